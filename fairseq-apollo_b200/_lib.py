@@ -87,6 +87,11 @@ SIGNATURES = {
     "mega_attention_bias_grad": [c_p, c_p, c_i, c_i, c_l, c_i, c_i, c_p],
     "mega_block_step": [c_p, c_p],
     "mega_block_cache_fill": [c_p, c_l, c_l, c_p, c_l, c_l, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_p, c_p, c_l, c_p],
+    "mega_gated_recurrence_fwd": [c_p] * 4 + [c_i] * 4 + [c_l] * 8 + [c_p] * 5 + [c_u, c_p],
+    "mega_gated_recurrence_bwd": [c_p] * 7 + [c_i] * 4 + [c_l] * 14 + [c_p] * 5 + [c_u, c_p],
+    "mega_gated_recurrence_step": [c_p] * 4 + [c_i] * 3 + [c_l] * 4 + [c_p] * 3,
+    "mega_group_norm_fwd": [c_p] * 2 + [c_i] * 4 + [c_l] * 4 + [c_p] * 3 + [c_i, c_d, c_u] + [c_p] * 5,
+    "mega_group_norm_bwd": [c_p] * 3 + [c_i] * 4 + [c_l] * 6 + [c_p] * 3 + [c_i, c_u] + [c_p] * 7,
     "mega_set_option": [c_i, c_i],
     "mega_debug_device_error": [ctypes.POINTER(c_i), c_i],
 }
@@ -95,6 +100,8 @@ OTHER = {
     "mega_last_cuda_error": ([], ctypes.c_char_p),
     "mega_abi_version": ([], c_i),
     "mega_block_step_work": ([c_i, c_i, c_i, c_i, c_i, c_l], c_l),
+    "mega_gated_recurrence_segment": ([c_i, c_i], c_i),
+    "mega_group_norm_work": ([c_i] * 5, c_l),
     "mega_launch_count": ([], ctypes.c_uint64),
     "mega_debug_last_kernel": ([], ctypes.c_char_p),
 }

@@ -41,3 +41,21 @@ def sequence_norm(x, weight, bias, padding_mask, eps, length_last, num_groups=No
     """y = SequenceNorm(x), per channel or per channel group, from the module's parameters."""
     return _lib.host().sequence_norm_train(x, weight, bias, padding_mask, eps, length_last,
                                            0 if num_groups is None else num_groups)
+
+
+def gated_recurrence(x, forget, input_gate=None, padding_mask=None, reset_mask=None, h_in=None, want_state=False, reverse=False):
+    """ops.gated_recurrence_fwd with gradients of x, both gates and h_in (through y and through the state that leaves)."""
+    r = _lib.host().gated_recurrence_train(x, forget, input_gate, padding_mask, reset_mask, h_in, want_state, reverse)
+    return tuple(r) if want_state else r[0]
+
+
+def gated_recurrence_packed(z, gated=False, padding_mask=None, reset_mask=None, h_in=None, want_state=False, reverse=False):
+    """gated_recurrence on z (B, L, 2 D), x and the forget gate side by side (with ``gated`` (B, L, 3 D), the input gate behind
+    them), as one projection leaves them; z's gradient is written in place of its parts."""
+    r = _lib.host().gated_recurrence_packed(z, gated, padding_mask, reset_mask, h_in, want_state, reverse)
+    return tuple(r) if want_state else r[0]
+
+
+def group_norm(x, weight, bias, num_groups, padding_mask, eps, activation):
+    """y = act(GroupNorm(x)) from the module's parameters (effective scale weight + 1)."""
+    return _lib.host().group_norm_train(x, weight, bias, num_groups, padding_mask, eps, ops._silu(activation))

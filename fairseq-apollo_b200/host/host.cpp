@@ -16,6 +16,8 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <climits>
+#include <cmath>
 #include <tuple>
 #include <unordered_map>
 #include <vector>
@@ -758,6 +760,307 @@ std::tuple<Tensor, Tensor> gate_qk(const Tensor& z, const Tensor& gamma, const T
   return {q, k};
 }
 
+// ------------------------------------------------------------------------------- gated linear recurrence
+// (the package's other operators take what a caller hands them; these check it all, as their operands come from several places)
+void same_kind(const Tensor& t, const Tensor& x, const char* what) {
+  if (!t.defined()) return;
+  if (t.scalar_type() != x.scalar_type()) throw py::type_error(std::string(what) + " must have x's type");
+  if (t.device() != x.device()) throw py::value_error(std::string(what) + " must be on x's device");
+  if (t.sizes() != x.sizes()) throw py::value_error(std::string(what) + " must have x's shape");
+}
+Tensor mask_on(const Tensor& mask, const Tensor& x, const char* what) {
+  if (!mask.defined()) return mask;
+  if (mask.device() != x.device()) throw py::value_error(std::string(what) + " must be on x's device");
+  if (mask.dim() != 2 || mask.size(0) != x.size(0) || mask.size(1) != x.size(1))
+    throw py::value_error(std::string(what) + " must be (batch, length) = (" + std::to_string(x.size(0)) + ", " + std::to_string(x.size(1)) + ")");
+  return mask.scalar_type() == at::kBool ? mask.contiguous() : mask.ne(0).contiguous();
+}
+void check_state(const Tensor& h, const Tensor& x, int64_t dim, const char* what) {
+  if (!h.defined()) return;
+  if (h.device() != x.device()) throw py::value_error(std::string(what) + " must be on x's device");
+  if (!at::isFloatingType(h.scalar_type())) throw py::type_error(std::string(what) + " must be a floating-point tensor");
+  if (h.dim() != 2 || h.size(0) != x.size(0) || h.size(1) != dim)
+    throw py::value_error(std::string(what) + " must be (batch, channels) = (" + std::to_string(x.size(0)) + ", " + std::to_string(dim) + ")");
+}
+int extent(int64_t n) {
+  expect(n <= INT_MAX, "an extent does not fit 32 bits");
+  return (int)n;
+}
+// contiguous channels; the strides of the axes before them are free
+Tensor channels(const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+struct Rec {
+  Tensor x, f, i, pad, reset, h_in;
+  int B, L, D;
+  unsigned flags;
+};
+Rec rec_args(const Tensor& x, const Tensor& f, const Tensor& i, const Tensor& pad, const Tensor& reset, const Tensor& h_in, bool reverse) {
+  on_cuda(x, f, i, pad, reset, h_in);
+  expect(x.dim() == 3, "x must be (batch, length, channels)");
+  dtype_of(x);
+  same_kind(f, x, "the forget gate");
+  same_kind(i, x, "the input gate");
+  check_state(h_in, x, x.size(2), "h_in");
+  Rec r = {channels(x.detach()), channels(f.detach()), i.defined() ? channels(i.detach()) : i};
+  r.pad = mask_on(pad, x, "padding_mask");
+  r.reset = mask_on(reset, x, "reset_mask");
+  r.h_in = f32c(h_in);
+  r.B = extent(x.size(0)), r.L = extent(x.size(1)), r.D = extent(x.size(2));
+  r.flags = reverse ? MEGA_REC_REVERSE : 0u;
+  return r;
+}
+#define STRIDES2(t) ((t).defined() ? (t).stride(0) : 0), ((t).defined() ? (t).stride(1) : 0)
+
+void run_rec(const Rec& r, const Tensor& y, const Tensor& h_out, const Tensor& starts, const Where& w) {
+  check(mega_gated_recurrence_fwd(r.x.data_ptr(), r.f.data_ptr(), ptr(r.i), y.data_ptr(), dtype_of(r.x), r.B, r.L, r.D, STRIDES2(r.x),
+                                  STRIDES2(r.f), STRIDES2(r.i), STRIDES2(y), ptr<uint8_t>(r.pad), ptr<uint8_t>(r.reset), fptr(r.h_in),
+                                  fptr(h_out), fptr(starts), r.flags, w.stream), "gated_recurrence_fwd");
+}
+// the output of (B, L, D) operands: time-major ones give a time-major result
+Tensor rec_like(const Tensor& x) {
+  Tensor y = like(x);
+  return y.size(-1) == 1 || y.stride(-1) == 1 ? y : at::empty(x.sizes(), x.options().requires_grad(false));
+}
+
+// (y, state behind the last step or None)
+std::tuple<Tensor, OptTensor> gated_recurrence(const Tensor& x, const Tensor& f, const OptTensor& i, const OptTensor& pad,
+                                               const OptTensor& reset, const OptTensor& h_in, bool want_state, bool reverse) {
+  const Rec r = rec_args(x, f, given(i), given(pad), given(reset), given(h_in), reverse);
+  const Where w(x);
+  const Tensor y = rec_like(x);
+  Tensor h = want_state ? floats({r.B, r.D}, x) : Tensor();
+  if (x.numel() == 0) {   // (no step: the state stays)
+    if (h.defined()) r.h_in.defined() ? h.copy_(r.h_in) : h.zero_();
+  } else {
+    run_rec(r, y, h, none(), w);
+  }
+  if (!want_state) return {y, std::nullopt};
+  return {y, h};
+}
+
+// one step: x, f, i (B, D) -> (y, h'); h' is `h_out` where given, which may be h
+std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x_, const Tensor& f_, const OptTensor& i_, const OptTensor& h_,
+                                                 const OptTensor& h_out_) {
+  on_cuda(x_, f_, given(i_), given(h_), given(h_out_));
+  expect(x_.dim() == 2, "x must be (batch, channels)");
+  const int dt = dtype_of(x_);
+  same_kind(f_, x_, "the forget gate");
+  same_kind(given(i_), x_, "the input gate");
+  check_state(given(h_), x_, x_.size(1), "h");
+  const Where w(x_);
+  const Tensor x = channels(x_), f = channels(f_), i = channels(given(i_)), h = f32c(given(h_));
+  const int B = extent(x.size(0)), D = extent(x.size(1));
+  Tensor y = at::empty(x.sizes(), x.options().requires_grad(false)), out = given(h_out_);
+  if (out.defined()) {
+    check_state(out, x_, D, "h_out");
+    expect(out.scalar_type() == at::kFloat && out.is_contiguous(), "h_out must be contiguous float32");
+  } else {
+    out = floats({B, D}, x);
+  }
+  if (x.numel())
+    check(mega_gated_recurrence_step(x.data_ptr(), f.data_ptr(), ptr(i), y.data_ptr(), dt, B, D, x.stride(0), f.stride(0),
+                                     i.defined() ? i.stride(0) : 0, D, fptr(h), fptr(out), w.stream), "gated_recurrence_step");
+  return {y, out};
+}
+
+void first_order() {
+  if (at::GradMode::is_enabled()) throw std::runtime_error("mega_b200: second derivatives of this operator are not available");
+}
+// a gradient of (B, L, D) values in x's type with contiguous channels
+Tensor rec_grad(const Tensor& g, const Tensor& x) {
+  return channels(g.scalar_type() == x.scalar_type() ? g : g.to(x.scalar_type()));
+}
+
+// Separate operands, or one tensor z (B, L, 2 D or 3 D) that holds x, f (and i) side by side, whose gradient then comes as
+// one tensor too (the gradients of three slices would be three tensors of z's size, added up).
+class RecFn : public torch::autograd::Function<RecFn> {
+ public:
+  static variable_list forward(AutogradContext* ctx, Tensor x, OptTensor f, OptTensor i, OptTensor pad, OptTensor reset, OptTensor h_in,
+                               bool want_state, bool reverse, int64_t packed) {
+    const int64_t d = packed ? x.size(2) / packed : x.size(2);
+    auto part = [&](int64_t k) { return x.detach().narrow(2, k * d, d); };
+    const Rec r = packed ? rec_args(part(0), part(1), packed == 3 ? part(2) : Tensor(), given(pad), given(reset), given(h_in), reverse)
+                         : rec_args(x, given(f), given(i), given(pad), given(reset), given(h_in), reverse);
+    const Where w(x);
+    const int64_t seg = mega_gated_recurrence_segment(dtype_of(r.x), r.i.defined());
+    Tensor y = rec_like(r.x), h = want_state ? floats({r.B, r.D}, x) : Tensor(), starts = floats({r.B, (r.L + seg - 1) / seg, r.D}, x);
+    run_rec(r, y, h, starts, w);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, given(f), given(i), r.pad, r.reset, given(h_in), starts});
+    ctx->saved_data["reverse"] = reverse;
+    ctx->saved_data["packed"] = packed;
+    if (!want_state) return {y};
+    return {y, h};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order();
+    const auto s = ctx->get_saved_variables();
+    const int64_t packed = ctx->saved_data["packed"].toInt();
+    const Tensor &z = s[0], &starts = s[6], &h_in = s[5];
+    const Where w(z);
+    const int64_t d = packed ? z.size(2) / packed : z.size(2);
+    auto part = [&](const Tensor& t, int64_t k) { return t.narrow(2, k * d, d); };
+    const Tensor x = channels(packed ? part(z, 0) : z), f = channels(packed ? part(z, 1) : s[1]);
+    const Tensor i = channels(packed == 3 ? part(z, 2) : s[2]);
+    const bool dh = grads.size() > 1 && grads[1].defined();
+    const Tensor dy = grads[0].defined() ? rec_grad(grads[0], x) : at::zeros(x.sizes(), x.options());
+    const Tensor dh_out = dh ? f32c(grads[1]) : Tensor();
+    Tensor dz = packed ? at::empty(z.sizes(), z.options().requires_grad(false)) : Tensor();
+    Tensor dx = packed ? part(dz, 0) : rec_like(x), df = packed ? part(dz, 1) : rec_like(f), di;
+    if (i.defined()) di = packed ? part(dz, 2) : rec_like(i);
+    Tensor dh_in = h_in.defined() ? floats({x.size(0), d}, x) : Tensor();
+    check(mega_gated_recurrence_bwd(dy.data_ptr(), x.data_ptr(), f.data_ptr(), ptr(i), dx.data_ptr(), df.data_ptr(), ptr(di),
+                                    dtype_of(x), (int)x.size(0), (int)x.size(1), (int)d, STRIDES2(dy), STRIDES2(x), STRIDES2(f),
+                                    STRIDES2(i), STRIDES2(dx), STRIDES2(df), STRIDES2(di), ptr<uint8_t>(s[3]), ptr<uint8_t>(s[4]),
+                                    fptr(starts), fptr(dh_out), fptr(dh_in), ctx->saved_data["reverse"].toBool() ? MEGA_REC_REVERSE : 0u,
+                                    w.stream), "gated_recurrence_bwd");
+    if (dh_in.defined()) dh_in = dh_in.to(h_in.scalar_type());
+    return {packed ? dz : dx, packed ? Tensor() : df, packed ? Tensor() : di, Tensor(), Tensor(), dh_in, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// (y, h) or (y,); differentiable
+variable_list gated_recurrence_train(const Tensor& x, const Tensor& f, const OptTensor& i, const OptTensor& pad, const OptTensor& reset,
+                                     const OptTensor& h_in, bool want_state, bool reverse) {
+  rec_args(x, f, given(i), given(pad), given(reset), given(h_in), reverse);
+  if (x.numel() == 0) {
+    variable_list r = {i.has_value() ? x + f + *i : x + f};   // (no values, but gradients of that shape)
+    if (want_state) r.push_back(h_in.has_value() ? h_in->to(at::kFloat, false, true) : at::zeros({x.size(0), x.size(2)}, x.options().dtype(at::kFloat)));
+    return r;
+  }
+  return RecFn::apply(x, OptTensor(f), i, pad, reset, h_in, want_state, reverse, (int64_t)0);
+}
+variable_list gated_recurrence_packed(const Tensor& z, bool gated, const OptTensor& pad, const OptTensor& reset, const OptTensor& h_in,
+                                      bool want_state, bool reverse) {
+  const int64_t k = gated ? 3 : 2;
+  on_cuda(z);
+  expect(z.dim() == 3 && z.size(2) % k == 0, "the packed operand must be (batch, length, 2 or 3 times the channels)");
+  const int64_t d = z.size(2) / k;
+  if (z.numel() == 0)
+    return gated_recurrence_train(z.narrow(2, 0, d), z.narrow(2, d, d), gated ? OptTensor(z.narrow(2, 2 * d, d)) : std::nullopt, pad, reset,
+                                  h_in, want_state, reverse);
+  return RecFn::apply(z, OptTensor(), OptTensor(), pad, reset, h_in, want_state, reverse, k);
+}
+
+// ----------------------------------------------------------------------- group norm with an activation
+// x (B, ..., D) as (B, L, D) with contiguous channels
+Tensor gn_rows(const Tensor& x) {
+  expect(x.dim() >= 2, "x must be (batch, ..., channels)");
+  if (x.dim() == 3) return channels(x);
+  return channels(x.dim() == 2 ? x.unsqueeze(1) : x.reshape({x.size(0), -1, x.size(-1)}));
+}
+struct Gn {
+  Tensor x, gamma, beta, mask;
+  int B, L, D, G;
+  unsigned flags;
+};
+Gn gn_args(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, const Tensor& mask, bool silu, bool offset,
+           const Where& w) {
+  on_cuda(x, weight, bias, mask);
+  dtype_of(x);
+  const Tensor rows = x.numel() ? gn_rows(x) : x;
+  const int64_t d = x.size(-1);
+  expect(groups >= 1 && d % groups == 0, "num_groups must divide the channels");
+  expect_numel(weight, d, "weight");
+  expect_numel(bias, d, "bias");
+  if (weight.device() != x.device() || bias.device() != x.device()) throw py::value_error("weight and bias must be on x's device");
+  Gn r = {rows};
+  if (x.numel()) {
+    Tensor m = mask;
+    if (m.defined() && m.dim() != 2 && m.dim() == x.dim() - 1) {
+      expect(m.sizes() == x.sizes().slice(0, x.dim() - 1), "padding_mask must have x's shape without its channels");
+      m = m.reshape({m.size(0), -1});
+    } else if (m.defined() && x.dim() == 2 && m.dim() == 1) {
+      m = m.unsqueeze(1);
+    }
+    r.mask = mask_on(m, rows, "padding_mask");
+    const auto p = f32_all({weight.detach(), bias.detach()}, w.stream);
+    r.gamma = p[0], r.beta = p[1];
+    r.B = extent(rows.size(0)), r.L = extent(rows.size(1)), r.D = extent(d), r.G = (int)groups;
+  }
+  r.flags = (silu ? MEGA_GN_SILU : 0u) | (offset ? MEGA_GN_OFFSET : 0u);
+  return r;
+}
+Tensor gn_work(const Gn& r) {
+  return at::empty({mega_group_norm_work(dtype_of(r.x), r.B, r.L, r.D, r.G)}, at::TensorOptions().dtype(at::kByte).device(r.x.device()));
+}
+// A result of x's shape for rows r, and its own rows (a tensor of its own: a view could not be changed in place)
+std::pair<Tensor, Tensor> gn_like(const Tensor& x, const Tensor& rows) {
+  if (x.dim() == 3) {
+    Tensor y = rec_like(rows);
+    return {y, y};
+  }
+  Tensor y = at::empty(x.sizes(), x.options().requires_grad(false));
+  return {y, y.view(rows.sizes())};
+}
+// y like x and its statistics (count, mean, rstd)
+std::tuple<Tensor, Tensor, Tensor, Tensor> run_gn(const Tensor& x, const Gn& r, double eps, const Where& w) {
+  auto [out, y] = gn_like(x, r.x);
+  Tensor count = counts(r.B, r.x), st = floats({2, r.B, r.G}, r.x);
+  Tensor mean = st.select(0, 0), rstd = st.select(0, 1);
+  const Tensor work = gn_work(r);
+  check(mega_group_norm_fwd(r.x.data_ptr(), y.data_ptr(), dtype_of(r.x), r.B, r.L, r.D, STRIDES2(r.x), STRIDES2(y), fptr(r.gamma),
+                            fptr(r.beta), ptr<uint8_t>(r.mask), r.G, eps, r.flags, ptr<int64_t>(count), fptr(mean), fptr(rstd),
+                            work.data_ptr(), w.stream), "group_norm_fwd");
+  return {out, count, mean, rstd};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> group_norm_fwd(const Tensor& x, const Tensor& gamma, const Tensor& beta, int64_t groups,
+                                                          const OptTensor& mask, double eps, bool silu, bool offset) {
+  on_cuda(x);
+  const Where w(x);
+  const Gn r = gn_args(x, gamma, beta, groups, given(mask), silu, offset, w);
+  if (x.numel() == 0) {
+    const int64_t b = x.size(0);
+    Tensor rstd = floats({b, groups}, x);
+    rstd.fill_(1.0 / std::sqrt(eps));
+    return {fresh(x), counts(b, x).zero_(), floats({b, groups}, x).zero_(), rstd};
+  }
+  return run_gn(x, r, eps, w);
+}
+
+class GnFn : public torch::autograd::Function<GnFn> {
+ public:
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor weight, Tensor bias, int64_t groups, OptTensor mask, double eps, bool silu) {
+    on_cuda(x);
+    const Where w(x);
+    const Gn r = gn_args(x, weight, bias, groups, given(mask), silu, true, w);
+    auto [y, count, mean, rstd] = run_gn(x.detach(), r, eps, w);
+    ctx->save_for_backward({x, weight, bias, r.mask, count, mean, rstd});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["silu"] = silu;
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order();
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &weight = s[1], &bias = s[2];
+    const Where w(x);
+    const Gn r = gn_args(x, weight, bias, ctx->saved_data["groups"].toInt(), Tensor(), ctx->saved_data["silu"].toBool(), true, w);
+    Tensor dy = grads[0];
+    dy = gn_rows(dy.scalar_type() == x.scalar_type() ? dy : dy.to(x.scalar_type()));
+    auto [out, dx] = gn_like(x, r.x);
+    Tensor f = floats({2, r.D}, x);
+    const Tensor work = gn_work(r);
+    check(mega_group_norm_bwd(dy.data_ptr(), r.x.data_ptr(), dx.data_ptr(), dtype_of(r.x), r.B, r.L, r.D, STRIDES2(dy), STRIDES2(r.x),
+                              STRIDES2(dx), fptr(r.gamma), fptr(r.beta), ptr<uint8_t>(s[3]), r.G, r.flags, ptr<int64_t>(s[4]),
+                              fptr(s[5]), fptr(s[6]), fptr(f), fptr(f) + r.D, work.data_ptr(), w.stream), "group_norm_bwd");
+    auto own = [&](int64_t k, const Tensor& p) { return f.select(0, k).view(p.sizes()).to(p.scalar_type()); };
+    return {out, own(0, weight), own(1, bias), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor group_norm_train(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, const OptTensor& mask, double eps,
+                        bool silu) {
+  if (x.numel() == 0) {   // (no values, but gradients of that shape)
+    on_cuda(x, weight, bias);
+    return (x * (weight + bias)).to(x.scalar_type());
+  }
+  return GnFn::apply(x, weight, bias, groups, mask, eps, silu);
+}
+
 Tensor softmax_fwd(const Tensor& x, bool causal) {
   on_cuda(x);
   const Where w(x);
@@ -1396,6 +1699,12 @@ PYBIND11_MODULE(_mega_host, m) {
   m.def("gate_output", &gate_output);
   m.def("gate_qk", &gate_qk);
   m.def("attention_softmax_fwd", &softmax_fwd);
+  m.def("gated_recurrence", &gated_recurrence);
+  m.def("gated_recurrence_step", &gated_recurrence_step);
+  m.def("gated_recurrence_train", &gated_recurrence_train);
+  m.def("gated_recurrence_packed", &gated_recurrence_packed);
+  m.def("group_norm_fwd", &group_norm_fwd);
+  m.def("group_norm_train", &group_norm_train);
   m.def("block_train", &block_train);
   m.def("block_infer", &block_infer);
 }

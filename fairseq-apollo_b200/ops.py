@@ -512,6 +512,41 @@ def cema_coeffs_bwd(alpha, delta, theta, q, dp, dq, dg, dtype=torch.float32):
     return da.view(k, n, 1), dd.view(k, n, 1), dt.view(k, 1, 1), dgm.view(k, n, 2)
 
 
+# --------------------------------------------------------- gated linear recurrence
+def gated_recurrence_fwd(x, forget, input_gate=None, padding_mask=None, reset_mask=None, h_in=None, want_state=False,
+                         reverse=False):
+    """h_t = (1 - l_t) h_{t-1} + l_t x_t with l = sigmoid(-forget), or + sigmoid(input_gate_t) x_t, over the steps of x (B, L, D);
+    y_t = h_t.  x, forget and input_gate share shape and dtype; their strides are free (column slices, time-major memory), a copy
+    is made where the channels are not contiguous.
+    padding_mask (B, L), non-zero = padded: the state stays as it is, y = 0.  reset_mask (B, L), non-zero: the step starts from
+    a zero state (the first step of a document in a packed sequence).  h_in (B, D): the state that comes in.
+    ``reverse`` walks from the last step to the first.
+    Returns y like x, and the state behind the walk's last step (B, D) fp32 when ``want_state``."""
+    y, h = _lib.host().gated_recurrence(x, forget, input_gate, padding_mask, reset_mask, h_in, want_state, reverse)
+    return (y, h) if want_state else y
+
+
+def gated_recurrence_step(x, forget, input_gate=None, h=None, h_out=None):
+    """One step: x, forget, input_gate (B, D), h (B, D) the state (None: zero) -> (y like x, h' (B, D) fp32).  ``h_out``: the
+    contiguous fp32 tensor that takes h', ``h`` itself for an update in place."""
+    return _lib.host().gated_recurrence_step(x, forget, input_gate, h, h_out)
+
+
+# ------------------------------------------------------ group norm with an activation
+def group_norm_fwd(x, gamma, beta, num_groups, padding_mask=None, eps=1e-5, activation=None, offset=False):
+    """Group norm of x (B, ..., D), channels last: mean and variance of a group of D / num_groups adjacent channels over all
+    positions of a sequence that are not padded (padding_mask: x's shape without the channels, non-zero = padded, y = 0 there);
+    y = act((x - mean) * rstd * gamma + beta), ``activation`` None or 'silu'; with ``offset`` the scale is gamma + 1.
+    Returns (y, count (B) int64, mean, rstd (B, G) fp32)."""
+    return _lib.host().group_norm_fwd(x, gamma, beta, int(num_groups), padding_mask, float(eps), _silu(activation), offset)
+
+
+def _silu(activation):
+    if activation not in (None, "silu"):
+        raise ValueError("activation must be None or 'silu', got %r" % (activation,))
+    return activation == "silu"
+
+
 # ----------------------------------------------------------------------- attention
 def attention_softmax_fwd(x, causal=True):
     """softmax over the last axis of the score tensor x (..., C_q, C_k); with ``causal`` row r keeps

@@ -614,6 +614,66 @@ MEGA_API int mega_block_cache_fill(const void* k, int64_t ksb, int64_t ksl, cons
                           const float* rot, int positions, int dtype, int batch, int n, int zdim, int hdim, void* keys,
                           void* keys_rot, void* values, int64_t cap, mega_stream_t stream);
 
+/*
+ * ---- Gated linear recurrence -----------------------------------------------------------------
+ * One state per sequence and channel, a decay that depends on the step:
+ *   h_t = (1 - l_t) h_{t-1} + l_t x_t            l = sigmoid(-f)          (i == NULL: tied gates)
+ *   h_t = (1 - l_t) h_{t-1} + sigmoid(i_t) x_t                            (an input gate of its own)
+ * y_t = h_t.  f and i are what the sigmoids take.  A step whose byte of reset_mask is set starts from a zero state; a
+ * step whose byte of pad_mask is set leaves the state as it is (after the reset, when both are set), gives y = 0, and
+ * what lies there in x, f, i is not used.  A state that is not finite reaches no step behind a reset.
+ *
+ * x, f, i, y (and the gradients) are (B, L, D) with contiguous channels; the strides of the other two axes are free, 0
+ * and negative ones among them for what is read, and outputs do not overlap one another or an input.  Masks are (B, L)
+ * uint8, either may be NULL.
+ * h_in, h_out, dh_out, dh_in are (B, D) fp32, either may be NULL (a NULL h_in is zero); h_out may be h_in, dh_in may be
+ * dh_out.  MEGA_REC_REVERSE walks from the last step to the first (h_in enters behind the last step, h_out is the state at
+ * the first).  At most 65535 sequences (MEGA_ERR_UNSUPPORTED).
+ *
+ * mega_gated_recurrence_fwd: with `starts` also the state before every segment of mega_gated_recurrence_segment() steps,
+ * counted in the order of the walk: (B, ceil(L / segment), D) fp32, all that the backward needs besides the inputs.
+ * mega_gated_recurrence_bwd: dy is y's gradient, dh_out h_out's (NULL: zero).  Outputs dx, df, di (with i) in the
+ * activations' type, 0 at padded steps, and dh_in where it is not NULL.
+ * mega_gated_recurrence_step: one step of every sequence, x, f, i, y (B, D).
+ */
+#define MEGA_REC_REVERSE 1u
+MEGA_API int mega_gated_recurrence_segment(int dtype, int gated);
+MEGA_API int mega_gated_recurrence_fwd(const void* x, const void* f, const void* i, void* y, int dtype, int B, int L, int D,
+                              int64_t xsb, int64_t xsl, int64_t fsb, int64_t fsl, int64_t isb, int64_t isl, int64_t ysb,
+                              int64_t ysl, const uint8_t* pad_mask, const uint8_t* reset_mask, const float* h_in, float* h_out,
+                              float* starts, unsigned flags, mega_stream_t stream);
+MEGA_API int mega_gated_recurrence_bwd(const void* dy, const void* x, const void* f, const void* i, void* dx, void* df, void* di,
+                              int dtype, int B, int L, int D, int64_t gsb, int64_t gsl, int64_t xsb, int64_t xsl, int64_t fsb,
+                              int64_t fsl, int64_t isb, int64_t isl, int64_t dxb, int64_t dxl, int64_t dfb, int64_t dfl,
+                              int64_t dib, int64_t dil, const uint8_t* pad_mask, const uint8_t* reset_mask, const float* starts,
+                              const float* dh_out, float* dh_in, unsigned flags, mega_stream_t stream);
+MEGA_API int mega_gated_recurrence_step(const void* x, const void* f, const void* i, void* y, int dtype, int B, int D, int64_t xsb,
+                               int64_t fsb, int64_t isb, int64_t ysb, const float* h_in, float* h_out, mega_stream_t stream);
+
+/*
+ * ---- Group norm with an activation, channels last ----------------------------------------------
+ * x (B, L, D) with contiguous channels (the strides of the other two axes are free), num_groups groups of D / num_groups
+ * adjacent channels.  Mean and variance of a (sequence, group) are taken over its channels and the steps that are not
+ * padded; y = act((x - mean) * rstd * scale + beta), 0 at padded steps, whatever lies there in x.  act is SiLU with
+ * MEGA_GN_SILU, else nothing.  gamma, beta are (D) fp32; scale = gamma, or gamma + 1 with MEGA_GN_OFFSET.
+ * Statistics: count (B) int64 (steps that are not padded), mean, rstd (B, G) fp32 (0 and 1 / sqrt(eps) without a step).
+ *
+ * mega_group_norm_bwd: dx like x (0 at padded steps), dgamma, dbeta (D) fp32, summed over sequences and steps in a fixed
+ * order.  `work`: device memory of mega_group_norm_work() bytes, 16-byte aligned, used by this call alone until it is done;
+ * forward and backward take the same size.
+ * At most 65535 sequences and groups (MEGA_ERR_UNSUPPORTED).
+ */
+#define MEGA_GN_SILU 1u
+#define MEGA_GN_OFFSET 2u
+MEGA_API int64_t mega_group_norm_work(int dtype, int B, int L, int D, int num_groups);
+MEGA_API int mega_group_norm_fwd(const void* x, void* y, int dtype, int B, int L, int D, int64_t xsb, int64_t xsl, int64_t ysb,
+                        int64_t ysl, const float* gamma, const float* beta, const uint8_t* pad_mask, int num_groups, double eps,
+                        unsigned flags, int64_t* count, float* mean, float* rstd, void* work, mega_stream_t stream);
+MEGA_API int mega_group_norm_bwd(const void* dy, const void* x, void* dx, int dtype, int B, int L, int D, int64_t gsb, int64_t gsl,
+                        int64_t xsb, int64_t xsl, int64_t dsb, int64_t dsl, const float* gamma, const float* beta,
+                        const uint8_t* pad_mask, int num_groups, unsigned flags, const int64_t* count, const float* mean,
+                        const float* rstd, float* dgamma, float* dbeta, void* work, mega_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
