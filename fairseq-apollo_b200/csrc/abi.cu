@@ -11,7 +11,7 @@ namespace mega {
 
 std::atomic<uint64_t> g_launches{0};
 thread_local char g_cuda_err[256] = "";
-std::atomic<int> g_options[8];
+std::atomic<int> g_options[9];
 std::atomic<const char*> g_last_kernel{"none"};
 
 void allow_smem(const void* kernel, size_t bytes) {
@@ -60,7 +60,7 @@ extern "C" uint64_t mega_launch_count(void) { return mega::g_launches.load(); }
 extern "C" MEGA_API const char* mega_debug_last_kernel(void) { return mega::g_last_kernel.load(); }
 
 extern "C" MEGA_API int mega_set_option(int key, int value) {
-  if (key < 0 || key >= 8) return MEGA_ERR_SHAPE;
+  if (key < 0 || key >= 9) return MEGA_ERR_SHAPE;
   mega::g_options[key].store(value);
   return MEGA_OK;
 }

@@ -1,119 +1,531 @@
-// Gated linear recurrence: a decay per step, sequence and channel.
+// Gated linear recurrence: a decay per step, sequence and channel; forward, backward, single step.
 //
 //   l_t = sigmoid(-f_t),  h_t = h_{t-1} - l_t h_{t-1} + c_t,  c_t = l_t x_t  or  sigmoid(i_t) x_t
 //
 // written with the leak l instead of the decay 1 - l: a gate that stands open (f >> 0) has a leak far below the spacing of
-// floats next to 1, and 1 - l would round it to a few bits.
+// floats next to 1, and 1 - l would round it to a few bits, the same way at every step.
+//
+// A run of steps maps the state that enters it linearly to the one that leaves, h -> h_loc + A h (h_loc: from a zero state,
+// A: the product of the decays), and such maps compose, so the time axis is split: a warp takes 64 channels (two to a lane) of
+// kS steps, a block kW such segments, a cluster of up to eight blocks as many block tiles, and walks the sequence in
+// strides of the cluster.  A segment is walked once, h_loc and A of every step staying in registers; its map goes through
+// shared memory to the block's other warps, the block's through distributed shared memory to the cluster's other blocks;
+// then y_t = h_loc,t + A_t h for the state h that enters.  Inputs are read once, by cp.async into a ring of the warp's own, so
+// the next tile is on its way while this one is worked on and exchanged.
+//
+// Backward, with q the gradient that flows into the state behind a step: g_t = dy_t + q, q' = (1 - l_t) g_t, a linear map
+// of the same kind walked the other way.  The states are walked again from one that the forward left for each segment.
+//   tied gates   dx = l g,  df = q' l (h_{t-1} - x)       input gate s   dx = s g,  df = q' l h_{t-1},  di = s (1 - s) x g
+//
+// A reset is a map that ignores what enters: its A is -0 (the decays are never negative), and A = -0 means h_loc alone, so
+// that nothing infinite or NaN passes.
+// Bound: HBM.
 #include <algorithm>
+#include <climits>
+#include <type_traits>
 
 #include "common.cuh"
+#include "tma.cuh"
 
 namespace mega {
 
 namespace {
 
-constexpr int kSeg = 16;   // steps between two saved states
+constexpr int kW = 8;        // segments (warps) of a block
+constexpr int kC = 64;       // channels of a tile
+constexpr int kStages = 2;   // tiles of a warp's ring
 
 struct RecArgs {
   const void *x, *f, *i, *dy;
   void *y, *dx, *df, *di;
+  // strides in elements of the axes before the channels; a walk from the last step has its pointers there and these negative
   long long xsb, xsl, fsb, fsl, isb, isl, ysb, ysl, gsb, gsl, dxb, dxl, dfb, dfl, dib, dil;
   const unsigned char *pad, *reset;
+  long long msb, msl;
   const float *h_in, *dh_out;
   float *h_out, *starts, *dh_in;
-  int B, L, D, reverse;
+  int L, D, pairs;   // pairs: whether two floats of a state lie on 8 bytes
 };
 
-template <typename T>
-__device__ __forceinline__ float leak_of(float f) {
-  const float e = 1.f + exp_of<T>(f);
-  return sizeof(T) == 4 ? 1.f / e : rcp_approx(e);
+// Steps of a segment: what h_loc and A of every step (the backward: leak, state and, with an input gate, its two factors) leave of
+// 128 registers.
+template <typename T, bool kGate>
+constexpr int kSteps = sizeof(T) == 4 || kGate ? 8 : 16;
+
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void put_peer(float4* p, int rank, float4 v) {   // to the same place in another block's shared memory
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int valid) {   // the rest of kBytes is zeroed
+  if (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// -sigmoid(-f): minus the leak
 template <typename T>
-__global__ void __launch_bounds__(128) rec_fwd_kernel(RecArgs a) {
-  const int b = blockIdx.y, d = blockIdx.x * 128 + threadIdx.x;
-  if (d >= a.D) return;
-  float h = a.h_in ? a.h_in[(long long)b * a.D + d] : 0.f;
-  const int nseg = (a.L + kSeg - 1) / kSeg;
-  for (int k = 0; k < a.L; ++k) {
-    const int t = a.reverse ? a.L - 1 - k : k;
-    if (a.starts && k % kSeg == 0) a.starts[((long long)b * nseg + k / kSeg) * a.D + d] = h;
-    if (a.reset && a.reset[(long long)b * a.L + t]) h = 0.f;
-    float y = 0.f;
-    if (!(a.pad && a.pad[(long long)b * a.L + t])) {
-      const float x = Elem<T>::ld((const T*)a.x + b * a.xsb + t * a.xsl + d);
-      const float l = leak_of<T>(Elem<T>::ld((const T*)a.f + b * a.fsb + t * a.fsl + d));
-      h = a.i ? fmaf(-l, h, fmaf(leak_of<T>(-Elem<T>::ld((const T*)a.i + b * a.isb + t * a.isl + d)), x, h)) : fmaf(l, x - h, h);
-      y = h;
-    }
-    Elem<T>::st((T*)a.y + b * a.ysb + t * a.ysl + d, y);
+__device__ __forceinline__ float minus_leak(float f) {
+  return sizeof(T) == 4 ? -1.f / (1.f + expf(f)) : rcp_approx(-1.f - __expf(f));
+}
+template <typename T>
+__device__ __forceinline__ f32x2 minus_leak2(f32x2 f) {
+  float a, b;
+  if (sizeof(T) == 4) {
+    unpack2(f, a, b);
+    return pack2(minus_leak<T>(a), minus_leak<T>(b));
   }
-  if (a.h_out) a.h_out[(long long)b * a.D + d] = h;
+  unpack2(mul2(f, pack2(1.4426950408889634f, 1.4426950408889634f)), a, b);   // e^f = 2^(f / ln 2)
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+  unpack2(add2(mul2(pack2(a, b), pack2(-1.f, -1.f)), pack2(-1.f, -1.f)), a, b);
+  return pack2(rcp_approx(a), rcp_approx(b));
+}
+// sigmoid(i), and sigmoid(i) sigmoid(-i) where the caller asks for it
+template <typename T, bool kSlope>
+__device__ __forceinline__ float gate_one(float i, float& slope) {
+  const float e = exp_of<T>(-i), s = sizeof(T) == 4 ? 1.f / (1.f + e) : rcp_approx(1.f + e);
+  if (kSlope) slope = s * (fminf(e, 3.4e38f) * s);   // (e s = sigmoid(-i); an infinite e comes with s = 0)
+  return s;
+}
+template <typename T, bool kSlope>
+__device__ __forceinline__ f32x2 gate2(f32x2 i, f32x2& slope) {
+  float a, b, p = 0.f, q = 0.f;
+  unpack2(i, a, b);
+  const f32x2 s = pack2(gate_one<T, kSlope>(a, p), gate_one<T, kSlope>(b, q));
+  if (kSlope) slope = pack2(p, q);
+  return s;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(128) rec_bwd_kernel(RecArgs a) {
-  const int b = blockIdx.y, d = blockIdx.x * 128 + threadIdx.x;
-  if (d >= a.D) return;
-  float q = a.dh_out ? a.dh_out[(long long)b * a.D + d] : 0.f;
-  const int nseg = (a.L + kSeg - 1) / kSeg;
-  for (int s = nseg - 1; s >= 0; --s) {
-    const int n = min(kSeg, a.L - s * kSeg);
-    float h = a.starts[((long long)b * nseg + s) * a.D + d];
-    float hp[kSeg];
-    for (int j = 0; j < n; ++j) {
-      const int k = s * kSeg + j, t = a.reverse ? a.L - 1 - k : k;
-      if (a.reset && a.reset[(long long)b * a.L + t]) h = 0.f;
-      hp[j] = h;
-      if (a.pad && a.pad[(long long)b * a.L + t]) continue;
-      const float x = Elem<T>::ld((const T*)a.x + b * a.xsb + t * a.xsl + d);
-      const float l = leak_of<T>(Elem<T>::ld((const T*)a.f + b * a.fsb + t * a.fsl + d));
-      h = a.i ? fmaf(-l, h, fmaf(leak_of<T>(-Elem<T>::ld((const T*)a.i + b * a.isb + t * a.isl + d)), x, h)) : fmaf(l, x - h, h);
+// two neighbouring values of shared memory
+__device__ __forceinline__ f32x2 two(const float* p) {
+  const float2 v = *reinterpret_cast<const float2*>(p);
+  return pack2(v.x, v.y);
+}
+__device__ __forceinline__ f32x2 two(const __nv_bfloat16* p) {
+  const unsigned v = *reinterpret_cast<const unsigned*>(p);
+  return pack2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ f32x2 two(const __half* p) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(p));
+  return pack2(v.x, v.y);
+}
+// two values to memory: as one word where kPair, `n` of them (0 .. 2) are inside
+template <bool kPair>
+__device__ __forceinline__ void put(float* p, f32x2 v, int n) {
+  float a, b;
+  unpack2(v, a, b);
+  if (kPair && n == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(a, b);
+  } else {
+    if (n > 0) p[0] = a;
+    if (n > 1) p[1] = b;
+  }
+}
+template <bool kPair>
+__device__ __forceinline__ void put(__nv_bfloat16* p, f32x2 v, int n) {
+  float a, b;
+  unpack2(v, a, b);
+  if (kPair && n == 2) {
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+  } else {
+    if (n > 0) p[0] = __float2bfloat16_rn(a);
+    if (n > 1) p[1] = __float2bfloat16_rn(b);
+  }
+}
+template <bool kPair>
+__device__ __forceinline__ void put(__half* p, f32x2 v, int n) {
+  float a, b;
+  unpack2(v, a, b);
+  if (kPair && n == 2) {
+    *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b);
+  } else {
+    if (n > 0) p[0] = __float2half_rn(a);
+    if (n > 1) p[1] = __float2half_rn(b);
+  }
+}
+__device__ __forceinline__ f32x2 neg2(f32x2 v) { return v ^ 0x8000000080000000ull; }
+__device__ __forceinline__ f32x2 minus_zero() { return 0x8000000080000000ull; }
+
+__device__ __forceinline__ f32x2 get_state(const float* p, int n, bool pairs) {
+  if (p == nullptr || n == 0) return pack2(0.f, 0.f);
+  if (pairs && n == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    return pack2(v.x, v.y);
+  }
+  return pack2(p[0], n > 1 ? p[1] : 0.f);
+}
+__device__ __forceinline__ void put_state(float* p, f32x2 v, int n, bool pairs) {
+  if (pairs)
+    put<true>(p, v, n);
+  else
+    put<false>(p, v, n);
+}
+
+// a map of the state: what a run makes of zero, and the factor of what enters
+struct Map {
+  f32x2 a, h;
+  __device__ __forceinline__ float4 words() const {
+    float4 v;
+    unpack2(a, v.x, v.y);
+    unpack2(h, v.z, v.w);
+    return v;
+  }
+  __device__ __forceinline__ static Map of(float4 v) { return {pack2(v.x, v.y), pack2(v.z, v.w)}; }
+  template <bool kReset>
+  __device__ __forceinline__ f32x2 operator()(f32x2 in) const {
+    f32x2 r = fma2(a, in, h);
+    if (kReset) {
+      float a0, a1, h0, h1, r0, r1;
+      unpack2(a, a0, a1), unpack2(h, h0, h1), unpack2(r, r0, r1);
+      r = pack2(__float_as_int(a0) == (int)0x80000000 ? h0 : r0, __float_as_int(a1) == (int)0x80000000 ? h1 : r1);
     }
-    for (int j = n - 1; j >= 0; --j) {
-      const int k = s * kSeg + j, t = a.reverse ? a.L - 1 - k : k;
-      float dx = 0.f, df = 0.f, di = 0.f;
-      if (!(a.pad && a.pad[(long long)b * a.L + t])) {
-        const float x = Elem<T>::ld((const T*)a.x + b * a.xsb + t * a.xsl + d);
-        const float l = leak_of<T>(Elem<T>::ld((const T*)a.f + b * a.fsb + t * a.fsl + d));
-        const float g = q + Elem<T>::ld((const T*)a.dy + b * a.gsb + t * a.gsl + d);
-        q = fmaf(-l, g, g);
-        if (a.i) {
-          const float w = Elem<T>::ld((const T*)a.i + b * a.isb + t * a.isl + d), s1 = leak_of<T>(-w);
-          dx = s1 * g;
-          df = q * l * hp[j];
-          di = dx * leak_of<T>(w) * x;
-        } else {
-          dx = l * g;
-          df = q * l * (hp[j] - x);
-        }
+    return r;
+  }
+};
+// first, then second
+__device__ __forceinline__ Map then(const Map& first, const Map& second) {
+  float a0, a1, b0, b1;
+  unpack2(first.a, a0, a1), unpack2(second.a, b0, b1);
+  return {pack2(__float_as_int(b0) == (int)0x80000000 ? b0 : a0 * b0, __float_as_int(b1) == (int)0x80000000 ? b1 : a1 * b1),
+          second.operator()<true>(first.h)};
+}
+
+// One operand's tiles: [kS][kC] values of a warp, kMode bytes to a copy (2: through registers, for rows of 16-bit values that lie
+// on odd ones).
+template <typename T, int kS, int kMode>
+struct Tile {
+  static constexpr int kBytes = kS * kC * (int)sizeof(T);
+  static constexpr int kRow = kC * (int)sizeof(T);
+  // rows t0 .. t0 + kS of p (at the tile's first channel), of which `rows` are inside, and `chans` channels
+  static __device__ __forceinline__ void fetch(char* dst, const T* p, long long stride, int t0, int rows, int chans, int lane) {
+    if (kMode == 2) {
+      unsigned short v[2 * kS];
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p + (long long)t0 * stride);
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        v[2 * s] = s < rows && lane < chans ? __ldg(q + s * stride + lane) : (unsigned short)0;
+        v[2 * s + 1] = s < rows && lane + 32 < chans ? __ldg(q + s * stride + lane + 32) : (unsigned short)0;
       }
-      if (a.reset && a.reset[(long long)b * a.L + t]) q = 0.f;
-      Elem<T>::st((T*)a.dx + b * a.dxb + t * a.dxl + d, dx);
-      Elem<T>::st((T*)a.df + b * a.dfb + t * a.dfl + d, df);
-      if (a.i) Elem<T>::st((T*)a.di + b * a.dib + t * a.dil + d, di);
+      unsigned short* d = reinterpret_cast<unsigned short*>(dst);
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        d[s * kC + lane] = v[2 * s];
+        d[s * kC + lane + 32] = v[2 * s + 1];
+      }
+      return;
+    }
+    constexpr int kPer = kRow / (kMode == 16 ? 16 : 4);                // copies to a row
+    constexpr int kRows = kPer >= 32 ? 1 : 32 / kPer;                 // rows to a round of the warp
+    constexpr int kOver = kPer >= 32 ? kPer / 32 : 1;                 // rounds to a row
+    const int row = kPer >= 32 ? 0 : lane / kPer, col = (kPer >= 32 ? lane : lane % kPer) * kMode;
+    const char* base = reinterpret_cast<const char*>(p);
+    const uint32_t to = smem_u32(dst) + row * kRow + col;
+    const char* from = base + ((long long)(t0 + row) * stride) * (int)sizeof(T) + col;
+    const long long next = stride * (kRows * (int)sizeof(T));
+#pragma unroll
+    for (int s = 0; s < kS; s += kRows) {
+#pragma unroll
+      for (int o = 0; o < kOver; ++o) {
+        const int left = min(max(chans * (int)sizeof(T) - col - o * 32 * kMode, 0), kMode);
+        const int n = s + row < rows ? left : 0;
+        copy_async<kMode == 16 ? 16 : 4>(to + s * kRow + o * 32 * kMode, n ? from + o * 32 * kMode : base, n);
+      }
+      from += next;
     }
   }
-  if (a.dh_in) a.dh_in[(long long)b * a.D + d] = q;
+};
+
+// the padding (bits 0 ..) and resets (bits 16 ..) of a segment, one byte to a lane; steps behind the end are padded
+__device__ __forceinline__ bool flag_of(const RecArgs& a, int b, int t0, int steps, int lane) {
+  const int s = lane & 15, t = t0 + s;
+  if (s >= steps) return false;
+  if (lane < 16) return t >= a.L || (a.pad && a.pad[b * a.msb + t * a.msl]);
+  return t < a.L && a.reset && a.reset[b * a.msb + t * a.msl];
 }
 
+// Exchange: every warp's map -> the state that enters each, and the carry behind the whole stride.  kDir > 0: in the order
+// of warps and ranks, else the other way.
+template <int kDir>
+__device__ __forceinline__ f32x2 exchange(const Map& own, f32x2& carry, float4 (*warp_maps)[32], float4 (*block_maps)[32], int w, int lane,
+                                          int rank, int size, bool reset) {
+  warp_maps[w][lane] = own.words();
+  __syncthreads();
+  f32x2 in = carry;
+  if (size > 1) {
+    if (w == 0) {
+      Map m = Map::of(warp_maps[kDir > 0 ? 0 : kW - 1][lane]);
+#pragma unroll
+      for (int k = 1; k < kW; ++k) m = then(m, Map::of(warp_maps[kDir > 0 ? k : kW - 1 - k][lane]));
+      const float4 v = m.words();
+      for (int r = 0; r < size; ++r) put_peer(&block_maps[rank][lane], r, v);
+    }
+    cluster_arrive();
+    cluster_wait();
+    for (int k = 0; k < size; ++k) {
+      const int r = kDir > 0 ? k : size - 1 - k;
+      if (r == rank) in = carry;
+      const Map m = Map::of(block_maps[r][lane]);
+      carry = reset ? m.operator()<true>(carry) : m.operator()<false>(carry);
+    }
+  }
+  f32x2 at = in;
+#pragma unroll
+  for (int k = 0; k < kW; ++k) {
+    const int v = kDir > 0 ? k : kW - 1 - k;
+    if (v == w) in = at;
+    const Map m = Map::of(warp_maps[v][lane]);
+    at = reset ? m.operator()<true>(at) : m.operator()<false>(at);
+  }
+  if (size == 1) carry = at;
+  return in;
+}
+
+// ---- forward ---------------------------------------------------------------------------------
+template <typename T, bool kGate, int kMode>
+__global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
+  constexpr int kS = kSteps<T, kGate>, kOps = kGate ? 3 : 2;
+  using Op = Tile<T, kS, kMode>;
+  constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float4 warp_maps[2][kW][32], block_maps[2][8][32];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
+  const int size = cluster_size(), rank = size > 1 ? cluster_rank() : 0;
+  const int c0 = (blockIdx.x / size) * kC, chans = min(a.D - c0, kC), n = min(max(chans - 2 * lane, 0), 2);
+  const long long state = (long long)b * a.D + c0 + 2 * lane;
+  const T *x = (const T*)a.x + b * a.xsb + c0, *f = (const T*)a.f + b * a.fsb + c0, *i = kGate ? (const T*)a.i + b * a.isb + c0 : nullptr;
+  T* y = (T*)a.y + b * a.ysb + c0 + 2 * lane;
+  char* ring = smem + w * (kStages * kOps * Op::kBytes);
+  const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
+  const bool masks = a.pad || a.reset, reset = a.reset != nullptr;
+
+  auto fetch = [&](int k) {
+    const int t0 = (k * size + rank) * (kW * kS) + w * kS, rows = min(max(a.L - t0, 0), kS);
+    char* at = ring + (k % kStages) * (kOps * Op::kBytes);
+    if (k < rounds) {
+      const int t = rows > 0 ? t0 : 0;
+      Op::fetch(at, x, a.xsl, t, rows, chans, lane);
+      Op::fetch(at + Op::kBytes, f, a.fsl, t, rows, chans, lane);
+      if (kGate) Op::fetch(at + 2 * Op::kBytes, i, a.isl, t, rows, chans, lane);
+    }
+    copies_commit();
+    return masks && k < rounds ? flag_of(a, b, t0, kS, lane) : (lane < kS && t0 + lane >= a.L);
+  };
+
+  if (size > 1) cluster_arrive();   // (every block has begun before another writes into its shared memory)
+  f32x2 carry = get_state(a.h_in ? a.h_in + state : nullptr, n, a.pairs);
+  bool flag = fetch(0);
+  for (int k = 0; k < rounds; ++k) {
+    const unsigned flags = __ballot_sync(0xffffffffu, flag);
+    __syncwarp();   // (the stage that is fetched into next has been read by every lane)
+    flag = fetch(k + 1);
+    copies_wait<kStages - 1>();
+    __syncwarp();
+    const T* op = reinterpret_cast<const T*>(ring + (k % kStages) * (kOps * Op::kBytes)) + 2 * lane;
+    Map loc[kS];
+    f32x2 h = pack2(0.f, 0.f), A = pack2(1.f, 1.f);
+    auto step = [&](int s) {
+      const f32x2 nl = minus_leak2<T>(two(op + kS * kC + s * kC)), xv = two(op + s * kC);
+      if (kGate) {
+        f32x2 none;
+        h = fma2(nl, h, fma2(gate2<T, false>(two(op + 2 * kS * kC + s * kC), none), xv, h));
+      } else {
+        h = fma2(nl, sub2(h, xv), h);
+      }
+      A = fma2(nl, A, A);
+    };
+    if (flags == 0) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        step(s);
+        loc[s] = {A, h};
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        if ((flags >> (16 + s)) & 1u) h = pack2(0.f, 0.f), A = minus_zero();
+        if (!((flags >> s) & 1u)) {
+          const f32x2 before = A;
+          step(s);
+          if (before == minus_zero()) A = minus_zero();
+        }
+        loc[s] = {A, h};
+      }
+    }
+    if (size > 1 && k == 0) cluster_wait();
+    const f32x2 in = exchange<1>(loc[kS - 1], carry, warp_maps[k & 1], block_maps[k & 1], w, lane, rank, size, reset);
+    const int t0 = (k * size + rank) * (kW * kS) + w * kS;
+    if (a.starts && t0 < a.L) put_state(a.starts + ((long long)b * segs + t0 / kS) * a.D + c0 + 2 * lane, in, n, a.pairs);
+    T* yt = y + t0 * a.ysl;
+    if (flags == 0) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) put<kPair>(yt + s * a.ysl, loc[s].operator()<false>(in), n);
+    } else {
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+        if (t0 + s < a.L) put<kPair>(yt + s * a.ysl, (flags >> s) & 1u ? pack2(0.f, 0.f) : loc[s].operator()<true>(in), n);
+    }
+  }
+  if (a.h_out && rank == 0 && w == 0) put_state(a.h_out + state, carry, n, a.pairs);
+}
+
+// ---- backward --------------------------------------------------------------------------------
+template <typename T, bool kGate, int kMode>
+__global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
+  constexpr int kS = kSteps<T, kGate>, kOps = kGate ? 4 : 3;
+  using Op = Tile<T, kS, kMode>;
+  constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float4 warp_maps[2][kW][32], block_maps[2][8][32];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
+  const int size = cluster_size(), rank = size > 1 ? cluster_rank() : 0;
+  const int c0 = (blockIdx.x / size) * kC, chans = min(a.D - c0, kC), n = min(max(chans - 2 * lane, 0), 2);
+  const long long state = (long long)b * a.D + c0 + 2 * lane;
+  const T *x = (const T*)a.x + b * a.xsb + c0, *f = (const T*)a.f + b * a.fsb + c0, *dy = (const T*)a.dy + b * a.gsb + c0;
+  const T* i = kGate ? (const T*)a.i + b * a.isb + c0 : nullptr;
+  T *dx = (T*)a.dx + b * a.dxb + c0 + 2 * lane, *df = (T*)a.df + b * a.dfb + c0 + 2 * lane;
+  T* di = kGate ? (T*)a.di + b * a.dib + c0 + 2 * lane : nullptr;
+  char* ring = smem + w * (kStages * kOps * Op::kBytes);
+  const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
+  const bool masks = a.pad || a.reset, reset = a.reset != nullptr;
+
+  f32x2 start = pack2(0.f, 0.f);
+  auto fetch = [&](int k) {   // (round k is the k-th from the end)
+    const int t0 = ((rounds - 1 - k) * size + rank) * (kW * kS) + w * kS, rows = min(max(a.L - t0, 0), kS);
+    char* at = ring + (k % kStages) * (kOps * Op::kBytes);
+    if (k < rounds) {
+      const int t = rows > 0 ? t0 : 0;
+      Op::fetch(at, x, a.xsl, t, rows, chans, lane);
+      Op::fetch(at + Op::kBytes, f, a.fsl, t, rows, chans, lane);
+      Op::fetch(at + 2 * Op::kBytes, dy, a.gsl, t, rows, chans, lane);
+      if (kGate) Op::fetch(at + 3 * Op::kBytes, i, a.isl, t, rows, chans, lane);
+      if (rows > 0) start = get_state(a.starts + ((long long)b * segs + t0 / kS) * a.D + c0 + 2 * lane, n, a.pairs);
+    }
+    copies_commit();
+    return masks && k < rounds ? flag_of(a, b, t0, kS, lane) : (lane < kS && t0 + lane >= a.L);
+  };
+
+  if (size > 1) cluster_arrive();
+  f32x2 carry = get_state(a.dh_out ? a.dh_out + state : nullptr, n, a.pairs);
+  bool flag = fetch(0);
+  for (int k = 0; k < rounds; ++k) {
+    const unsigned flags = __ballot_sync(0xffffffffu, flag);
+    f32x2 h = start;
+    __syncwarp();
+    flag = fetch(k + 1);
+    copies_wait<kStages - 1>();
+    __syncwarp();
+    const T* op = reinterpret_cast<const T*>(ring + (k % kStages) * (kOps * Op::kBytes)) + 2 * lane;
+    const T* gy = op + 2 * kS * kC;
+    f32x2 nl[kS], v[kS], gate[kGate ? kS : 1], slope[kGate ? kS : 1];   // v: h_{t-1} - x, with an input gate h_{t-1}
+    auto state_step = [&](int s) {
+      nl[s] = minus_leak2<T>(two(op + kS * kC + s * kC));
+      const f32x2 xv = two(op + s * kC);
+      if (kGate) {
+        v[s] = h;
+        gate[s] = gate2<T, true>(two(op + 3 * kS * kC + s * kC), slope[s]);
+        h = fma2(nl[s], h, fma2(gate[s], xv, h));
+      } else {
+        v[s] = sub2(h, xv);
+        h = fma2(nl[s], v[s], h);
+      }
+    };
+    Map m = {pack2(1.f, 1.f), pack2(0.f, 0.f)};
+    auto grad_step = [&](int s) {
+      const f32x2 g = add2(m.h, two(gy + s * kC));
+      m.h = fma2(nl[s], g, g);
+      m.a = fma2(nl[s], m.a, m.a);
+    };
+    if (flags == 0) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) state_step(s);
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) grad_step(s);
+    } else {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        if ((flags >> (16 + s)) & 1u) h = pack2(0.f, 0.f);
+        nl[s] = v[s] = pack2(0.f, 0.f);
+        if (kGate) gate[s] = slope[s] = pack2(0.f, 0.f);
+        if (!((flags >> s) & 1u)) state_step(s);
+      }
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) {
+        if (!((flags >> s) & 1u)) {
+          const f32x2 before = m.a;
+          grad_step(s);
+          if (before == minus_zero()) m.a = minus_zero();
+        }
+        if ((flags >> (16 + s)) & 1u) m = {minus_zero(), pack2(0.f, 0.f)};
+      }
+    }
+    if (size > 1 && k == 0) cluster_wait();
+    f32x2 q = exchange<-1>(m, carry, warp_maps[k & 1], block_maps[k & 1], w, lane, rank, size, reset);
+    const int t0 = ((rounds - 1 - k) * size + rank) * (kW * kS) + w * kS;
+    T *xt = dx + t0 * a.dxl, *ft = df + t0 * a.dfl, *it = kGate ? di + t0 * a.dil : nullptr;
+    auto out_step = [&](int s, bool pad) {
+      const f32x2 g = add2(q, two(gy + s * kC));
+      if (!pad) q = fma2(nl[s], g, g);
+      // (the leak and the slope, which may be subnormal, come last: a product of theirs would be rounded to few bits first)
+      f32x2 ox = kGate ? mul2(gate[s], g) : neg2(mul2(nl[s], g)), of = neg2(mul2(mul2(v[s], q), nl[s])), oi = pack2(0.f, 0.f);
+      if (kGate) oi = mul2(mul2(two(op + s * kC), g), slope[s]);
+      if (pad) ox = of = oi = pack2(0.f, 0.f);
+      put<kPair>(xt + s * a.dxl, ox, n);
+      put<kPair>(ft + s * a.dfl, of, n);
+      if (kGate) put<kPair>(it + s * a.dil, oi, n);
+    };
+    if (flags == 0) {
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) out_step(s, false);
+    } else {
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) {
+        if (t0 + s < a.L) out_step(s, (flags >> s) & 1u);
+        if ((flags >> (16 + s)) & 1u) q = pack2(0.f, 0.f);
+      }
+    }
+  }
+  if (a.dh_in && rank == 0 && w == 0) put_state(a.dh_in + state, carry, n, a.pairs);
+}
+
+// ---- single step -----------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(128) rec_step_kernel(RecArgs a) {
   const int b = blockIdx.y, d = blockIdx.x * 128 + threadIdx.x;
   if (d >= a.D) return;
   const long long at = (long long)b * a.D + d;
   const float h = a.h_in ? a.h_in[at] : 0.f, x = Elem<T>::ld((const T*)a.x + b * a.xsb + d);
-  const float l = leak_of<T>(Elem<T>::ld((const T*)a.f + b * a.fsb + d));
-  const float v = a.i ? fmaf(-l, h, fmaf(leak_of<T>(-Elem<T>::ld((const T*)a.i + b * a.isb + d)), x, h)) : fmaf(l, x - h, h);
+  const float nl = minus_leak<T>(Elem<T>::ld((const T*)a.f + b * a.fsb + d));
+  float none;
+  const float v = a.i ? fmaf(nl, h, fmaf(gate_one<T, false>(Elem<T>::ld((const T*)a.i + b * a.isb + d), none), x, h)) : fmaf(nl, h - x, h);
   Elem<T>::st((T*)a.y + b * a.ysb + d, v);
   a.h_out[at] = v;
 }
 
+// ---- host ------------------------------------------------------------------------------------
 int check_rec(int dtype, int B, int L, int D, std::initializer_list<const void*> acts, std::initializer_list<const void*> f32) {
   if (!valid_dtype(dtype)) return MEGA_ERR_DTYPE;
   if (B <= 0 || L <= 0 || D <= 0) return MEGA_ERR_SHAPE;
-  if (B > 65535) return MEGA_ERR_UNSUPPORTED;
+  if (B > 65535 || L > INT_MAX - 8192) return MEGA_ERR_UNSUPPORTED;   // (steps are counted past the end by up to two strides)
   for (const void* p : acts)
     if (!aligned_to(p, elem_size(dtype))) return MEGA_ERR_ALIGN;
   for (const void* p : f32)
@@ -121,12 +533,81 @@ int check_rec(int dtype, int B, int L, int D, std::initializer_list<const void*>
   return MEGA_OK;
 }
 
+struct Operand {
+  const void* p;
+  long long sb, sl;
+  bool on(int bytes, int es) const { return !p || (aligned_to(p, bytes) && sb * es % bytes == 0 && sl * es % bytes == 0); }
+};
+// bytes of a copy: 16 or 4 where every row of the inputs starts on them (and pairs of outputs on theirs), else 2
+int mode_of(int es, std::initializer_list<Operand> in, std::initializer_list<Operand> out) {
+  auto all = [&](std::initializer_list<Operand> ops, int bytes) { return std::all_of(ops.begin(), ops.end(), [&](const Operand& o) { return o.on(bytes, es); }); };
+  if (all(in, 16) && all(out, 2 * es)) return 16;
+  return es == 4 || (all(in, 4) && all(out, 4)) ? 4 : 2;
+}
+
+// Blocks to a cluster.
+int cluster_of(int tiles, int B, int L, int steps) {
+  const int forced = g_options[OPT_REC_CLUSTER].load(std::memory_order_relaxed);
+  if (forced == 1 || forced == 2 || forced == 4 || forced == 8) return forced;
+  int c = 1;
+  while (c < 8 && (long long)tiles * B * c < 240 && c * kW * steps < L) c *= 2;
+  return c;
+}
+
+template <typename Kernel>
+void launch_rec(Kernel kernel, int tiles, int B, int cluster, size_t smem, cudaStream_t s, const RecArgs& a) {
+  allow_smem(reinterpret_cast<const void*>(kernel), smem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles * cluster, B);
+  cfg.blockDim = dim3(kW * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, a);
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  g_last_kernel.store("gated_recurrence", std::memory_order_relaxed);
+}
+
+template <typename T, bool kGate, int kMode>
+void run_mode(bool bwd, int B, const RecArgs& a, cudaStream_t s) {
+  constexpr int kS = kSteps<T, kGate>;
+  const int tiles = (a.D + kC - 1) / kC, cluster = cluster_of(tiles, B, a.L, kS);
+  const size_t smem = size_t(kW) * kStages * ((kGate ? 3 : 2) + (bwd ? 1 : 0)) * Tile<T, kS, kMode>::kBytes;
+  launch_rec(bwd ? rec_bwd_kernel<T, kGate, kMode> : rec_fwd_kernel<T, kGate, kMode>, tiles, B, cluster, smem, s, a);
+}
+template <typename T>
+void run_rec(bool bwd, int mode, int B, const RecArgs& a, cudaStream_t s) {
+  auto go = [&](auto gate) {
+    constexpr bool kGate = decltype(gate)::value;
+    if (mode == 16) return run_mode<T, kGate, 16>(bwd, B, a, s);
+    if constexpr (sizeof(T) == 2) {
+      if (mode == 2) return run_mode<T, kGate, 2>(bwd, B, a, s);
+    }
+    run_mode<T, kGate, 4>(bwd, B, a, s);
+  };
+  a.i ? go(std::true_type{}) : go(std::false_type{});
+}
+
+// operands at the walk's first step, strides in its direction
+template <typename P>
+void turn(P& p, long long& stride, int L, int es) {
+  if (p) p = (P)((const char*)p + (long long)(L - 1) * stride * es);
+  stride = -stride;
+}
+
 }  // namespace
 }  // namespace mega
 
 using namespace mega;
 
-extern "C" int mega_gated_recurrence_segment(int dtype, int gated) { return valid_dtype(dtype) ? kSeg : 0; }
+extern "C" int mega_gated_recurrence_segment(int dtype, int gated) {
+  return !valid_dtype(dtype) ? 0 : dtype == MEGA_F32 ? kSteps<float, false> : gated ? kSteps<__half, true> : kSteps<__half, false>;
+}
 
 extern "C" int mega_gated_recurrence_fwd(const void* x, const void* f, const void* i, void* y, int dtype, int B, int L, int D,
                                          int64_t xsb, int64_t xsl, int64_t fsb, int64_t fsl, int64_t isb, int64_t isl, int64_t ysb,
@@ -138,8 +619,16 @@ extern "C" int mega_gated_recurrence_fwd(const void* x, const void* f, const voi
   a.x = x, a.f = f, a.i = i, a.y = y;
   a.xsb = xsb, a.xsl = xsl, a.fsb = fsb, a.fsl = fsl, a.isb = isb, a.isl = isl, a.ysb = ysb, a.ysl = ysl;
   a.pad = pad_mask, a.reset = reset_mask, a.h_in = h_in, a.h_out = h_out, a.starts = starts;
-  a.B = B, a.L = L, a.D = D, a.reverse = (flags & MEGA_REC_REVERSE) != 0;
-  MEGA_DISPATCH_DTYPE(dtype, launch(rec_fwd_kernel<T>, dim3((D + 127) / 128, B), dim3(128), 0, stream, a));
+  a.msb = L, a.msl = 1, a.L = L, a.D = D;
+  a.pairs = D % 2 == 0 && aligned_to(h_in, 8) && aligned_to(h_out, 8) && aligned_to(starts, 8);
+  const int es = elem_size(dtype), mode = mode_of(es, {{x, xsb, xsl}, {f, fsb, fsl}, {i, isb, isl}}, {{y, ysb, ysl}});
+  if (flags & MEGA_REC_REVERSE) {
+    turn(a.x, a.xsl, L, es), turn(a.f, a.fsl, L, es), turn(a.i, a.isl, L, es), turn(a.y, a.ysl, L, es);
+    if (a.pad) a.pad += L - 1;
+    if (a.reset) a.reset += L - 1;
+    a.msl = -1;
+  }
+  MEGA_DISPATCH_DTYPE(dtype, run_rec<T>(false, mode, B, a, (cudaStream_t)stream));
   return check_launch("gated_recurrence_fwd");
 }
 
@@ -156,8 +645,18 @@ extern "C" int mega_gated_recurrence_bwd(const void* dy, const void* x, const vo
   a.gsb = gsb, a.gsl = gsl, a.xsb = xsb, a.xsl = xsl, a.fsb = fsb, a.fsl = fsl, a.isb = isb, a.isl = isl;
   a.dxb = dxb, a.dxl = dxl, a.dfb = dfb, a.dfl = dfl, a.dib = dib, a.dil = dil;
   a.pad = pad_mask, a.reset = reset_mask, a.starts = const_cast<float*>(starts), a.dh_out = dh_out, a.dh_in = dh_in;
-  a.B = B, a.L = L, a.D = D, a.reverse = (flags & MEGA_REC_REVERSE) != 0;
-  MEGA_DISPATCH_DTYPE(dtype, launch(rec_bwd_kernel<T>, dim3((D + 127) / 128, B), dim3(128), 0, stream, a));
+  a.msb = L, a.msl = 1, a.L = L, a.D = D;
+  a.pairs = D % 2 == 0 && aligned_to(dh_in, 8) && aligned_to(dh_out, 8) && aligned_to(starts, 8);
+  const int es = elem_size(dtype);
+  const int mode = mode_of(es, {{dy, gsb, gsl}, {x, xsb, xsl}, {f, fsb, fsl}, {i, isb, isl}}, {{dx, dxb, dxl}, {df, dfb, dfl}, {i ? di : nullptr, dib, dil}});
+  if (flags & MEGA_REC_REVERSE) {
+    turn(a.dy, a.gsl, L, es), turn(a.x, a.xsl, L, es), turn(a.f, a.fsl, L, es), turn(a.i, a.isl, L, es);
+    turn(a.dx, a.dxl, L, es), turn(a.df, a.dfl, L, es), turn(a.di, a.dil, L, es);
+    if (a.pad) a.pad += L - 1;
+    if (a.reset) a.reset += L - 1;
+    a.msl = -1;
+  }
+  MEGA_DISPATCH_DTYPE(dtype, run_rec<T>(true, mode, B, a, (cudaStream_t)stream));
   return check_launch("gated_recurrence_bwd");
 }
 
@@ -168,7 +667,7 @@ extern "C" int mega_gated_recurrence_step(const void* x, const void* f, const vo
   if (int rc = check_rec(dtype, B, 1, D, {x, f, i, y}, {h_in, h_out})) return rc;
   RecArgs a = {};
   a.x = x, a.f = f, a.i = i, a.y = y, a.xsb = xsb, a.fsb = fsb, a.isb = isb, a.ysb = ysb;
-  a.h_in = h_in, a.h_out = h_out, a.B = B, a.L = 1, a.D = D;
+  a.h_in = h_in, a.h_out = h_out, a.L = 1, a.D = D;
   MEGA_DISPATCH_DTYPE(dtype, launch(rec_step_kernel<T>, dim3((D + 127) / 128, B), dim3(128), 0, stream, a));
   return check_launch("gated_recurrence_step");
 }
