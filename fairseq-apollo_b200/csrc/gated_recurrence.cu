@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "gated_recurrence.cuh"
 #include "tma.cuh"
 
 namespace mega {
@@ -64,10 +65,34 @@ __device__ __forceinline__ unsigned cluster_size() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void put_peer(float4* p, int rank, float4 v) {   // to the same place in another block's shared memory
-  uint32_t at;
+// 16 bytes to the same place in another block's shared memory, counted by the barrier at that block's `bar`
+__device__ __forceinline__ void send(float4* p, uint64_t* bar, int rank, float4 v) {
+  uint32_t at, to;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "f"(v.x),
+               "f"(v.y), "f"(v.z), "f"(v.w), "r"(to)
+               : "memory");
+}
+// What the cluster's blocks sent for this phase has arrived.  Bounded: false, with the error word raised, after about 2 s.
+__device__ __forceinline__ bool received(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  const long long start = clock64();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (clock64() - start > 4000000000LL) {
+      g_device_error = 1;
+      return false;
+    }
+  }
 }
 template <int kBytes>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int valid) {   // the rest of kBytes is zeroed
@@ -97,7 +122,7 @@ __device__ __forceinline__ f32x2 minus_leak2(f32x2 f) {
   unpack2(mul2(f, pack2(1.4426950408889634f, 1.4426950408889634f)), a, b);   // e^f = 2^(f / ln 2)
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-  unpack2(add2(mul2(pack2(a, b), pack2(-1.f, -1.f)), pack2(-1.f, -1.f)), a, b);
+  unpack2(fma2(pack2(a, b), pack2(-1.f, -1.f), pack2(-1.f, -1.f)), a, b);
   return pack2(rcp_approx(a), rcp_approx(b));
 }
 // sigmoid(i), and sigmoid(i) sigmoid(-i) where the caller asks for it
@@ -203,11 +228,15 @@ struct Map {
   }
 };
 // first, then second
+template <bool kReset>
 __device__ __forceinline__ Map then(const Map& first, const Map& second) {
-  float a0, a1, b0, b1;
-  unpack2(first.a, a0, a1), unpack2(second.a, b0, b1);
-  return {pack2(__float_as_int(b0) == (int)0x80000000 ? b0 : a0 * b0, __float_as_int(b1) == (int)0x80000000 ? b1 : a1 * b1),
-          second.operator()<true>(first.h)};
+  Map r = {mul2(first.a, second.a), second.operator()<kReset>(first.h)};
+  if (kReset) {
+    float b0, b1, r0, r1;
+    unpack2(second.a, b0, b1), unpack2(r.a, r0, r1);
+    r.a = pack2(__float_as_int(b0) == (int)0x80000000 ? b0 : r0, __float_as_int(b1) == (int)0x80000000 ? b1 : r1);
+  }
+  return r;
 }
 
 // One operand's tiles: [kS][kC] values of a warp, kMode bytes to a copy (2: through registers, for rows of 16-bit values that lie
@@ -242,6 +271,15 @@ struct Tile {
     const uint32_t to = smem_u32(dst) + row * kRow + col;
     const char* from = base + ((long long)(t0 + row) * stride) * (int)sizeof(T) + col;
     const long long next = stride * (kRows * (int)sizeof(T));
+    if (rows == kS && chans == kC) {
+#pragma unroll
+      for (int s = 0; s < kS; s += kRows) {
+#pragma unroll
+        for (int o = 0; o < kOver; ++o) copy_async<kMode == 16 ? 16 : 4>(to + s * kRow + o * 32 * kMode, from + o * 32 * kMode, kMode);
+        from += next;
+      }
+      return;
+    }
 #pragma unroll
     for (int s = 0; s < kS; s += kRows) {
 #pragma unroll
@@ -263,41 +301,61 @@ __device__ __forceinline__ bool flag_of(const RecArgs& a, int b, int t0, int ste
   return t < a.L && a.reset && a.reset[b * a.msb + t * a.msl];
 }
 
-// Exchange: every warp's map -> the state that enters each, and the carry behind the whole stride.  kDir > 0: in the order
-// of warps and ranks, else the other way.
-template <int kDir>
-__device__ __forceinline__ f32x2 exchange(const Map& own, f32x2& carry, float4 (*warp_maps)[32], float4 (*block_maps)[32], int w, int lane,
-                                          int rank, int size, bool reset) {
-  warp_maps[w][lane] = own.words();
+// What the warps of a block, and the blocks of a cluster, tell one another.  Two of each: a place is written again only after every
+// reader has taken part in the round between.
+struct Post {
+  float4 warps[2][kW][32], blocks[2][8][32];
+  f32x2 carry[2][32];
+  uint64_t bar[2];
+};
+
+// Every warp's map -> the state that enters each; `carry` is the state that enters the whole stride, then the next one (in a block
+// by itself: in the last warp alone, the others find it here in the next round).  kDir > 0: in the order of warps and ranks, else
+// the other way.  A warp reads the maps before its own only: all eight in every warp are a third of the shared memory traffic, and
+// their loads, issued together, crowd out the registers.  Returns false once a wait has given up: the rounds go on, without
+// waiting.
+template <int kDir, bool kReset>
+__device__ __forceinline__ bool exchange(const Map& own, f32x2& carry, f32x2& in, Post& post, int round, int w, int lane, int rank, int size,
+                                         bool alive) {
+  const int at = round & 1, place = kDir > 0 ? w : kW - 1 - w;
+  post.warps[at][w][lane] = own.words();
   __syncthreads();
-  f32x2 in = carry;
-  if (size > 1) {
-    if (w == 0) {
-      Map m = Map::of(warp_maps[kDir > 0 ? 0 : kW - 1][lane]);
+  if (size == 1) {
+    if (round > 0 && place < kW - 1) carry = post.carry[at][lane];
+    in = carry;
 #pragma unroll
-      for (int k = 1; k < kW; ++k) m = then(m, Map::of(warp_maps[kDir > 0 ? k : kW - 1 - k][lane]));
-      const float4 v = m.words();
-      for (int r = 0; r < size; ++r) put_peer(&block_maps[rank][lane], r, v);
+    for (int k = 0; k < kW - 1; ++k) {
+      if (k >= place) break;
+      in = Map::of(post.warps[at][kDir > 0 ? k : kW - 1 - k][lane]).template operator()<kReset>(in);
     }
-    cluster_arrive();
-    cluster_wait();
-    for (int k = 0; k < size; ++k) {
-      const int r = kDir > 0 ? k : size - 1 - k;
-      if (r == rank) in = carry;
-      const Map m = Map::of(block_maps[r][lane]);
-      carry = reset ? m.operator()<true>(carry) : m.operator()<false>(carry);
+    if (place == kW - 1) {
+      carry = own.operator()<kReset>(in);
+      post.carry[at ^ 1][lane] = carry;
     }
+    return true;
   }
-  f32x2 at = in;
+  Map pre = {pack2(1.f, 1.f), pack2(0.f, 0.f)};
 #pragma unroll
-  for (int k = 0; k < kW; ++k) {
-    const int v = kDir > 0 ? k : kW - 1 - k;
-    if (v == w) in = at;
-    const Map m = Map::of(warp_maps[v][lane]);
-    at = reset ? m.operator()<true>(at) : m.operator()<false>(at);
+  for (int k = 0; k < kW - 1; ++k) {
+    if (k >= place) break;
+    const Map m = Map::of(post.warps[at][kDir > 0 ? k : kW - 1 - k][lane]);
+    pre = k == 0 ? m : then<kReset>(pre, m);
   }
-  if (size == 1) carry = at;
-  return in;
+  if (round == 0) cluster_wait();
+  if (place == kW - 1) {
+    if (lane == 0) mbar_expect_tx(&post.bar[at], size * 512);
+    const float4 v = then<kReset>(pre, own).words();
+    for (int r = 0; r < size; ++r) send(&post.blocks[at][rank][lane], &post.bar[at], r, v);
+  }
+  if (alive) alive = received(&post.bar[at], (round >> 1) & 1);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int r = kDir > 0 ? k : 7 - k;   // (ranks from the cluster's size on are passed over)
+    if (r == rank) in = carry;
+    if (r < size) carry = Map::of(post.blocks[at][r][lane]).template operator()<kReset>(carry);
+  }
+  in = pre.operator()<kReset>(in);
+  return alive;
 }
 
 // ---- forward ---------------------------------------------------------------------------------
@@ -307,7 +365,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
   using Op = Tile<T, kS, kMode>;
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
   extern __shared__ __align__(16) char smem[];
-  __shared__ float4 warp_maps[2][kW][32], block_maps[2][8][32];
+  __shared__ Post post;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
   const int size = cluster_size(), rank = size > 1 ? cluster_rank() : 0;
   const int c0 = (blockIdx.x / size) * kC, chans = min(a.D - c0, kC), n = min(max(chans - 2 * lane, 0), 2);
@@ -316,7 +374,8 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
   T* y = (T*)a.y + b * a.ysb + c0 + 2 * lane;
   char* ring = smem + w * (kStages * kOps * Op::kBytes);
   const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
-  const bool masks = a.pad || a.reset, reset = a.reset != nullptr;
+  const bool masks = a.pad || a.reset, reset = a.reset != nullptr, whole = kPair && chans == kC;
+  bool alive = true;
 
   auto fetch = [&](int k) {
     const int t0 = (k * size + rank) * (kW * kS) + w * kS, rows = min(max(a.L - t0, 0), kS);
@@ -331,7 +390,14 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
     return masks && k < rounds ? flag_of(a, b, t0, kS, lane) : (lane < kS && t0 + lane >= a.L);
   };
 
-  if (size > 1) cluster_arrive();   // (every block has begun before another writes into its shared memory)
+  if (size > 1) {
+    if (threadIdx.x == 0) {
+      mbar_init(&post.bar[0], 1);
+      mbar_init(&post.bar[1], 1);
+      mbar_fence_init();
+    }
+    cluster_arrive();   // (every block has begun, and its barriers are there, before another writes to it)
+  }
   f32x2 carry = get_state(a.h_in ? a.h_in + state : nullptr, n, a.pairs);
   bool flag = fetch(0);
   for (int k = 0; k < rounds; ++k) {
@@ -371,21 +437,29 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
         loc[s] = {A, h};
       }
     }
-    if (size > 1 && k == 0) cluster_wait();
-    const f32x2 in = exchange<1>(loc[kS - 1], carry, warp_maps[k & 1], block_maps[k & 1], w, lane, rank, size, reset);
+    f32x2 in;
+    alive = reset ? exchange<1, true>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive)
+                  : exchange<1, false>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive);
     const int t0 = (k * size + rank) * (kW * kS) + w * kS;
     if (a.starts && t0 < a.L) put_state(a.starts + ((long long)b * segs + t0 / kS) * a.D + c0 + 2 * lane, in, n, a.pairs);
     T* yt = y + t0 * a.ysl;
-    if (flags == 0) {
+    if (flags == 0 && whole) {
 #pragma unroll
-      for (int s = 0; s < kS; ++s) put<kPair>(yt + s * a.ysl, loc[s].operator()<false>(in), n);
+      for (int s = 0; s < kS; ++s) {
+        put<kPair>(yt, loc[s].operator()<false>(in), 2);
+        yt += a.ysl;
+      }
     } else {
 #pragma unroll
       for (int s = 0; s < kS; ++s)
         if (t0 + s < a.L) put<kPair>(yt + s * a.ysl, (flags >> s) & 1u ? pack2(0.f, 0.f) : loc[s].operator()<true>(in), n);
     }
   }
-  if (a.h_out && rank == 0 && w == 0) put_state(a.h_out + state, carry, n, a.pairs);
+  if (size > 1) {   // (no block's shared memory goes before all are through)
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (a.h_out && rank == 0 && w == kW - 1) put_state(a.h_out + state, carry, n, a.pairs);
 }
 
 // ---- backward --------------------------------------------------------------------------------
@@ -395,7 +469,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
   using Op = Tile<T, kS, kMode>;
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
   extern __shared__ __align__(16) char smem[];
-  __shared__ float4 warp_maps[2][kW][32], block_maps[2][8][32];
+  __shared__ Post post;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
   const int size = cluster_size(), rank = size > 1 ? cluster_rank() : 0;
   const int c0 = (blockIdx.x / size) * kC, chans = min(a.D - c0, kC), n = min(max(chans - 2 * lane, 0), 2);
@@ -406,7 +480,8 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
   T* di = kGate ? (T*)a.di + b * a.dib + c0 + 2 * lane : nullptr;
   char* ring = smem + w * (kStages * kOps * Op::kBytes);
   const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
-  const bool masks = a.pad || a.reset, reset = a.reset != nullptr;
+  const bool masks = a.pad || a.reset, reset = a.reset != nullptr, whole = kPair && chans == kC;
+  bool alive = true;
 
   f32x2 start = pack2(0.f, 0.f);
   auto fetch = [&](int k) {   // (round k is the k-th from the end)
@@ -424,7 +499,14 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
     return masks && k < rounds ? flag_of(a, b, t0, kS, lane) : (lane < kS && t0 + lane >= a.L);
   };
 
-  if (size > 1) cluster_arrive();
+  if (size > 1) {
+    if (threadIdx.x == 0) {
+      mbar_init(&post.bar[0], 1);
+      mbar_init(&post.bar[1], 1);
+      mbar_fence_init();
+    }
+    cluster_arrive();
+  }
   f32x2 carry = get_state(a.dh_out ? a.dh_out + state : nullptr, n, a.pairs);
   bool flag = fetch(0);
   for (int k = 0; k < rounds; ++k) {
@@ -478,31 +560,36 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
         if ((flags >> (16 + s)) & 1u) m = {minus_zero(), pack2(0.f, 0.f)};
       }
     }
-    if (size > 1 && k == 0) cluster_wait();
-    f32x2 q = exchange<-1>(m, carry, warp_maps[k & 1], block_maps[k & 1], w, lane, rank, size, reset);
+    f32x2 q;
+    alive = reset ? exchange<-1, true>(m, carry, q, post, k, w, lane, rank, size, alive)
+                  : exchange<-1, false>(m, carry, q, post, k, w, lane, rank, size, alive);
     const int t0 = ((rounds - 1 - k) * size + rank) * (kW * kS) + w * kS;
     T *xt = dx + t0 * a.dxl, *ft = df + t0 * a.dfl, *it = kGate ? di + t0 * a.dil : nullptr;
-    auto out_step = [&](int s, bool pad) {
+    auto out_step = [&](int s, bool pad, int count) {
       const f32x2 g = add2(q, two(gy + s * kC));
       if (!pad) q = fma2(nl[s], g, g);
       // (the leak and the slope, which may be subnormal, come last: a product of theirs would be rounded to few bits first)
       f32x2 ox = kGate ? mul2(gate[s], g) : neg2(mul2(nl[s], g)), of = neg2(mul2(mul2(v[s], q), nl[s])), oi = pack2(0.f, 0.f);
       if (kGate) oi = mul2(mul2(two(op + s * kC), g), slope[s]);
       if (pad) ox = of = oi = pack2(0.f, 0.f);
-      put<kPair>(xt + s * a.dxl, ox, n);
-      put<kPair>(ft + s * a.dfl, of, n);
-      if (kGate) put<kPair>(it + s * a.dil, oi, n);
+      put<kPair>(xt + s * a.dxl, ox, count);
+      put<kPair>(ft + s * a.dfl, of, count);
+      if (kGate) put<kPair>(it + s * a.dil, oi, count);
     };
-    if (flags == 0) {
+    if (flags == 0 && whole) {
 #pragma unroll
-      for (int s = kS - 1; s >= 0; --s) out_step(s, false);
+      for (int s = kS - 1; s >= 0; --s) out_step(s, false, 2);
     } else {
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) {
-        if (t0 + s < a.L) out_step(s, (flags >> s) & 1u);
+        if (t0 + s < a.L) out_step(s, (flags >> s) & 1u, n);
         if ((flags >> (16 + s)) & 1u) q = pack2(0.f, 0.f);
       }
     }
+  }
+  if (size > 1) {
+    cluster_arrive();
+    cluster_wait();
   }
   if (a.dh_in && rank == 0 && w == 0) put_state(a.dh_in + state, carry, n, a.pairs);
 }
@@ -601,6 +688,9 @@ void turn(P& p, long long& stride, int L, int es) {
 }
 
 }  // namespace
+
+cudaError_t gated_recurrence_read_device_error(int* v, bool reset) { return read_device_error(v, reset); }
+
 }  // namespace mega
 
 using namespace mega;

@@ -9,6 +9,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "gated_recurrence.cuh"
 #include "tma.cuh"
 #include "stream_cl.cuh"
 #include "stream_bwd.cuh"
@@ -432,6 +433,8 @@ extern "C" MEGA_API int mega_debug_device_error(int* host_value, int reset) {
   if (mega::mma_cl_read_device_error(&v2, reset != 0) != cudaSuccess) return mega::check_launch("device_error");
   int v3 = 0;
   if (mega::stream_bwd_read_device_error(&v3, reset != 0) != cudaSuccess) return mega::check_launch("device_error");
+  v2 |= v3;
+  if (mega::gated_recurrence_read_device_error(&v3, reset != 0) != cudaSuccess) return mega::check_launch("device_error");
   v2 |= v3;
   *host_value = v | v2;
   return MEGA_OK;
