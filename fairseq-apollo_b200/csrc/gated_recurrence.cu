@@ -347,14 +347,18 @@ __device__ __forceinline__ bool exchange(const Map& own, f32x2& carry, f32x2& in
     const float4 v = then<kReset>(pre, own).words();
     for (int r = 0; r < size; ++r) send(&post.blocks[at][rank][lane], &post.bar[at], r, v);
   }
-  if (alive) alive = received(&post.bar[at], (round >> 1) & 1);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int r = kDir > 0 ? k : 7 - k;   // (ranks from the cluster's size on are passed over)
-    if (r == rank) in = carry;
-    if (r < size) carry = Map::of(post.blocks[at][r][lane]).template operator()<kReset>(carry);
+  if (place == kW - 1) {
+    if (alive) alive = received(&post.bar[at], (round >> 1) & 1);
+#pragma unroll 1
+    for (int k = 0; k < size; ++k) {
+      const int r = kDir > 0 ? k : size - 1 - k;
+      if (r == rank) in = carry;
+      carry = Map::of(post.blocks[at][r][lane]).template operator()<kReset>(carry);
+    }
+    post.carry[at][lane] = in;
   }
-  in = pre.operator()<kReset>(in);
+  __syncthreads();
+  in = pre.operator()<kReset>(post.carry[at][lane]);
   return alive;
 }
 
