@@ -662,7 +662,7 @@ MEGA_API int mega_gated_recurrence_step(const void* x, const void* f, const void
  * mega_group_norm_bwd: dx like x (0 at padded steps), dgamma, dbeta (D) fp32, summed over sequences and steps in a fixed
  * order.  `work`: device memory of mega_group_norm_work() bytes, 16-byte aligned, used by this call alone until it is done;
  * forward and backward take the same size.
- * At most 65535 sequences and groups (MEGA_ERR_UNSUPPORTED).
+ * At most 65535 sequences and groups, and 2^24 steps (MEGA_ERR_UNSUPPORTED).
  */
 #define MEGA_GN_SILU 1u
 #define MEGA_GN_OFFSET 2u

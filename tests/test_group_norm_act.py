@@ -278,8 +278,9 @@ def test_axes_memory_orders_and_alignment():
 
             for shape in (sliced, lambda t: t.transpose(0, 1).contiguous().transpose(0, 1),
                           lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)):
+                # (not bit for bit: rows that start elsewhere take other vectors, and so another order of the sums)
                 got = run_all(M, x, dy, w, c, mask, G, "silu", shape)
-                assert all(torch.equal(plain[k], got[k]) for k in plain)
+                check_all(got, x, dy, w, c, mask, G, "silu")
             norm = M.GroupNorm(D, G, activation="silu").cuda()   # maps of 5 x 12 positions
             with torch.no_grad():
                 norm.weight.copy_(w)
