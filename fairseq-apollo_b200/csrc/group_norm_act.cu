@@ -17,6 +17,7 @@
 // counts, means and squared deviations: the mean of all first, then the deviations about it.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tma.cuh"
@@ -27,7 +28,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRun = 64;        // steps of a thread at most
-constexpr int kBatch = 4;       // rows that a thread loads at once
 constexpr int kGroups = 256;    // groups of a tile at most (a vector or more each, or the 128 bytes of a narrow tile)
 
 struct GnArgs {
@@ -49,56 +49,83 @@ struct GnArgs {
   int params;                  // blocks behind the others that add up dgamma, dbeta
 };
 
-// kV channels in a register or four
+// kV neighbouring channels: as pairs of fp32 values (packed arithmetic; with one channel the second of the pair is idle)
 template <typename T, int kV>
 struct Vec {
-  static constexpr int kBytes = kV * (int)sizeof(T);
-  static constexpr int kWords = kBytes >= 4 ? kBytes / 4 : 1;
-  unsigned w[kWords];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kBytes == 16) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (kBytes == 4) {
-      w[0] = __ldg(reinterpret_cast<const unsigned*>(p));
-    } else {
-      w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
-    }
-  }
-  __device__ __forceinline__ void get(float (&f)[kV]) const {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int j = 0; j < kV; ++j) f[j] = __uint_as_float(w[j]);
-    } else {
-      const T* e = reinterpret_cast<const T*>(w);
-#pragma unroll
-      for (int j = 0; j < kV; ++j) f[j] = Elem<T>::ld_shared(e + j);
-    }
-  }
-  __device__ __forceinline__ void set(const float (&f)[kV]) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int j = 0; j < kV; ++j) w[j] = __float_as_uint(f[j]);
-    } else {
-      T* e = reinterpret_cast<T*>(w);
-#pragma unroll
-      for (int j = 0; j < kV; ++j) Elem<T>::st(e + j, f[j]);
-    }
-  }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (kBytes == 16)
-      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else if constexpr (kBytes == 4)
-      *reinterpret_cast<unsigned*>(p) = w[0];
+  static constexpr int kBytes = kV * (int)sizeof(T), kP = (kV + 1) / 2;
+  static __device__ __forceinline__ void fetch(uint32_t slot, const T* p) {   // to shared memory, asynchronously
+    static_assert(kBytes == 16 || kBytes == 4, "");
+    if (kBytes == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot), "l"(p) : "memory");
     else
-      *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(slot), "l"(p) : "memory");
+  }
+  static __device__ __forceinline__ void read(const char* slot, f32x2 (&f)[kP]) {
+    if constexpr (kBytes == 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(slot);
+      const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < kP; ++j) f[j] = sizeof(T) == 4 ? pack2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1])) : two(w[j]);
+    } else {
+      const unsigned w = *reinterpret_cast<const unsigned*>(slot);
+      f[0] = sizeof(T) == 4 ? pack2(__uint_as_float(w), 0.f) : two(w);
+    }
+  }
+  static __device__ __forceinline__ f32x2 two(unsigned w) {   // a pair of 16-bit values
+    if constexpr (sizeof(T) == 2) {
+      const T* e = reinterpret_cast<const T*>(&w);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+      return pack2(Elem<T>::ld_shared(e), Elem<T>::ld_shared(e + 1));
+    }
+    return 0;
+  }
+  static __device__ __forceinline__ unsigned one(f32x2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+      return *reinterpret_cast<const unsigned*>(&r);
+    }
+    const __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&r);
+  }
+  static __device__ __forceinline__ void store(T* p, const f32x2 (&f)[kP]) {
+    if constexpr (kV == 1) {
+      float a, b;
+      unpack2(f[0], a, b);
+      Elem<T>::st(p, a);
+    } else if constexpr (sizeof(T) == 4) {
+      float4 v;
+      unpack2(f[0], v.x, v.y);
+      unpack2(f[kP - 1], v.z, v.w);
+      *reinterpret_cast<float4*>(p) = v;
+    } else if constexpr (kBytes == 16) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(one(f[0]), one(f[kP > 1 ? 1 : 0]), one(f[kP > 2 ? 2 : 0]), one(f[kP - 1]));
+    } else {
+      *reinterpret_cast<unsigned*>(p) = one(f[0]);
+    }
   }
 };
+__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
 
 // sigmoid(z): fp32 with the full-range exponential and division, 16-bit types with the approximate ones (relative 2^-22 or so)
 template <typename T>
 __device__ __forceinline__ float sig(float z) {
   return sizeof(T) == 4 ? 1.f / (1.f + expf(-z)) : rcp_approx(1.f + __expf(-z));
+}
+// minus the sigmoids of a pair
+template <typename T>
+__device__ __forceinline__ f32x2 minus_sig2(f32x2 z) {
+  float a, b;
+  if (sizeof(T) == 4) {
+    unpack2(z, a, b);
+    return pack2(-1.f / (1.f + expf(-a)), -1.f / (1.f + expf(-b)));
+  }
+  unpack2(mul2(z, both(-1.4426950408889634f)), a, b);   // e^-z = 2^(-z / ln 2)
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+  unpack2(fma2(pack2(a, b), both(-1.f), both(-1.f)), a, b);
+  return pack2(rcp_approx(a), rcp_approx(b));
 }
 
 // What a block works on.
@@ -120,8 +147,13 @@ struct Where {
   }
 };
 
+// Shared memory.  While rows are walked: a thread's own ring of vectors that are on their way; then the block's sums.
+constexpr int kRing = 32 << 10;   // bytes of the ring: eight rows of one operand, four of two
 struct Sums {
-  float a[2][kThreads * 8];   // [row of the block][channel of the tile]
+  union {
+    char ring[kRing];
+    float a[2][kThreads * 8];   // [row of the block][channel of the tile]
+  };
   float n[kThreads];
   float g[3][kGroups];        // of a group: mean, rstd; backward the two sums
 };
@@ -132,35 +164,61 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// calls f(row, step, live) for the thread's rows of the block, live: not padded; loads go ahead, kN at a time
-template <typename T, int kV, int kOps, int kN, typename Load, typename F>
-__device__ __forceinline__ void rows(const GnArgs& a, const Where<kV>& p, bool back, Load&& load, F&& f) {
-  const unsigned char* mask = a.mask ? a.mask + (long long)p.b * a.L : nullptr;
-  const int total = p.t1 - p.t0, mine = p.on && p.r < total ? (total - p.r + p.lanes - 1) / p.lanes : 0;
+// Calls f(values, step, live) for the thread's rows of the block (live: not padded), in order or back.  ptr(operand): its
+// vector at step 0; the rows ahead are on their way to the thread's own places in shared memory, as many as fit there: what
+// a block has under way does not take registers.
+template <typename T, int kV, int kOps, typename F>
+__device__ __forceinline__ void rows(const GnArgs& a, const Where<kV>& p, Sums& s, bool back, const T* const (&ptr)[kOps],
+                                     const long long (&stride)[kOps], F&& f) {
+  using V = Vec<T, kV>;
+  constexpr int kP = V::kP, kDepth = kRing / (kThreads * 16 * kOps);
+  const int total = p.t1 - p.t0, mine = p.on && p.r < total ? (total - p.r + p.lanes - 1) / p.lanes : 0;   // (at most kRun)
   const int first = back ? p.t0 + p.r + (mine - 1) * p.lanes : p.t0 + p.r, step = back ? -p.lanes : p.lanes;
-  int k = 0;
-  if (mask == nullptr) {
-    for (; k + kN <= mine; k += kN) {
-      Vec<T, kV> v[kN][kOps];
-#pragma unroll
-      for (int u = 0; u < kN; ++u) load(v[u], first + (k + u) * step);
-#pragma unroll
-      for (int u = 0; u < kN; ++u) f(v[u], first + (k + u) * step, true);
-    }
+  unsigned long long dead = 0;
+  if (a.mask != nullptr) {
+    const unsigned char* mask = a.mask + (long long)p.b * a.L;
+#pragma unroll 8
+    for (int k = 0; k < mine; ++k) dead |= (unsigned long long)(mask[first + k * step] != 0) << k;
   }
-  for (; k < mine; k += kN) {
-    Vec<T, kV> v[kN][kOps];
-    bool live[kN];
+  if constexpr (V::kBytes == 2) {   // (no copy is that short: eight rows at a time through registers)
+    constexpr int kN = 8 / kOps;
+    for (int k = 0; k < mine; k += kN) {
+      float v[kN][kOps];
 #pragma unroll
-    for (int u = 0; u < kN; ++u) {
-      const int t = first + (k + u) * step;
-      live[u] = k + u < mine && !(mask && mask[t]);
-      if (live[u]) load(v[u], t);
+      for (int u = 0; u < kN; ++u)
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) v[u][o] = k + u < mine ? Elem<T>::ld(ptr[o] + (first + (k + u) * step) * stride[o]) : 0.f;
+#pragma unroll
+      for (int u = 0; u < kN; ++u) {
+        f32x2 w[kOps][kP];
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) w[o][0] = pack2(v[u][o], 0.f);
+        if (k + u < mine) f(w, first + (k + u) * step, !((dead >> (k + u)) & 1u));
+      }
     }
+  } else {
+    char* const own = s.ring + threadIdx.x * 16;
+    auto place = [&](int k, int o) { return own + ((k % kDepth) * kOps + o) * (kThreads * 16); };
+    auto fetch = [&](int k) {
+      if (k < mine) {
 #pragma unroll
-    for (int u = 0; u < kN; ++u)
-      if (k + u < mine) f(v[u], first + (k + u) * step, live[u]);
+        for (int o = 0; o < kOps; ++o) V::fetch(smem_u32(place(k, o)), ptr[o] + (first + k * step) * stride[o]);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int k = 0; k < kDepth - 1; ++k) fetch(k);
+    for (int k = 0; k < mine; ++k) {
+      fetch(k + kDepth - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      f32x2 w[kOps][kP];
+#pragma unroll
+      for (int o = 0; o < kOps; ++o) V::read(place(k, o), w[o]);
+      f(w, first + k * step, !((dead >> k) & 1u));
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
+  __syncthreads();   // (the ring is free)
 }
 
 // ---- forward -----------------------------------------------------------------------------------
@@ -170,51 +228,51 @@ __device__ __forceinline__ void rows(const GnArgs& a, const Where<kV>& p, bool b
 // kOne: a vector lies in one group; its values are then one entry.
 template <typename T, int kV, bool kOne>
 __device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sums& s) {
-  constexpr int kE = kOne ? 1 : kV;   // entries that a thread leaves
-  const T* x = (const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV;
-  float cnt = 0.f, pv[kV], S[kV], Q[kV];
+  constexpr int kE = kOne ? 1 : kV, kP = Vec<T, kV>::kP;   // entries that a thread leaves, pairs
+  float cnt = 0.f;
+  f32x2 pv[kP], S[kP], Q[kP];
 #pragma unroll
-  for (int j = 0; j < kV; ++j) S[j] = Q[j] = pv[j] = 0.f;
-  rows<T, kV, 1, kBatch>(a, p, false, [&](Vec<T, kV>(&v)[1], int t) { v[0].load(x + t * a.xsl); },
-                         [&](Vec<T, kV>(&v)[1], int, bool live) {
-                           if (!live) return;
-                           float f[kV];
-                           v[0].get(f);
-                           if (cnt == 0.f) {
+  for (int j = 0; j < kP; ++j) S[j] = Q[j] = pv[j] = both(0.f);
+  const T* const ptr[1] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV};
+  const long long stride[1] = {a.xsl};
+  rows<T, kV, 1>(a, p, s, false, ptr, stride, [&](f32x2(&f)[1][kP], int, bool live) {
+    if (!live) return;
+    if (cnt == 0.f) {
 #pragma unroll
-                             for (int j = 0; j < kV; ++j) pv[j] = f[j];
-                           }
-                           cnt += 1.f;
+      for (int j = 0; j < kP; ++j) pv[j] = f[0][j];
+    }
+    cnt += 1.f;
 #pragma unroll
-                           for (int j = 0; j < kV; ++j) {
-                             const float d = f[j] - pv[j];
-                             S[j] += d;
-                             Q[j] = fmaf(d, d, Q[j]);
-                           }
-                         });
+    for (int j = 0; j < kP; ++j) {
+      const f32x2 d = sub2(f[0][j], pv[j]);
+      S[j] = add2(S[j], d);
+      Q[j] = fma2(d, d, Q[j]);
+    }
+  });
   const float inv = cnt > 0.f ? 1.f / cnt : 0.f;
   const int width = p.nv * kE;
   if (p.r < p.lanes) {
-    float m[kV];
+    float m[2 * kP], q[2 * kP];
 #pragma unroll
-    for (int j = 0; j < kV; ++j) {
-      const float d = S[j] * inv;
-      m[j] = pv[j] + d;
-      Q[j] = not_negative(fmaf(-S[j], d, Q[j]));
+    for (int j = 0; j < kP; ++j) {
+      float s0, s1, q0, q1;
+      unpack2(S[j], s0, s1), unpack2(Q[j], q0, q1), unpack2(pv[j], m[2 * j], m[2 * j + 1]);
+      m[2 * j] = fmaf(s0, inv, m[2 * j]), m[2 * j + 1] = fmaf(s1, inv, m[2 * j + 1]);
+      q[2 * j] = not_negative(fmaf(-s0 * inv, s0, q0)), q[2 * j + 1] = not_negative(fmaf(-s1 * inv, s1, q1));
     }
     if (kOne) {
-      float mean = 0.f, q = 0.f;
+      float mean = 0.f, all = 0.f;
 #pragma unroll
       for (int j = 0; j < kV; ++j) mean += m[j];
       mean *= 1.f / kV;
 #pragma unroll
-      for (int j = 0; j < kV; ++j) q += fmaf(cnt * (m[j] - mean), m[j] - mean, Q[j]);
-      m[0] = mean, Q[0] = q;
+      for (int j = 0; j < kV; ++j) all += fmaf(cnt * (m[j] - mean), m[j] - mean, q[j]);
+      m[0] = mean, q[0] = all;
     }
 #pragma unroll
     for (int j = 0; j < kE; ++j) {
       s.a[0][p.r * width + p.v * kE + j] = m[j];
-      s.a[1][p.r * width + p.v * kE + j] = Q[j];
+      s.a[1][p.r * width + p.v * kE + j] = q[j];
     }
     if (p.v == 0) s.n[p.r] = cnt;
   }
@@ -269,32 +327,41 @@ __device__ __forceinline__ int group_of(const GnArgs& a, const Where<kV>& p, int
   return p.on ? (p.v * kV + (kOne ? 0 : j)) / a.size : 0;
 }
 
+// a pair of the thread's channels: what `of` says for each (0 for the idle one)
+template <int kV, typename F>
+__device__ __forceinline__ f32x2 pair_of(int j, F&& of) {
+  return pack2(of(2 * j), kV == 1 ? 0.f : of(2 * j + 1));
+}
+
 template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, const Sums& s) {
-  constexpr int kE = kOne ? 1 : kV;
-  float m[kE], scale[kV], beta[kV];
+__device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, Sums& s) {
+  constexpr int kP = Vec<T, kV>::kP, kM = kOne ? 1 : kP;
+  f32x2 m[kM], scale[kP], beta[kP];
 #pragma unroll
-  for (int j = 0; j < kE; ++j) m[j] = s.g[0][group_of<kV, kOne>(a, p, j)];
+  for (int j = 0; j < kM; ++j) m[j] = pair_of<kOne ? 2 : kV>(j, [&](int c) { return s.g[0][group_of<kV, kOne>(a, p, c)]; });
 #pragma unroll
-  for (int j = 0; j < kV; ++j) {
-    scale[j] = p.on ? s.g[1][group_of<kV, kOne>(a, p, j)] * (a.gamma[p.c0 + p.v * kV + j] + a.offset) : 0.f;
-    beta[j] = p.on ? a.beta[p.c0 + p.v * kV + j] : 0.f;
+  for (int j = 0; j < kP; ++j) {
+    const float *w = a.gamma + p.c0 + p.v * kV, *c = a.beta + p.c0 + p.v * kV;
+    scale[j] = pair_of<kV>(j, [&](int k) { return p.on ? s.g[1][group_of<kV, kOne>(a, p, k)] * (w[k] + a.offset) : 0.f; });
+    beta[j] = pair_of<kV>(j, [&](int k) { return p.on ? c[k] : 0.f; });
   }
-  const T* x = (const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV;
+  const T* const ptr[1] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV};
+  const long long stride[1] = {a.xsl};
   T* y = (T*)a.out + p.b * a.osb + p.c0 + p.v * kV;
-  rows<T, kV, 1, kBatch>(a, p, true, [&](Vec<T, kV>(&v)[1], int t) { v[0].load(x + t * a.xsl); },
-                         [&](Vec<T, kV>(&v)[1], int t, bool live) {
-                           float f[kV];
-                           Vec<T, kV> o;
-                           v[0].get(f);
+  rows<T, kV, 1>(a, p, s, true, ptr, stride, [&](f32x2(&f)[1][kP], int t, bool live) {
+    f32x2 o[kP];
 #pragma unroll
-                           for (int j = 0; j < kV; ++j) {
-                             const float z = fmaf(f[j] - m[kOne ? 0 : j], scale[j], beta[j]);
-                             f[j] = live ? (a.silu ? z * sig<T>(z) : z) : 0.f;
-                           }
-                           o.set(f);
-                           o.store(y + t * a.osl);
-                         });
+    for (int j = 0; j < kP; ++j) o[j] = fma2(sub2(f[0][j], m[kOne ? 0 : j]), scale[j], beta[j]);
+    if (a.silu) {
+#pragma unroll
+      for (int j = 0; j < kP; ++j) o[j] = mul2(o[j], minus_sig2<T>(o[j]) ^ 0x8000000080000000ull);
+    }
+    if (!live) {
+#pragma unroll
+      for (int j = 0; j < kP; ++j) o[j] = both(0.f);
+    }
+    Vec<T, kV>::store(y + t * a.osl, o);
+  });
 }
 
 // the partial results of the tile's groups, of every run (steps, mean, squared deviations)
@@ -320,8 +387,9 @@ __device__ __forceinline__ void fold(const GnArgs& a, int b, int tile, int group
 }
 
 template <typename T, int kV, bool kOne>
-__global__ void __launch_bounds__(kThreads, 3) gn_first_kernel(GnArgs a) {
-  __shared__ Sums s;
+__global__ void __launch_bounds__(kThreads, 4) gn_first_kernel(GnArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  Sums& s = *reinterpret_cast<Sums*>(smem);
   pdl_wait();
   const Where<kV> p(a, a.first + blockIdx.y, blockIdx.x);
   moments<T, kV, kOne>(a, p, s);
@@ -338,8 +406,9 @@ __global__ void __launch_bounds__(kThreads, 3) gn_first_kernel(GnArgs a) {
 }
 
 template <typename T, int kV, bool kOne>
-__global__ void __launch_bounds__(kThreads, 3) gn_second_kernel(GnArgs a) {
-  __shared__ Sums s;
+__global__ void __launch_bounds__(kThreads, 4) gn_second_kernel(GnArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  Sums& s = *reinterpret_cast<Sums*>(smem);
   const int slice = a.slices - 1 - blockIdx.y, run = a.runs - 1 - blockIdx.x;
   const Where<kV> p(a, a.first + slice, run);
   pdl_wait();
@@ -360,55 +429,70 @@ __device__ __forceinline__ float slope_of(float d, float dy, float scale, float 
 
 template <typename T, int kV, bool kOne>
 struct Back {
-  static constexpr int kE = kOne ? 1 : kV;
-  const T *x, *dy;
-  float m[kE], scale[kV], beta[kV];
+  static constexpr int kP = Vec<T, kV>::kP, kM = kOne ? 1 : kP;
+  f32x2 m[kM], scale[kP], beta[kP];
   __device__ __forceinline__ Back(const GnArgs& a, const Where<kV>& p) {
     const long long at = (long long)p.b * a.G + p.tile * a.ng;
-    x = (const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV;
-    dy = (const T*)a.dy + p.b * a.gsb + p.c0 + p.v * kV;
+    const float *w = a.gamma + p.c0 + p.v * kV, *c = a.beta + p.c0 + p.v * kV, *mean = a.mean + at, *rstd = a.rstd + at;
 #pragma unroll
-    for (int j = 0; j < kE; ++j) m[j] = a.mean[at + group_of<kV, kOne>(a, p, j)];
+    for (int j = 0; j < kM; ++j) m[j] = pair_of<kOne ? 2 : kV>(j, [&](int k) { return mean[group_of<kV, kOne>(a, p, k)]; });
 #pragma unroll
-    for (int j = 0; j < kV; ++j) {
-      scale[j] = p.on ? a.rstd[at + group_of<kV, kOne>(a, p, j)] * (a.gamma[p.c0 + p.v * kV + j] + a.offset) : 0.f;
-      beta[j] = p.on ? a.beta[p.c0 + p.v * kV + j] : 0.f;
+    for (int j = 0; j < kP; ++j) {
+      scale[j] = pair_of<kV>(j, [&](int k) { return p.on ? rstd[group_of<kV, kOne>(a, p, k)] * (w[k] + a.offset) : 0.f; });
+      beta[j] = pair_of<kV>(j, [&](int k) { return p.on ? c[k] : 0.f; });
     }
   }
-  __device__ __forceinline__ void load(const GnArgs& a, Vec<T, kV> (&v)[2], int t) const {
-    v[0].load(x + t * a.xsl);
-    v[1].load(dy + t * a.gsl);
+  // d = x - mean, and minus dz
+  __device__ __forceinline__ void slopes(const GnArgs& a, const f32x2 (&x)[kP], const f32x2 (&dy)[kP], f32x2 (&d)[kP], f32x2 (&ndz)[kP]) const {
+#pragma unroll
+    for (int j = 0; j < kP; ++j) d[j] = sub2(x[j], m[kOne ? 0 : j]);
+    if (a.silu) {
+#pragma unroll
+      for (int j = 0; j < kP; ++j) {
+        const f32x2 z = fma2(d[j], scale[j], beta[j]), ns = minus_sig2<T>(z);
+        ndz[j] = mul2(mul2(dy[j], ns), add2(fma2(z, ns, z), both(1.f)));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kP; ++j) ndz[j] = dy[j] ^ 0x8000000080000000ull;
+    }
   }
 };
 
 // sums of dz and dz xhat of every channel over the block's steps -> a.chan, of dn and dn xhat of every group -> s.g[0], s.g[1]
 template <typename T, int kV, bool kOne>
 __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& s) {
-  float S[kV], Q[kV];   // (Q: of dz d, xhat being rstd d)
+  constexpr int kP = Vec<T, kV>::kP;
+  f32x2 nS[kP], nQ[kP];   // minus the sums of dz and of dz d (xhat being rstd d)
 #pragma unroll
-  for (int j = 0; j < kV; ++j) S[j] = Q[j] = 0.f;
+  for (int j = 0; j < kP; ++j) nS[j] = nQ[j] = both(0.f);
+  const T* const ptr[2] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV, (const T*)a.dy + p.b * a.gsb + p.c0 + p.v * kV};
+  const long long stride[2] = {a.xsl, a.gsl};
   {
     const Back<T, kV, kOne> k(a, p);
-    rows<T, kV, 2, kBatch / 2>(a, p, false, [&](Vec<T, kV>(&v)[2], int t) { k.load(a, v, t); },
-                               [&](Vec<T, kV>(&v)[2], int, bool live) {
-                                 if (!live) return;
-                                 float f[kV], g[kV];
-                                 v[0].get(f);
-                                 v[1].get(g);
+    rows<T, kV, 2>(a, p, s, false, ptr, stride, [&](f32x2(&f)[2][kP], int, bool live) {
+      if (!live) return;
+      f32x2 d[kP], ndz[kP];
+      k.slopes(a, f[0], f[1], d, ndz);
 #pragma unroll
-                                 for (int j = 0; j < kV; ++j) {
-                                   const float d = f[j] - k.m[kOne ? 0 : j], dz = slope_of<T>(d, g[j], k.scale[j], k.beta[j], a.silu);
-                                   S[j] += dz;
-                                   Q[j] = fmaf(dz, d, Q[j]);
-                                 }
-                               });
+      for (int j = 0; j < kP; ++j) {
+        nS[j] = add2(nS[j], ndz[j]);
+        nQ[j] = fma2(ndz[j], d[j], nQ[j]);
+      }
+    });
+  }
+  float S[2 * kP], Q[2 * kP];
+#pragma unroll
+  for (int j = 0; j < kP; ++j) {
+    unpack2(nS[j], S[2 * j], S[2 * j + 1]);
+    unpack2(nQ[j], Q[2 * j], Q[2 * j + 1]);
   }
   const int width = p.nv * kV;
   if (p.r < p.lanes) {
 #pragma unroll
     for (int j = 0; j < kV; ++j) {
-      s.a[0][p.r * width + p.v * kV + j] = S[j];
-      s.a[1][p.r * width + p.v * kV + j] = Q[j];
+      s.a[0][p.r * width + p.v * kV + j] = -S[j];
+      s.a[1][p.r * width + p.v * kV + j] = -Q[j];
     }
   }
   __syncthreads();
@@ -446,38 +530,43 @@ __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& 
 
 // sums of dn, dn xhat in s.g[0], s.g[1] -> dx = rstd dn - rstd mean(dn) - d rstd^2 mean(dn xhat)
 template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, const Sums& s) {
-  constexpr int kE = kOne ? 1 : kV;
+__device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, Sums& s) {
+  constexpr int kP = Vec<T, kV>::kP, kM = kOne ? 1 : kP;
   const Back<T, kV, kOne> k(a, p);
   const float n = (float)a.count[p.b] * (float)a.size, inv = n > 0.f ? 1.f / n : 0.f;
-  float m1[kE], m2[kE];
+  const float* rstd = a.rstd + (long long)p.b * a.G + p.tile * a.ng;
+  f32x2 m1[kM], m2[kM];   // rstd times the one mean, rstd^2 times the other
 #pragma unroll
-  for (int j = 0; j < kE; ++j) {
-    const int g = group_of<kV, kOne>(a, p, j);
-    const float r = a.rstd[(long long)p.b * a.G + p.tile * a.ng + g];
-    m1[j] = s.g[0][g] * inv * r;
-    m2[j] = s.g[1][g] * inv * r * r;
+  for (int j = 0; j < kM; ++j) {
+    m1[j] = pair_of<kOne ? 2 : kV>(j, [&](int c) {
+      const int g = group_of<kV, kOne>(a, p, c);
+      return s.g[0][g] * inv * rstd[g];
+    });
+    m2[j] = pair_of<kOne ? 2 : kV>(j, [&](int c) {
+      const int g = group_of<kV, kOne>(a, p, c);
+      return s.g[1][g] * inv * rstd[g] * rstd[g];
+    });
   }
+  const T* const ptr[2] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV, (const T*)a.dy + p.b * a.gsb + p.c0 + p.v * kV};
+  const long long stride[2] = {a.xsl, a.gsl};
   T* dx = (T*)a.out + p.b * a.osb + p.c0 + p.v * kV;
-  rows<T, kV, 2, kBatch / 2>(a, p, true, [&](Vec<T, kV>(&v)[2], int t) { k.load(a, v, t); },
-                             [&](Vec<T, kV>(&v)[2], int t, bool live) {
-                               float f[kV], g[kV];
-                               Vec<T, kV> o;
-                               v[0].get(f);
-                               v[1].get(g);
+  rows<T, kV, 2>(a, p, s, true, ptr, stride, [&](f32x2(&f)[2][kP], int t, bool live) {
+    f32x2 d[kP], ndz[kP], o[kP];
+    k.slopes(a, f[0], f[1], d, ndz);
 #pragma unroll
-                               for (int j = 0; j < kV; ++j) {
-                                 const float d = f[j] - k.m[kOne ? 0 : j], dz = slope_of<T>(d, g[j], k.scale[j], k.beta[j], a.silu);
-                                 f[j] = live ? fmaf(dz, k.scale[j], -m1[kOne ? 0 : j]) - d * m2[kOne ? 0 : j] : 0.f;
-                               }
-                               o.set(f);
-                               o.store(dx + t * a.osl);
-                             });
+    for (int j = 0; j < kP; ++j) {
+      // dz scale - m1 - d m2, the signs turned twice
+      const f32x2 v = fma2(ndz[j], k.scale[j], fma2(d[j], m2[kOne ? 0 : j], m1[kOne ? 0 : j]));
+      o[j] = live ? v ^ 0x8000000080000000ull : both(0.f);
+    }
+    Vec<T, kV>::store(dx + t * a.osl, o);
+  });
 }
 
 template <typename T, int kV, bool kOne>
-__global__ void __launch_bounds__(kThreads, 3) gn_sums_kernel(GnArgs a) {
-  __shared__ Sums s;
+__global__ void __launch_bounds__(kThreads, 4) gn_sums_kernel(GnArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  Sums& s = *reinterpret_cast<Sums*>(smem);
   pdl_wait();
   const Where<kV> p(a, a.first + blockIdx.y, blockIdx.x);
   sums<T, kV, kOne>(a, p, s);
@@ -494,8 +583,9 @@ __global__ void __launch_bounds__(kThreads, 3) gn_sums_kernel(GnArgs a) {
 }
 
 template <typename T, int kV, bool kOne>
-__global__ void __launch_bounds__(kThreads, 3) gn_grads_kernel(GnArgs a) {
-  __shared__ Sums s;
+__global__ void __launch_bounds__(kThreads, 4) gn_grads_kernel(GnArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  Sums& s = *reinterpret_cast<Sums*>(smem);
   const int slice = a.slices - 1 - blockIdx.y, run = a.runs - 1 - blockIdx.x, lane = threadIdx.x & 31;
   const Where<kV> p(a, a.first + slice, run);
   pdl_wait();
@@ -742,10 +832,10 @@ void passes(First first, Second second, GnArgs a, int slices, int piece, cudaStr
     a.first = at;
     a.slices = std::min(piece, slices - at);
     if (at == 0)
-      launch(first, dim3(a.runs, a.slices), dim3(kThreads), 0, s, a);
+      launch(first, dim3(a.runs, a.slices), dim3(kThreads), sizeof(Sums), s, a);
     else
-      launch_after(first, dim3(a.runs, a.slices), dim3(kThreads), 0, s, a);
-    if (a.runs > 1) launch_after(second, dim3(a.runs, a.slices), dim3(kThreads), 0, s, a);
+      launch_after(first, dim3(a.runs, a.slices), dim3(kThreads), sizeof(Sums), s, a);
+    if (a.runs > 1) launch_after(second, dim3(a.runs, a.slices), dim3(kThreads), sizeof(Sums), s, a);
   }
 }
 template <typename T, int kV, bool kOne>
