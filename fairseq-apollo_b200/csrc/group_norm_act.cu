@@ -156,6 +156,7 @@ struct Sums {
   };
   float n[kThreads];
   float g[3][kGroups];        // of a group: mean, rstd; backward the two sums
+  unsigned bits[kRun * kThreads / 32];   // padded steps of the block
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -164,61 +165,105 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Calls f(values, step, live) for the thread's rows of the block (live: not padded), in order or back.  ptr(operand): its
-// vector at step 0; the rows ahead are on their way to the thread's own places in shared memory, as many as fit there: what
-// a block has under way does not take registers.
-template <typename T, int kV, int kOps, typename F>
-__device__ __forceinline__ void rows(const GnArgs& a, const Where<kV>& p, Sums& s, bool back, const T* const (&ptr)[kOps],
-                                     const long long (&stride)[kOps], F&& f) {
+// the padded steps of the block as bits
+template <int kV>
+__device__ __forceinline__ void read_mask(const GnArgs& a, const Where<kV>& p, Sums& s) {
+  if (a.mask == nullptr) return;
+  const unsigned char* mask = a.mask + (long long)p.b * a.L + p.t0;
+  const int n = p.t1 - p.t0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < (n + 31) / 32 * 32; i += kThreads) {
+    const unsigned bits = __ballot_sync(0xffffffffu, i < n && mask[i] != 0);
+    if ((threadIdx.x & 31) == 0) s.bits[i >> 5] = bits;
+  }
+  __syncthreads();
+}
+
+// Calls f(values, address, first, live) for the thread's rows of the block (live: not padded), in order or back; address: of `out`'s
+// vector there.  ptr(operand): its vector at step 0; the rows ahead are on their way to the thread's own places in shared
+// memory, as many as fit there: what a block has under way does not take registers.
+template <typename T, int kV, int kOps, bool kMask, typename F>
+__device__ __forceinline__ void walk(const GnArgs& a, const Where<kV>& p, Sums& s, bool back, const T* const (&ptr)[kOps],
+                                     const long long (&stride)[kOps], T* out, long long outs, F&& f) {
   using V = Vec<T, kV>;
   constexpr int kP = V::kP, kDepth = kRing / (kThreads * 16 * kOps);
   const int total = p.t1 - p.t0, mine = p.on && p.r < total ? (total - p.r + p.lanes - 1) / p.lanes : 0;   // (at most kRun)
-  const int first = back ? p.t0 + p.r + (mine - 1) * p.lanes : p.t0 + p.r, step = back ? -p.lanes : p.lanes;
-  unsigned long long dead = 0;
-  if (a.mask != nullptr) {
-    const unsigned char* mask = a.mask + (long long)p.b * a.L;
-#pragma unroll 8
-    for (int k = 0; k < mine; ++k) dead |= (unsigned long long)(mask[first + k * step] != 0) << k;
-  }
-  if constexpr (V::kBytes == 2) {   // (no copy is that short: eight rows at a time through registers)
+  const int start = back ? p.r + (mine - 1) * p.lanes : p.r, step = back ? -p.lanes : p.lanes;
+  const T* q[kOps];
+  long long hop[kOps];
+#pragma unroll
+  for (int o = 0; o < kOps; ++o) q[o] = ptr[o] + (long long)(p.t0 + start) * stride[o], hop[o] = step * stride[o];
+  T* at = out + (long long)(p.t0 + start) * outs;
+  const long long next = step * outs;
+  auto live = [&](int k) {
+    const int i = start + k * step;
+    return !kMask || !((s.bits[i >> 5] >> (i & 31)) & 1u);
+  };
+  if constexpr (V::kBytes == 2) {   // (no copy is that short: eight at a time through registers)
     constexpr int kN = 8 / kOps;
     for (int k = 0; k < mine; k += kN) {
       float v[kN][kOps];
 #pragma unroll
       for (int u = 0; u < kN; ++u)
 #pragma unroll
-        for (int o = 0; o < kOps; ++o) v[u][o] = k + u < mine ? Elem<T>::ld(ptr[o] + (first + (k + u) * step) * stride[o]) : 0.f;
+        for (int o = 0; o < kOps; ++o) v[u][o] = k + u < mine ? Elem<T>::ld(q[o] + (k + u) * hop[o]) : 0.f;
 #pragma unroll
       for (int u = 0; u < kN; ++u) {
         f32x2 w[kOps][kP];
 #pragma unroll
         for (int o = 0; o < kOps; ++o) w[o][0] = pack2(v[u][o], 0.f);
-        if (k + u < mine) f(w, first + (k + u) * step, !((dead >> (k + u)) & 1u));
+        if (k + u < mine) f(w, at, k + u == 0, live(k + u));
+        at += next;
       }
     }
   } else {
-    char* const own = s.ring + threadIdx.x * 16;
-    auto place = [&](int k, int o) { return own + ((k % kDepth) * kOps + o) * (kThreads * 16); };
-    auto fetch = [&](int k) {
-      if (k < mine) {
+    const uint32_t own = smem_u32(s.ring) + threadIdx.x * 16;
+    int ahead = 0;
+    auto fetch = [&](int u) {   // (the next row, into place u)
+      if (ahead < mine) {
 #pragma unroll
-        for (int o = 0; o < kOps; ++o) V::fetch(smem_u32(place(k, o)), ptr[o] + (first + k * step) * stride[o]);
+        for (int o = 0; o < kOps; ++o) {
+          V::fetch(own + (u * kOps + o) * (kThreads * 16), q[o]);
+          q[o] += hop[o];
+        }
       }
+      ++ahead;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
-    for (int k = 0; k < kDepth - 1; ++k) fetch(k);
-    for (int k = 0; k < mine; ++k) {
-      fetch(k + kDepth - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    auto use = [&](int k, int u) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
       f32x2 w[kOps][kP];
 #pragma unroll
-      for (int o = 0; o < kOps; ++o) V::read(place(k, o), w[o]);
-      f(w, first + k * step, !((dead >> k) & 1u));
+      for (int o = 0; o < kOps; ++o) V::read(s.ring + threadIdx.x * 16 + (u * kOps + o) * (kThreads * 16), w[o]);
+      f(w, at, k == 0, live(k));
+      at += next;
+    };
+#pragma unroll
+    for (int u = 0; u < kDepth - 1; ++u) fetch(u);
+    int k = 0;
+    for (; k + kDepth <= mine; k += kDepth) {
+#pragma unroll
+      for (int u = 0; u < kDepth; ++u) {
+        use(k + u, u);
+        fetch((u + kDepth - 1) % kDepth);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kDepth - 1; ++u) {
+      if (k + u < mine) use(k + u, u);
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
   __syncthreads();   // (the ring is free)
+}
+template <typename T, int kV, int kOps, typename F>
+__device__ __forceinline__ void rows(const GnArgs& a, const Where<kV>& p, Sums& s, bool back, const T* const (&ptr)[kOps],
+                                     const long long (&stride)[kOps], T* out, long long outs, F&& f) {
+  if (a.mask != nullptr)
+    walk<T, kV, kOps, true>(a, p, s, back, ptr, stride, out, outs, f);
+  else
+    walk<T, kV, kOps, false>(a, p, s, back, ptr, stride, out, outs, f);
 }
 
 // ---- forward -----------------------------------------------------------------------------------
@@ -235,9 +280,9 @@ __device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sum
   for (int j = 0; j < kP; ++j) S[j] = Q[j] = pv[j] = both(0.f);
   const T* const ptr[1] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV};
   const long long stride[1] = {a.xsl};
-  rows<T, kV, 1>(a, p, s, false, ptr, stride, [&](f32x2(&f)[1][kP], int, bool live) {
+  rows<T, kV, 1>(a, p, s, false, ptr, stride, (T*)nullptr, 0ll, [&](f32x2(&f)[1][kP], T*, bool first, bool live) {
     if (!live) return;
-    if (cnt == 0.f) {
+    if (a.mask != nullptr ? cnt == 0.f : first) {
 #pragma unroll
       for (int j = 0; j < kP; ++j) pv[j] = f[0][j];
     }
@@ -348,7 +393,7 @@ __device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, Sums&
   const T* const ptr[1] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV};
   const long long stride[1] = {a.xsl};
   T* y = (T*)a.out + p.b * a.osb + p.c0 + p.v * kV;
-  rows<T, kV, 1>(a, p, s, true, ptr, stride, [&](f32x2(&f)[1][kP], int t, bool live) {
+  rows<T, kV, 1>(a, p, s, true, ptr, stride, y, a.osl, [&](f32x2(&f)[1][kP], T* at, bool, bool live) {
     f32x2 o[kP];
 #pragma unroll
     for (int j = 0; j < kP; ++j) o[j] = fma2(sub2(f[0][j], m[kOne ? 0 : j]), scale[j], beta[j]);
@@ -360,7 +405,7 @@ __device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, Sums&
 #pragma unroll
       for (int j = 0; j < kP; ++j) o[j] = both(0.f);
     }
-    Vec<T, kV>::store(y + t * a.osl, o);
+    Vec<T, kV>::store(at, o);
   });
 }
 
@@ -392,6 +437,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_first_kernel(GnArgs a) {
   Sums& s = *reinterpret_cast<Sums*>(smem);
   pdl_wait();
   const Where<kV> p(a, a.first + blockIdx.y, blockIdx.x);
+  read_mask(a, p, s);
   moments<T, kV, kOne>(a, p, s);
   if (a.runs == 1) {
     finish(a, p, s, true);
@@ -411,6 +457,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_second_kernel(GnArgs a) {
   Sums& s = *reinterpret_cast<Sums*>(smem);
   const int slice = a.slices - 1 - blockIdx.y, run = a.runs - 1 - blockIdx.x;
   const Where<kV> p(a, a.first + slice, run);
+  read_mask(a, p, s);
   pdl_wait();
   fold(a, p.b, p.tile, p.groups, s);
   finish(a, p, s, run == 0);
@@ -470,7 +517,7 @@ __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& 
   const long long stride[2] = {a.xsl, a.gsl};
   {
     const Back<T, kV, kOne> k(a, p);
-    rows<T, kV, 2>(a, p, s, false, ptr, stride, [&](f32x2(&f)[2][kP], int, bool live) {
+    rows<T, kV, 2>(a, p, s, false, ptr, stride, (T*)nullptr, 0ll, [&](f32x2(&f)[2][kP], T*, bool, bool live) {
       if (!live) return;
       f32x2 d[kP], ndz[kP];
       k.slopes(a, f[0], f[1], d, ndz);
@@ -550,7 +597,7 @@ __device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, Sums&
   const T* const ptr[2] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV, (const T*)a.dy + p.b * a.gsb + p.c0 + p.v * kV};
   const long long stride[2] = {a.xsl, a.gsl};
   T* dx = (T*)a.out + p.b * a.osb + p.c0 + p.v * kV;
-  rows<T, kV, 2>(a, p, s, true, ptr, stride, [&](f32x2(&f)[2][kP], int t, bool live) {
+  rows<T, kV, 2>(a, p, s, true, ptr, stride, dx, a.osl, [&](f32x2(&f)[2][kP], T* at, bool, bool live) {
     f32x2 d[kP], ndz[kP], o[kP];
     k.slopes(a, f[0], f[1], d, ndz);
 #pragma unroll
@@ -559,16 +606,17 @@ __device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, Sums&
       const f32x2 v = fma2(ndz[j], k.scale[j], fma2(d[j], m2[kOne ? 0 : j], m1[kOne ? 0 : j]));
       o[j] = live ? v ^ 0x8000000080000000ull : both(0.f);
     }
-    Vec<T, kV>::store(dx + t * a.osl, o);
+    Vec<T, kV>::store(at, o);
   });
 }
 
 template <typename T, int kV, bool kOne>
-__global__ void __launch_bounds__(kThreads, 4) gn_sums_kernel(GnArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) gn_sums_kernel(GnArgs a) {
   extern __shared__ __align__(16) char smem[];
   Sums& s = *reinterpret_cast<Sums*>(smem);
   pdl_wait();
   const Where<kV> p(a, a.first + blockIdx.y, blockIdx.x);
+  read_mask(a, p, s);
   sums<T, kV, kOne>(a, p, s);
   if (a.runs == 1) {
     grads<T, kV, kOne>(a, p, s);
@@ -583,11 +631,12 @@ __global__ void __launch_bounds__(kThreads, 4) gn_sums_kernel(GnArgs a) {
 }
 
 template <typename T, int kV, bool kOne>
-__global__ void __launch_bounds__(kThreads, 4) gn_grads_kernel(GnArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) gn_grads_kernel(GnArgs a) {
   extern __shared__ __align__(16) char smem[];
   Sums& s = *reinterpret_cast<Sums*>(smem);
   const int slice = a.slices - 1 - blockIdx.y, run = a.runs - 1 - blockIdx.x, lane = threadIdx.x & 31;
   const Where<kV> p(a, a.first + slice, run);
+  read_mask(a, p, s);
   pdl_wait();
   for (int g = threadIdx.x >> 5; g < p.groups; g += kThreads / 32) {
     const float* q = a.part + (((long long)p.b * a.G + p.tile * a.ng + g) * a.runs) * 2;
