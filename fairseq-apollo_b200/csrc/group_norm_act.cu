@@ -10,7 +10,7 @@
 // one run needs no partial results: the same block does both, in one launch.
 //
 // Bound: HBM, each value once: the second pass goes backwards, over what the first has just left in L2, and a call that is larger
-// than that goes through L2 in pieces of sequences and tiles.
+// much larger than that goes through L2 in pieces of sequences.
 //
 // Statistics: a thread adds up d = x - p and d^2 with p the first value of its run.  p being one of the n values, the squares about
 // it are at most n + 1 times those about the mean, so n <= kRun bounds what their difference loses; such entries are then joined by
@@ -38,8 +38,10 @@ struct GnArgs {
   const unsigned char* mask;
   int B, L, D, G, size;        // size: channels of a group
   int ng, tiles;               // groups of a tile, tiles of a row
+  int nv, lanes;               // vectors of a tile's row, rows that a block takes at once
   int steps, runs;             // steps of a block, blocks of a sequence
-  int first, slices;           // this launch: (sequence, tile) pairs first .. first + slices
+  int from;                    // this launch's first sequence
+  float over_nv, over_size, over_vectors;   // reciprocals: of a row's vectors, a group's channels, a group's vectors
   float eps, offset;
   int silu;
   long long* count;
@@ -128,32 +130,35 @@ __device__ __forceinline__ f32x2 minus_sig2(f32x2 z) {
   return pack2(rcp_approx(a), rcp_approx(b));
 }
 
+// a / b for 0 <= a < 2^16 and b's reciprocal (off by less than 2^-23 of it: the half keeps the quotient on its side)
+__device__ __forceinline__ int quotient(int a, float over) { return __float2int_rd(((float)a + 0.5f) * over); }
+
 // What a block works on.
 template <int kV>
 struct Where {
   int b, tile, run, c0, chans, groups, t0, t1;   // first channel, channels, groups; steps
   int nv, lanes, v, r;                           // vectors of a row, rows at once; this thread's vector and row
   bool on;
-  __device__ __forceinline__ Where(const GnArgs& a, int slice, int run_) {
-    b = slice / a.tiles, tile = slice % a.tiles, run = run_;
+  __device__ __forceinline__ Where(const GnArgs& a, bool back) {
+    b = a.from + (back ? gridDim.z - 1 - blockIdx.z : blockIdx.z);
+    tile = back ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
+    run = back ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
     c0 = tile * a.ng * a.size;
     groups = min(a.ng, a.G - tile * a.ng);
     chans = groups * a.size;
     t0 = run * a.steps, t1 = min(t0 + a.steps, a.L);
-    nv = a.ng * a.size / kV;
-    lanes = kThreads / nv;
-    r = threadIdx.x / nv, v = threadIdx.x - r * nv;
+    nv = a.nv;
+    lanes = a.lanes;
+    r = quotient(threadIdx.x, a.over_nv), v = threadIdx.x - r * nv;
     on = r < lanes && v * kV < chans;
   }
 };
 
-// Shared memory.  While rows are walked: a thread's own ring of vectors that are on their way; then the block's sums.
+// Shared memory: every thread's own ring of vectors that are on their way, the block's sums.
 constexpr int kRing = 32 << 10;   // bytes of the ring: eight rows of one operand, four of two
 struct Sums {
-  union {
-    char ring[kRing];
-    float a[2][kThreads * 8];   // [row of the block][channel of the tile]
-  };
+  char ring[kRing];
+  float a[2][kThreads * 8];   // [row of the block][channel of the tile]
   float n[kThreads];
   float g[3][kGroups];        // of a group: mean, rstd; backward the two sums
   unsigned bits[kRun * kThreads / 32];   // padded steps of the block
@@ -179,47 +184,30 @@ __device__ __forceinline__ void read_mask(const GnArgs& a, const Where<kV>& p, S
   __syncthreads();
 }
 
-// Calls f(values, address, first, live) for the thread's rows of the block (live: not padded), in order or back; address: of `out`'s
-// vector there.  ptr(operand): its vector at step 0; the rows ahead are on their way to the thread's own places in shared
-// memory, as many as fit there: what a block has under way does not take registers.
-template <typename T, int kV, int kOps, bool kMask, typename F>
-__device__ __forceinline__ void walk(const GnArgs& a, const Where<kV>& p, Sums& s, bool back, const T* const (&ptr)[kOps],
-                                     const long long (&stride)[kOps], T* out, long long outs, F&& f) {
+// The thread's rows of the block, in order or back.  begin() sets the first of them on their way to the thread's own places in
+// shared memory, run(f) calls f(values, address, first, live) for each (live: not padded; address: of the output's vector
+// there).  What a block has under way so takes no registers, and begins before what the rows are needed for is known.
+template <typename T, int kV, int kOps>
+struct Walk {
   using V = Vec<T, kV>;
-  constexpr int kP = V::kP, kDepth = kRing / (kThreads * 16 * kOps);
-  const int total = p.t1 - p.t0, mine = p.on && p.r < total ? (total - p.r + p.lanes - 1) / p.lanes : 0;   // (at most kRun)
-  const int start = back ? p.r + (mine - 1) * p.lanes : p.r, step = back ? -p.lanes : p.lanes;
+  static constexpr int kP = V::kP, kDepth = kRing / (kThreads * 16 * kOps);
   const T* q[kOps];
-  long long hop[kOps];
-#pragma unroll
-  for (int o = 0; o < kOps; ++o) q[o] = ptr[o] + (long long)(p.t0 + start) * stride[o], hop[o] = step * stride[o];
-  T* at = out + (long long)(p.t0 + start) * outs;
-  const long long next = step * outs;
-  auto live = [&](int k) {
-    const int i = start + k * step;
-    return !kMask || !((s.bits[i >> 5] >> (i & 31)) & 1u);
-  };
-  if constexpr (V::kBytes == 2) {   // (no copy is that short: eight at a time through registers)
-    constexpr int kN = 8 / kOps;
-    for (int k = 0; k < mine; k += kN) {
-      float v[kN][kOps];
-#pragma unroll
-      for (int u = 0; u < kN; ++u)
-#pragma unroll
-        for (int o = 0; o < kOps; ++o) v[u][o] = k + u < mine ? Elem<T>::ld(q[o] + (k + u) * hop[o]) : 0.f;
-#pragma unroll
-      for (int u = 0; u < kN; ++u) {
-        f32x2 w[kOps][kP];
-#pragma unroll
-        for (int o = 0; o < kOps; ++o) w[o][0] = pack2(v[u][o], 0.f);
-        if (k + u < mine) f(w, at, k + u == 0, live(k + u));
-        at += next;
-      }
-    }
-  } else {
-    const uint32_t own = smem_u32(s.ring) + threadIdx.x * 16;
-    int ahead = 0;
-    auto fetch = [&](int u) {   // (the next row, into place u)
+  long long hop[kOps], next;
+  T* at;
+  int mine, start, step, ahead = 0;
+  uint32_t own;
+  __device__ __forceinline__ Walk(const GnArgs& a, const Where<kV>& p, Sums& s, bool back, T* out) {
+    const int total = p.t1 - p.t0;
+    mine = p.on && p.r < total ? quotient(total - p.r + p.lanes - 1, 1.f / (float)p.lanes) : 0;   // (at most kRun)
+    start = back ? p.r + (mine - 1) * p.lanes : p.r, step = back ? -p.lanes : p.lanes;
+    const int c = p.c0 + p.v * kV;
+    q[0] = (const T*)a.x + p.b * a.xsb + (p.t0 + start) * a.xsl + c, hop[0] = step * a.xsl;
+    if (kOps == 2) q[kOps - 1] = (const T*)a.dy + p.b * a.gsb + (p.t0 + start) * a.gsl + c, hop[kOps - 1] = step * a.gsl;
+    at = out + p.b * a.osb + (p.t0 + start) * a.osl + c, next = step * a.osl;
+    own = smem_u32(s.ring) + threadIdx.x * 16;
+  }
+  __device__ __forceinline__ void fetch(int u) {   // the next row, into place u
+    if constexpr (V::kBytes != 2) {
       if (ahead < mine) {
 #pragma unroll
         for (int o = 0; o < kOps; ++o) {
@@ -229,42 +217,62 @@ __device__ __forceinline__ void walk(const GnArgs& a, const Where<kV>& p, Sums& 
       }
       ++ahead;
       asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    auto use = [&](int k, int u) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
-      f32x2 w[kOps][kP];
-#pragma unroll
-      for (int o = 0; o < kOps; ++o) V::read(s.ring + threadIdx.x * 16 + (u * kOps + o) * (kThreads * 16), w[o]);
-      f(w, at, k == 0, live(k));
-      at += next;
-    };
+    }
+  }
+  __device__ __forceinline__ void begin() {
 #pragma unroll
     for (int u = 0; u < kDepth - 1; ++u) fetch(u);
-    int k = 0;
-    for (; k + kDepth <= mine; k += kDepth) {
-#pragma unroll
-      for (int u = 0; u < kDepth; ++u) {
-        use(k + u, u);
-        fetch((u + kDepth - 1) % kDepth);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kDepth - 1; ++u) {
-      if (k + u < mine) use(k + u, u);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  __syncthreads();   // (the ring is free)
-}
-template <typename T, int kV, int kOps, typename F>
-__device__ __forceinline__ void rows(const GnArgs& a, const Where<kV>& p, Sums& s, bool back, const T* const (&ptr)[kOps],
-                                     const long long (&stride)[kOps], T* out, long long outs, F&& f) {
-  if (a.mask != nullptr)
-    walk<T, kV, kOps, true>(a, p, s, back, ptr, stride, out, outs, f);
-  else
-    walk<T, kV, kOps, false>(a, p, s, back, ptr, stride, out, outs, f);
-}
+  template <typename F>
+  __device__ __forceinline__ void run(const Sums& s, bool masked, F&& f) {
+    auto live = [&](int k) {
+      if (!masked) return true;
+      const int i = start + k * step;
+      return !((s.bits[i >> 5] >> (i & 31)) & 1u);
+    };
+    if constexpr (V::kBytes == 2) {   // (no copy is that short: eight at a time through registers)
+      constexpr int kN = 8 / kOps;
+      for (int k = 0; k < mine; k += kN) {
+        float v[kN][kOps];
+#pragma unroll
+        for (int u = 0; u < kN; ++u)
+#pragma unroll
+          for (int o = 0; o < kOps; ++o) v[u][o] = k + u < mine ? Elem<T>::ld(q[o] + (k + u) * hop[o]) : 0.f;
+#pragma unroll
+        for (int u = 0; u < kN; ++u) {
+          f32x2 w[kOps][kP];
+#pragma unroll
+          for (int o = 0; o < kOps; ++o) w[o][0] = pack2(v[u][o], 0.f);
+          if (k + u < mine) f(w, at, k + u == 0, live(k + u));
+          at += next;
+        }
+      }
+    } else {
+      auto use = [&](int k, int u) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+        f32x2 w[kOps][kP];
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) V::read(s.ring + threadIdx.x * 16 + (u * kOps + o) * (kThreads * 16), w[o]);
+        f(w, at, k == 0, live(k));
+        at += next;
+      };
+      int k = 0;
+      for (; k + kDepth <= mine; k += kDepth) {
+#pragma unroll
+        for (int u = 0; u < kDepth; ++u) {
+          use(k + u, u);
+          fetch((u + kDepth - 1) % kDepth);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kDepth - 1; ++u) {
+        if (k + u < mine) use(k + u, u);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+  }
+};
 
 // ---- forward -----------------------------------------------------------------------------------
 // Statistics of n values, means m[k] of counts c[k] and squared deviations q[k]: mean = sum c m / n, then sum q + c (m - mean)^2.
@@ -272,15 +280,13 @@ __device__ __forceinline__ void rows(const GnArgs& a, const Where<kV>& p, Sums& 
 // Of the tile's groups over the block's steps -> s.g: steps, mean, squared deviations of all channels over their number.
 // kOne: a vector lies in one group; its values are then one entry.
 template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sums& s) {
+__device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sums& s, Walk<T, kV, 1>& walk, Walk<T, kV, 1>* then) {
   constexpr int kE = kOne ? 1 : kV, kP = Vec<T, kV>::kP;   // entries that a thread leaves, pairs
   float cnt = 0.f;
   f32x2 pv[kP], S[kP], Q[kP];
 #pragma unroll
   for (int j = 0; j < kP; ++j) S[j] = Q[j] = pv[j] = both(0.f);
-  const T* const ptr[1] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV};
-  const long long stride[1] = {a.xsl};
-  rows<T, kV, 1>(a, p, s, false, ptr, stride, (T*)nullptr, 0ll, [&](f32x2(&f)[1][kP], T*, bool first, bool live) {
+  walk.run(s, a.mask != nullptr, [&](f32x2(&f)[1][kP], T*, bool first, bool live) {
     if (!live) return;
     if (a.mask != nullptr ? cnt == 0.f : first) {
 #pragma unroll
@@ -294,6 +300,7 @@ __device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sum
       Q[j] = fma2(d, d, Q[j]);
     }
   });
+  if (then) then->begin();
   const float inv = cnt > 0.f ? 1.f / cnt : 0.f;
   const int width = p.nv * kE;
   if (p.r < p.lanes) {
@@ -322,7 +329,8 @@ __device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sum
     if (p.v == 0) s.n[p.r] = cnt;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31, per = a.size * kE / kV;   // entries of a row and group
+  const int lane = threadIdx.x & 31, per = kOne ? quotient(a.size, 1.f / kV) : a.size;   // entries of a row and group
+  const float over_per = kOne ? a.over_vectors : a.over_size;
   float n = 0.f;
   for (int r = lane; r < p.lanes; r += 32) n += s.n[r];
   n = warp_sum(n);
@@ -330,12 +338,12 @@ __device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sum
   for (int g = threadIdx.x >> 5; g < p.groups; g += kThreads / 32) {
     float sum = 0.f, dev = 0.f;
     for (int e = lane; e < p.lanes * per; e += 32) {
-      const int r = e / per;
+      const int r = quotient(e, over_per);
       sum = fmaf(s.n[r], s.a[0][r * width + g * per + e - r * per], sum);
     }
     const float mean = warp_sum(sum) * over;
     for (int e = lane; e < p.lanes * per; e += 32) {
-      const int r = e / per, at = r * width + g * per + e - r * per;
+      const int r = quotient(e, over_per), at = r * width + g * per + e - r * per;
       const float d = s.a[0][at] - mean, c = s.n[r] * (float)(kV / kE);
       if (c > 0.f) dev += fmaf(c * d, d, s.a[1][at]);   // (an empty row has no mean)
     }
@@ -369,34 +377,41 @@ __device__ __forceinline__ void finish(const GnArgs& a, const Where<kV>& p, Sums
 // the group of a thread's j-th channel
 template <int kV, bool kOne>
 __device__ __forceinline__ int group_of(const GnArgs& a, const Where<kV>& p, int j) {
-  return p.on ? (p.v * kV + (kOne ? 0 : j)) / a.size : 0;
+  return p.on ? quotient(p.v * kV + (kOne ? 0 : j), a.over_size) : 0;
 }
-
 // a pair of the thread's channels: what `of` says for each (0 for the idle one)
 template <int kV, typename F>
 __device__ __forceinline__ f32x2 pair_of(int j, F&& of) {
   return pack2(of(2 * j), kV == 1 ? 0.f : of(2 * j + 1));
 }
 
+// the thread's channels of gamma (+ 1) and beta
+template <int kV>
+struct Params {
+  static constexpr int kP = (kV + 1) / 2;
+  f32x2 w[kP], c[kP];
+  __device__ __forceinline__ Params(const GnArgs& a, const Where<kV>& p) {
+    const float *gamma = a.gamma + p.c0 + p.v * kV, *beta = a.beta + p.c0 + p.v * kV;
+#pragma unroll
+    for (int j = 0; j < kP; ++j) {
+      w[j] = pair_of<kV>(j, [&](int k) { return p.on ? gamma[k] + a.offset : 0.f; });
+      c[j] = pair_of<kV>(j, [&](int k) { return p.on ? beta[k] : 0.f; });
+    }
+  }
+};
+
 template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, Sums& s) {
+__device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, Sums& s, Walk<T, kV, 1>& walk, const Params<kV>& k) {
   constexpr int kP = Vec<T, kV>::kP, kM = kOne ? 1 : kP;
-  f32x2 m[kM], scale[kP], beta[kP];
+  f32x2 m[kM], scale[kP];
 #pragma unroll
   for (int j = 0; j < kM; ++j) m[j] = pair_of<kOne ? 2 : kV>(j, [&](int c) { return s.g[0][group_of<kV, kOne>(a, p, c)]; });
 #pragma unroll
-  for (int j = 0; j < kP; ++j) {
-    const float *w = a.gamma + p.c0 + p.v * kV, *c = a.beta + p.c0 + p.v * kV;
-    scale[j] = pair_of<kV>(j, [&](int k) { return p.on ? s.g[1][group_of<kV, kOne>(a, p, k)] * (w[k] + a.offset) : 0.f; });
-    beta[j] = pair_of<kV>(j, [&](int k) { return p.on ? c[k] : 0.f; });
-  }
-  const T* const ptr[1] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV};
-  const long long stride[1] = {a.xsl};
-  T* y = (T*)a.out + p.b * a.osb + p.c0 + p.v * kV;
-  rows<T, kV, 1>(a, p, s, true, ptr, stride, y, a.osl, [&](f32x2(&f)[1][kP], T* at, bool, bool live) {
+  for (int j = 0; j < kP; ++j) scale[j] = mul2(k.w[j], pair_of<kV>(j, [&](int c) { return s.g[1][group_of<kV, kOne>(a, p, c)]; }));
+  walk.run(s, a.mask != nullptr, [&](f32x2(&f)[1][kP], T* at, bool, bool live) {
     f32x2 o[kP];
 #pragma unroll
-    for (int j = 0; j < kP; ++j) o[j] = fma2(sub2(f[0][j], m[kOne ? 0 : j]), scale[j], beta[j]);
+    for (int j = 0; j < kP; ++j) o[j] = fma2(sub2(f[0][j], m[kOne ? 0 : j]), scale[j], k.c[j]);
     if (a.silu) {
 #pragma unroll
       for (int j = 0; j < kP; ++j) o[j] = mul2(o[j], minus_sig2<T>(o[j]) ^ 0x8000000080000000ull);
@@ -414,14 +429,17 @@ __device__ __forceinline__ void fold(const GnArgs& a, int b, int tile, int group
   const int lane = threadIdx.x & 31;
   for (int g = threadIdx.x >> 5; g < groups; g += kThreads / 32) {
     const float* q = a.part + (((long long)b * a.G + tile * a.ng + g) * a.runs) * 3;
-    float n = 0.f, sum = 0.f, dev = 0.f;
-    for (int r = lane; r < a.runs; r += 32) {
+    float n = 0.f, sum = 0.f, dev = 0.f, c0 = 0.f, m0 = 0.f, q0 = 0.f;
+    if (lane < a.runs) c0 = q[3 * lane], m0 = q[3 * lane + 1], q0 = q[3 * lane + 2];
+    n = c0, sum = c0 * m0;
+    for (int r = lane + 32; r < a.runs; r += 32) {
       n += q[3 * r];
       sum = fmaf(q[3 * r], q[3 * r + 1], sum);
     }
     n = warp_sum(n), sum = warp_sum(sum);
     const float mean = n > 0.f ? sum / n : 0.f;
-    for (int r = lane; r < a.runs; r += 32) {
+    if (c0 > 0.f) dev = fmaf(c0 * (m0 - mean), m0 - mean, q0);
+    for (int r = lane + 32; r < a.runs; r += 32) {
       const float d = q[3 * r + 1] - mean;
       if (q[3 * r] > 0.f) dev += fmaf(q[3 * r] * d, d, q[3 * r + 2]);
     }
@@ -436,33 +454,41 @@ __global__ void __launch_bounds__(kThreads, 4) gn_first_kernel(GnArgs a) {
   extern __shared__ __align__(16) char smem[];
   Sums& s = *reinterpret_cast<Sums*>(smem);
   pdl_wait();
-  const Where<kV> p(a, a.first + blockIdx.y, blockIdx.x);
-  read_mask(a, p, s);
-  moments<T, kV, kOne>(a, p, s);
-  if (a.runs == 1) {
-    finish(a, p, s, true);
-    apply<T, kV, kOne>(a, p, s);
-  } else {
-    for (int g = threadIdx.x; g < p.groups; g += kThreads) {
-      float* q = a.part + (((long long)p.b * a.G + p.tile * a.ng + g) * a.runs + p.run) * 3;
-      q[0] = s.g[0][g], q[1] = s.g[1][g], q[2] = s.g[2][g];
-    }
-  }
+  const Where<kV> p(a, false);
+  Walk<T, kV, 1> walk(a, p, s, false, (T*)a.out);
+  walk.begin();
   pdl_next();
+  read_mask(a, p, s);
+  if (a.runs == 1) {
+    Walk<T, kV, 1> again(a, p, s, true, (T*)a.out);
+    moments<T, kV, kOne>(a, p, s, walk, &again);
+    const Params<kV> k(a, p);
+    finish(a, p, s, true);
+    apply<T, kV, kOne>(a, p, s, again, k);
+    return;
+  }
+  moments<T, kV, kOne>(a, p, s, walk, nullptr);
+  for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+    float* q = a.part + (((long long)p.b * a.G + p.tile * a.ng + g) * a.runs + p.run) * 3;
+    q[0] = s.g[0][g], q[1] = s.g[1][g], q[2] = s.g[2][g];
+  }
 }
 
+// (what it reads of the caller's is there before the first pass begins, so its rows are on their way before that has ended)
 template <typename T, int kV, bool kOne>
 __global__ void __launch_bounds__(kThreads, 4) gn_second_kernel(GnArgs a) {
   extern __shared__ __align__(16) char smem[];
   Sums& s = *reinterpret_cast<Sums*>(smem);
-  const int slice = a.slices - 1 - blockIdx.y, run = a.runs - 1 - blockIdx.x;
-  const Where<kV> p(a, a.first + slice, run);
+  const Where<kV> p(a, true);
+  Walk<T, kV, 1> walk(a, p, s, true, (T*)a.out);
+  walk.begin();
+  const Params<kV> k(a, p);
   read_mask(a, p, s);
   pdl_wait();
-  fold(a, p.b, p.tile, p.groups, s);
-  finish(a, p, s, run == 0);
-  apply<T, kV, kOne>(a, p, s);
   pdl_next();
+  fold(a, p.b, p.tile, p.groups, s);
+  finish(a, p, s, p.run == 0);
+  apply<T, kV, kOne>(a, p, s, walk, k);
 }
 
 // ---- backward --------------------------------------------------------------------------------
@@ -480,13 +506,14 @@ struct Back {
   f32x2 m[kM], scale[kP], beta[kP];
   __device__ __forceinline__ Back(const GnArgs& a, const Where<kV>& p) {
     const long long at = (long long)p.b * a.G + p.tile * a.ng;
-    const float *w = a.gamma + p.c0 + p.v * kV, *c = a.beta + p.c0 + p.v * kV, *mean = a.mean + at, *rstd = a.rstd + at;
+    const float *mean = a.mean + at, *rstd = a.rstd + at;
+    const Params<kV> k(a, p);
 #pragma unroll
-    for (int j = 0; j < kM; ++j) m[j] = pair_of<kOne ? 2 : kV>(j, [&](int k) { return mean[group_of<kV, kOne>(a, p, k)]; });
+    for (int j = 0; j < kM; ++j) m[j] = pair_of<kOne ? 2 : kV>(j, [&](int c) { return mean[group_of<kV, kOne>(a, p, c)]; });
 #pragma unroll
     for (int j = 0; j < kP; ++j) {
-      scale[j] = pair_of<kV>(j, [&](int k) { return p.on ? rstd[group_of<kV, kOne>(a, p, k)] * (w[k] + a.offset) : 0.f; });
-      beta[j] = pair_of<kV>(j, [&](int k) { return p.on ? c[k] : 0.f; });
+      scale[j] = mul2(k.w[j], pair_of<kV>(j, [&](int c) { return rstd[group_of<kV, kOne>(a, p, c)]; }));
+      beta[j] = k.c[j];
     }
   }
   // d = x - mean, and minus dz
@@ -508,26 +535,23 @@ struct Back {
 
 // sums of dz and dz xhat of every channel over the block's steps -> a.chan, of dn and dn xhat of every group -> s.g[0], s.g[1]
 template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& s) {
+__device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& s, const Back<T, kV, kOne>& k, Walk<T, kV, 2>& walk,
+                                     Walk<T, kV, 2>* then) {
   constexpr int kP = Vec<T, kV>::kP;
   f32x2 nS[kP], nQ[kP];   // minus the sums of dz and of dz d (xhat being rstd d)
 #pragma unroll
   for (int j = 0; j < kP; ++j) nS[j] = nQ[j] = both(0.f);
-  const T* const ptr[2] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV, (const T*)a.dy + p.b * a.gsb + p.c0 + p.v * kV};
-  const long long stride[2] = {a.xsl, a.gsl};
-  {
-    const Back<T, kV, kOne> k(a, p);
-    rows<T, kV, 2>(a, p, s, false, ptr, stride, (T*)nullptr, 0ll, [&](f32x2(&f)[2][kP], T*, bool, bool live) {
-      if (!live) return;
-      f32x2 d[kP], ndz[kP];
-      k.slopes(a, f[0], f[1], d, ndz);
+  walk.run(s, a.mask != nullptr, [&](f32x2(&f)[2][kP], T*, bool, bool live) {
+    if (!live) return;
+    f32x2 d[kP], ndz[kP];
+    k.slopes(a, f[0], f[1], d, ndz);
 #pragma unroll
-      for (int j = 0; j < kP; ++j) {
-        nS[j] = add2(nS[j], ndz[j]);
-        nQ[j] = fma2(ndz[j], d[j], nQ[j]);
-      }
-    });
-  }
+    for (int j = 0; j < kP; ++j) {
+      nS[j] = add2(nS[j], ndz[j]);
+      nQ[j] = fma2(ndz[j], d[j], nQ[j]);
+    }
+  });
+  if (then) then->begin();
   float S[2 * kP], Q[2 * kP];
 #pragma unroll
   for (int j = 0; j < kP; ++j) {
@@ -544,9 +568,9 @@ __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& 
   }
   __syncthreads();
   // rows of the block: some threads to a channel, each every parts-th row, into that part's row
-  const int parts = min(max(1, kThreads / width), p.lanes);
+  const int parts = min(max(1, quotient(kThreads, 1.f / (float)width)), p.lanes);
   for (int e = threadIdx.x; e < parts * width; e += kThreads) {
-    const int part = e / width, c = e - part * width;
+    const int part = quotient(e, 1.f / (float)width), c = e - part * width;
     float u = 0.f, q = 0.f;
     for (int r = part; r < p.lanes; r += parts) u += s.a[0][r * width + c], q += s.a[1][r * width + c];
     s.a[0][e] = u;
@@ -557,7 +581,7 @@ __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& 
   for (int c = threadIdx.x; c < p.chans; c += kThreads) {
     float u = 0.f, q = 0.f;
     for (int k = 0; k < parts; ++k) u += s.a[0][k * width + c], q += s.a[1][k * width + c];
-    q *= a.rstd[at + c / a.size];
+    q *= a.rstd[at + quotient(c, a.over_size)];
     a.chan[row + p.c0 + c] = u;
     a.chan[row + a.D + p.c0 + c] = q;
     const float w = a.gamma[p.c0 + c] + a.offset;
@@ -577,9 +601,8 @@ __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& 
 
 // sums of dn, dn xhat in s.g[0], s.g[1] -> dx = rstd dn - rstd mean(dn) - d rstd^2 mean(dn xhat)
 template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, Sums& s) {
+__device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, Sums& s, const Back<T, kV, kOne>& k, Walk<T, kV, 2>& walk) {
   constexpr int kP = Vec<T, kV>::kP, kM = kOne ? 1 : kP;
-  const Back<T, kV, kOne> k(a, p);
   const float n = (float)a.count[p.b] * (float)a.size, inv = n > 0.f ? 1.f / n : 0.f;
   const float* rstd = a.rstd + (long long)p.b * a.G + p.tile * a.ng;
   f32x2 m1[kM], m2[kM];   // rstd times the one mean, rstd^2 times the other
@@ -594,10 +617,7 @@ __device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, Sums&
       return s.g[1][g] * inv * rstd[g] * rstd[g];
     });
   }
-  const T* const ptr[2] = {(const T*)a.x + p.b * a.xsb + p.c0 + p.v * kV, (const T*)a.dy + p.b * a.gsb + p.c0 + p.v * kV};
-  const long long stride[2] = {a.xsl, a.gsl};
-  T* dx = (T*)a.out + p.b * a.osb + p.c0 + p.v * kV;
-  rows<T, kV, 2>(a, p, s, true, ptr, stride, dx, a.osl, [&](f32x2(&f)[2][kP], T* at, bool, bool live) {
+  walk.run(s, a.mask != nullptr, [&](f32x2(&f)[2][kP], T* at, bool, bool live) {
     f32x2 d[kP], ndz[kP], o[kP];
     k.slopes(a, f[0], f[1], d, ndz);
 #pragma unroll
@@ -615,29 +635,38 @@ __global__ void __launch_bounds__(kThreads, 3) gn_sums_kernel(GnArgs a) {
   extern __shared__ __align__(16) char smem[];
   Sums& s = *reinterpret_cast<Sums*>(smem);
   pdl_wait();
-  const Where<kV> p(a, a.first + blockIdx.y, blockIdx.x);
-  read_mask(a, p, s);
-  sums<T, kV, kOne>(a, p, s);
-  if (a.runs == 1) {
-    grads<T, kV, kOne>(a, p, s);
-  } else {
-    const long long at = (long long)p.b * a.G + p.tile * a.ng;
-    for (int g = threadIdx.x; g < p.groups; g += kThreads) {
-      float* q = a.part + ((at + g) * a.runs + p.run) * 2;
-      q[0] = s.g[0][g], q[1] = s.g[1][g];
-    }
-  }
+  const Where<kV> p(a, false);
+  Walk<T, kV, 2> walk(a, p, s, false, (T*)a.out);
+  walk.begin();
   pdl_next();
+  const Back<T, kV, kOne> k(a, p);
+  read_mask(a, p, s);
+  if (a.runs == 1) {
+    Walk<T, kV, 2> again(a, p, s, true, (T*)a.out);
+    sums<T, kV, kOne>(a, p, s, k, walk, &again);
+    grads<T, kV, kOne>(a, p, s, k, again);
+    return;
+  }
+  sums<T, kV, kOne>(a, p, s, k, walk, nullptr);
+  const long long at = (long long)p.b * a.G + p.tile * a.ng;
+  for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+    float* q = a.part + ((at + g) * a.runs + p.run) * 2;
+    q[0] = s.g[0][g], q[1] = s.g[1][g];
+  }
 }
 
 template <typename T, int kV, bool kOne>
 __global__ void __launch_bounds__(kThreads, 3) gn_grads_kernel(GnArgs a) {
   extern __shared__ __align__(16) char smem[];
   Sums& s = *reinterpret_cast<Sums*>(smem);
-  const int slice = a.slices - 1 - blockIdx.y, run = a.runs - 1 - blockIdx.x, lane = threadIdx.x & 31;
-  const Where<kV> p(a, a.first + slice, run);
+  const int lane = threadIdx.x & 31;
+  const Where<kV> p(a, true);
+  Walk<T, kV, 2> walk(a, p, s, true, (T*)a.out);
+  walk.begin();
+  const Back<T, kV, kOne> k(a, p);
   read_mask(a, p, s);
   pdl_wait();
+  pdl_next();
   for (int g = threadIdx.x >> 5; g < p.groups; g += kThreads / 32) {
     const float* q = a.part + (((long long)p.b * a.G + p.tile * a.ng + g) * a.runs) * 2;
     float u = 0.f, w = 0.f;
@@ -646,8 +675,7 @@ __global__ void __launch_bounds__(kThreads, 3) gn_grads_kernel(GnArgs a) {
     if (lane == 0) s.g[0][g] = u, s.g[1][g] = w;
   }
   __syncthreads();
-  grads<T, kV, kOne>(a, p, s);
-  pdl_next();
+  grads<T, kV, kOne>(a, p, s, k, walk);
 }
 
 // dgamma, dbeta of 32 channels: the partial results of all sequences and runs, 32 rows at a time
@@ -826,33 +854,31 @@ int check_gn(int dtype, int B, int L, int D, int G, std::initializer_list<const 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 struct Plan {
-  int ng, tiles, steps, runs, piece;   // piece: slices that a pass leaves in L2 for the next
+  int ng, tiles, steps, runs, piece;   // piece: sequences that a pass leaves in L2 for the next
 };
-constexpr long long kL2 = 48ll << 20;   // bytes of inputs that the second pass finds in L2
+constexpr long long kL2 = 200ll << 20;   // bytes of inputs of such a piece
 
 Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
-  const int es = elem_size(dtype), size = D / G, arrays = bwd ? 2 : 1;
+  const int es = elem_size(dtype), size = D / G, arrays = bwd ? 2 : 1, blocks = (bwd ? 3 : 4) * 148;   // (all at once on the device)
+  if (vec == 0) return {G, 1, L, 1, B};
   Plan p;
-  if (vec == 0) return {G, 1, L, 1, 1};
-  // a tile: whole groups and whole vectors, 128 bytes or more of a row where there are as many
+  // a tile: whole groups and whole vectors, 128 bytes or more of a row where there are as many; wider while the device stays full,
+  // as a block's fixed part is worth some ten rows of a thread
   const int unit = vec / gcd(size, vec);
+  auto tiles_of = [&](int ng) { return (G + ng - 1) / ng; };
   p.ng = unit;
   while (p.ng < G && p.ng * size * es < 128) p.ng += unit;
+  while (p.ng < G && 2 * p.ng * size <= kThreads * vec && 2 * p.ng <= kGroups && (long long)B * tiles_of(2 * p.ng) >= blocks) p.ng *= 2;
   while (p.ng > G) p.ng -= unit;
   if (p.ng <= 0) p.ng = G;   // (D is whole vectors: the row is)
-  p.tiles = (G + p.ng - 1) / p.ng;
-  const long long slices = (long long)B * p.tiles, row = (long long)p.ng * size * es * arrays;
-  // a block's run of steps: some 64 KB, fewer where the device would not be full, one run where a sequence is little more
-  long long steps = std::max<long long>(1, (64 << 10) / row);
-  const long long blocks = 4 * 148;
-  if (slices * ((L + steps - 1) / steps) < blocks) steps = std::max<long long>((L * slices + blocks - 1) / blocks, std::max<long long>(1, (8 << 10) / row));
-  if (L <= 2 * steps || (slices >= 296 && L * row <= (256 << 10))) steps = L;
-  const int nv = std::max(1, p.ng * size / vec);
-  steps = std::min<long long>(steps, (long long)kRun * std::max(1, kThreads / nv));
-  p.steps = (int)std::min<long long>(steps, L);
+  p.tiles = tiles_of(p.ng);
+  const long long slices = (long long)B * p.tiles;
+  const int lanes = std::max(1, kThreads / std::max(1, p.ng * size / vec));
+  // runs: as many as fill the device once, of eight rows to a thread at least and kRun at most
+  const long long runs = std::max<long long>(1, std::min<long long>(blocks / slices, L / (8ll * lanes)));
+  p.steps = (int)std::min<long long>((L + runs - 1) / runs, (long long)kRun * lanes);
   p.runs = (L + p.steps - 1) / p.steps;
-  p.piece = (int)std::min<long long>(slices, std::max<long long>(1, kL2 / (row * L)));
-  if (p.runs == 1) p.piece = (int)std::min<long long>(slices, 65535);
+  p.piece = p.runs == 1 ? B : (int)std::min<long long>(B, std::max<long long>(1, kL2 / std::max<long long>(1, (long long)L * D * es * arrays)));
   return p;
 }
 
@@ -870,30 +896,31 @@ int vec_of(int dtype, int D, int G, std::initializer_list<std::pair<const void*,
   return fits(16) ? 16 / es : fits(4) ? 4 / es : fits(es) ? 1 : 0;
 }
 
-void fill(GnArgs& a, const Plan& p) {
+void fill(GnArgs& a, const Plan& p, int vec) {
   a.ng = p.ng, a.tiles = p.tiles, a.steps = p.steps, a.runs = p.runs;
+  if (vec == 0) return;
+  a.nv = p.ng * a.size / vec, a.lanes = kThreads / a.nv;
+  a.over_nv = 1.f / (float)a.nv, a.over_size = 1.f / (float)a.size, a.over_vectors = 1.f / (float)std::max(1, a.size / vec);
 }
 
 // first pass, second pass, piece by piece
 template <typename First, typename Second>
-void passes(First first, Second second, GnArgs a, int slices, int piece, cudaStream_t s) {
-  for (int at = 0; at < slices; at += piece) {
-    a.first = at;
-    a.slices = std::min(piece, slices - at);
-    if (at == 0)
-      launch(first, dim3(a.runs, a.slices), dim3(kThreads), sizeof(Sums), s, a);
+void passes(First first, Second second, GnArgs a, int piece, cudaStream_t s) {
+  for (a.from = 0; a.from < a.B; a.from += piece) {
+    const dim3 grid(a.runs, a.tiles, std::min(piece, a.B - a.from));
+    if (a.from == 0)
+      launch(first, grid, dim3(kThreads), sizeof(Sums), s, a);
     else
-      launch_after(first, dim3(a.runs, a.slices), dim3(kThreads), sizeof(Sums), s, a);
-    if (a.runs > 1) launch_after(second, dim3(a.runs, a.slices), dim3(kThreads), sizeof(Sums), s, a);
+      launch_after(first, grid, dim3(kThreads), sizeof(Sums), s, a);
+    if (a.runs > 1) launch_after(second, grid, dim3(kThreads), sizeof(Sums), s, a);
   }
 }
 template <typename T, int kV, bool kOne>
 void run_one(bool bwd, const GnArgs& a, const Plan& p, cudaStream_t s) {
-  const int slices = a.B * p.tiles, piece = std::min(p.piece, 65535);
   if (bwd)
-    passes(gn_sums_kernel<T, kV, kOne>, gn_grads_kernel<T, kV, kOne>, a, slices, piece, s);
+    passes(gn_sums_kernel<T, kV, kOne>, gn_grads_kernel<T, kV, kOne>, a, p.piece, s);
   else
-    passes(gn_first_kernel<T, kV, kOne>, gn_second_kernel<T, kV, kOne>, a, slices, piece, s);
+    passes(gn_first_kernel<T, kV, kOne>, gn_second_kernel<T, kV, kOne>, a, p.piece, s);
 }
 template <typename T, int kV>
 void run_vec(bool bwd, const GnArgs& a, const Plan& p, cudaStream_t s) {
@@ -954,7 +981,7 @@ extern "C" int mega_group_norm_fwd(const void* x, void* y, int dtype, int B, int
   a.count = (long long*)count, a.mean = mean, a.rstd = rstd, a.part = (float*)work;
   const int vec = vec_of(dtype, D, num_groups, {{x, {xsb, xsl}}, {y, {ysb, ysl}}});
   const Plan p = plan_of(dtype, B, L, D, num_groups, vec, false);
-  fill(a, p);
+  fill(a, p, vec);
   MEGA_DISPATCH_DTYPE(dtype, run_gn<T>(false, vec, a, p, (cudaStream_t)stream));
   return check_launch("group_norm_fwd");
 }
@@ -975,7 +1002,7 @@ extern "C" int mega_group_norm_bwd(const void* dy, const void* x, void* dx, int 
   a.dgamma = dgamma, a.dbeta = dbeta;
   const int vec = vec_of(dtype, D, num_groups, {{dy, {gsb, gsl}}, {x, {xsb, xsl}}, {dx, {dsb, dsl}}});
   const Plan p = plan_of(dtype, B, L, D, num_groups, vec, true);
-  fill(a, p);
+  fill(a, p, vec);
   a.chan = (float*)work, a.part = a.chan + (size_t)B * p.runs * 2 * D;
   MEGA_DISPATCH_DTYPE(dtype, run_gn<T>(true, vec, a, p, (cudaStream_t)stream));
   launch_after(gn_params_kernel, dim3((D + 31) / 32), dim3(1024), 0, stream, a);
