@@ -156,13 +156,14 @@ struct Where {
 
 // Shared memory: every thread's own ring of vectors that are on their way, the block's sums.
 constexpr int kRing = 32 << 10;   // bytes of the ring: eight rows of one operand, four of two
+constexpr int kHeld = 16;         // vectors that a thread keeps where a cluster holds a sequence
 struct Sums {
-  char ring[kRing];
   float a[2][kThreads * 8];   // [row of the block][channel of the tile]
   float n[kThreads];
   float g[3][kGroups];        // of a group: mean, rstd; backward the two sums
   unsigned bits[kRun * kThreads / 32];   // padded steps of the block
 };
+constexpr int kPlaces = (sizeof(Sums) + 15) / 16 * 16;   // behind it the ring, or what is held
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -195,8 +196,8 @@ struct Walk {
   long long hop[kOps], next;
   T* at;
   int mine, start, step, ahead = 0;
-  uint32_t own;
-  __device__ __forceinline__ Walk(const GnArgs& a, const Where<kV>& p, Sums& s, bool back, T* out) {
+  const char* own;
+  __device__ __forceinline__ Walk(const GnArgs& a, const Where<kV>& p, char* place, bool back, T* out) {
     const int total = p.t1 - p.t0;
     mine = p.on && p.r < total ? quotient(total - p.r + p.lanes - 1, 1.f / (float)p.lanes) : 0;   // (at most kRun)
     start = back ? p.r + (mine - 1) * p.lanes : p.r, step = back ? -p.lanes : p.lanes;
@@ -204,14 +205,14 @@ struct Walk {
     q[0] = (const T*)a.x + p.b * a.xsb + (p.t0 + start) * a.xsl + c, hop[0] = step * a.xsl;
     if (kOps == 2) q[kOps - 1] = (const T*)a.dy + p.b * a.gsb + (p.t0 + start) * a.gsl + c, hop[kOps - 1] = step * a.gsl;
     at = out + p.b * a.osb + (p.t0 + start) * a.osl + c, next = step * a.osl;
-    own = smem_u32(s.ring) + threadIdx.x * 16;
+    own = place + threadIdx.x * 16;
   }
   __device__ __forceinline__ void fetch(int u) {   // the next row, into place u
     if constexpr (V::kBytes != 2) {
       if (ahead < mine) {
 #pragma unroll
         for (int o = 0; o < kOps; ++o) {
-          V::fetch(own + (u * kOps + o) * (kThreads * 16), q[o]);
+          V::fetch(smem_u32(own) + (u * kOps + o) * (kThreads * 16), q[o]);
           q[o] += hop[o];
         }
       }
@@ -252,7 +253,7 @@ struct Walk {
         asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
         f32x2 w[kOps][kP];
 #pragma unroll
-        for (int o = 0; o < kOps; ++o) V::read(s.ring + threadIdx.x * 16 + (u * kOps + o) * (kThreads * 16), w[o]);
+        for (int o = 0; o < kOps; ++o) V::read(own + (u * kOps + o) * (kThreads * 16), w[o]);
         f(w, at, k == 0, live(k));
         at += next;
       };
@@ -274,13 +275,87 @@ struct Walk {
   }
 };
 
+// The same with every row kept: a block's steps are what its threads' places hold, and rows are there for a second run.
+template <typename T, int kV, int kOps>
+struct Held {
+  using V = Vec<T, kV>;
+  static constexpr int kP = V::kP, kRows = kHeld / kOps;
+  int mine, start, step;
+  T* at;
+  long long next;
+  const char* own;
+  // (a thread's rows lie next to one another: only the places of one row are a whole block apart)
+  __device__ __forceinline__ Held(const GnArgs& a, const Where<kV>& p, char* place, T* out) {
+    const int total = p.t1 - p.t0, c = p.c0 + p.v * kV;
+    mine = p.on && p.r < total ? quotient(total - p.r + p.lanes - 1, 1.f / (float)p.lanes) : 0;   // (at most kRows)
+    start = p.r, step = p.lanes;
+    own = place + threadIdx.x * 16;
+    const T *x = (const T*)a.x + p.b * a.xsb + (p.t0 + start) * a.xsl + c, *dy = nullptr;
+    if (kOps == 2) dy = (const T*)a.dy + p.b * a.gsb + (p.t0 + start) * a.gsl + c;
+    const uint32_t to = smem_u32(own);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (k < mine) {
+        V::fetch(to + k * kOps * (kThreads * 16), x);
+        x += step * a.xsl;
+        if (kOps == 2) {
+          V::fetch(to + (k * kOps + 1) * (kThreads * 16), dy);
+          dy += step * a.gsl;
+        }
+      }
+      if (k % 4 == 3 || k == kRows - 1) asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    at = out + p.b * a.osb + (p.t0 + start) * a.osl + c, next = step * a.osl;
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(const Sums& s, bool masked, int from, F&& f) {
+#pragma unroll 2
+    for (int k = from; k < min(from + 4, mine); ++k) {
+      f32x2 w[kOps][kP];
+#pragma unroll
+      for (int o = 0; o < kOps; ++o) V::read(own + (k * kOps + o) * (kThreads * 16), w[o]);
+      const int i = start + k * step;
+      f(w, at + k * next, k == 0, !(masked && ((s.bits[i >> 5] >> (i & 31)) & 1u)));
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void run(const Sums& s, bool masked, F&& f) {
+    static_assert(kRows <= 16, "");
+    asm volatile("cp.async.wait_group %0;" ::"n"((kRows + 3) / 4 - 1) : "memory");
+    each(s, masked, 0, f);
+    if (kRows > 4) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRows > 4 ? (kRows + 3) / 4 - 2 : 0) : "memory");
+      each(s, masked, 4, f);
+    }
+    if (kRows > 8) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRows > 8 ? (kRows + 3) / 4 - 3 : 0) : "memory");
+      each(s, masked, 8, f);
+    }
+    if (kRows > 12) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRows > 12 ? (kRows + 3) / 4 - 4 : 0) : "memory");
+      each(s, masked, 12, f);
+    }
+  }
+};
+
+// the blocks of a cluster, which share a sequence's steps
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float peer(const float* p, int rank) {   // a float of another block's shared memory
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
 // ---- forward -----------------------------------------------------------------------------------
 // Statistics of n values, means m[k] of counts c[k] and squared deviations q[k]: mean = sum c m / n, then sum q + c (m - mean)^2.
 //
 // Of the tile's groups over the block's steps -> s.g: steps, mean, squared deviations of all channels over their number.
 // kOne: a vector lies in one group; its values are then one entry.
-template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sums& s, Walk<T, kV, 1>& walk, Walk<T, kV, 1>* then) {
+template <typename T, int kV, bool kOne, typename W>
+__device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sums& s, W& walk, Walk<T, kV, 1>* then) {
   constexpr int kE = kOne ? 1 : kV, kP = Vec<T, kV>::kP;   // entries that a thread leaves, pairs
   float cnt = 0.f;
   f32x2 pv[kP], S[kP], Q[kP];
@@ -400,8 +475,8 @@ struct Params {
   }
 };
 
-template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, Sums& s, Walk<T, kV, 1>& walk, const Params<kV>& k) {
+template <typename T, int kV, bool kOne, typename W>
+__device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, Sums& s, W& walk, const Params<kV>& k) {
   constexpr int kP = Vec<T, kV>::kP, kM = kOne ? 1 : kP;
   f32x2 m[kM], scale[kP];
 #pragma unroll
@@ -455,12 +530,12 @@ __global__ void __launch_bounds__(kThreads, 4) gn_first_kernel(GnArgs a) {
   Sums& s = *reinterpret_cast<Sums*>(smem);
   pdl_wait();
   const Where<kV> p(a, false);
-  Walk<T, kV, 1> walk(a, p, s, false, (T*)a.out);
+  Walk<T, kV, 1> walk(a, p, smem + kPlaces, false, (T*)a.out);
   walk.begin();
   pdl_next();
   read_mask(a, p, s);
   if (a.runs == 1) {
-    Walk<T, kV, 1> again(a, p, s, true, (T*)a.out);
+    Walk<T, kV, 1> again(a, p, smem + kPlaces, true, (T*)a.out);
     moments<T, kV, kOne>(a, p, s, walk, &again);
     const Params<kV> k(a, p);
     finish(a, p, s, true);
@@ -480,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_second_kernel(GnArgs a) {
   extern __shared__ __align__(16) char smem[];
   Sums& s = *reinterpret_cast<Sums*>(smem);
   const Where<kV> p(a, true);
-  Walk<T, kV, 1> walk(a, p, s, true, (T*)a.out);
+  Walk<T, kV, 1> walk(a, p, smem + kPlaces, true, (T*)a.out);
   walk.begin();
   const Params<kV> k(a, p);
   read_mask(a, p, s);
@@ -489,6 +564,43 @@ __global__ void __launch_bounds__(kThreads, 4) gn_second_kernel(GnArgs a) {
   fold(a, p.b, p.tile, p.groups, s);
   finish(a, p, s, p.run == 0);
   apply<T, kV, kOne>(a, p, s, walk, k);
+}
+
+// In one pass: a cluster's blocks hold the sequence's steps of the tile, and tell one another their statistics.
+template <typename T, int kV>
+__global__ void __launch_bounds__(kThreads, 3) gn_held_kernel(GnArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  Sums& s = *reinterpret_cast<Sums*>(smem);
+  const Where<kV> p(a, false);
+  Held<T, kV, 1> rows(a, p, smem + kPlaces, (T*)a.out);
+  const Params<kV> k(a, p);
+  read_mask(a, p, s);
+  moments<T, kV, true>(a, p, s, rows, nullptr);
+  if (a.runs > 1) {
+    cluster_arrive();
+    cluster_wait();
+    const int g = threadIdx.x;
+    float n = 0.f, sum = 0.f, dev = 0.f;
+    if (g < p.groups) {
+      for (int r = 0; r < a.runs; ++r) {
+        const float c = peer(&s.g[0][g], r);
+        n += c;
+        sum = fmaf(c, peer(&s.g[1][g], r), sum);
+      }
+      const float mean = n > 0.f ? sum / n : 0.f;
+      for (int r = 0; r < a.runs; ++r) {
+        const float c = peer(&s.g[0][g], r), d = peer(&s.g[1][g], r) - mean;
+        if (c > 0.f) dev += fmaf(c * d, d, peer(&s.g[2][g], r));
+      }
+      sum = mean;
+    }
+    cluster_arrive();   // (all have read)
+    cluster_wait();
+    if (g < p.groups) s.g[0][g] = n, s.g[1][g] = sum, s.g[2][g] = dev;
+    __syncthreads();
+  }
+  finish(a, p, s, p.run == 0);
+  apply<T, kV, true>(a, p, s, rows, k);
 }
 
 // ---- backward --------------------------------------------------------------------------------
@@ -534,9 +646,8 @@ struct Back {
 };
 
 // sums of dz and dz xhat of every channel over the block's steps -> a.chan, of dn and dn xhat of every group -> s.g[0], s.g[1]
-template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& s, const Back<T, kV, kOne>& k, Walk<T, kV, 2>& walk,
-                                     Walk<T, kV, 2>* then) {
+template <typename T, int kV, bool kOne, typename W>
+__device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& s, const Back<T, kV, kOne>& k, W& walk, Walk<T, kV, 2>* then) {
   constexpr int kP = Vec<T, kV>::kP;
   f32x2 nS[kP], nQ[kP];   // minus the sums of dz and of dz d (xhat being rstd d)
 #pragma unroll
@@ -600,8 +711,8 @@ __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& 
 }
 
 // sums of dn, dn xhat in s.g[0], s.g[1] -> dx = rstd dn - rstd mean(dn) - d rstd^2 mean(dn xhat)
-template <typename T, int kV, bool kOne>
-__device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, Sums& s, const Back<T, kV, kOne>& k, Walk<T, kV, 2>& walk) {
+template <typename T, int kV, bool kOne, typename W>
+__device__ __forceinline__ void grads(const GnArgs& a, const Where<kV>& p, Sums& s, const Back<T, kV, kOne>& k, W& walk) {
   constexpr int kP = Vec<T, kV>::kP, kM = kOne ? 1 : kP;
   const float n = (float)a.count[p.b] * (float)a.size, inv = n > 0.f ? 1.f / n : 0.f;
   const float* rstd = a.rstd + (long long)p.b * a.G + p.tile * a.ng;
@@ -636,13 +747,13 @@ __global__ void __launch_bounds__(kThreads, 3) gn_sums_kernel(GnArgs a) {
   Sums& s = *reinterpret_cast<Sums*>(smem);
   pdl_wait();
   const Where<kV> p(a, false);
-  Walk<T, kV, 2> walk(a, p, s, false, (T*)a.out);
+  Walk<T, kV, 2> walk(a, p, smem + kPlaces, false, (T*)a.out);
   walk.begin();
   pdl_next();
   const Back<T, kV, kOne> k(a, p);
   read_mask(a, p, s);
   if (a.runs == 1) {
-    Walk<T, kV, 2> again(a, p, s, true, (T*)a.out);
+    Walk<T, kV, 2> again(a, p, smem + kPlaces, true, (T*)a.out);
     sums<T, kV, kOne>(a, p, s, k, walk, &again);
     grads<T, kV, kOne>(a, p, s, k, again);
     return;
@@ -661,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 3) gn_grads_kernel(GnArgs a) {
   Sums& s = *reinterpret_cast<Sums*>(smem);
   const int lane = threadIdx.x & 31;
   const Where<kV> p(a, true);
-  Walk<T, kV, 2> walk(a, p, s, true, (T*)a.out);
+  Walk<T, kV, 2> walk(a, p, smem + kPlaces, true, (T*)a.out);
   walk.begin();
   const Back<T, kV, kOne> k(a, p);
   read_mask(a, p, s);
@@ -676,6 +787,31 @@ __global__ void __launch_bounds__(kThreads, 3) gn_grads_kernel(GnArgs a) {
   }
   __syncthreads();
   grads<T, kV, kOne>(a, p, s, k, walk);
+}
+
+template <typename T, int kV>
+__global__ void __launch_bounds__(kThreads, 3) gn_held_back_kernel(GnArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  Sums& s = *reinterpret_cast<Sums*>(smem);
+  const Where<kV> p(a, false);
+  Held<T, kV, 2> rows(a, p, smem + kPlaces, (T*)a.out);
+  pdl_next();
+  const Back<T, kV, true> k(a, p);
+  read_mask(a, p, s);
+  sums<T, kV, true>(a, p, s, k, rows, nullptr);
+  if (a.runs > 1) {
+    cluster_arrive();
+    cluster_wait();
+    const int g = threadIdx.x;
+    float u = 0.f, q = 0.f;
+    if (g < p.groups)
+      for (int r = 0; r < a.runs; ++r) u += peer(&s.g[0][g], r), q += peer(&s.g[1][g], r);
+    cluster_arrive();   // (all have read)
+    cluster_wait();
+    if (g < p.groups) s.g[0][g] = u, s.g[1][g] = q;
+    __syncthreads();
+  }
+  grads<T, kV, true>(a, p, s, k, rows);
 }
 
 // dgamma, dbeta of 32 channels: the partial results of all sequences and runs, 32 rows at a time
@@ -855,13 +991,33 @@ int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 struct Plan {
   int ng, tiles, steps, runs, piece;   // piece: sequences that a pass leaves in L2 for the next
+  bool held;                           // in one pass, the runs of a sequence a cluster
 };
+constexpr int kHeldRow = 64;   // bytes of a row of a held tile at least
 constexpr long long kL2 = 200ll << 20;   // bytes of inputs of such a piece
 
 Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
   const int es = elem_size(dtype), size = D / G, arrays = bwd ? 2 : 1, blocks = (bwd ? 3 : 4) * 148;   // (all at once on the device)
-  if (vec == 0) return {G, 1, L, 1, B};
+  if (vec == 0) return {G, 1, L, 1, B, false};
   Plan p;
+  p.held = false;
+  if (vec * es == 16 && size % vec == 0) {
+    // Held in one pass where eight blocks hold a sequence's steps of a tile of 64 bytes or more; wider tiles as long as no further
+    // block is needed for them and the device stays full.
+    const int places = kHeld / arrays;
+    auto lanes_of = [&](int ng) { return kThreads / (ng * size / vec); };
+    auto blocks_of = [&](int ng) { return (L + places * lanes_of(ng) - 1) / (places * lanes_of(ng)); };
+    int ng = 1;
+    while (ng < G && ng * size * es < kHeldRow) ++ng;
+    if (ng * size <= kThreads * vec && blocks_of(ng) <= 8) {
+      while (2 * ng <= G && 2 * ng * size <= kThreads * vec && blocks_of(2 * ng) == blocks_of(ng) &&
+             (long long)B * ((G + 2 * ng - 1) / (2 * ng)) * blocks_of(ng) >= 3 * 148)
+        ng *= 2;
+      p.ng = ng, p.tiles = (G + ng - 1) / ng, p.runs = blocks_of(ng), p.piece = B, p.held = true;
+      p.steps = (L + p.runs - 1) / p.runs;
+      return p;
+    }
+  }
   // a tile: whole groups and whole vectors, 128 bytes or more of a row where there are as many; wider while the device stays full,
   // as a block's fixed part is worth some ten rows of a thread
   const int unit = vec / gcd(size, vec);
@@ -909,10 +1065,10 @@ void passes(First first, Second second, GnArgs a, int piece, cudaStream_t s) {
   for (a.from = 0; a.from < a.B; a.from += piece) {
     const dim3 grid(a.runs, a.tiles, std::min(piece, a.B - a.from));
     if (a.from == 0)
-      launch(first, grid, dim3(kThreads), sizeof(Sums), s, a);
+      launch(first, grid, dim3(kThreads), kPlaces + kRing, s, a);
     else
-      launch_after(first, grid, dim3(kThreads), sizeof(Sums), s, a);
-    if (a.runs > 1) launch_after(second, grid, dim3(kThreads), sizeof(Sums), s, a);
+      launch_after(first, grid, dim3(kThreads), kPlaces + kRing, s, a);
+    if (a.runs > 1) launch_after(second, grid, dim3(kThreads), kPlaces + kRing, s, a);
   }
 }
 template <typename T, int kV, bool kOne>
@@ -922,9 +1078,29 @@ void run_one(bool bwd, const GnArgs& a, const Plan& p, cudaStream_t s) {
   else
     passes(gn_first_kernel<T, kV, kOne>, gn_second_kernel<T, kV, kOne>, a, p.piece, s);
 }
+template <typename Kernel>
+void launch_held(Kernel kernel, const GnArgs& a, cudaStream_t s) {
+  const size_t smem = kPlaces + kHeld * kThreads * 16;
+  allow_smem(reinterpret_cast<const void*>(kernel), smem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.runs, a.tiles, a.B);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = a.runs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, a);
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  g_last_kernel.store("group_norm_held", std::memory_order_relaxed);
+}
 template <typename T, int kV>
 void run_vec(bool bwd, const GnArgs& a, const Plan& p, cudaStream_t s) {
   if constexpr (kV * sizeof(T) == 16) {
+    if (p.held) return launch_held(bwd ? gn_held_back_kernel<T, kV> : gn_held_kernel<T, kV>, a, s);
     if (a.size % kV == 0) return run_one<T, kV, true>(bwd, a, p, s);
   }
   run_one<T, kV, kV == 1>(bwd, a, p, s);
