@@ -26,6 +26,7 @@
 
 #include "common.cuh"
 #include "gated_recurrence.cuh"
+#include "gates.cuh"
 #include "tma.cuh"
 
 namespace mega {
@@ -107,38 +108,23 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+__device__ __forceinline__ f32x2 neg2(f32x2 v) { return v ^ 0x8000000080000000ull; }
+
 // -sigmoid(-f): minus the leak
 template <typename T>
-__device__ __forceinline__ float minus_leak(float f) {
-  return sizeof(T) == 4 ? -1.f / (1.f + expf(f)) : rcp_approx(-1.f - __expf(f));
-}
-template <typename T>
 __device__ __forceinline__ f32x2 minus_leak2(f32x2 f) {
-  float a, b;
-  if (sizeof(T) == 4) {
-    unpack2(f, a, b);
-    return pack2(minus_leak<T>(a), minus_leak<T>(b));
-  }
-  unpack2(mul2(f, pack2(1.4426950408889634f, 1.4426950408889634f)), a, b);   // e^f = 2^(f / ln 2)
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-  unpack2(fma2(pack2(a, b), pack2(-1.f, -1.f), pack2(-1.f, -1.f)), a, b);
-  return pack2(rcp_approx(a), rcp_approx(b));
+  return minus_sigmoid2<T, 1>(f);
 }
 // sigmoid(i), and sigmoid(i) sigmoid(-i) where the caller asks for it
 template <typename T, bool kSlope>
-__device__ __forceinline__ float gate_one(float i, float& slope) {
-  const float e = exp_of<T>(-i), s = sizeof(T) == 4 ? 1.f / (1.f + e) : rcp_approx(1.f + e);
-  if (kSlope) slope = s * (fminf(e, 3.4e38f) * s);   // (e s = sigmoid(-i); an infinite e comes with s = 0)
-  return s;
-}
-template <typename T, bool kSlope>
 __device__ __forceinline__ f32x2 gate2(f32x2 i, f32x2& slope) {
-  float a, b, p = 0.f, q = 0.f;
-  unpack2(i, a, b);
-  const f32x2 s = pack2(gate_one<T, kSlope>(a, p), gate_one<T, kSlope>(b, q));
-  if (kSlope) slope = pack2(p, q);
-  return s;
+  const f32x2 e = exp_pair<T, -1>(i), ns = minus_over_one_and(e);
+  if (kSlope) {   // s (e s): 1 - s would lose what there is of it when the gate stands open; an infinite e comes with s = 0
+    float a, b;
+    unpack2(e, a, b);
+    slope = mul2(mul2(pack2(fminf(a, 3.4e38f), fminf(b, 3.4e38f)), ns), ns);
+  }
+  return neg2(ns);
 }
 
 // two neighbouring values of shared memory
@@ -188,7 +174,6 @@ __device__ __forceinline__ void put(__half* p, f32x2 v, int n) {
     if (n > 1) p[1] = __float2half_rn(b);
   }
 }
-__device__ __forceinline__ f32x2 neg2(f32x2 v) { return v ^ 0x8000000080000000ull; }
 __device__ __forceinline__ f32x2 minus_zero() { return 0x8000000080000000ull; }
 
 __device__ __forceinline__ f32x2 get_state(const float* p, int n, bool pairs) {
@@ -605,9 +590,9 @@ __global__ void __launch_bounds__(128) rec_step_kernel(RecArgs a) {
   if (d >= a.D) return;
   const long long at = (long long)b * a.D + d;
   const float h = a.h_in ? a.h_in[at] : 0.f, x = Elem<T>::ld((const T*)a.x + b * a.xsb + d);
-  const float nl = minus_leak<T>(Elem<T>::ld((const T*)a.f + b * a.fsb + d));
-  float none;
-  const float v = a.i ? fmaf(nl, h, fmaf(gate_one<T, false>(Elem<T>::ld((const T*)a.i + b * a.isb + d), none), x, h)) : fmaf(nl, h - x, h);
+  float nl, ns;   // (the input gate beside the leak)
+  unpack2(minus_sigmoid2<T, 1>(pack2(Elem<T>::ld((const T*)a.f + b * a.fsb + d), a.i ? -Elem<T>::ld((const T*)a.i + b * a.isb + d) : 0.f)), nl, ns);
+  const float v = a.i ? fmaf(nl, h, fmaf(-ns, x, h)) : fmaf(nl, h - x, h);
   Elem<T>::st((T*)a.y + b * a.ysb + d, v);
   a.h_out[at] = v;
 }

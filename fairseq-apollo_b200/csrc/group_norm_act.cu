@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "gates.cuh"
 #include "tma.cuh"
 
 namespace mega {
@@ -115,21 +116,6 @@ template <typename T>
 __device__ __forceinline__ float sig(float z) {
   return sizeof(T) == 4 ? 1.f / (1.f + expf(-z)) : rcp_approx(1.f + __expf(-z));
 }
-// minus the sigmoids of a pair
-template <typename T>
-__device__ __forceinline__ f32x2 minus_sig2(f32x2 z) {
-  float a, b;
-  if (sizeof(T) == 4) {
-    unpack2(z, a, b);
-    return pack2(-1.f / (1.f + expf(-a)), -1.f / (1.f + expf(-b)));
-  }
-  unpack2(mul2(z, both(-1.4426950408889634f)), a, b);   // e^-z = 2^(-z / ln 2)
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-  unpack2(fma2(pack2(a, b), both(-1.f), both(-1.f)), a, b);
-  return pack2(rcp_approx(a), rcp_approx(b));
-}
-
 // a / b for 0 <= a < 2^16 and b's reciprocal (off by less than 2^-23 of it: the half keeps the quotient on its side)
 __device__ __forceinline__ int quotient(int a, float over) { return __float2int_rd(((float)a + 0.5f) * over); }
 
@@ -156,14 +142,15 @@ struct Where {
 
 // Shared memory: every thread's own ring of vectors that are on their way, the block's sums.
 constexpr int kRing = 32 << 10;   // bytes of the ring: eight rows of one operand, four of two
-constexpr int kHeld = 16;         // vectors that a thread keeps where a cluster holds a sequence
+constexpr int kHeld = 16, kHeldBack = 12;   // vectors that a thread keeps where a cluster holds a sequence: three blocks fit a multiprocessor
 struct Sums {
-  float a[2][kThreads * 8];   // [row of the block][channel of the tile]
   float n[kThreads];
   float g[3][kGroups];        // of a group: mean, rstd; backward the two sums
   unsigned bits[kRun * kThreads / 32];   // padded steps of the block
+  float a[2 * kThreads * 8];   // two arrays [row of the block][channel of the tile] (or vector, where it is one entry)
 };
-constexpr int kPlaces = (sizeof(Sums) + 15) / 16 * 16;   // behind it the ring, or what is held
+// behind it the ring, or what is held; a forward pass of one entry to a vector needs an eighth of the arrays
+constexpr int kPlaces = (sizeof(Sums) + 15) / 16 * 16, kFewer = kPlaces - 2 * kThreads * 7 * (int)sizeof(float);
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -279,62 +266,69 @@ struct Walk {
 template <typename T, int kV, int kOps>
 struct Held {
   using V = Vec<T, kV>;
-  static constexpr int kP = V::kP, kRows = kHeld / kOps;
+  static constexpr int kP = V::kP, kRows = (kOps == 1 ? kHeld : kHeldBack) / kOps, kSteps = (kRows + 3) / 4;
   int mine, start, step;
-  T* at;
+  T* to;
   long long next;
   const char* own;
-  // (a thread's rows lie next to one another: only the places of one row are a whole block apart)
   __device__ __forceinline__ Held(const GnArgs& a, const Where<kV>& p, char* place, T* out) {
     const int total = p.t1 - p.t0, c = p.c0 + p.v * kV;
     mine = p.on && p.r < total ? quotient(total - p.r + p.lanes - 1, 1.f / (float)p.lanes) : 0;   // (at most kRows)
     start = p.r, step = p.lanes;
     own = place + threadIdx.x * 16;
     const T *x = (const T*)a.x + p.b * a.xsb + (p.t0 + start) * a.xsl + c, *dy = nullptr;
+    const long long hx = step * a.xsl, hy = kOps == 2 ? step * a.gsl : 0;
     if (kOps == 2) dy = (const T*)a.dy + p.b * a.gsb + (p.t0 + start) * a.gsl + c;
-    const uint32_t to = smem_u32(own);
+    const uint32_t at = smem_u32(own);
+    auto row = [&](int k) {
+      V::fetch(at + k * kOps * (kThreads * 16), x);
+      x += hx;
+      if (kOps == 2) {
+        V::fetch(at + (k * kOps + 1) * (kThreads * 16), dy);
+        dy += hy;
+      }
+    };
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      if (k < mine) {
-        V::fetch(to + k * kOps * (kThreads * 16), x);
-        x += step * a.xsl;
-        if (kOps == 2) {
-          V::fetch(to + (k * kOps + 1) * (kThreads * 16), dy);
-          dy += step * a.gsl;
+    for (int q = 0; q < kSteps; ++q) {
+      if (mine >= min(4 * q + 4, kRows)) {
+#pragma unroll
+        for (int k = 4 * q; k < min(4 * q + 4, kRows); ++k) row(k);
+      } else {
+        for (int k = 4 * q; k < mine; ++k) row(k);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    to = out + p.b * a.osb + (p.t0 + start) * a.osl + c, next = step * a.osl;
+  }
+  template <int kQ, typename F>
+  __device__ __forceinline__ void quarter(const Sums& s, bool masked, T*& at, F&& f) {
+    if constexpr (kQ < kSteps) {
+      constexpr int kEnd = 4 * kQ + 4 < kRows ? 4 * kQ + 4 : kRows;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kSteps - 1 - kQ) : "memory");
+      auto use = [&](int k, bool live) {
+        f32x2 w[kOps][kP];
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) V::read(own + (k * kOps + o) * (kThreads * 16), w[o]);
+        f(w, at, k == 0, live);
+        at += next;
+      };
+      if (mine >= kEnd && !masked) {
+#pragma unroll
+        for (int k = 4 * kQ; k < kEnd; ++k) use(k, true);
+      } else {
+#pragma unroll 1
+        for (int k = 4 * kQ; k < min(kEnd, mine); ++k) {
+          const int i = start + k * step;
+          use(k, !(masked && ((s.bits[i >> 5] >> (i & 31)) & 1u)));
         }
       }
-      if (k % 4 == 3 || k == kRows - 1) asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    at = out + p.b * a.osb + (p.t0 + start) * a.osl + c, next = step * a.osl;
-  }
-  template <typename F>
-  __device__ __forceinline__ void each(const Sums& s, bool masked, int from, F&& f) {
-#pragma unroll 2
-    for (int k = from; k < min(from + 4, mine); ++k) {
-      f32x2 w[kOps][kP];
-#pragma unroll
-      for (int o = 0; o < kOps; ++o) V::read(own + (k * kOps + o) * (kThreads * 16), w[o]);
-      const int i = start + k * step;
-      f(w, at + k * next, k == 0, !(masked && ((s.bits[i >> 5] >> (i & 31)) & 1u)));
+      quarter<kQ + 1>(s, masked, at, f);
     }
   }
   template <typename F>
   __device__ __forceinline__ void run(const Sums& s, bool masked, F&& f) {
-    static_assert(kRows <= 16, "");
-    asm volatile("cp.async.wait_group %0;" ::"n"((kRows + 3) / 4 - 1) : "memory");
-    each(s, masked, 0, f);
-    if (kRows > 4) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRows > 4 ? (kRows + 3) / 4 - 2 : 0) : "memory");
-      each(s, masked, 4, f);
-    }
-    if (kRows > 8) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRows > 8 ? (kRows + 3) / 4 - 3 : 0) : "memory");
-      each(s, masked, 8, f);
-    }
-    if (kRows > 12) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRows > 12 ? (kRows + 3) / 4 - 4 : 0) : "memory");
-      each(s, masked, 12, f);
-    }
+    T* at = to;
+    quarter<0>(s, masked, at, f);
   }
 };
 
@@ -356,7 +350,7 @@ __device__ __forceinline__ float peer(const float* p, int rank) {   // a float o
 // kOne: a vector lies in one group; its values are then one entry.
 template <typename T, int kV, bool kOne, typename W>
 __device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sums& s, W& walk, Walk<T, kV, 1>* then) {
-  constexpr int kE = kOne ? 1 : kV, kP = Vec<T, kV>::kP;   // entries that a thread leaves, pairs
+  constexpr int kE = kOne ? 1 : kV, kP = Vec<T, kV>::kP, kPlane = kThreads * kE;   // entries that a thread leaves, pairs
   float cnt = 0.f;
   f32x2 pv[kP], S[kP], Q[kP];
 #pragma unroll
@@ -398,8 +392,8 @@ __device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sum
     }
 #pragma unroll
     for (int j = 0; j < kE; ++j) {
-      s.a[0][p.r * width + p.v * kE + j] = m[j];
-      s.a[1][p.r * width + p.v * kE + j] = q[j];
+      s.a[p.r * width + p.v * kE + j] = m[j];
+      s.a[kPlane + p.r * width + p.v * kE + j] = q[j];
     }
     if (p.v == 0) s.n[p.r] = cnt;
   }
@@ -414,13 +408,13 @@ __device__ __forceinline__ void moments(const GnArgs& a, const Where<kV>& p, Sum
     float sum = 0.f, dev = 0.f;
     for (int e = lane; e < p.lanes * per; e += 32) {
       const int r = quotient(e, over_per);
-      sum = fmaf(s.n[r], s.a[0][r * width + g * per + e - r * per], sum);
+      sum = fmaf(s.n[r], s.a[r * width + g * per + e - r * per], sum);
     }
     const float mean = warp_sum(sum) * over;
     for (int e = lane; e < p.lanes * per; e += 32) {
       const int r = quotient(e, over_per), at = r * width + g * per + e - r * per;
-      const float d = s.a[0][at] - mean, c = s.n[r] * (float)(kV / kE);
-      if (c > 0.f) dev += fmaf(c * d, d, s.a[1][at]);   // (an empty row has no mean)
+      const float d = s.a[at] - mean, c = s.n[r] * (float)(kV / kE);
+      if (c > 0.f) dev += fmaf(c * d, d, s.a[kPlane + at]);   // (an empty row has no mean)
     }
     dev = warp_sum(dev);
     if (lane == 0) {
@@ -489,7 +483,7 @@ __device__ __forceinline__ void apply(const GnArgs& a, const Where<kV>& p, Sums&
     for (int j = 0; j < kP; ++j) o[j] = fma2(sub2(f[0][j], m[kOne ? 0 : j]), scale[j], k.c[j]);
     if (a.silu) {
 #pragma unroll
-      for (int j = 0; j < kP; ++j) o[j] = mul2(o[j], minus_sig2<T>(o[j]) ^ 0x8000000080000000ull);
+      for (int j = 0; j < kP; ++j) o[j] = mul2(o[j], minus_sigmoid2<T, -1>(o[j]) ^ 0x8000000080000000ull);
     }
     if (!live) {
 #pragma unroll
@@ -572,31 +566,25 @@ __global__ void __launch_bounds__(kThreads, 3) gn_held_kernel(GnArgs a) {
   extern __shared__ __align__(16) char smem[];
   Sums& s = *reinterpret_cast<Sums*>(smem);
   const Where<kV> p(a, false);
-  Held<T, kV, 1> rows(a, p, smem + kPlaces, (T*)a.out);
+  Held<T, kV, 1> rows(a, p, smem + kFewer, (T*)a.out);
   const Params<kV> k(a, p);
   read_mask(a, p, s);
   moments<T, kV, true>(a, p, s, rows, nullptr);
   if (a.runs > 1) {
     cluster_arrive();
     cluster_wait();
-    const int g = threadIdx.x;
-    float n = 0.f, sum = 0.f, dev = 0.f;
-    if (g < p.groups) {
-      for (int r = 0; r < a.runs; ++r) {
-        const float c = peer(&s.g[0][g], r);
-        n += c;
-        sum = fmaf(c, peer(&s.g[1][g], r), sum);
-      }
-      const float mean = n > 0.f ? sum / n : 0.f;
-      for (int r = 0; r < a.runs; ++r) {
-        const float c = peer(&s.g[0][g], r), d = peer(&s.g[1][g], r) - mean;
-        if (c > 0.f) dev += fmaf(c * d, d, peer(&s.g[2][g], r));
-      }
-      sum = mean;
+    // a lane to a block (their results stay where they are until all have read them, the own ones go to where the counts were)
+    const int lane = threadIdx.x & 31;
+    for (int g = threadIdx.x >> 5; g < p.groups; g += kThreads / 32) {
+      float n = 0.f, m = 0.f, q = 0.f;
+      if (lane < a.runs) n = peer(&s.g[0][g], lane), m = peer(&s.g[1][g], lane), q = peer(&s.g[2][g], lane);
+      const float all = warp_sum(n), mean = all > 0.f ? warp_sum(n * m) / all : 0.f;
+      const float dev = warp_sum(n > 0.f ? fmaf(n * (m - mean), m - mean, q) : 0.f);
+      if (lane == 0) s.a[3 * g] = all, s.a[3 * g + 1] = mean, s.a[3 * g + 2] = dev;
     }
-    cluster_arrive();   // (all have read)
+    cluster_arrive();
     cluster_wait();
-    if (g < p.groups) s.g[0][g] = n, s.g[1][g] = sum, s.g[2][g] = dev;
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) s.g[0][g] = s.a[3 * g], s.g[1][g] = s.a[3 * g + 1], s.g[2][g] = s.a[3 * g + 2];
     __syncthreads();
   }
   finish(a, p, s, p.run == 0);
@@ -635,7 +623,7 @@ struct Back {
     if (a.silu) {
 #pragma unroll
       for (int j = 0; j < kP; ++j) {
-        const f32x2 z = fma2(d[j], scale[j], beta[j]), ns = minus_sig2<T>(z);
+        const f32x2 z = fma2(d[j], scale[j], beta[j]), ns = minus_sigmoid2<T, -1>(z);
         ndz[j] = mul2(mul2(dy[j], ns), add2(fma2(z, ns, z), both(1.f)));
       }
     } else {
@@ -648,7 +636,7 @@ struct Back {
 // sums of dz and dz xhat of every channel over the block's steps -> a.chan, of dn and dn xhat of every group -> s.g[0], s.g[1]
 template <typename T, int kV, bool kOne, typename W>
 __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& s, const Back<T, kV, kOne>& k, W& walk, Walk<T, kV, 2>* then) {
-  constexpr int kP = Vec<T, kV>::kP;
+  constexpr int kP = Vec<T, kV>::kP, kPlane = kThreads * kV;
   f32x2 nS[kP], nQ[kP];   // minus the sums of dz and of dz d (xhat being rstd d)
 #pragma unroll
   for (int j = 0; j < kP; ++j) nS[j] = nQ[j] = both(0.f);
@@ -673,8 +661,8 @@ __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& 
   if (p.r < p.lanes) {
 #pragma unroll
     for (int j = 0; j < kV; ++j) {
-      s.a[0][p.r * width + p.v * kV + j] = -S[j];
-      s.a[1][p.r * width + p.v * kV + j] = -Q[j];
+      s.a[p.r * width + p.v * kV + j] = -S[j];
+      s.a[kPlane + p.r * width + p.v * kV + j] = -Q[j];
     }
   }
   __syncthreads();
@@ -683,27 +671,27 @@ __device__ __forceinline__ void sums(const GnArgs& a, const Where<kV>& p, Sums& 
   for (int e = threadIdx.x; e < parts * width; e += kThreads) {
     const int part = quotient(e, 1.f / (float)width), c = e - part * width;
     float u = 0.f, q = 0.f;
-    for (int r = part; r < p.lanes; r += parts) u += s.a[0][r * width + c], q += s.a[1][r * width + c];
-    s.a[0][e] = u;
-    s.a[1][e] = q;
+    for (int r = part; r < p.lanes; r += parts) u += s.a[r * width + c], q += s.a[kPlane + r * width + c];
+    s.a[e] = u;
+    s.a[kPlane + e] = q;
   }
   __syncthreads();
   const long long row = ((long long)p.b * a.runs + p.run) * 2 * a.D, at = (long long)p.b * a.G + p.tile * a.ng;
   for (int c = threadIdx.x; c < p.chans; c += kThreads) {
     float u = 0.f, q = 0.f;
-    for (int k = 0; k < parts; ++k) u += s.a[0][k * width + c], q += s.a[1][k * width + c];
+    for (int k = 0; k < parts; ++k) u += s.a[k * width + c], q += s.a[kPlane + k * width + c];
     q *= a.rstd[at + quotient(c, a.over_size)];
     a.chan[row + p.c0 + c] = u;
     a.chan[row + a.D + p.c0 + c] = q;
     const float w = a.gamma[p.c0 + c] + a.offset;
-    s.a[0][c] = u * w;   // (this thread alone has read the place)
-    s.a[1][c] = q * w;
+    s.a[c] = u * w;   // (this thread alone has read the place)
+    s.a[kPlane + c] = q * w;
   }
   __syncthreads();
   const int lane = threadIdx.x & 31;
   for (int g = threadIdx.x >> 5; g < p.groups; g += kThreads / 32) {
     float u = 0.f, q = 0.f;
-    for (int c = lane; c < a.size; c += 32) u += s.a[0][g * a.size + c], q += s.a[1][g * a.size + c];
+    for (int c = lane; c < a.size; c += 32) u += s.a[g * a.size + c], q += s.a[kPlane + g * a.size + c];
     u = warp_sum(u), q = warp_sum(q);
     if (lane == 0) s.g[0][g] = u, s.g[1][g] = q;
   }
@@ -802,13 +790,16 @@ __global__ void __launch_bounds__(kThreads, 3) gn_held_back_kernel(GnArgs a) {
   if (a.runs > 1) {
     cluster_arrive();
     cluster_wait();
-    const int g = threadIdx.x;
-    float u = 0.f, q = 0.f;
-    if (g < p.groups)
-      for (int r = 0; r < a.runs; ++r) u += peer(&s.g[0][g], r), q += peer(&s.g[1][g], r);
+    const int lane = threadIdx.x & 31;
+    for (int g = threadIdx.x >> 5; g < p.groups; g += kThreads / 32) {
+      float u = 0.f, q = 0.f;
+      if (lane < a.runs) u = peer(&s.g[0][g], lane), q = peer(&s.g[1][g], lane);
+      u = warp_sum(u), q = warp_sum(q);
+      if (lane == 0) s.a[2 * g] = u, s.a[2 * g + 1] = q;
+    }
     cluster_arrive();   // (all have read)
     cluster_wait();
-    if (g < p.groups) s.g[0][g] = u, s.g[1][g] = q;
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) s.g[0][g] = s.a[2 * g], s.g[1][g] = s.a[2 * g + 1];
     __syncthreads();
   }
   grads<T, kV, true>(a, p, s, k, rows);
@@ -1004,12 +995,12 @@ Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
   if (vec * es == 16 && size % vec == 0) {
     // Held in one pass where eight blocks hold a sequence's steps of a tile of 64 bytes or more; wider tiles as long as no further
     // block is needed for them and the device stays full.
-    const int places = kHeld / arrays;
+    const int places = bwd ? kHeldBack / 2 : kHeld;
     auto lanes_of = [&](int ng) { return kThreads / (ng * size / vec); };
     auto blocks_of = [&](int ng) { return (L + places * lanes_of(ng) - 1) / (places * lanes_of(ng)); };
     int ng = 1;
     while (ng < G && ng * size * es < kHeldRow) ++ng;
-    if (ng * size <= kThreads * vec && blocks_of(ng) <= 8) {
+    if (ng * size <= kThreads * vec && blocks_of(ng) <= 8 && (long long)B * ((G + ng - 1) / ng) * blocks_of(ng) <= 3 * 148) {
       while (2 * ng <= G && 2 * ng * size <= kThreads * vec && blocks_of(2 * ng) == blocks_of(ng) &&
              (long long)B * ((G + 2 * ng - 1) / (2 * ng)) * blocks_of(ng) >= 3 * 148)
         ng *= 2;
@@ -1018,21 +1009,24 @@ Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
       return p;
     }
   }
-  // a tile: whole groups and whole vectors, 128 bytes or more of a row where there are as many; wider while the device stays full,
+  // a tile: whole groups and whole vectors, 256 bytes or more of a row where there are as many (B = 2, L = 32768, D = 1024, 16 groups,
+  // bf16 forward: 81 us with 128, 76 with 256, 76 with 512); wider while the device stays full,
   // as a block's fixed part is worth some ten rows of a thread
   const int unit = vec / gcd(size, vec);
   auto tiles_of = [&](int ng) { return (G + ng - 1) / ng; };
   p.ng = unit;
-  while (p.ng < G && p.ng * size * es < 128) p.ng += unit;
+  while (p.ng < G && p.ng * size * es < 256) p.ng += unit;
   while (p.ng < G && 2 * p.ng * size <= kThreads * vec && 2 * p.ng <= kGroups && (long long)B * tiles_of(2 * p.ng) >= blocks) p.ng *= 2;
   while (p.ng > G) p.ng -= unit;
   if (p.ng <= 0) p.ng = G;   // (D is whole vectors: the row is)
   p.tiles = tiles_of(p.ng);
   const long long slices = (long long)B * p.tiles;
   const int lanes = std::max(1, kThreads / std::max(1, p.ng * size / vec));
-  // runs: as many as fill the device once, of eight rows to a thread at least and kRun at most
-  const long long runs = std::max<long long>(1, std::min<long long>(blocks / slices, L / (8ll * lanes)));
-  p.steps = (int)std::min<long long>((L + runs - 1) / runs, (long long)kRun * lanes);
+  // runs: as many as fill the device once (or, where a thread's kRun rows are fewer, a whole number of times), of eight rows to a
+  // thread at least
+  const long long least = (L + (long long)kRun * lanes - 1) / ((long long)kRun * lanes), waves = (least * slices + blocks - 1) / blocks;
+  const long long runs = std::max<long long>(least, std::min<long long>(waves * blocks / slices, L / (8ll * lanes)));
+  p.steps = (int)((L + runs - 1) / runs);
   p.runs = (L + p.steps - 1) / p.steps;
   p.piece = p.runs == 1 ? B : (int)std::min<long long>(B, std::max<long long>(1, kL2 / std::max<long long>(1, (long long)L * D * es * arrays)));
   return p;
@@ -1079,8 +1073,8 @@ void run_one(bool bwd, const GnArgs& a, const Plan& p, cudaStream_t s) {
     passes(gn_first_kernel<T, kV, kOne>, gn_second_kernel<T, kV, kOne>, a, p.piece, s);
 }
 template <typename Kernel>
-void launch_held(Kernel kernel, const GnArgs& a, cudaStream_t s) {
-  const size_t smem = kPlaces + kHeld * kThreads * 16;
+void launch_held(Kernel kernel, bool bwd, const GnArgs& a, cudaStream_t s) {
+  const size_t smem = bwd ? kPlaces + kHeldBack * kThreads * 16 : kFewer + kHeld * kThreads * 16;
   allow_smem(reinterpret_cast<const void*>(kernel), smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.runs, a.tiles, a.B);
@@ -1100,7 +1094,7 @@ void launch_held(Kernel kernel, const GnArgs& a, cudaStream_t s) {
 template <typename T, int kV>
 void run_vec(bool bwd, const GnArgs& a, const Plan& p, cudaStream_t s) {
   if constexpr (kV * sizeof(T) == 16) {
-    if (p.held) return launch_held(bwd ? gn_held_back_kernel<T, kV> : gn_held_kernel<T, kV>, a, s);
+    if (p.held) return launch_held(bwd ? gn_held_back_kernel<T, kV> : gn_held_kernel<T, kV>, bwd, a, s);
     if (a.size % kV == 0) return run_one<T, kV, true>(bwd, a, p, s);
   }
   run_one<T, kV, kV == 1>(bwd, a, p, s);
