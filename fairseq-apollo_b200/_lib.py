@@ -101,7 +101,7 @@ OTHER = {
     "mega_abi_version": ([], c_i),
     "mega_block_step_work": ([c_i, c_i, c_i, c_i, c_i, c_l], c_l),
     "mega_gated_recurrence_segment": ([c_i, c_i], c_i),
-    "mega_group_norm_work": ([c_i] * 5, c_l),
+    "mega_group_norm_work": ([c_i] * 6, c_l),
     "mega_launch_count": ([], ctypes.c_uint64),
     "mega_debug_last_kernel": ([], ctypes.c_char_p),
 }

@@ -1129,11 +1129,11 @@ size_t work_bytes(const Plan& p, int B, int D, int G, bool bwd) {
 
 using namespace mega;
 
-extern "C" int64_t mega_group_norm_work(int dtype, int B, int L, int D, int num_groups) {
+extern "C" int64_t mega_group_norm_work(int dtype, int B, int L, int D, int num_groups, int backward) {
   if (check_gn(dtype, B, L, D, num_groups, {})) return 0;
-  size_t most = 0;
+  size_t most = 0;   // (of the vectors that addresses may allow)
   for (int vec : {16 / elem_size(dtype), 4 / elem_size(dtype), 1, 0})
-    for (bool bwd : {false, true}) most = std::max(most, work_bytes(plan_of(dtype, B, L, D, num_groups, vec, bwd), B, D, num_groups, bwd));
+    most = std::max(most, work_bytes(plan_of(dtype, B, L, D, num_groups, vec, backward != 0), B, D, num_groups, backward != 0));
   return (int64_t)most;
 }
 

@@ -58,4 +58,5 @@ def gated_recurrence_packed(z, gated=False, padding_mask=None, reset_mask=None, 
 
 def group_norm(x, weight, bias, num_groups, padding_mask, eps, activation):
     """y = act(GroupNorm(x)) from the module's parameters (effective scale weight + 1)."""
-    return _lib.host().group_norm_train(x, weight, bias, num_groups, padding_mask, eps, ops._silu(activation))
+    fn = _lib.host().group_norm_train if needs_grad(x, weight, bias) else _lib.host().group_norm
+    return fn(x, weight, bias, num_groups, padding_mask, eps, ops._silu(activation))

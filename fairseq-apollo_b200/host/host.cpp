@@ -955,35 +955,31 @@ struct Gn {
   int B, L, D, G;
   unsigned flags;
 };
-Gn gn_args(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, const Tensor& mask, bool silu, bool offset,
-           const Where& w) {
+Tensor gn_param(const Tensor& p) {
+  return p.scalar_type() == at::kFloat && p.is_contiguous() ? p : f32c(p);
+}
+Gn gn_args(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, const Tensor& mask, bool silu, bool offset) {
   on_cuda(x, weight, bias, mask);
   dtype_of(x);
-  const Tensor rows = x.numel() ? gn_rows(x) : x;
+  expect(x.dim() >= 2, "x must be (batch, ..., channels)");
   const int64_t d = x.size(-1);
   expect(groups >= 1 && d % groups == 0, "num_groups must divide the channels");
   expect_numel(weight, d, "weight");
   expect_numel(bias, d, "bias");
   if (weight.device() != x.device() || bias.device() != x.device()) throw py::value_error("weight and bias must be on x's device");
-  Gn r = {rows};
-  if (x.numel()) {
-    Tensor m = mask;
-    if (m.defined() && m.dim() != 2 && m.dim() == x.dim() - 1) {
-      expect(m.sizes() == x.sizes().slice(0, x.dim() - 1), "padding_mask must have x's shape without its channels");
-      m = m.reshape({m.size(0), -1});
-    } else if (m.defined() && x.dim() == 2 && m.dim() == 1) {
-      m = m.unsqueeze(1);
-    }
-    r.mask = mask_on(m, rows, "padding_mask");
-    const auto p = f32_all({weight.detach(), bias.detach()}, w.stream);
-    r.gamma = p[0], r.beta = p[1];
-    r.B = extent(rows.size(0)), r.L = extent(rows.size(1)), r.D = extent(d), r.G = (int)groups;
-  }
+  Gn r;
   r.flags = (silu ? MEGA_GN_SILU : 0u) | (offset ? MEGA_GN_OFFSET : 0u);
+  if (x.numel() == 0) return r;
+  r.x = gn_rows(x);
+  Tensor m = mask;
+  if (m.defined() && m.dim() != 2 && m.dim() == x.dim() - 1) {
+    expect(m.sizes() == x.sizes().slice(0, x.dim() - 1), "padding_mask must have x's shape without its channels");
+    m = x.dim() == 2 ? m.unsqueeze(1) : m.reshape({m.size(0), -1});
+  }
+  r.mask = mask_on(m, r.x, "padding_mask");
+  r.gamma = gn_param(weight), r.beta = gn_param(bias);
+  r.B = extent(r.x.size(0)), r.L = extent(r.x.size(1)), r.D = extent(d), r.G = (int)groups;
   return r;
-}
-Tensor gn_work(const Gn& r) {
-  return at::empty({mega_group_norm_work(dtype_of(r.x), r.B, r.L, r.D, r.G)}, at::TensorOptions().dtype(at::kByte).device(r.x.device()));
 }
 // A result of x's shape for rows r, and its own rows (a tensor of its own: a view could not be changed in place)
 std::pair<Tensor, Tensor> gn_like(const Tensor& x, const Tensor& rows) {
@@ -994,40 +990,58 @@ std::pair<Tensor, Tensor> gn_like(const Tensor& x, const Tensor& rows) {
   Tensor y = at::empty(x.sizes(), x.options().requires_grad(false));
   return {y, y.view(rows.sizes())};
 }
-// y like x and its statistics (count, mean, rstd)
-std::tuple<Tensor, Tensor, Tensor, Tensor> run_gn(const Tensor& x, const Gn& r, double eps, const Where& w) {
+// (count (B) int64, mean, rstd (B, G) fp32) in one piece, which is one allocation to a call
+struct Stats {
+  int64_t* count;
+  float *mean, *rstd;
+  char* end;
+  Stats(const Tensor& t, int64_t b, int64_t g)
+      : count(static_cast<int64_t*>(t.data_ptr())), mean(reinterpret_cast<float*>(count + b)), rstd(mean + b * g),
+        end(static_cast<char*>(t.data_ptr()) + bytes(b, g)) {}
+  static int64_t bytes(int64_t b, int64_t g) { return (8 * b * (1 + g) + 15) / 16 * 16; }
+};
+Tensor bytes_of(int64_t n, const Tensor& like) { return at::empty({n}, at::TensorOptions().dtype(at::kByte).device(like.device())); }
+// y like x; its statistics, with the call's workspace behind them
+std::pair<Tensor, Tensor> run_gn(const Tensor& x, const Gn& r, double eps, const Where& w) {
+  const int dt = dtype_of(r.x);
   auto [out, y] = gn_like(x, r.x);
-  Tensor count = counts(r.B, r.x), st = floats({2, r.B, r.G}, r.x);
-  Tensor mean = st.select(0, 0), rstd = st.select(0, 1);
-  const Tensor work = gn_work(r);
-  check(mega_group_norm_fwd(r.x.data_ptr(), y.data_ptr(), dtype_of(r.x), r.B, r.L, r.D, STRIDES2(r.x), STRIDES2(y), fptr(r.gamma),
-                            fptr(r.beta), ptr<uint8_t>(r.mask), r.G, eps, r.flags, ptr<int64_t>(count), fptr(mean), fptr(rstd),
-                            work.data_ptr(), w.stream), "group_norm_fwd");
-  return {out, count, mean, rstd};
+  const Tensor stats = bytes_of(Stats::bytes(r.B, r.G) + mega_group_norm_work(dt, r.B, r.L, r.D, r.G, 0), r.x);
+  const Stats st(stats, r.B, r.G);
+  check(mega_group_norm_fwd(r.x.data_ptr(), y.data_ptr(), dt, r.B, r.L, r.D, STRIDES2(r.x), STRIDES2(y), fptr(r.gamma), fptr(r.beta),
+                            ptr<uint8_t>(r.mask), r.G, eps, r.flags, st.count, st.mean, st.rstd, st.end, w.stream), "group_norm_fwd");
+  return {out, stats};
 }
 
+Tensor group_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, const OptTensor& mask, double eps, bool silu) {
+  const Gn r = gn_args(x, weight, bias, groups, given(mask), silu, true);
+  if (x.numel() == 0) return fresh(x);
+  const Where w(x);
+  return run_gn(x, r, eps, w).first;
+}
+
+// (y, count, mean, rstd)
 std::tuple<Tensor, Tensor, Tensor, Tensor> group_norm_fwd(const Tensor& x, const Tensor& gamma, const Tensor& beta, int64_t groups,
                                                           const OptTensor& mask, double eps, bool silu, bool offset) {
-  on_cuda(x);
+  const Gn r = gn_args(x, gamma, beta, groups, given(mask), silu, offset);
   const Where w(x);
-  const Gn r = gn_args(x, gamma, beta, groups, given(mask), silu, offset, w);
+  const int64_t b = x.size(0);
   if (x.numel() == 0) {
-    const int64_t b = x.size(0);
     Tensor rstd = floats({b, groups}, x);
     rstd.fill_(1.0 / std::sqrt(eps));
     return {fresh(x), counts(b, x).zero_(), floats({b, groups}, x).zero_(), rstd};
   }
-  return run_gn(x, r, eps, w);
+  auto [y, stats] = run_gn(x, r, eps, w);
+  const Tensor f = stats.narrow(0, 8 * b, 8 * b * groups).view(at::kFloat).view({2, b, groups});
+  return {y, stats.narrow(0, 0, 8 * b).view(at::kLong), f.select(0, 0), f.select(0, 1)};
 }
 
 class GnFn : public torch::autograd::Function<GnFn> {
  public:
   static Tensor forward(AutogradContext* ctx, Tensor x, Tensor weight, Tensor bias, int64_t groups, OptTensor mask, double eps, bool silu) {
-    on_cuda(x);
+    const Gn r = gn_args(x, weight, bias, groups, given(mask), silu, true);
     const Where w(x);
-    const Gn r = gn_args(x, weight, bias, groups, given(mask), silu, true, w);
-    auto [y, count, mean, rstd] = run_gn(x.detach(), r, eps, w);
-    ctx->save_for_backward({x, weight, bias, r.mask, count, mean, rstd});
+    auto [y, stats] = run_gn(x, r, eps, w);
+    ctx->save_for_backward({x, weight, bias, r.mask, stats});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["silu"] = silu;
     return y;
@@ -1037,18 +1051,23 @@ class GnFn : public torch::autograd::Function<GnFn> {
     first_order();
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &weight = s[1], &bias = s[2];
+    const Gn r = gn_args(x, weight, bias, ctx->saved_data["groups"].toInt(), Tensor(), ctx->saved_data["silu"].toBool(), true);
     const Where w(x);
-    const Gn r = gn_args(x, weight, bias, ctx->saved_data["groups"].toInt(), Tensor(), ctx->saved_data["silu"].toBool(), true, w);
+    const int dt = dtype_of(x);
     Tensor dy = grads[0];
     dy = gn_rows(dy.scalar_type() == x.scalar_type() ? dy : dy.to(x.scalar_type()));
     auto [out, dx] = gn_like(x, r.x);
-    Tensor f = floats({2, r.D}, x);
-    const Tensor work = gn_work(r);
-    check(mega_group_norm_bwd(dy.data_ptr(), r.x.data_ptr(), dx.data_ptr(), dtype_of(r.x), r.B, r.L, r.D, STRIDES2(dy), STRIDES2(r.x),
-                              STRIDES2(dx), fptr(r.gamma), fptr(r.beta), ptr<uint8_t>(s[3]), r.G, r.flags, ptr<int64_t>(s[4]),
-                              fptr(s[5]), fptr(s[6]), fptr(f), fptr(f) + r.D, work.data_ptr(), w.stream), "group_norm_bwd");
-    auto own = [&](int64_t k, const Tensor& p) { return f.select(0, k).view(p.sizes()).to(p.scalar_type()); };
-    return {out, own(0, weight), own(1, bias), Tensor(), Tensor(), Tensor(), Tensor()};
+    Tensor dw = floats({r.D}, x), db = floats({r.D}, x);
+    const Tensor work = bytes_of(mega_group_norm_work(dt, r.B, r.L, r.D, r.G, 1), x);
+    const Stats st(s[4], r.B, r.G);
+    check(mega_group_norm_bwd(dy.data_ptr(), r.x.data_ptr(), dx.data_ptr(), dt, r.B, r.L, r.D, STRIDES2(dy), STRIDES2(r.x), STRIDES2(dx),
+                              fptr(r.gamma), fptr(r.beta), ptr<uint8_t>(s[3]), r.G, r.flags, st.count, st.mean, st.rstd, fptr(dw), fptr(db),
+                              work.data_ptr(), w.stream), "group_norm_bwd");
+    auto own = [&](const Tensor& g, const Tensor& p) {
+      const Tensor v = p.dim() == 1 ? g : g.view(p.sizes());
+      return p.scalar_type() == at::kFloat ? v : v.to(p.scalar_type());
+    };
+    return {out, own(dw, weight), own(db, bias), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -1703,6 +1722,7 @@ PYBIND11_MODULE(_mega_host, m) {
   m.def("gated_recurrence_step", &gated_recurrence_step);
   m.def("gated_recurrence_train", &gated_recurrence_train);
   m.def("gated_recurrence_packed", &gated_recurrence_packed);
+  m.def("group_norm", &group_norm);
   m.def("group_norm_fwd", &group_norm_fwd);
   m.def("group_norm_train", &group_norm_train);
   m.def("block_train", &block_train);

@@ -11,7 +11,7 @@ import torch.nn as nn
 from torch.nn.parameter import Parameter
 
 from .. import ops
-from ..functions import group_norm, needs_grad
+from ..functions import group_norm
 
 
 class GroupNorm(nn.Module):
@@ -30,9 +30,7 @@ class GroupNorm(nn.Module):
         """x (B, ..., D); padding_mask of x's shape without the channels, non-zero = padded (0 in the result)."""
         if x.size(-1) != self.num_features:
             raise ValueError("x has %d channels, not %d" % (x.size(-1), self.num_features))
-        if needs_grad(x, self.weight, self.bias):
-            return group_norm(x, self.weight, self.bias, self.num_groups, padding_mask, self.eps, self.activation)
-        return ops.group_norm_fwd(x, self.weight, self.bias, self.num_groups, padding_mask, self.eps, self.activation, True)[0]
+        return group_norm(x, self.weight, self.bias, self.num_groups, padding_mask, self.eps, self.activation)
 
     def extra_repr(self) -> str:
         return 'num_features={num_features}, num_groups={num_groups}, eps={eps}, activation={activation}'.format(**self.__dict__)

@@ -660,13 +660,12 @@ MEGA_API int mega_gated_recurrence_step(const void* x, const void* f, const void
  * Statistics: count (B) int64 (steps that are not padded), mean, rstd (B, G) fp32 (0 and 1 / sqrt(eps) without a step).
  *
  * mega_group_norm_bwd: dx like x (0 at padded steps), dgamma, dbeta (D) fp32, summed over sequences and steps in a fixed
- * order.  `work`: device memory of mega_group_norm_work() bytes, 16-byte aligned, used by this call alone until it is done;
- * forward and backward take the same size.
+ * order.  `work`: device memory of mega_group_norm_work() bytes, 16-byte aligned, used by this call alone until it is done.
  * At most 65535 sequences and groups, and 2^24 steps (MEGA_ERR_UNSUPPORTED).
  */
 #define MEGA_GN_SILU 1u
 #define MEGA_GN_OFFSET 2u
-MEGA_API int64_t mega_group_norm_work(int dtype, int B, int L, int D, int num_groups);
+MEGA_API int64_t mega_group_norm_work(int dtype, int B, int L, int D, int num_groups, int backward);
 MEGA_API int mega_group_norm_fwd(const void* x, void* y, int dtype, int B, int L, int D, int64_t xsb, int64_t xsl, int64_t ysb,
                         int64_t ysl, const float* gamma, const float* beta, const uint8_t* pad_mask, int num_groups, double eps,
                         unsigned flags, int64_t* count, float* mean, float* rstd, void* work, mega_stream_t stream);

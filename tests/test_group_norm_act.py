@@ -162,7 +162,8 @@ def test_abi_refusals():
     assert fwd(G=3) == 3 and fwd(G=0) == 3 and fwd(L=0) == 3 and bwd(G=5) == 3
     assert fwd(B=65536) == 7 and fwd(G=70000, D=70000) == 7
     assert fwd(x=odd) == 5 and bwd(dy=odd) == 5
-    assert lib.mega_group_norm_work(1, 4, 100, 64, 8) > 0 and lib.mega_group_norm_work(1, 4, 100, 64, 7) == 0
+    for backward in (0, 1):
+        assert lib.mega_group_norm_work(1, 4, 100, 64, 8, backward) > 0 and lib.mega_group_norm_work(1, 4, 100, 64, 7, backward) == 0
 
 
 def test_reference_gradients_against_differences():
