@@ -1009,14 +1009,17 @@ Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
       return p;
     }
   }
-  // a tile: whole groups and whole vectors, 256 bytes or more of a row where there are as many (B = 2, L = 32768, D = 1024, 16 groups,
-  // bf16 forward: 81 us with 128, 76 with 256, 76 with 512); wider while the device stays full,
-  // as a block's fixed part is worth some ten rows of a thread
+  // a tile: whole groups and whole vectors, 64 bytes or more of a row where there are as many; up to 256 while runs of eight rows to a
+  // thread still fill the device (B = 2, L = 32768, D = 1024, 16 groups, bf16 forward: 81 us with 128 bytes, 76 with 256, 76 with
+  // 512), and further while whole sequences do, as a block's fixed part is worth some ten rows of a thread
   const int unit = vec / gcd(size, vec);
   auto tiles_of = [&](int ng) { return (G + ng - 1) / ng; };
+  auto most = [&](int ng) { return (long long)B * tiles_of(ng) * std::max<long long>(1, L / (8ll * std::max(1, kThreads / (ng * size / vec)))); };
   p.ng = unit;
-  while (p.ng < G && p.ng * size * es < 256) p.ng += unit;
-  while (p.ng < G && 2 * p.ng * size <= kThreads * vec && 2 * p.ng <= kGroups && (long long)B * tiles_of(2 * p.ng) >= blocks) p.ng *= 2;
+  while (p.ng < G && p.ng * size * es < 64) p.ng += unit;
+  while (p.ng < G && 2 * p.ng * size <= kThreads * vec && 2 * p.ng <= kGroups &&
+         (p.ng * size * es < 256 ? most(2 * p.ng) >= blocks : (long long)B * tiles_of(2 * p.ng) >= blocks))
+    p.ng *= 2;
   while (p.ng > G) p.ng -= unit;
   if (p.ng <= 0) p.ng = G;   // (D is whole vectors: the row is)
   p.tiles = tiles_of(p.ng);
