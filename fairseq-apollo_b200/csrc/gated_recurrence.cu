@@ -286,6 +286,15 @@ __device__ __forceinline__ bool flag_of(const RecArgs& a, int b, int t0, int ste
   return t < a.L && a.reset && a.reset[b * a.msb + t * a.msl];
 }
 
+template <int kS>
+__device__ __forceinline__ bool all_padded(unsigned flags) {
+  return (flags & ((1u << kS) - 1u)) == (1u << kS) - 1u;
+}
+template <int kS>
+__device__ __forceinline__ bool idle(unsigned flags) {   // all padded, and no reset
+  return flags == (1u << kS) - 1u;
+}
+
 // What the warps of a block, and the blocks of a cluster, tell one another.  Two of each: a place is written again only after every
 // reader has taken part in the round between.
 struct Post {
@@ -363,20 +372,25 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
   T* y = (T*)a.y + b * a.ysb + c0 + 2 * lane;
   char* ring = smem + w * (kStages * kOps * Op::kBytes);
   const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
-  const bool masks = a.pad || a.reset, reset = a.reset != nullptr, whole = kPair && chans == kC;
+  const bool reset = a.reset != nullptr, whole = kPair && chans == kC;
   bool alive = true;
 
+  auto first = [&](int k) { return (k * size + rank) * (kW * kS) + w * kS; };
+  bool flag = flag_of(a, b, first(0), kS, lane);
+  // sets round k's tile on its way and returns its padding and resets, which came a round earlier: a segment of padding is not read
   auto fetch = [&](int k) {
-    const int t0 = (k * size + rank) * (kW * kS) + w * kS, rows = min(max(a.L - t0, 0), kS);
+    const unsigned flags = __ballot_sync(0xffffffffu, flag);
+    if (k + 1 < rounds) flag = flag_of(a, b, first(k + 1), kS, lane);
+    const int t0 = first(k), rows = min(max(a.L - t0, 0), kS);
     char* at = ring + (k % kStages) * (kOps * Op::kBytes);
-    if (k < rounds) {
+    if (k < rounds && !all_padded<kS>(flags)) {
       const int t = rows > 0 ? t0 : 0;
       Op::fetch(at, x, a.xsl, t, rows, chans, lane);
       Op::fetch(at + Op::kBytes, f, a.fsl, t, rows, chans, lane);
       if (kGate) Op::fetch(at + 2 * Op::kBytes, i, a.isl, t, rows, chans, lane);
     }
     copies_commit();
-    return masks && k < rounds ? flag_of(a, b, t0, kS, lane) : (lane < kS && t0 + lane >= a.L);
+    return flags;
   };
 
   if (size > 1) {
@@ -388,11 +402,11 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
     cluster_arrive();   // (every block has begun, and its barriers are there, before another writes to it)
   }
   f32x2 carry = get_state(a.h_in ? a.h_in + state : nullptr, n, a.pairs);
-  bool flag = fetch(0);
+  unsigned flags, next = fetch(0);
   for (int k = 0; k < rounds; ++k) {
-    const unsigned flags = __ballot_sync(0xffffffffu, flag);
+    flags = next;
     __syncwarp();   // (the stage that is fetched into next has been read by every lane)
-    flag = fetch(k + 1);
+    next = fetch(k + 1);
     copies_wait<kStages - 1>();
     __syncwarp();
     const T* op = reinterpret_cast<const T*>(ring + (k % kStages) * (kOps * Op::kBytes)) + 2 * lane;
@@ -414,6 +428,8 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
         step(s);
         loc[s] = {A, h};
       }
+    } else if (idle<kS>(flags)) {
+      loc[kS - 1] = {A, h};
     } else {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
@@ -429,13 +445,19 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
     f32x2 in;
     alive = reset ? exchange<1, true>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive)
                   : exchange<1, false>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive);
-    const int t0 = (k * size + rank) * (kW * kS) + w * kS;
+    const int t0 = first(k);
     if (a.starts && t0 < a.L) put_state(a.starts + ((long long)b * segs + t0 / kS) * a.D + c0 + 2 * lane, in, n, a.pairs);
     T* yt = y + t0 * a.ysl;
     if (flags == 0 && whole) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         put<kPair>(yt, loc[s].operator()<false>(in), 2);
+        yt += a.ysl;
+      }
+    } else if (idle<kS>(flags)) {
+#pragma unroll 4
+      for (int s = 0; s < min(kS, a.L - t0); ++s) {
+        put<kPair>(yt, pack2(0.f, 0.f), n);
         yt += a.ysl;
       }
     } else {
@@ -469,14 +491,18 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
   T* di = kGate ? (T*)a.di + b * a.dib + c0 + 2 * lane : nullptr;
   char* ring = smem + w * (kStages * kOps * Op::kBytes);
   const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
-  const bool masks = a.pad || a.reset, reset = a.reset != nullptr, whole = kPair && chans == kC;
+  const bool reset = a.reset != nullptr, whole = kPair && chans == kC;
   bool alive = true;
 
   f32x2 start = pack2(0.f, 0.f);
-  auto fetch = [&](int k) {   // (round k is the k-th from the end)
-    const int t0 = ((rounds - 1 - k) * size + rank) * (kW * kS) + w * kS, rows = min(max(a.L - t0, 0), kS);
+  auto first = [&](int k) { return ((rounds - 1 - k) * size + rank) * (kW * kS) + w * kS; };   // (round k is the k-th from the end)
+  bool flag = flag_of(a, b, first(0), kS, lane);
+  auto fetch = [&](int k) {
+    const unsigned flags = __ballot_sync(0xffffffffu, flag);
+    if (k + 1 < rounds) flag = flag_of(a, b, first(k + 1), kS, lane);
+    const int t0 = first(k), rows = min(max(a.L - t0, 0), kS);
     char* at = ring + (k % kStages) * (kOps * Op::kBytes);
-    if (k < rounds) {
+    if (k < rounds && !all_padded<kS>(flags)) {
       const int t = rows > 0 ? t0 : 0;
       Op::fetch(at, x, a.xsl, t, rows, chans, lane);
       Op::fetch(at + Op::kBytes, f, a.fsl, t, rows, chans, lane);
@@ -485,7 +511,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
       if (rows > 0) start = get_state(a.starts + ((long long)b * segs + t0 / kS) * a.D + c0 + 2 * lane, n, a.pairs);
     }
     copies_commit();
-    return masks && k < rounds ? flag_of(a, b, t0, kS, lane) : (lane < kS && t0 + lane >= a.L);
+    return flags;
   };
 
   if (size > 1) {
@@ -497,12 +523,12 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
     cluster_arrive();
   }
   f32x2 carry = get_state(a.dh_out ? a.dh_out + state : nullptr, n, a.pairs);
-  bool flag = fetch(0);
+  unsigned flags, next = fetch(0);
   for (int k = 0; k < rounds; ++k) {
-    const unsigned flags = __ballot_sync(0xffffffffu, flag);
+    flags = next;
     f32x2 h = start;
     __syncwarp();
-    flag = fetch(k + 1);
+    next = fetch(k + 1);
     copies_wait<kStages - 1>();
     __syncwarp();
     const T* op = reinterpret_cast<const T*>(ring + (k % kStages) * (kOps * Op::kBytes)) + 2 * lane;
@@ -531,7 +557,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
       for (int s = 0; s < kS; ++s) state_step(s);
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) grad_step(s);
-    } else {
+    } else if (!idle<kS>(flags)) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         if ((flags >> (16 + s)) & 1u) h = pack2(0.f, 0.f);
@@ -552,7 +578,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
     f32x2 q;
     alive = reset ? exchange<-1, true>(m, carry, q, post, k, w, lane, rank, size, alive)
                   : exchange<-1, false>(m, carry, q, post, k, w, lane, rank, size, alive);
-    const int t0 = ((rounds - 1 - k) * size + rank) * (kW * kS) + w * kS;
+    const int t0 = first(k);
     T *xt = dx + t0 * a.dxl, *ft = df + t0 * a.dfl, *it = kGate ? di + t0 * a.dil : nullptr;
     auto out_step = [&](int s, bool pad, int count) {
       const f32x2 g = add2(q, two(gy + s * kC));
@@ -568,6 +594,15 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
     if (flags == 0 && whole) {
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) out_step(s, false, 2);
+    } else if (idle<kS>(flags)) {
+#pragma unroll 4
+      for (int s = 0; s < min(kS, a.L - t0); ++s) {
+        put<kPair>(xt, pack2(0.f, 0.f), n);
+        put<kPair>(ft, pack2(0.f, 0.f), n);
+        if (kGate) put<kPair>(it, pack2(0.f, 0.f), n);
+        xt += a.dxl, ft += a.dfl;
+        if (kGate) it += a.dil;
+      }
     } else {
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) {
