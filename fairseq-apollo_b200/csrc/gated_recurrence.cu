@@ -50,9 +50,12 @@ struct RecArgs {
 };
 
 // Steps of a segment: what h_loc and A of every step (the backward: leak, state and, with an input gate, its two factors) leave of
-// 128 registers.
+// 128 registers; fp32 tiles would not fit the shared memory of two blocks otherwise.  The forward saves the states that the
+// backward's segments start from.
 template <typename T, bool kGate>
-constexpr int kSteps = sizeof(T) == 4 || kGate ? 8 : 16;
+constexpr int kBackSteps = sizeof(T) == 4 || kGate ? 8 : 16;
+template <typename T>
+constexpr int kForwardSteps = sizeof(T) == 4 ? 8 : 16;
 
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
@@ -359,7 +362,7 @@ __device__ __forceinline__ bool exchange(const Map& own, f32x2& carry, f32x2& in
 // ---- forward ---------------------------------------------------------------------------------
 template <typename T, bool kGate, int kMode>
 __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
-  constexpr int kS = kSteps<T, kGate>, kOps = kGate ? 3 : 2;
+  constexpr int kS = kForwardSteps<T>, kSave = kBackSteps<T, kGate>, kOps = kGate ? 3 : 2;
   using Op = Tile<T, kS, kMode>;
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
   extern __shared__ __align__(16) char smem[];
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
   const T *x = (const T*)a.x + b * a.xsb + c0, *f = (const T*)a.f + b * a.fsb + c0, *i = kGate ? (const T*)a.i + b * a.isb + c0 : nullptr;
   T* y = (T*)a.y + b * a.ysb + c0 + 2 * lane;
   char* ring = smem + w * (kStages * kOps * Op::kBytes);
-  const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
+  const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kSave - 1) / kSave;
   const bool reset = a.reset != nullptr, whole = kPair && chans == kC;
   bool alive = true;
 
@@ -446,7 +449,13 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
     alive = reset ? exchange<1, true>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive)
                   : exchange<1, false>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive);
     const int t0 = first(k);
-    if (a.starts && t0 < a.L) put_state(a.starts + ((long long)b * segs + t0 / kS) * a.D + c0 + 2 * lane, in, n, a.pairs);
+    if (a.starts) {
+#pragma unroll
+      for (int s = 0; s < kS; s += kSave) {
+        const f32x2 from = s == 0 || idle<kS>(flags) ? in : loc[s > 0 ? s - 1 : 0].operator()<true>(in);
+        if (t0 + s < a.L) put_state(a.starts + ((long long)b * segs + (t0 + s) / kSave) * a.D + c0 + 2 * lane, from, n, a.pairs);
+      }
+    }
     T* yt = y + t0 * a.ysl;
     if (flags == 0 && whole) {
 #pragma unroll
@@ -476,7 +485,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
 // ---- backward --------------------------------------------------------------------------------
 template <typename T, bool kGate, int kMode>
 __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
-  constexpr int kS = kSteps<T, kGate>, kOps = kGate ? 4 : 3;
+  constexpr int kS = kBackSteps<T, kGate>, kOps = kGate ? 4 : 3;
   using Op = Tile<T, kS, kMode>;
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
   extern __shared__ __align__(16) char smem[];
@@ -686,9 +695,8 @@ void launch_rec(Kernel kernel, int tiles, int B, int cluster, size_t smem, cudaS
 
 template <typename T, bool kGate, int kMode>
 void run_mode(bool bwd, int B, const RecArgs& a, cudaStream_t s) {
-  constexpr int kS = kSteps<T, kGate>;
-  const int tiles = (a.D + kC - 1) / kC, cluster = cluster_of(tiles, B, a.L, kS);
-  const size_t smem = size_t(kW) * kStages * ((kGate ? 3 : 2) + (bwd ? 1 : 0)) * Tile<T, kS, kMode>::kBytes;
+  const int steps = bwd ? kBackSteps<T, kGate> : kForwardSteps<T>, tiles = (a.D + kC - 1) / kC, cluster = cluster_of(tiles, B, a.L, steps);
+  const size_t smem = size_t(kW) * kStages * ((kGate ? 3 : 2) + (bwd ? 1 : 0)) * steps * kC * sizeof(T);
   launch_rec(bwd ? rec_bwd_kernel<T, kGate, kMode> : rec_fwd_kernel<T, kGate, kMode>, tiles, B, cluster, smem, s, a);
 }
 template <typename T>
@@ -720,7 +728,7 @@ cudaError_t gated_recurrence_read_device_error(int* v, bool reset) { return read
 using namespace mega;
 
 extern "C" int mega_gated_recurrence_segment(int dtype, int gated) {
-  return !valid_dtype(dtype) ? 0 : dtype == MEGA_F32 ? kSteps<float, false> : gated ? kSteps<__half, true> : kSteps<__half, false>;
+  return !valid_dtype(dtype) ? 0 : dtype == MEGA_F32 ? kBackSteps<float, false> : gated ? kBackSteps<__half, true> : kBackSteps<__half, false>;
 }
 
 extern "C" int mega_gated_recurrence_fwd(const void* x, const void* f, const void* i, void* y, int dtype, int B, int L, int D,
