@@ -311,7 +311,7 @@ struct Post {
 // the other way.  A warp reads the maps before its own only: all eight in every warp are a third of the shared memory traffic, and
 // their loads, issued together, crowd out the registers.  Returns false once a wait has given up: the rounds go on, without
 // waiting.
-template <int kDir, bool kReset>
+template <int kDir, bool kReset, bool kFour>
 __device__ __forceinline__ bool exchange(const Map& own, f32x2& carry, f32x2& in, Post& post, int round, int w, int lane, int rank, int size,
                                          bool alive) {
   const int at = round & 1, place = kDir > 0 ? w : kW - 1 - w;
@@ -346,11 +346,30 @@ __device__ __forceinline__ bool exchange(const Map& own, f32x2& carry, f32x2& in
   }
   if (place == kW - 1) {
     if (alive) alive = received(&post.bar[at], (round >> 1) & 1);
+    if constexpr (kFour) {   // (maps read four at a time)
+#pragma unroll
+      for (int k0 = 0; k0 < 8; k0 += 4) {
+        if (k0 >= size) break;
+        float4 m[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = kDir > 0 ? k0 + k : size - 1 - k0 - k;
+          if (k0 + k < size) m[k] = post.blocks[at][r][lane];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = kDir > 0 ? k0 + k : size - 1 - k0 - k;
+          if (r == rank) in = carry;
+          if (k0 + k < size) carry = Map::of(m[k]).template operator()<kReset>(carry);
+        }
+      }
+    } else {
 #pragma unroll 1
-    for (int k = 0; k < size; ++k) {
-      const int r = kDir > 0 ? k : size - 1 - k;
-      if (r == rank) in = carry;
-      carry = Map::of(post.blocks[at][r][lane]).template operator()<kReset>(carry);
+      for (int k = 0; k < size; ++k) {
+        const int r = kDir > 0 ? k : size - 1 - k;
+        if (r == rank) in = carry;
+        carry = Map::of(post.blocks[at][r][lane]).template operator()<kReset>(carry);
+      }
     }
     post.carry[at][lane] = in;
   }
@@ -365,6 +384,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
   constexpr int kS = kForwardSteps<T>, kSave = kBackSteps<T, kGate>, kOps = kGate ? 3 : 2;
   using Op = Tile<T, kS, kMode>;
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
+  constexpr bool kFour = kMode == 16 && sizeof(T) == 2;   // (the other forms have no registers left for it)
   extern __shared__ __align__(16) char smem[];
   __shared__ Post post;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
@@ -446,8 +466,8 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
       }
     }
     f32x2 in;
-    alive = reset ? exchange<1, true>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive)
-                  : exchange<1, false>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive);
+    alive = reset ? exchange<1, true, kFour>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive)
+                  : exchange<1, false, kFour>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive);
     const int t0 = first(k);
     if (a.starts) {
 #pragma unroll
@@ -488,6 +508,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
   constexpr int kS = kBackSteps<T, kGate>, kOps = kGate ? 4 : 3;
   using Op = Tile<T, kS, kMode>;
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
+  constexpr bool kFour = kMode == 16 && sizeof(T) == 2;   // (the other forms have no registers left for it)
   extern __shared__ __align__(16) char smem[];
   __shared__ Post post;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
@@ -585,8 +606,8 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
       }
     }
     f32x2 q;
-    alive = reset ? exchange<-1, true>(m, carry, q, post, k, w, lane, rank, size, alive)
-                  : exchange<-1, false>(m, carry, q, post, k, w, lane, rank, size, alive);
+    alive = reset ? exchange<-1, true, kFour>(m, carry, q, post, k, w, lane, rank, size, alive)
+                  : exchange<-1, false, kFour>(m, carry, q, post, k, w, lane, rank, size, alive);
     const int t0 = first(k);
     T *xt = dx + t0 * a.dxl, *ft = df + t0 * a.dfl, *it = kGate ? di + t0 * a.dil : nullptr;
     auto out_step = [&](int s, bool pad, int count) {
@@ -665,13 +686,28 @@ int mode_of(int es, std::initializer_list<Operand> in, std::initializer_list<Ope
   return es == 4 || (all(in, 4) && all(out, 4)) ? 4 : 2;
 }
 
-// Blocks to a cluster.
+// Blocks to a cluster: what is predicted to take the least time.  A round takes two blocks on a multiprocessor about 2.4 us and one
+// block 1.6 (bf16 forward; the other forms' ratios are alike), a cluster's exchange some more; a launch is rounds and one to begin
+// with, in as many waves as it has blocks for (the device holds that many clusters at once).  Measured, bf16 forward, clusters of
+// 1, 2, 4, 8: B = 8, L = 4096, D = 1024 56, 49, 54, 61 us; B = 1, L = 65536, D = 2048 791, 498, 262, 190; B = 8, L = 4096,
+// D = 2048 74, 91, 103, 120.
 int cluster_of(int tiles, int B, int L, int steps) {
   const int forced = g_options[OPT_REC_CLUSTER].load(std::memory_order_relaxed);
   if (forced == 1 || forced == 2 || forced == 4 || forced == 8) return forced;
-  int c = 1;
-  while (c < 8 && (long long)tiles * B * c < 240 && c * kW * steps < L) c *= 2;
-  return c;
+  struct Form {
+    int size, slots;
+    double round;
+  };
+  constexpr Form kForms[] = {{1, 296, 1.}, {2, 296, 1.2}, {4, 284, 1.25}, {8, 264, 1.3}};
+  int best = 1;
+  double least = 1e300;
+  for (const Form& f : kForms) {
+    const long long blocks = (long long)tiles * B * f.size, last = blocks % f.slots;
+    const double waves = (double)(blocks / f.slots) + (last == 0 ? 0. : last <= f.slots / 2 ? 1.6 / 2.4 : 1.);
+    const double cost = waves * ((L + f.size * kW * steps - 1) / (f.size * kW * steps) + 1) * f.round;
+    if (cost < least * 0.999) least = cost, best = f.size;
+  }
+  return best;
 }
 
 template <typename Kernel>
