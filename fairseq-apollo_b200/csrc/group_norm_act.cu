@@ -9,8 +9,12 @@
 // Second pass: every block folds the partial results of its groups, in their order, and does the elementwise part.  A sequence of
 // one run needs no partial results: the same block does both, in one launch.
 //
-// Bound: HBM, each value once: the second pass goes backwards, over what the first has just left in L2, and a call that is larger
-// much larger than that goes through L2 in pieces of sequences.
+// Small calls are held in shared memory by clusters of blocks, in one pass (gn_held_*).
+//
+// Bound: HBM, but for the held calls with every input twice: what the second pass, which goes backwards, finds in L2 of the first
+// saves it little, as its 16 special-function operations to a vector take as long (16 x 4096 x 512 bf16, 32 groups, forward: 17 us
+// for the first pass, 28 for the second, 25 for a copy; 6 x 32768 x 1024 207 us, 0.89 of the measured copy rate over the three
+// passes).  Calls in pieces that fit L2 were slower by their launches (54 against 45 us, 324 against 445 backward at the larger).
 //
 // Statistics: a thread adds up d = x - p and d^2 with p the first value of its run.  p being one of the n values, the squares about
 // it are at most n + 1 times those about the mean, so n <= kRun bounds what their difference loses; such entries are then joined by
@@ -29,7 +33,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRun = 64;        // steps of a thread at most
-constexpr int kGroups = 256;    // groups of a tile at most (a vector or more each, or the 128 bytes of a narrow tile)
+constexpr int kGroups = 256;    // groups of a tile at most
 
 struct GnArgs {
   const void *x, *dy;
@@ -41,7 +45,6 @@ struct GnArgs {
   int ng, tiles;               // groups of a tile, tiles of a row
   int nv, lanes;               // vectors of a tile's row, rows that a block takes at once
   int steps, runs;             // steps of a block, blocks of a sequence
-  int from;                    // this launch's first sequence
   float over_nv, over_size, over_vectors;   // reciprocals: of a row's vectors, a group's channels, a group's vectors
   float eps, offset;
   int silu;
@@ -49,7 +52,6 @@ struct GnArgs {
   float *mean, *rstd;
   float *part, *chan;          // partial results of a run: of its groups (3 or 2 values), backward: of its channels (2)
   float *dgamma, *dbeta;
-  int params;                  // blocks behind the others that add up dgamma, dbeta
 };
 
 // kV neighbouring channels: as pairs of fp32 values (packed arithmetic; with one channel the second of the pair is idle)
@@ -126,7 +128,7 @@ struct Where {
   int nv, lanes, v, r;                           // vectors of a row, rows at once; this thread's vector and row
   bool on;
   __device__ __forceinline__ Where(const GnArgs& a, bool back) {
-    b = a.from + (back ? gridDim.z - 1 - blockIdx.z : blockIdx.z);
+    b = back ? gridDim.z - 1 - blockIdx.z : blockIdx.z;
     tile = back ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
     run = back ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
     c0 = tile * a.ng * a.size;
@@ -981,20 +983,21 @@ int check_gn(int dtype, int B, int L, int D, int G, std::initializer_list<const 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 struct Plan {
-  int ng, tiles, steps, runs, piece;   // piece: sequences that a pass leaves in L2 for the next
-  bool held;                           // in one pass, the runs of a sequence a cluster
+  int ng, tiles, steps, runs;
+  bool held;   // in one pass, the runs of a sequence a cluster
 };
 constexpr int kHeldRow = 64;   // bytes of a row of a held tile at least
-constexpr long long kL2 = 200ll << 20;   // bytes of inputs of such a piece
 
 Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
   const int es = elem_size(dtype), size = D / G, arrays = bwd ? 2 : 1, blocks = (bwd ? 3 : 4) * 148;   // (all at once on the device)
-  if (vec == 0) return {G, 1, L, 1, B, false};
+  if (vec == 0) return {G, 1, L, 1, false};
   Plan p;
   p.held = false;
   if (vec * es == 16 && size % vec == 0) {
-    // Held in one pass where eight blocks hold a sequence's steps of a tile of 64 bytes or more; wider tiles as long as no further
-    // block is needed for them and the device stays full.
+    // Held in one pass where eight blocks hold a sequence's steps of a tile of 64 bytes or more, and all of the call are on the device
+    // at once (B = 7, L = 314, D = 768, 16 groups forward and backward 8.6 and 13.9 us, in two passes 10.6 and 17.6; in several
+    // waves, which load and compute by turns, B = 32, L = 1024, D = 1024 backward 97 us against 75); wider tiles as long as no
+    // further block is needed for them and the device stays full.
     const int places = bwd ? kHeldBack / 2 : kHeld;
     auto lanes_of = [&](int ng) { return kThreads / (ng * size / vec); };
     auto blocks_of = [&](int ng) { return (L + places * lanes_of(ng) - 1) / (places * lanes_of(ng)); };
@@ -1004,7 +1007,7 @@ Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
       while (2 * ng <= G && 2 * ng * size <= kThreads * vec && blocks_of(2 * ng) == blocks_of(ng) &&
              (long long)B * ((G + 2 * ng - 1) / (2 * ng)) * blocks_of(ng) >= 3 * 148)
         ng *= 2;
-      p.ng = ng, p.tiles = (G + ng - 1) / ng, p.runs = blocks_of(ng), p.piece = B, p.held = true;
+      p.ng = ng, p.tiles = (G + ng - 1) / ng, p.runs = blocks_of(ng), p.held = true;
       p.steps = (L + p.runs - 1) / p.runs;
       return p;
     }
@@ -1031,7 +1034,6 @@ Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
   const long long runs = std::max<long long>(least, std::min<long long>(waves * blocks / slices, L / (8ll * lanes)));
   p.steps = (int)((L + runs - 1) / runs);
   p.runs = (L + p.steps - 1) / p.steps;
-  p.piece = p.runs == 1 ? B : (int)std::min<long long>(B, std::max<long long>(1, kL2 / std::max<long long>(1, (long long)L * D * es * arrays)));
   return p;
 }
 
@@ -1056,24 +1058,18 @@ void fill(GnArgs& a, const Plan& p, int vec) {
   a.over_nv = 1.f / (float)a.nv, a.over_size = 1.f / (float)a.size, a.over_vectors = 1.f / (float)std::max(1, a.size / vec);
 }
 
-// first pass, second pass, piece by piece
 template <typename First, typename Second>
-void passes(First first, Second second, GnArgs a, int piece, cudaStream_t s) {
-  for (a.from = 0; a.from < a.B; a.from += piece) {
-    const dim3 grid(a.runs, a.tiles, std::min(piece, a.B - a.from));
-    if (a.from == 0)
-      launch(first, grid, dim3(kThreads), kPlaces + kRing, s, a);
-    else
-      launch_after(first, grid, dim3(kThreads), kPlaces + kRing, s, a);
-    if (a.runs > 1) launch_after(second, grid, dim3(kThreads), kPlaces + kRing, s, a);
-  }
+void passes(First first, Second second, const GnArgs& a, cudaStream_t s) {
+  const dim3 grid(a.runs, a.tiles, a.B);
+  launch(first, grid, dim3(kThreads), kPlaces + kRing, s, a);
+  if (a.runs > 1) launch_after(second, grid, dim3(kThreads), kPlaces + kRing, s, a);
 }
 template <typename T, int kV, bool kOne>
-void run_one(bool bwd, const GnArgs& a, const Plan& p, cudaStream_t s) {
+void run_one(bool bwd, const GnArgs& a, cudaStream_t s) {
   if (bwd)
-    passes(gn_sums_kernel<T, kV, kOne>, gn_grads_kernel<T, kV, kOne>, a, p.piece, s);
+    passes(gn_sums_kernel<T, kV, kOne>, gn_grads_kernel<T, kV, kOne>, a, s);
   else
-    passes(gn_first_kernel<T, kV, kOne>, gn_second_kernel<T, kV, kOne>, a, p.piece, s);
+    passes(gn_first_kernel<T, kV, kOne>, gn_second_kernel<T, kV, kOne>, a, s);
 }
 template <typename Kernel>
 void launch_held(Kernel kernel, bool bwd, const GnArgs& a, cudaStream_t s) {
@@ -1098,9 +1094,9 @@ template <typename T, int kV>
 void run_vec(bool bwd, const GnArgs& a, const Plan& p, cudaStream_t s) {
   if constexpr (kV * sizeof(T) == 16) {
     if (p.held) return launch_held(bwd ? gn_held_back_kernel<T, kV> : gn_held_kernel<T, kV>, bwd, a, s);
-    if (a.size % kV == 0) return run_one<T, kV, true>(bwd, a, p, s);
+    if (a.size % kV == 0) return run_one<T, kV, true>(bwd, a, s);
   }
-  run_one<T, kV, kV == 1>(bwd, a, p, s);
+  run_one<T, kV, kV == 1>(bwd, a, s);
 }
 template <typename T>
 void run_gn(bool bwd, int vec, const GnArgs& a, const Plan& p, cudaStream_t s) {

@@ -854,6 +854,9 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x_, const Tensor&
   if (out.defined()) {
     check_state(out, x_, D, "h_out");
     expect(out.scalar_type() == at::kFloat && out.is_contiguous(), "h_out must be contiguous float32");
+    // (each value is read where it is written, so the whole of h or nothing of it)
+    const char *to = static_cast<const char*>(out.data_ptr()), *from = h.defined() ? static_cast<const char*>(h.data_ptr()) : nullptr;
+    expect(!from || to == from || to + out.nbytes() <= from || from + h.nbytes() <= to, "h_out overlaps h and is not h");
   } else {
     out = floats({B, D}, x);
   }

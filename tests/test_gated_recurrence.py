@@ -280,6 +280,26 @@ def test_long_and_wide(long, gate):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cluster", [1, 2, 4, 8])
+def test_every_split_of_the_time_axis(cluster):
+    """the same call over clusters of 1 to 8 blocks, padded, with documents, reversed; no wait gave up"""
+    import fairseq_apollo_b200 as M
+    from fairseq_apollo_b200 import _lib
+    _lib.device_error(reset=True)
+    try:
+        _lib.set_option(8, cluster)
+        for dtype, gate, D in ((torch.bfloat16, False, 64), (torch.float16, True, 70), (torch.float32, True, 65), (torch.float32, False, 128),
+                               (torch.bfloat16, True, 33)):
+            for L in (3, 700, 2049):
+                r = inputs(2, L, D, dtype, gate, L + cluster, "any" if L == 700 else None, "docs" if L > 700 else None)
+                check_all(run_all(M, r, L == 700), r, L == 700, dtype)
+                assert _lib.last_kernel() == "gated_recurrence"
+    finally:
+        _lib.set_option(8, 0)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.gpu
 def test_gates_far_open_and_closed():
     """f up to +-200: leaks that vanish, states that are forgotten at once; everything stays finite"""
     import fairseq_apollo_b200 as M
@@ -489,6 +509,9 @@ def test_refusals():
                                     h_out=torch.zeros(8, 2, device="cuda").t())
     with pytest.raises(ValueError):
         M.ops.gated_recurrence_step(x, x)
+    states = torch.zeros(3, 8, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        M.ops.gated_recurrence_step(x[:, 0], x[:, 0], h=states[:2], h_out=states[1:])
     xg = x.clone().requires_grad_()
     g = M.gated_recurrence(xg, x)
     with pytest.raises(RuntimeError, match="second"):

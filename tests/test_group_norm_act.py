@@ -209,12 +209,24 @@ def test_against_64_bits(shape, dtype, activation):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(1, 40000, 16, 2), (2, 5000, 520, 8), (150, 64, 64, 1), (40, 600, 128, 64), (1, 20000, 130, 1), (3, 4096, 256, 8),
-                                   (1, 9000, 64, 2)])
+                                   (1, 9000, 64, 2), (1, 30000, 96, 32), (6, 6000, 264, 11)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_long_and_wide(shape, dtype):
     import fairseq_apollo_b200 as M
     args = inputs(*shape[:3], dtype, 5, "right" if shape[0] == 3 else None)
     check_all(run_all(M, *args, shape[3], "silu"), *args, shape[3], "silu")
+
+
+@pytest.mark.gpu
+def test_forms():
+    """small calls in one pass over clusters, larger ones in two: the shapes above reach both"""
+    import fairseq_apollo_b200 as M
+    from fairseq_apollo_b200 import _lib
+    for shape, groups, held in (((3, 4096, 256), 8, True), ((2, 1000, 64), 8, True), ((1, 40000, 16), 2, False), ((6, 6000, 264), 11, False)):
+        norm = M.GroupNorm(shape[2], groups, activation="silu").cuda()
+        with torch.no_grad():
+            norm(torch.randn(shape, device="cuda").bfloat16())
+        assert (_lib.last_kernel() == "group_norm_held") == held, shape
 
 
 @pytest.mark.gpu
