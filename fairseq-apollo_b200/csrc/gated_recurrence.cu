@@ -47,6 +47,7 @@ struct RecArgs {
   const float *h_in, *dh_out;
   float *h_out, *starts, *dh_in;
   int L, D, pairs;   // pairs: whether two floats of a state lie on 8 bytes
+  int tiles, units;   // of a row's channels, of the call
 };
 
 // Steps of a segment: what h_loc and A of every step (the backward: leak, state and, with an input gate, its two factors) leave of
@@ -298,6 +299,22 @@ __device__ __forceinline__ bool idle(unsigned flags) {   // all padded, and no r
   return flags == (1u << kS) - 1u;
 }
 
+// Where a warp is: its sequence (-1: behind the last), the tile's first channel, its place in time.  Serial: a warp walks a sequence's
+// tile by itself, and nobody waits for anybody, which is what many short sequences take.
+struct Place {
+  int w, lane, b, size, rank, c0;
+  __device__ __forceinline__ Place(const RecArgs& a, bool serial) {
+    w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (serial) {
+      const int unit = blockIdx.x * kW + w;
+      b = unit < a.units ? unit / a.tiles : -1;
+      c0 = (unit % a.tiles) * kC, size = 1, rank = 0;
+    } else {
+      b = blockIdx.y, size = cluster_size(), rank = size > 1 ? cluster_rank() : 0, c0 = (blockIdx.x / size) * kC;
+    }
+  }
+};
+
 // What the warps of a block, and the blocks of a cluster, tell one another.  Two of each: a place is written again only after every
 // reader has taken part in the round between.
 struct Post {
@@ -379,7 +396,7 @@ __device__ __forceinline__ bool exchange(const Map& own, f32x2& carry, f32x2& in
 }
 
 // ---- forward ---------------------------------------------------------------------------------
-template <typename T, bool kGate, int kMode>
+template <typename T, bool kGate, int kMode, bool kSerial>
 __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
   constexpr int kS = kForwardSteps<T>, kSave = kBackSteps<T, kGate>, kOps = kGate ? 3 : 2;
   using Op = Tile<T, kS, kMode>;
@@ -387,18 +404,19 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
   constexpr bool kFour = kMode == 16 && sizeof(T) == 2;   // (the other forms have no registers left for it)
   extern __shared__ __align__(16) char smem[];
   __shared__ Post post;
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
-  const int size = cluster_size(), rank = size > 1 ? cluster_rank() : 0;
-  const int c0 = (blockIdx.x / size) * kC, chans = min(a.D - c0, kC), n = min(max(chans - 2 * lane, 0), 2);
+  const Place p(a, kSerial);
+  if (kSerial && p.b < 0) return;
+  const int w = p.w, lane = p.lane, b = p.b, size = p.size, rank = p.rank, c0 = p.c0, chans = min(a.D - c0, kC);
+  const int n = min(max(chans - 2 * lane, 0), 2);
   const long long state = (long long)b * a.D + c0 + 2 * lane;
   const T *x = (const T*)a.x + b * a.xsb + c0, *f = (const T*)a.f + b * a.fsb + c0, *i = kGate ? (const T*)a.i + b * a.isb + c0 : nullptr;
   T* y = (T*)a.y + b * a.ysb + c0 + 2 * lane;
   char* ring = smem + w * (kStages * kOps * Op::kBytes);
-  const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kSave - 1) / kSave;
+  const int stride = kSerial ? kS : size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kSave - 1) / kSave;
   const bool reset = a.reset != nullptr, whole = kPair && chans == kC;
   bool alive = true;
 
-  auto first = [&](int k) { return (k * size + rank) * (kW * kS) + w * kS; };
+  auto first = [&](int k) { return kSerial ? k * kS : (k * size + rank) * (kW * kS) + w * kS; };
   bool flag = flag_of(a, b, first(0), kS, lane);
   // sets round k's tile on its way and returns its padding and resets, which came a round earlier: a segment of padding is not read
   auto fetch = [&](int k) {
@@ -416,7 +434,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
     return flags;
   };
 
-  if (size > 1) {
+  if (!kSerial && size > 1) {
     if (threadIdx.x == 0) {
       mbar_init(&post.bar[0], 1);
       mbar_init(&post.bar[1], 1);
@@ -466,8 +484,14 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
       }
     }
     f32x2 in;
-    alive = reset ? exchange<1, true, kFour>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive)
-                  : exchange<1, false, kFour>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive);
+    if (kSerial) {
+      in = carry;
+      const Map m = idle<kS>(flags) ? Map{pack2(1.f, 1.f), pack2(0.f, 0.f)} : loc[kS - 1];
+      carry = reset ? m.operator()<true>(in) : m.operator()<false>(in);
+    } else {
+      alive = reset ? exchange<1, true, kFour>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive)
+                    : exchange<1, false, kFour>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive);
+    }
     const int t0 = first(k);
     if (a.starts) {
 #pragma unroll
@@ -495,15 +519,15 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
         if (t0 + s < a.L) put<kPair>(yt + s * a.ysl, (flags >> s) & 1u ? pack2(0.f, 0.f) : loc[s].operator()<true>(in), n);
     }
   }
-  if (size > 1) {   // (no block's shared memory goes before all are through)
+  if (!kSerial && size > 1) {   // (no block's shared memory goes before all are through)
     cluster_arrive();
     cluster_wait();
   }
-  if (a.h_out && rank == 0 && w == kW - 1) put_state(a.h_out + state, carry, n, a.pairs);
+  if (a.h_out && (kSerial || (rank == 0 && w == kW - 1))) put_state(a.h_out + state, carry, n, a.pairs);
 }
 
 // ---- backward --------------------------------------------------------------------------------
-template <typename T, bool kGate, int kMode>
+template <typename T, bool kGate, int kMode, bool kSerial>
 __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
   constexpr int kS = kBackSteps<T, kGate>, kOps = kGate ? 4 : 3;
   using Op = Tile<T, kS, kMode>;
@@ -511,21 +535,22 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
   constexpr bool kFour = kMode == 16 && sizeof(T) == 2;   // (the other forms have no registers left for it)
   extern __shared__ __align__(16) char smem[];
   __shared__ Post post;
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
-  const int size = cluster_size(), rank = size > 1 ? cluster_rank() : 0;
-  const int c0 = (blockIdx.x / size) * kC, chans = min(a.D - c0, kC), n = min(max(chans - 2 * lane, 0), 2);
+  const Place p(a, kSerial);
+  if (kSerial && p.b < 0) return;
+  const int w = p.w, lane = p.lane, b = p.b, size = p.size, rank = p.rank, c0 = p.c0, chans = min(a.D - c0, kC);
+  const int n = min(max(chans - 2 * lane, 0), 2);
   const long long state = (long long)b * a.D + c0 + 2 * lane;
   const T *x = (const T*)a.x + b * a.xsb + c0, *f = (const T*)a.f + b * a.fsb + c0, *dy = (const T*)a.dy + b * a.gsb + c0;
   const T* i = kGate ? (const T*)a.i + b * a.isb + c0 : nullptr;
   T *dx = (T*)a.dx + b * a.dxb + c0 + 2 * lane, *df = (T*)a.df + b * a.dfb + c0 + 2 * lane;
   T* di = kGate ? (T*)a.di + b * a.dib + c0 + 2 * lane : nullptr;
   char* ring = smem + w * (kStages * kOps * Op::kBytes);
-  const int stride = size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
+  const int stride = kSerial ? kS : size * kW * kS, rounds = (a.L + stride - 1) / stride, segs = (a.L + kS - 1) / kS;
   const bool reset = a.reset != nullptr, whole = kPair && chans == kC;
   bool alive = true;
 
   f32x2 start = pack2(0.f, 0.f);
-  auto first = [&](int k) { return ((rounds - 1 - k) * size + rank) * (kW * kS) + w * kS; };   // (round k is the k-th from the end)
+  auto first = [&](int k) { return kSerial ? (rounds - 1 - k) * kS : ((rounds - 1 - k) * size + rank) * (kW * kS) + w * kS; };   // (round k is the k-th from the end)
   bool flag = flag_of(a, b, first(0), kS, lane);
   auto fetch = [&](int k) {
     const unsigned flags = __ballot_sync(0xffffffffu, flag);
@@ -544,7 +569,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
     return flags;
   };
 
-  if (size > 1) {
+  if (!kSerial && size > 1) {
     if (threadIdx.x == 0) {
       mbar_init(&post.bar[0], 1);
       mbar_init(&post.bar[1], 1);
@@ -606,8 +631,13 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
       }
     }
     f32x2 q;
-    alive = reset ? exchange<-1, true, kFour>(m, carry, q, post, k, w, lane, rank, size, alive)
-                  : exchange<-1, false, kFour>(m, carry, q, post, k, w, lane, rank, size, alive);
+    if (kSerial) {
+      q = carry;
+      carry = reset ? m.operator()<true>(q) : m.operator()<false>(q);
+    } else {
+      alive = reset ? exchange<-1, true, kFour>(m, carry, q, post, k, w, lane, rank, size, alive)
+                    : exchange<-1, false, kFour>(m, carry, q, post, k, w, lane, rank, size, alive);
+    }
     const int t0 = first(k);
     T *xt = dx + t0 * a.dxl, *ft = df + t0 * a.dfl, *it = kGate ? di + t0 * a.dil : nullptr;
     auto out_step = [&](int s, bool pad, int count) {
@@ -641,11 +671,11 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
       }
     }
   }
-  if (size > 1) {
+  if (!kSerial && size > 1) {
     cluster_arrive();
     cluster_wait();
   }
-  if (a.dh_in && rank == 0 && w == 0) put_state(a.dh_in + state, carry, n, a.pairs);
+  if (a.dh_in && (kSerial || (rank == 0 && w == 0))) put_state(a.dh_in + state, carry, n, a.pairs);
 }
 
 // ---- single step -----------------------------------------------------------------------------
@@ -666,7 +696,8 @@ __global__ void __launch_bounds__(128) rec_step_kernel(RecArgs a) {
 int check_rec(int dtype, int B, int L, int D, std::initializer_list<const void*> acts, std::initializer_list<const void*> f32) {
   if (!valid_dtype(dtype)) return MEGA_ERR_DTYPE;
   if (B <= 0 || L <= 0 || D <= 0) return MEGA_ERR_SHAPE;
-  if (B > 65535 || L > INT_MAX - 8192) return MEGA_ERR_UNSUPPORTED;   // (steps are counted past the end by up to two strides)
+  // (steps are counted past the end by up to two strides; tiles of all sequences by an int)
+  if (B > 65535 || L > INT_MAX - 8192 || ((long long)D + kC - 1) / kC * B > INT_MAX - kW) return MEGA_ERR_UNSUPPORTED;
   for (const void* p : acts)
     if (!aligned_to(p, elem_size(dtype))) return MEGA_ERR_ALIGN;
   for (const void* p : f32)
@@ -686,7 +717,7 @@ int mode_of(int es, std::initializer_list<Operand> in, std::initializer_list<Ope
   return es == 4 || (all(in, 4) && all(out, 4)) ? 4 : 2;
 }
 
-// Blocks to a cluster: what is predicted to take the least time.  A round takes two blocks on a multiprocessor about 2.4 us and one
+// Blocks to a cluster, 0 for serial warps: what is predicted to take the least time.  A round takes two blocks on a multiprocessor about 2.4 us and one
 // block 1.6 (bf16 forward; the other forms' ratios are alike), a cluster's exchange some more; a launch is rounds and one to begin
 // with, in as many waves as it has blocks for (the device holds that many clusters at once).  Measured, bf16 forward, clusters of
 // 1, 2, 4, 8: B = 8, L = 4096, D = 1024 56, 49, 54, 61 us; B = 1, L = 65536, D = 2048 791, 498, 262, 190; B = 8, L = 4096,
@@ -694,6 +725,8 @@ int mode_of(int es, std::initializer_list<Operand> in, std::initializer_list<Ope
 int cluster_of(int tiles, int B, int L, int steps) {
   const int forced = g_options[OPT_REC_CLUSTER].load(std::memory_order_relaxed);
   if (forced == 1 || forced == 2 || forced == 4 || forced == 8) return forced;
+  const long long units = (long long)tiles * B;
+  if (forced == 16) return 0;
   struct Form {
     int size, slots;
     double round;
@@ -707,11 +740,18 @@ int cluster_of(int tiles, int B, int L, int steps) {
     const double cost = waves * ((L + f.size * kW * steps - 1) / (f.size * kW * steps) + 1) * f.round;
     if (cost < least * 0.999) least = cost, best = f.size;
   }
-  return best;
+  const long long slots = 296 * kW, last = units % slots;
+  const double waves = (double)(units / slots) + (last == 0 ? 0. : last <= slots / 2 ? 1.6 / 2.4 : 1.);
+  return waves * ((L + steps - 1) / steps + 1) < least ? 0 : best;
 }
 
 template <typename Kernel>
 void launch_rec(Kernel kernel, int tiles, int B, int cluster, size_t smem, cudaStream_t s, const RecArgs& a) {
+  if (cluster == 0) {
+    launch(kernel, dim3((a.units + kW - 1) / kW), dim3(kW * 32), smem, s, a);
+    g_last_kernel.store("gated_recurrence serial", std::memory_order_relaxed);
+    return;
+  }
   allow_smem(reinterpret_cast<const void*>(kernel), smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * cluster, B);
@@ -730,10 +770,14 @@ void launch_rec(Kernel kernel, int tiles, int B, int cluster, size_t smem, cudaS
 }
 
 template <typename T, bool kGate, int kMode>
-void run_mode(bool bwd, int B, const RecArgs& a, cudaStream_t s) {
+void run_mode(bool bwd, int B, RecArgs a, cudaStream_t s) {
   const int steps = bwd ? kBackSteps<T, kGate> : kForwardSteps<T>, tiles = (a.D + kC - 1) / kC, cluster = cluster_of(tiles, B, a.L, steps);
   const size_t smem = size_t(kW) * kStages * ((kGate ? 3 : 2) + (bwd ? 1 : 0)) * steps * kC * sizeof(T);
-  launch_rec(bwd ? rec_bwd_kernel<T, kGate, kMode> : rec_fwd_kernel<T, kGate, kMode>, tiles, B, cluster, smem, s, a);
+  a.tiles = tiles, a.units = tiles * B;
+  if (cluster == 0)
+    launch_rec(bwd ? rec_bwd_kernel<T, kGate, kMode, true> : rec_fwd_kernel<T, kGate, kMode, true>, tiles, B, 0, smem, s, a);
+  else
+    launch_rec(bwd ? rec_bwd_kernel<T, kGate, kMode, false> : rec_fwd_kernel<T, kGate, kMode, false>, tiles, B, cluster, smem, s, a);
 }
 template <typename T>
 void run_rec(bool bwd, int mode, int B, const RecArgs& a, cudaStream_t s) {

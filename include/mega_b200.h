@@ -100,7 +100,7 @@ MEGA_API uint64_t mega_launch_count(void);
                             forward in leading parts alone),
                             0: where it is estimated to be faster */
 #define MEGA_OPT_CHUNK_STEPS 7 /* steps of a segment of that form, rounded up to a multiple of 64; 0: as estimated */
-#define MEGA_OPT_REC_CLUSTER 8 /* gated recurrence: 1, 2, 4, 8 blocks share the time axis of a tile; 0: as estimated */
+#define MEGA_OPT_REC_CLUSTER 8 /* gated recurrence: 1, 2, 4, 8 blocks share the time axis of a tile, 16: a warp by itself; 0: as estimated */
 MEGA_API int mega_set_option(int key, int value);
 /*
  * Test aid: name of the kernel family of this process's most recent launch ("tsn_ema_mma tile=7 pipe=1",

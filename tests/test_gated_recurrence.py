@@ -280,9 +280,9 @@ def test_long_and_wide(long, gate):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("cluster", [1, 2, 4, 8])
+@pytest.mark.parametrize("cluster", [1, 2, 4, 8, 16])
 def test_every_split_of_the_time_axis(cluster):
-    """the same call over clusters of 1 to 8 blocks, padded, with documents, reversed; no wait gave up"""
+    """the same call over clusters of 1 to 8 blocks and by warps alone, padded, with documents, reversed; no wait gave up"""
     import fairseq_apollo_b200 as M
     from fairseq_apollo_b200 import _lib
     _lib.device_error(reset=True)
@@ -293,7 +293,7 @@ def test_every_split_of_the_time_axis(cluster):
             for L in (3, 700, 2049):
                 r = inputs(2, L, D, dtype, gate, L + cluster, "any" if L == 700 else None, "docs" if L > 700 else None)
                 check_all(run_all(M, r, L == 700), r, L == 700, dtype)
-                assert _lib.last_kernel() == "gated_recurrence"
+                assert _lib.last_kernel() == "gated_recurrence" + (" serial" if cluster == 16 else "")
     finally:
         _lib.set_option(8, 0)
     assert _lib.device_error() == 0
