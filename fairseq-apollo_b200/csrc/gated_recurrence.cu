@@ -294,6 +294,13 @@ template <int kS>
 __device__ __forceinline__ bool all_padded(unsigned flags) {
   return (flags & ((1u << kS) - 1u)) == (1u << kS) - 1u;
 }
+// Resets alone: the walks then take them by selections instead of branches (a block waits for its slowest warp, and one of its eight
+// segments has a reset in every sixth round at documents of 700 steps).
+__device__ __forceinline__ bool only_resets(unsigned flags) { return flags != 0 && (flags & 0xffffu) == 0; }
+// whether a reset lies at step s of a segment; at it or before; at it or behind
+__device__ __forceinline__ bool cut_at(unsigned flags, int s) { return (flags >> (16 + s)) & 1u; }
+__device__ __forceinline__ bool cut_until(unsigned flags, int s) { return (flags >> 16) & ((2u << s) - 1u); }
+__device__ __forceinline__ bool cut_from(unsigned flags, int s) { return flags >> (16 + s); }
 template <int kS>
 __device__ __forceinline__ bool idle(unsigned flags) {   // all padded, and no reset
   return flags == (1u << kS) - 1u;
@@ -469,6 +476,14 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
         step(s);
         loc[s] = {A, h};
       }
+    } else if (only_resets(flags)) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        h = cut_at(flags, s) ? pack2(0.f, 0.f) : h;
+        step(s);
+        A = cut_until(flags, s) ? minus_zero() : A;
+        loc[s] = {A, h};
+      }
     } else if (idle<kS>(flags)) {
       loc[kS - 1] = {A, h};
     } else {
@@ -505,6 +520,12 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         put<kPair>(yt, loc[s].operator()<false>(in), 2);
+        yt += a.ysl;
+      }
+    } else if (only_resets(flags) && whole) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        put<kPair>(yt, cut_until(flags, s) ? loc[s].h : loc[s].operator()<false>(in), 2);
         yt += a.ysl;
       }
     } else if (idle<kS>(flags)) {
@@ -612,6 +633,18 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
       for (int s = 0; s < kS; ++s) state_step(s);
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) grad_step(s);
+    } else if (only_resets(flags)) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        h = cut_at(flags, s) ? pack2(0.f, 0.f) : h;
+        state_step(s);
+      }
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) {
+        grad_step(s);
+        m.h = cut_at(flags, s) ? pack2(0.f, 0.f) : m.h;
+        m.a = cut_from(flags, s) ? minus_zero() : m.a;
+      }
     } else if (!idle<kS>(flags)) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
@@ -654,6 +687,12 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_bwd_kernel(RecArgs a) {
     if (flags == 0 && whole) {
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) out_step(s, false, 2);
+    } else if (only_resets(flags) && whole) {
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) {
+        out_step(s, false, 2);
+        q = cut_at(flags, s) ? pack2(0.f, 0.f) : q;
+      }
     } else if (idle<kS>(flags)) {
 #pragma unroll 4
       for (int s = 0; s < min(kS, a.L - t0); ++s) {
