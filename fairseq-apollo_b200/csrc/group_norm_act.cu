@@ -18,7 +18,8 @@
 //
 // Statistics: a thread adds up d = x - p and d^2 with p the first value of its run.  p being one of the n values, the squares about
 // it are at most n + 1 times those about the mean, so n <= kRun bounds what their difference loses; such entries are then joined by
-// counts, means and squared deviations: the mean of all first, then the deviations about it.
+// counts, means and squared deviations: the mean of all first, then the deviations about it (Chan's rule, entry after entry with its
+// divisions, took the first pass 1.7 us a block).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -176,7 +177,8 @@ __device__ __forceinline__ void read_mask(const GnArgs& a, const Where<kV>& p, S
 
 // The thread's rows of the block, in order or back.  begin() sets the first of them on their way to the thread's own places in
 // shared memory, run(f) calls f(values, address, first, live) for each (live: not padded; address: of the output's vector
-// there).  What a block has under way so takes no registers, and begins before what the rows are needed for is known.
+// there).  What a block has under way so takes no registers, and begins before what the rows are needed for is known (16 x 4096 x
+// 512 bf16, 32 groups: 64 us with rows of the ring asked for in order, 45 with them under way before the launch before has ended).
 template <typename T, int kV, int kOps>
 struct Walk {
   using V = Vec<T, kV>;
