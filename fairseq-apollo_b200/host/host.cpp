@@ -889,7 +889,9 @@ class RecFn : public torch::autograd::Function<RecFn> {
     Tensor y = rec_like(r.x), h = want_state ? floats({r.B, r.D}, x) : Tensor(), starts = floats({r.B, (r.L + seg - 1) / seg, r.D}, x);
     run_rec(r, y, h, starts, w);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({x, given(f), given(i), r.pad, r.reset, given(h_in), starts});
+    ctx->save_for_backward({x, given(f), given(i), r.pad, r.reset, starts});
+    // (of the state that came in its type alone is needed: the caller may go on to write over it)
+    ctx->saved_data["state"] = r.h_in.defined() ? (int64_t)h_in->scalar_type() : (int64_t)-1;
     ctx->saved_data["reverse"] = reverse;
     ctx->saved_data["packed"] = packed;
     if (!want_state) return {y};
@@ -900,7 +902,8 @@ class RecFn : public torch::autograd::Function<RecFn> {
     first_order();
     const auto s = ctx->get_saved_variables();
     const int64_t packed = ctx->saved_data["packed"].toInt();
-    const Tensor &z = s[0], &starts = s[6], &h_in = s[5];
+    const Tensor &z = s[0], &starts = s[5];
+    const int64_t state = ctx->saved_data["state"].toInt();
     const Where w(z);
     const int64_t d = packed ? z.size(2) / packed : z.size(2);
     auto part = [&](const Tensor& t, int64_t k) { return t.narrow(2, k * d, d); };
@@ -912,13 +915,13 @@ class RecFn : public torch::autograd::Function<RecFn> {
     Tensor dz = packed ? at::empty(z.sizes(), z.options().requires_grad(false)) : Tensor();
     Tensor dx = packed ? part(dz, 0) : rec_like(x), df = packed ? part(dz, 1) : rec_like(f), di;
     if (i.defined()) di = packed ? part(dz, 2) : rec_like(i);
-    Tensor dh_in = h_in.defined() ? floats({x.size(0), d}, x) : Tensor();
+    Tensor dh_in = state >= 0 ? floats({x.size(0), d}, x) : Tensor();
     check(mega_gated_recurrence_bwd(dy.data_ptr(), x.data_ptr(), f.data_ptr(), ptr(i), dx.data_ptr(), df.data_ptr(), ptr(di),
                                     dtype_of(x), (int)x.size(0), (int)x.size(1), (int)d, STRIDES2(dy), STRIDES2(x), STRIDES2(f),
                                     STRIDES2(i), STRIDES2(dx), STRIDES2(df), STRIDES2(di), ptr<uint8_t>(s[3]), ptr<uint8_t>(s[4]),
                                     fptr(starts), fptr(dh_out), fptr(dh_in), ctx->saved_data["reverse"].toBool() ? MEGA_REC_REVERSE : 0u,
                                     w.stream), "gated_recurrence_bwd");
-    if (dh_in.defined()) dh_in = dh_in.to(h_in.scalar_type());
+    if (dh_in.defined()) dh_in = dh_in.to((at::ScalarType)state);
     return {packed ? dz : dx, packed ? Tensor() : df, packed ? Tensor() : di, Tensor(), Tensor(), dh_in, Tensor(), Tensor(), Tensor()};
   }
 };

@@ -460,6 +460,60 @@ def test_truncated_backpropagation_through_states():
 
 
 @pytest.mark.gpu
+def test_state_alone_and_states_written_over():
+    """a gradient through the state that leaves only; the state that came in, in 16 bits, overwritten before the backward"""
+    import fairseq_apollo_b200 as M
+    r = inputs(2, 50, 24, torch.float32, True, 31)
+    leaves = [r[k].cuda().requires_grad_() for k in ("x", "f", "i", "h_in")]
+    _, h = M.gated_recurrence(*leaves[:3], h_in=leaves[3], want_state=True)
+    got = torch.autograd.grad(h, leaves, r["dh"].cuda())
+    want = reference(r["x"], r["f"], r["i"], h_in=r["h_in"], dy=torch.zeros_like(r["dy"]), dh=r["dh"])
+    for g, k in zip(got, ("dx", "df", "di", "dh")):
+        close(g, want[k], k)
+    state = r["h_in"].cuda().bfloat16()
+    h0 = state.clone().requires_grad_()
+    y, h = M.gated_recurrence(leaves[0], leaves[1], h_in=h0 * 1, want_state=True)
+    assert torch.autograd.grad(y.sum(), h0, retain_graph=True)[0].dtype == torch.bfloat16
+    y, h = M.gated_recurrence(leaves[0], leaves[1], h_in=state, want_state=True)
+    state.copy_(h.detach())
+    y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_more_than_31_bits_of_values():
+    """offsets past 2^31 values: the end of a long call, against the same steps by themselves behind the state before them"""
+    import fairseq_apollo_b200 as M
+    L, D, tail = 270000, 8192, 300
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(1, L, D, device="cuda", dtype=torch.bfloat16, generator=gen)
+    f = torch.randn(1, L, D, device="cuda", dtype=torch.bfloat16, generator=gen)
+    assert x.numel() > 2 ** 31
+    with torch.no_grad():
+        y, h = M.gated_recurrence(x, f, want_state=True)
+        _, mid = M.gated_recurrence(x[:, :L - tail], f[:, :L - tail], want_state=True)
+        z, end = M.gated_recurrence(x[:, L - tail:], f[:, L - tail:], h_in=mid, want_state=True)
+    # (the same values joined at other places: states of size 1 within some 2^-21, outputs a bf16 step more)
+    assert float((h - end).abs().max()) < 2.0 ** -20
+    assert float((y[:, L - tail:].float() - z.float()).abs().max()) < 2.0 ** -7 * float(z.abs().max())
+    del y, z
+    xg, fg = x[:, L - 3 * tail:].clone(), f[:, L - 3 * tail:].clone()
+    x.requires_grad_(), f.requires_grad_()
+    y, h = M.gated_recurrence(x, f, want_state=True)
+    dx, df = torch.autograd.grad(h, [x, f], torch.ones_like(h))
+    xg.requires_grad_(), fg.requires_grad_()
+    with torch.no_grad():
+        _, mid = M.gated_recurrence(x[:, :L - 3 * tail], f[:, :L - 3 * tail], want_state=True)
+    _, h = M.gated_recurrence(xg, fg, h_in=mid, want_state=True)
+    a, b = torch.autograd.grad(h, [xg, fg], torch.ones_like(h))
+    # (segments begin elsewhere, so sums differ in their last bits and a rounding to bf16 may go the other way: one step, eps of the
+    # value.  dx is at most 1, df = q l (h - x) at most a quarter of |h| + |x| < 16)
+    for full, part, top in ((dx, a, 1.0), (df, b, 4.0)):
+        assert float((full[:, L - 3 * tail:].float() - part.float()).abs().max()) <= torch.finfo(torch.bfloat16).eps * top
+
+
+@pytest.mark.gpu
 def test_no_steps_no_sequences():
     import fairseq_apollo_b200 as M
     h = torch.randn(3, 8, device="cuda")

@@ -400,6 +400,30 @@ def test_repeats_bit_for_bit_on_streams_and_in_graphs():
 
 
 @pytest.mark.gpu
+def test_more_than_31_bits_of_values():
+    """offsets past 2^31 values: the last group of a long call against that group by itself"""
+    import fairseq_apollo_b200 as M
+    L, D, size = 270000, 8192, 16
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    x = torch.randn(1, L, D, device="cuda", dtype=torch.bfloat16, generator=torch.Generator(device="cuda").manual_seed(0))
+    x += 1
+    norm = M.GroupNorm(D, D // size, activation="silu").cuda()
+    x.requires_grad_()
+    y = norm(x)
+    dx, dw, db = torch.autograd.grad(y, [x, norm.weight, norm.bias], y.detach())
+    xl = x.detach()[..., -size:].to(F64).requires_grad_()
+    w, c = torch.zeros(size, device="cuda", dtype=F64, requires_grad=True), torch.zeros(size, device="cuda", dtype=F64, requires_grad=True)
+    z = (xl - xl.mean()) / (xl.var(unbiased=False) + 1e-5).sqrt() * (1 + w) + c
+    want = torch.nn.functional.silu(z)
+    grads = torch.autograd.grad(want, [xl, w, c], y.detach()[..., -size:].to(F64))
+    assert float((y.detach()[..., -size:].to(F64) - want).norm() / want.norm()) < 2.0 ** -8
+    assert float((dx[..., -size:].to(F64) - grads[0]).norm() / grads[0].norm()) < 2.0 ** -8
+    for a, b in ((dw, grads[1]), (db, grads[2])):
+        assert float((a[-size:].to(F64) - b).norm() / b.norm()) < 1e-5
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_norm_then_recurrence(dtype):
     """the two together, as a layer of an encoder takes them: norm and activation, gates, walks in both directions"""
