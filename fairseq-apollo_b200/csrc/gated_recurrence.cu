@@ -22,7 +22,7 @@
 // Bound: HBM where the blocks fill the device (B = 64, L = 1024, D = 2048 bf16: forward 135 us, backward 230, 0.91 and 0.89 of the
 // measured copy rate over 3 and 5 arrays).  With fewer it is the rounds: a multiprocessor takes some 1.2 us for a block's tile, of
 // which the special-function operations of the gates are 0.55 and its instructions 0.6, and an exchange through a cluster adds 0.3
-// to 0.7 (B = 8, L = 4096, D = 2048 76 and 130 us; B = 1, L = 65536, D = 2048 191 and 307, 0.64 and 0.67).
+// to 0.7 (B = 8, L = 4096, D = 2048 75 and 128 us; B = 1, L = 65536, D = 2048 190 and 305, 0.64 and 0.67).  Masks cost 2 % more.
 // What was tried there and no faster: leaks of the next tile taken while a block waits (203 and 347 us, registers); stages of the
 // gates' operations batched over 4, 8 and 16 rows (210, 210, 205); three stages of the ring (198); segments of 8 steps and three
 // blocks to a multiprocessor (255); blocks of four warps (better where there are four for each multiprocessor and more, worse
