@@ -48,4 +48,22 @@ __device__ __forceinline__ f32x2 minus_sigmoid2(f32x2 v) {
   return minus_over_one_and(exp_pair<T, kSign>(v));
 }
 
+// The sides of a gate, sigmoid(v) and sigmoid(-v), are held as the smaller of them, g <= 1/2, to its last places: the other is
+// 1 - g to its own.  v >= 0: c = -g = -sigmoid(-v); v < 0: c = g = sigmoid(v).
+template <typename T>
+__device__ __forceinline__ f32x2 gate_side2(f32x2 v) {
+  const f32x2 e = exp_pair<T, 1>(v | 0x8000000080000000ull);   // e^-|v|
+  return mul2(e, minus_over_one_and(e)) ^ (v & 0x8000000080000000ull);
+}
+// all bits where c says v >= 0 (by its sign: g may be 0)
+__device__ __forceinline__ f32x2 open_bits(f32x2 c) {
+  float a, b;
+  unpack2(c, a, b);
+  return pack2(__int_as_float(__float_as_int(a) >> 31), __int_as_float(__float_as_int(b) >> 31));
+}
+__device__ __forceinline__ f32x2 either(f32x2 bits, f32x2 a, f32x2 b) { return (a & bits) | (b & ~bits); }
+// u sigmoid(v) and u sigmoid(-v): u + c u and c u, or c u and u + c u
+__device__ __forceinline__ f32x2 pass(f32x2 c, f32x2 open, f32x2 u) { return fma2(c, u, u & open); }
+__device__ __forceinline__ f32x2 hold_back(f32x2 c, f32x2 open, f32x2 u) { return fma2(c ^ 0x8000000080000000ull, u, u & ~open); }
+
 }  // namespace mega
