@@ -6,7 +6,8 @@
 // round it to a few bits, the same way at every step.  Where a gate is closed (f << 0) it is the decay k that is small, and 1 - l
 // has few of its bits, or none: there h = x + k (h - x), and the gradient of f, k l times the rest, has k as it is.  fp32 calls take the
 // smaller of l and k at every step (gate_side2); 16-bit calls l alone, and walk a segment with the sides when one of its gates is
-// closed that far (the sides for all segments: B = 64, L = 1024, D = 2048 bf16 forward 150 us against 137, backward 292 against 231).
+// closed that far (the sides for all segments: B = 64, L = 1024, D = 2048 bf16 forward 150 us against 137, backward 292 against 231;
+// both walks where every segment has such a gate: B = 8, L = 4096, D = 2048 forward 156 us against 74, backward 335 against 122).
 //
 // A run of steps maps the state that enters it linearly to the one that leaves, h -> h_loc + A h (h_loc: from a zero state,
 // A: the product of the decays), and such maps compose, so the time axis is split: a warp takes 64 channels (two to a lane) of
@@ -22,6 +23,13 @@
 //
 // A reset is a map that ignores what enters: its A is -0 (the decays are never negative), and A = -0 means h_loc alone, so
 // that nothing infinite or NaN passes.
+//
+// Infinities.  As the recurrence has it, an infinite state stays until a reset or the other infinity comes, and a state between two
+// large values is no larger than they are.  h - x of such values overflows, an infinity less its leak is NaN, and so is one times a
+// product of decays that has underflowed: all of them mark the values behind them as not finite.  Each lane keeps what it has seen
+// of that (a product with 0 a round); where it has, one warp goes through the tile's steps in order at the end, and what had come out
+// not finite is replaced (0.5 us a step forward and 0.9 backward, until all is NaN: joining infinite maps as they come cost calls that
+// have none 3 to 12 %).
 // Bound: HBM where the blocks fill the device (B = 64, L = 1024, D = 2048 bf16: forward 135 us, backward 230, 0.91 and 0.89 of the
 // measured copy rate over 3 and 5 arrays).  With fewer it is the rounds: a multiprocessor takes some 1.2 us for a block's tile, of
 // which the special-function operations of the gates are 0.55 and its instructions 0.6, and an exchange through a cluster adds 0.3
@@ -371,6 +379,7 @@ struct Post {
   float4 warps[2][kW][32], blocks[2][8][32];
   f32x2 carry[2][32];
   uint64_t bar[2];
+  unsigned odd;   // lanes of the cluster (in its first block) that have seen values that are not finite
 };
 
 // Every warp's map -> the state that enters each; `carry` is the state that enters the whole stride, then the next one (in a block
@@ -445,13 +454,217 @@ __device__ __forceinline__ bool exchange(const Map& own, f32x2& carry, f32x2& in
   return alive;
 }
 
+// ---- values that are not finite ----------------------------------------------------------------
+// adds to what a lane has seen: NaN once it was not finite
+__device__ __forceinline__ float seen(float odd, f32x2 v) {
+  float a, b;
+  unpack2(v, a, b);
+  return fmaf(a, 0.f, fmaf(b, 0.f, odd));
+}
+__device__ __forceinline__ unsigned odd_lanes(float odd) {
+  return __ballot_sync(0xffffffffu, isnan(odd));
+}
+// The same of all warps of a block, or of a cluster for its first block, which then may write over what the others have written.
+__device__ __forceinline__ unsigned odd_lanes(float odd, Post& post, const Place& p) {
+  const unsigned own = odd_lanes(odd);
+  if (own && p.lane == 0) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(&post.odd)));
+    asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(at), "r"(own) : "memory");
+  }
+  if (p.size > 1) {   // (nor does any block's shared memory go before all are through)
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  return post.odd;
+}
+
+// which of a lane's values in a run of steps (bit 2 s + j) are not finite; plain loads, as this call has written them
+template <int kS, typename T>
+__device__ __forceinline__ unsigned not_finite(const T* p, long long stride, int rows, int n) {
+  float v[kS][2];
+#pragma unroll
+  for (int s = 0; s < kS; ++s)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[s][j] = s < rows && j < n ? Elem<T>::ld_shared(p + s * stride + j) : 0.f;
+  unsigned r = 0;
+#pragma unroll
+  for (int s = 0; s < kS; ++s)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) r |= (isfinite(v[s][j]) ? 0u : 1u) << (2 * s + j);
+  return r;
+}
+// the values that `which` asks for
+template <typename T>
+__device__ __forceinline__ void mend(T* p, unsigned which, const float (&v)[2]) {
+  if (which & 1u) Elem<T>::st(p, v[0]);
+  if (which & 2u) Elem<T>::st(p + 1, v[1]);
+}
+__device__ __forceinline__ f32x2 unless_finite(f32x2 v, f32x2 other) {
+  float a, b, c, d;
+  unpack2(v, a, b), unpack2(other, c, d);
+  return pack2(isfinite(a) ? a : c, isfinite(b) ? b : d);
+}
+
+// One step of one channel, any values: the gate's two sides, or with an input gate its side and slope, and what it makes of them.
+template <typename T, bool kGate>
+struct Step {
+  float c, side, into, slope;   // side: of the forget gate, the smaller; into: the input gate
+  bool open;
+  __device__ __forceinline__ Step(float f, float i) {
+    float s;
+    unpack2(gate_side2<T>(pack2(f, kGate ? i : 0.f)), c, s);
+    open = signbit(c), side = fabsf(c), into = signbit(s) ? 1.f + s : s, slope = fabsf(s) * (1.f - fabsf(s));
+  }
+  // a gate of this value on u; infinite u as it is (an infinity less a part of it, or 0 times it where the gate has underflowed, is
+  // NaN), NaN where the gate is
+  static __device__ __forceinline__ float on(float r, float u, float gate) { return isinf(u) ? fmaf(gate, 0.f, u) : r; }
+  __device__ __forceinline__ float keep(float u) const { return on(fmaf(c, u, open ? u : 0.f), u, c); }
+  __device__ __forceinline__ float leak(float u) const { return on(fmaf(-c, u, open ? 0.f : u), u, c); }
+  __device__ __forceinline__ float enter(float u) const { return kGate ? on(into * u, u, into) : leak(u); }
+  __device__ __forceinline__ float next(float h, float x) const { return keep(h) + enter(x); }
+};
+
+// NaN in all of these channels, to the end: there is no reset
+__device__ __forceinline__ bool nothing_left(const RecArgs& a, bool mine, const float (&v)[2], int n) {
+  return a.reset == nullptr && __all_sync(0xffffffffu, !mine || (isnan(v[0]) && (n < 2 || isnan(v[1]))));
+}
+
+// The forward of some lanes' channels, step by step, by a warp; the state behind the last one.  ring: tiles of the warp's own.
+template <typename T, bool kGate, int kMode>
+__device__ __noinline__ f32x2 forward_again(const RecArgs& a, char* ring, int b, int c0, unsigned lanes) {
+  constexpr int kS = kForwardSteps<T>, kSave = kBackSteps<T, kGate>;
+  using Op = Tile<T, kS, kMode>;
+  const int lane = threadIdx.x & 31, chans = min(a.D - c0, kC), n = min(max(chans - 2 * lane, 0), 2), c = c0 + 2 * lane;
+  const int segs = (a.L + kSave - 1) / kSave;
+  const bool mine = (lanes >> lane) & 1u;
+  const T* op = reinterpret_cast<const T*>(ring) + 2 * lane;
+  float h[2] = {0.f, 0.f};
+  for (int j = 0; j < n; ++j) h[j] = a.h_in ? a.h_in[(long long)b * a.D + c + j] : 0.f;
+#pragma unroll 1
+  for (int t0 = 0; t0 < a.L; t0 += kS) {
+    const int rows = min(kS, a.L - t0);
+    const unsigned flags = flags_of(flag_byte(a, b, t0, kS, lane));   // (and the tile before has been read)
+    Op::fetch(ring, (const T*)a.x + b * a.xsb + c0, a.xsl, t0, rows, chans, lane);
+    Op::fetch(ring + Op::kBytes, (const T*)a.f + b * a.fsb + c0, a.fsl, t0, rows, chans, lane);
+    if (kGate) Op::fetch(ring + 2 * Op::kBytes, (const T*)a.i + b * a.isb + c0, a.isl, t0, rows, chans, lane);
+    copies_commit();
+    T* y = (T*)a.y + b * a.ysb + t0 * a.ysl + c;
+    unsigned which = mine ? not_finite<kS>(y, a.ysl, rows, n) : 0u;
+    copies_wait<0>();
+    __syncwarp();
+    if (mine) {
+#pragma unroll 1
+      for (int s = 0; s < rows; ++s) {
+        if (a.starts && s % kSave == 0) {
+          float* p = a.starts + ((long long)b * segs + (t0 + s) / kSave) * a.D + c;
+          mend(p, not_finite<1>(p, 0, 1, n), h);
+        }
+        if ((flags >> (16 + s)) & 1u) h[0] = h[1] = 0.f;
+        if (!((flags >> s) & 1u)) {
+          float x[2], f[2], i[2] = {0.f, 0.f};
+          unpack2(two(op + s * kC), x[0], x[1]), unpack2(two(op + (kS + s) * kC), f[0], f[1]);
+          if (kGate) unpack2(two(op + (2 * kS + s) * kC), i[0], i[1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) h[j] = Step<T, kGate>(f[j], i[j]).next(h[j], x[j]);
+          mend(y, which >> (2 * s), h);
+        }
+        y += a.ysl;
+      }
+    }
+    if (nothing_left(a, mine, h, n)) break;
+  }
+  return pack2(h[0], h[1]);
+}
+
+// The backward: the states of a segment from the saved one, then its steps in reverse; the gradient of the state that came in.
+template <typename T, bool kGate, int kMode>
+__device__ __noinline__ f32x2 backward_again(const RecArgs& a, char* ring, int b, int c0, unsigned lanes) {
+  constexpr int kS = kBackSteps<T, kGate>, kOps = kGate ? 4 : 3;
+  using Op = Tile<T, kS, kMode>;
+  static_assert(kS * kC * (int)sizeof(float) <= (kStages - 1) * kOps * Op::kBytes, "states of a segment behind the operands");
+  const int lane = threadIdx.x & 31, chans = min(a.D - c0, kC), n = min(max(chans - 2 * lane, 0), 2), c = c0 + 2 * lane;
+  const int segs = (a.L + kS - 1) / kS;
+  const bool mine = (lanes >> lane) & 1u;
+  const T* op = reinterpret_cast<const T*>(ring) + 2 * lane;
+  float2* before = reinterpret_cast<float2*>(ring + kOps * Op::kBytes) + lane;
+  float q[2] = {0.f, 0.f};
+  for (int j = 0; j < n; ++j) q[j] = a.dh_out ? a.dh_out[(long long)b * a.D + c + j] : 0.f;
+#pragma unroll 1
+  for (int k = segs - 1; k >= 0; --k) {
+    const int t0 = k * kS, rows = min(kS, a.L - t0);
+    const unsigned flags = flags_of(flag_byte(a, b, t0, kS, lane));
+    Op::fetch(ring, (const T*)a.x + b * a.xsb + c0, a.xsl, t0, rows, chans, lane);
+    Op::fetch(ring + Op::kBytes, (const T*)a.f + b * a.fsb + c0, a.fsl, t0, rows, chans, lane);
+    Op::fetch(ring + 2 * Op::kBytes, (const T*)a.dy + b * a.gsb + c0, a.gsl, t0, rows, chans, lane);
+    if (kGate) Op::fetch(ring + 3 * Op::kBytes, (const T*)a.i + b * a.isb + c0, a.isl, t0, rows, chans, lane);
+    copies_commit();
+    T *dx = (T*)a.dx + b * a.dxb + t0 * a.dxl + c, *df = (T*)a.df + b * a.dfb + t0 * a.dfl + c;
+    T* di = kGate ? (T*)a.di + b * a.dib + t0 * a.dil + c : nullptr;
+    unsigned bad_x = 0, bad_f = 0, bad_i = 0;
+    float h[2] = {0.f, 0.f};
+    if (mine) {
+      for (int j = 0; j < n; ++j) h[j] = a.starts[((long long)b * segs + k) * a.D + c + j];
+      bad_x = not_finite<kS>(dx, a.dxl, rows, n), bad_f = not_finite<kS>(df, a.dfl, rows, n);
+      if (kGate) bad_i = not_finite<kS>(di, a.dil, rows, n);
+    }
+    copies_wait<0>();
+    __syncwarp();
+    auto gates = [&](int s, float (&f)[2], float (&i)[2]) {
+      unpack2(two(op + (kS + s) * kC), f[0], f[1]);
+      i[0] = i[1] = 0.f;
+      if (kGate) unpack2(two(op + (3 * kS + s) * kC), i[0], i[1]);
+    };
+    if (mine) {
+#pragma unroll 1
+      for (int s = 0; s < rows; ++s) {
+        if ((flags >> (16 + s)) & 1u) h[0] = h[1] = 0.f;
+        before[s * (kC / 2)] = make_float2(h[0], h[1]);
+        if ((flags >> s) & 1u) continue;
+        float x[2], f[2], i[2];
+        gates(s, f, i);
+        unpack2(two(op + s * kC), x[0], x[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) h[j] = Step<T, kGate>(f[j], i[j]).next(h[j], x[j]);
+      }
+#pragma unroll 1
+      for (int s = rows - 1; s >= 0; --s) {
+        if (!((flags >> s) & 1u)) {
+          const float2 hs = before[s * (kC / 2)];
+          float x[2], f[2], i[2], g[2], ox[2], of[2], oi[2];
+          gates(s, f, i);
+          unpack2(two(op + s * kC), x[0], x[1]), unpack2(two(op + (2 * kS + s) * kC), g[0], g[1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const Step<T, kGate> e(f[j], i[j]);
+            const float u = q[j] + g[j], rest = e.on(fmaf(-e.side, u, u), u, e.c), from = j ? hs.y : hs.x;
+            // (half of h - x, which may be past the largest value, and twice the side)
+            const float half = kGate ? 0.5f * from : fmaf(0.5f, from, -0.5f * x[j]);
+            ox[j] = e.enter(u), of[j] = (half * rest) * (2.f * e.side), oi[j] = (x[j] * u) * e.slope;
+            q[j] = e.keep(u);
+          }
+          mend(dx + s * a.dxl, bad_x >> (2 * s), ox);
+          mend(df + s * a.dfl, bad_f >> (2 * s), of);
+          if (kGate) mend(di + s * a.dil, bad_i >> (2 * s), oi);
+        }
+        if ((flags >> (16 + s)) & 1u) q[0] = q[1] = 0.f;
+      }
+    }
+    if (nothing_left(a, mine, q, n)) break;
+  }
+  return pack2(q[0], q[1]);
+}
+
 // ---- forward ---------------------------------------------------------------------------------
 template <typename T, bool kGate, int kMode, bool kSerial>
-__global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
+__global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(const __grid_constant__ RecArgs a) {
   constexpr int kS = kForwardSteps<T>, kSave = kBackSteps<T, kGate>, kOps = kGate ? 3 : 2;
   using Op = Tile<T, kS, kMode>;
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
-  constexpr bool kFour = kMode == 16 && sizeof(T) == 2;   // (the other forms have no registers left for it)
+  constexpr bool kFour = kMode == 16 && sizeof(T) == 2;   // (the other forms and the backward have no registers left for it)
   extern __shared__ __align__(16) char smem[];
   __shared__ Post post;
   const Place p(a, kSerial);
@@ -484,6 +697,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
     return flags;
   };
 
+  if (!kSerial && threadIdx.x == 0) post.odd = 0;   // (added to behind the first round's barriers)
   if (!kSerial && size > 1) {
     if (threadIdx.x == 0) {
       mbar_init(&post.bar[0], 1);
@@ -493,6 +707,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
     cluster_arrive();   // (every block has begun, and its barriers are there, before another writes to it)
   }
   f32x2 carry = get_state(a.h_in ? a.h_in + state : nullptr, n, a.pairs);
+  float odd = 0.f;   // see seen()
   unsigned flags, next = fetch(0);
   for (int k = 0; k < rounds; ++k) {
     flags = next;
@@ -516,43 +731,48 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
       } else {
         least.see(fs);
         const f32x2 nl = minus_leak2<T>(two(fs));
-        h = kGate ? fma2(nl, h, fma2(in, xv, h)) : fma2(nl, sub2(h, xv), h);
+        h = kGate ? fma2(in, xv, fma2(nl, h, h)) : fma2(nl, sub2(h, xv), h);
         A = fma2(nl, A, A);
       }
     };
-    bool walk = false;   // step by step, with the gates' sides
+    constexpr std::bool_constant<kSides<T>> usual;
+    auto by_step = [&](auto sides) {   // padded steps among them
+      h = pack2(0.f, 0.f), A = pack2(1.f, 1.f);
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        if ((flags >> (16 + s)) & 1u) odd = seen(odd, h), h = pack2(0.f, 0.f), A = minus_zero();
+        if (!((flags >> s) & 1u)) {
+          const f32x2 before = A;
+          step(s, sides);
+          if (before == minus_zero()) A = minus_zero();
+        }
+        loc[s] = {A, h};
+      }
+    };
+    bool walk = false;   // with the gates' sides
     if (flags == 0) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
-        step(s, std::bool_constant<kSides<T>>{});
+        step(s, usual);
         loc[s] = {A, h};
       }
     } else if (only_resets(flags)) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
+        odd = seen(odd, h);
         h = cut_at(flags, s) ? pack2(0.f, 0.f) : h;
-        step(s, std::bool_constant<kSides<T>>{});
+        step(s, usual);
         A = cut_until(flags, s) ? minus_zero() : A;
         loc[s] = {A, h};
       }
     } else if (idle<kS>(flags)) {
       loc[kS - 1] = {A, h};
+    } else if (!kSides<T>) {
+      by_step(usual);
     } else {
       walk = true;
     }
-    if (walk || least.closed()) {
-      h = pack2(0.f, 0.f), A = pack2(1.f, 1.f);
-#pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        if ((flags >> (16 + s)) & 1u) h = pack2(0.f, 0.f), A = minus_zero();
-        if (!((flags >> s) & 1u)) {
-          const f32x2 before = A;
-          step(s, std::true_type{});
-          if (before == minus_zero()) A = minus_zero();
-        }
-        loc[s] = {A, h};
-      }
-    }
+    if (walk || least.closed()) by_step(std::true_type{});
     f32x2 in;
     if (kSerial) {
       in = carry;
@@ -562,6 +782,7 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
       alive = reset ? exchange<1, true, kFour>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive)
                     : exchange<1, false, kFour>(loc[kS - 1], carry, in, post, k, w, lane, rank, size, alive);
     }
+    odd = seen(seen(odd, h), in);
     const int t0 = first(k);
     if (a.starts) {
 #pragma unroll
@@ -595,21 +816,25 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(RecArgs a) {
         if (t0 + s < a.L) put<kPair>(yt + s * a.ysl, (flags >> s) & 1u ? pack2(0.f, 0.f) : loc[s].operator()<true>(in), n);
     }
   }
-  if (!kSerial && size > 1) {   // (no block's shared memory goes before all are through)
-    cluster_arrive();
-    cluster_wait();
+  const Place e = kSerial ? p : Place(a, false);   // (again: it costs registers through the rounds)
+  const unsigned again = kSerial ? odd_lanes(odd) : odd_lanes(odd, post, e);
+  if (kSerial || (e.rank == 0 && e.w == kW - 1)) {
+    const int n = min(max(a.D - e.c0 - 2 * e.lane, 0), 2);
+    if (again) {
+      const f32x2 last = forward_again<T, kGate, kMode>(a, smem + e.w * (kStages * kOps * Op::kBytes), e.b, e.c0, again);
+      if ((again >> e.lane) & 1u) carry = unless_finite(carry, last);
+    }
+    if (a.h_out) put_state(a.h_out + (long long)e.b * a.D + e.c0 + 2 * e.lane, carry, n, a.pairs);
   }
-  if (a.h_out && (kSerial || (rank == 0 && w == kW - 1))) put_state(a.h_out + state, carry, n, a.pairs);
 }
 
 // ---- backward --------------------------------------------------------------------------------
 // (fp32 with an input gate: a block's 145 KB of shared memory leave a multiprocessor no second one, so it may have all registers)
 template <typename T, bool kGate, int kMode, bool kSerial>
-__global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_bwd_kernel(RecArgs a) {
+__global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_bwd_kernel(const __grid_constant__ RecArgs a) {
   constexpr int kS = kBackSteps<T, kGate>, kOps = kGate ? 4 : 3;
   using Op = Tile<T, kS, kMode>;
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
-  constexpr bool kFour = kMode == 16 && sizeof(T) == 2;   // (the other forms have no registers left for it)
   extern __shared__ __align__(16) char smem[];
   __shared__ Post post;
   const Place p(a, kSerial);
@@ -646,6 +871,7 @@ __global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_
     return flags;
   };
 
+  if (!kSerial && threadIdx.x == 0) post.odd = 0;   // (added to behind the first round's barriers)
   if (!kSerial && size > 1) {
     if (threadIdx.x == 0) {
       mbar_init(&post.bar[0], 1);
@@ -655,6 +881,7 @@ __global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_
     cluster_arrive();
   }
   f32x2 carry = get_state(a.dh_out ? a.dh_out + state : nullptr, n, a.pairs);
+  float odd = 0.f;   // see seen()
   unsigned flags, next = fetch(0);
   for (int k = 0; k < rounds; ++k) {
     flags = next;
@@ -681,7 +908,7 @@ __global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_
       } else {
         least.see(fs);
         c[s] = minus_leak2<T>(two(fs));
-        h = kGate ? fma2(c[s], h, fma2(gate[s], xv, h)) : fma2(c[s], v[s], h);
+        h = kGate ? fma2(gate[s], xv, fma2(c[s], h, h)) : fma2(c[s], v[s], h);
       }
     };
     Map m = {pack2(1.f, 1.f), pack2(0.f, 0.f)};
@@ -697,7 +924,27 @@ __global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_
       }
     };
     constexpr std::bool_constant<kSides<T>> usual;
-    bool walk = false;   // step by step, with the gates' sides
+    auto by_step = [&](auto sides) {   // padded steps among them
+      h = enters;
+      m = {pack2(1.f, 1.f), pack2(0.f, 0.f)};
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        if ((flags >> (16 + s)) & 1u) odd = seen(odd, h), h = pack2(0.f, 0.f);
+        c[s] = v[s] = pack2(0.f, 0.f);
+        if (kGate) gate[s] = slope[s] = pack2(0.f, 0.f);
+        if (!((flags >> s) & 1u)) state_step(s, sides);
+      }
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) {
+        if (!((flags >> s) & 1u)) {
+          const f32x2 before = m.a;
+          grad_step(s, sides);
+          if (before == minus_zero()) m.a = minus_zero();
+        }
+        if ((flags >> (16 + s)) & 1u) odd = seen(odd, m.h), m = {minus_zero(), pack2(0.f, 0.f)};
+      }
+    };
+    bool walk = false;   // with the gates' sides
     if (flags == 0) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) state_step(s, usual);
@@ -706,47 +953,34 @@ __global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_
     } else if (only_resets(flags)) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
+        odd = seen(odd, h);
         h = cut_at(flags, s) ? pack2(0.f, 0.f) : h;
         state_step(s, usual);
       }
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) {
         grad_step(s, usual);
+        odd = seen(odd, m.h);
         m.h = cut_at(flags, s) ? pack2(0.f, 0.f) : m.h;
         m.a = cut_from(flags, s) ? minus_zero() : m.a;
       }
+    } else if (!kSides<T> && !idle<kS>(flags)) {
+      by_step(usual);
     } else {
       walk = !idle<kS>(flags);
     }
     walk = walk || least.closed();
-    if (walk) {
-      h = enters;
-      m = {pack2(1.f, 1.f), pack2(0.f, 0.f)};
-#pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        if ((flags >> (16 + s)) & 1u) h = pack2(0.f, 0.f);
-        c[s] = v[s] = pack2(0.f, 0.f);
-        if (kGate) gate[s] = slope[s] = pack2(0.f, 0.f);
-        if (!((flags >> s) & 1u)) state_step(s, std::true_type{});
-      }
-#pragma unroll
-      for (int s = kS - 1; s >= 0; --s) {
-        if (!((flags >> s) & 1u)) {
-          const f32x2 before = m.a;
-          grad_step(s, std::true_type{});
-          if (before == minus_zero()) m.a = minus_zero();
-        }
-        if ((flags >> (16 + s)) & 1u) m = {minus_zero(), pack2(0.f, 0.f)};
-      }
-    }
+    if (walk) by_step(std::true_type{});
     f32x2 q;
     if (kSerial) {
       q = carry;
       carry = reset ? m.operator()<true>(q) : m.operator()<false>(q);
     } else {
-      alive = reset ? exchange<-1, true, kFour>(m, carry, q, post, k, w, lane, rank, size, alive)
-                    : exchange<-1, false, kFour>(m, carry, q, post, k, w, lane, rank, size, alive);
+      alive = reset ? exchange<-1, true, false>(m, carry, q, post, k, w, lane, rank, size, alive)
+                    : exchange<-1, false, false>(m, carry, q, post, k, w, lane, rank, size, alive);
     }
+    if (!idle<kS>(flags)) odd = seen(odd, h);   // (an idle segment has not read its state)
+    odd = seen(seen(odd, m.h), q);
     const int t0 = first(k);
     T *xt = dx + t0 * a.dxl, *ft = df + t0 * a.dfl, *it = kGate ? di + t0 * a.dil : nullptr;
     auto out_step = [&](int s, auto sides, bool pad, int count) {
@@ -795,11 +1029,16 @@ __global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_
       }
     }
   }
-  if (!kSerial && size > 1) {
-    cluster_arrive();
-    cluster_wait();
+  const Place e = kSerial ? p : Place(a, false);   // (again: it costs registers through the rounds)
+  const unsigned again = kSerial ? odd_lanes(odd) : odd_lanes(odd, post, e);
+  if (kSerial || (e.rank == 0 && e.w == 0)) {
+    const int n = min(max(a.D - e.c0 - 2 * e.lane, 0), 2);
+    if (again) {
+      const f32x2 last = backward_again<T, kGate, kMode>(a, smem + e.w * (kStages * kOps * Op::kBytes), e.b, e.c0, again);
+      if ((again >> e.lane) & 1u) carry = unless_finite(carry, last);
+    }
+    if (a.dh_in) put_state(a.dh_in + (long long)e.b * a.D + e.c0 + 2 * e.lane, carry, n, a.pairs);
   }
-  if (a.dh_in && (kSerial || (rank == 0 && w == 0))) put_state(a.dh_in + state, carry, n, a.pairs);
 }
 
 // ---- single step -----------------------------------------------------------------------------
@@ -810,10 +1049,8 @@ __global__ void __launch_bounds__(128) rec_step_kernel(RecArgs a) {
   if (d >= a.D) return;
   const long long at = (long long)b * a.D + d;
   const float h = a.h_in ? a.h_in[at] : 0.f, x = Elem<T>::ld((const T*)a.x + b * a.xsb + d);
-  float c, s;   // (the input gate beside the forget gate)
-  unpack2(gate_side2<T>(pack2(Elem<T>::ld((const T*)a.f + b * a.fsb + d), a.i ? Elem<T>::ld((const T*)a.i + b * a.isb + d) : 0.f)), c, s);
-  const bool open = signbit(c);
-  const float v = a.i ? fmaf(signbit(s) ? 1.f + s : s, x, fmaf(c, h, open ? h : 0.f)) : fmaf(c, h - x, open ? h : x);
+  const float f = Elem<T>::ld((const T*)a.f + b * a.fsb + d);
+  const float v = a.i ? Step<T, true>(f, Elem<T>::ld((const T*)a.i + b * a.isb + d)).next(h, x) : Step<T, false>(f, 0.f).next(h, x);
   Elem<T>::st((T*)a.y + b * a.ysb + d, v);
   a.h_out[at] = v;
 }

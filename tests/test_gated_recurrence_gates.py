@@ -167,3 +167,117 @@ def test_single_steps(dtype, gate):
         ys.append(y)
     close(torch.stack(ys, 1), want["y"], "y")
     close(state, want["h"], "h")
+
+
+# ------------------------------------------------------------ infinite, missing and very large values
+def same_or_close(got, want, what, dtype=None):
+    """within the bound where the 64-bit value is finite in the output's type, the same infinity or NaN elsewhere"""
+    value, bound = want
+    got = got.detach().cpu().to(F64)
+    top = torch.finfo(dtype or torch.float32).max
+    odd = ~(value.abs() <= top)
+    assert torch.equal(got[odd].isnan(), value[odd].isnan()), what
+    assert torch.equal(got[odd].nan_to_num(0.0, 1.0, -1.0).sign(), value[odd].nan_to_num(0.0, 1.0, -1.0).sign()), what
+    assert not torch.isfinite(got[odd]).any(), what
+    close(torch.where(odd, 0.0, got), (torch.where(odd, 0.0, value), torch.where(odd, 1.0, bound)), what)
+
+
+def check_odd(got, r, reverse=False):
+    want = tight(r["x"], r["f"], r["i"], r["pad"], r["reset"], r["h_in"], reverse, r["dy"], r["dh"])
+    for k, v in got.items():
+        same_or_close(v, want[k], k, v.dtype)
+
+
+def odd_values(B, L, D, dtype, gate, seed, what, **kw):
+    """ordinary inputs, some channels of which hold something that is not finite, at the ends and within segments"""
+    r = inputs(B, L, D, dtype, gate, seed, **kw)
+    inf, nan = float("inf"), float("nan")
+    if what in ("state", "all"):
+        r["h_in"][0, 1], r["h_in"][-1, 2], r["h_in"][0, D - 1] = inf, -inf, nan
+        r["h_in"][0, 3] = inf
+        r["x"][0, L // 2, 3] = -inf   # the other infinity: NaN from there
+    if what in ("input", "all"):
+        r["x"][0, L // 3, 5], r["x"][0, 0, 6], r["x"][-1, L - 1, 7] = inf, -inf, nan
+    if what in ("gradient", "all"):
+        r["dy"][0, L // 3, 9], r["dy"][0, 0, 10], r["dy"][-1, L - 1, 11], r["dy"][0, L - 1, 12] = inf, -inf, nan, inf
+        r["dh"][0, 13], r["dh"][-1, 14], r["dh"][0, 12] = inf, -inf, -inf
+    return r
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["state", "input", "gradient", "all"])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinite_values_stay(dtype, gate, what):
+    """an infinite state, input or gradient stays what it is until a reset or the other infinity, through decays whose product is 0 in
+    fp32 too, and changes nothing beside itself"""
+    import fairseq_apollo_b200 as M
+    for L, kw in ((1, {}), (2, {}), (45, {}), (45, {"pad": "any", "reset": "docs"}), (400, {"reset": "docs"}), (700, {})):
+        for reverse in (False, True):
+            r = odd_values(2, L, 66, dtype, gate, L + 1, what, **kw)
+            check_odd(run_all(M, r, reverse), r, reverse)
+    r = odd_values(2, 300, 32, dtype, gate, 3, what)
+    r["f"] = (r["f"] - 3).clamp(max=0).to(dtype)
+    check_odd(run_all(M, r, False), r)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cluster", [1, 2, 4, 8, 16])
+def test_infinite_values_over_every_split(cluster):
+    import fairseq_apollo_b200 as M
+    from fairseq_apollo_b200 import _lib
+    _lib.device_error(reset=True)
+    try:
+        _lib.set_option(8, cluster)
+        for dtype, gate in ((torch.bfloat16, False), (torch.float32, True), (torch.float16, True), (torch.float32, False)):
+            for L, kw in ((700, {"reset": "docs"}), (2100, {}), (90, {"pad": "any"})):
+                r = odd_values(2, L, 70, dtype, gate, L, "all", **kw)
+                check_odd(run_all(M, r, L == 90), r, L == 90)
+    finally:
+        _lib.set_option(8, 0)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinite_values_in_single_steps(dtype, gate):
+    import fairseq_apollo_b200 as M
+    r = odd_values(3, 9, 66, dtype, gate, 5, "all")
+    want = tight(r["x"], r["f"], r["i"], h_in=r["h_in"])
+    state, ys = cuda(r["h_in"]), []
+    for t in range(9):
+        y, state = M.ops.gated_recurrence_step(*(None if r[k] is None else cuda(r[k][:, t]) for k in ("x", "f", "i")), state)
+        ys.append(y)
+    same_or_close(torch.stack(ys, 1), want["y"], "y", dtype)
+    same_or_close(state, want["h"], "h")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_values_next_to_the_largest(dtype):
+    """states and inputs whose difference is past fp32's range: the state between them is not"""
+    import fairseq_apollo_b200 as M
+    for L in (1, 2, 37, 300):
+        r = inputs(2, L, 66, dtype, False, L)
+        r["f"] = (r["f"] - 2).to(dtype)
+        r["x"] = (3e38 * torch.randn(r["x"].shape, generator=torch.Generator().manual_seed(2)).sign()).to(dtype)
+        r["h_in"] = 3e38 * r["h_in"].sign()
+        r["dy"], r["dh"] = (r["dy"] * 0.1).to(dtype), r["dh"] * 0.1
+        got = run_all(M, r, False)
+        assert torch.isfinite(got["y"]).all() and torch.isfinite(got["h"]).all()
+        check_odd(got, r)
+    x, f = r["x"][:, 0], r["f"][:, 0]
+    y, h = M.ops.gated_recurrence_step(cuda(x), cuda(f), None, cuda(r["h_in"]))
+    want = tight(x[:, None], f[:, None], h_in=r["h_in"])
+    close(h, want["h"], "h")
+    close(y[:, None], want["y"], "y")
+    # an input gate: h = 3e38 and a value of the same size add up to no more than that where both are held back
+    big = torch.full((2, 66), 3e38)
+    f, i = torch.full((2, 1, 66), -1.0).to(dtype), torch.full((2, 1, 66), -1.0).to(dtype)
+    x = big[:, None].to(dtype)
+    for h_in in (big, -big):
+        want = tight(x, f, i, h_in=h_in)
+        y, h = M.gated_recurrence(cuda(x), cuda(f), cuda(i), h_in=cuda(h_in), want_state=True)
+        close(h, want["h"], "h")
+        close(M.ops.gated_recurrence_step(cuda(x[:, 0]), cuda(f[:, 0]), cuda(i[:, 0]), cuda(h_in))[1], want["h"], "h")
