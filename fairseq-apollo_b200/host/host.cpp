@@ -818,8 +818,7 @@ void run_rec(const Rec& r, const Tensor& y, const Tensor& h_out, const Tensor& s
 }
 // the output of (B, L, D) operands: time-major ones give a time-major result
 Tensor rec_like(const Tensor& x) {
-  Tensor y = like(x);
-  return y.size(-1) == 1 || y.stride(-1) == 1 ? y : at::empty(x.sizes(), x.options().requires_grad(false));
+  return x.size(-1) == 1 || x.stride(-1) == 1 ? like(x) : at::empty(x.sizes(), x.options().requires_grad(false));
 }
 
 // (y, state behind the last step or None)
@@ -880,7 +879,7 @@ class RecFn : public torch::autograd::Function<RecFn> {
  public:
   static variable_list forward(AutogradContext* ctx, Tensor x, OptTensor f, OptTensor i, OptTensor pad, OptTensor reset, OptTensor h_in,
                                bool want_state, bool reverse, int64_t packed) {
-    const int64_t d = packed ? x.size(2) / packed : x.size(2);
+    const int64_t d = packed ? x.size(2) / packed : 0;   // (x is not checked yet where it is an operand by itself)
     auto part = [&](int64_t k) { return x.detach().narrow(2, k * d, d); };
     const Rec r = packed ? rec_args(part(0), part(1), packed == 3 ? part(2) : Tensor(), given(pad), given(reset), given(h_in), reverse)
                          : rec_args(x, given(f), given(i), given(pad), given(reset), given(h_in), reverse);
@@ -929,8 +928,8 @@ class RecFn : public torch::autograd::Function<RecFn> {
 // (y, h) or (y,); differentiable
 variable_list gated_recurrence_train(const Tensor& x, const Tensor& f, const OptTensor& i, const OptTensor& pad, const OptTensor& reset,
                                      const OptTensor& h_in, bool want_state, bool reverse) {
-  rec_args(x, f, given(i), given(pad), given(reset), given(h_in), reverse);
-  if (x.numel() == 0) {
+  if (x.numel() == 0) {   // (else RecFn checks them, and converts what it has to once)
+    rec_args(x, f, given(i), given(pad), given(reset), given(h_in), reverse);
     variable_list r = {i.has_value() ? x + f + *i : x + f};   // (no values, but gradients of that shape)
     if (want_state) r.push_back(h_in.has_value() ? h_in->to(at::kFloat, false, true) : at::zeros({x.size(0), x.size(2)}, x.options().dtype(at::kFloat)));
     return r;

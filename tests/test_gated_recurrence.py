@@ -683,3 +683,22 @@ def test_module(gate, bidirectional):
     other = M.GatedRecurrence(48, input_gate=gate, bidirectional=bidirectional)
     other.load_state_dict(layer.state_dict())
 
+
+
+@pytest.mark.gpu
+def test_training_converts_its_operands_once():
+    """channels that are not adjacent, integer masks, a 16-bit state: a training forward allocates what inference does, and the saved states"""
+    import fairseq_apollo_b200 as M
+    x, f, i = (torch.randn(2, 24, 40, device="cuda").transpose(1, 2) for _ in range(3))
+    pad, reset = torch.zeros(2, 40, dtype=torch.int32, device="cuda"), torch.zeros(2, 40, dtype=torch.uint8, device="cuda")
+    h = torch.zeros(2, 24, dtype=torch.bfloat16, device="cuda")
+
+    def allocations(x):
+        M.gated_recurrence(x, f, i, pad, reset, h, want_state=True)
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        M.gated_recurrence(x, f, i, pad, reset, h, want_state=True)
+        return torch.cuda.memory_stats()["allocation.all.allocated"] - before
+
+    with torch.no_grad():
+        plain = allocations(x)
+    assert allocations(x.detach().requires_grad_()) == plain + 1
