@@ -837,6 +837,15 @@ std::tuple<Tensor, OptTensor> gated_recurrence(const Tensor& x, const Tensor& f,
   return {y, h};
 }
 
+// Whether a call that reads each value of t (B, D) where it writes that of `out` may do so: t is `out`, value for value, or elsewhere.
+bool in_place_or_apart(const Tensor& out, const Tensor& t) {
+  if (!t.defined() || t.numel() == 0) return true;
+  const char *to = static_cast<const char*>(out.data_ptr()), *from = static_cast<const char*>(t.data_ptr());
+  const int64_t span = ((t.size(0) - 1) * t.stride(0) + (t.size(1) - 1) * t.stride(1) + 1) * t.element_size();
+  if (to + out.nbytes() <= from || from + span <= to) return true;
+  return to == from && t.scalar_type() == out.scalar_type() && t.is_contiguous();
+}
+
 // one step: x, f, i (B, D) -> (y, h'); h' is `h_out` where given, which may be h
 std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x_, const Tensor& f_, const OptTensor& i_, const OptTensor& h_,
                                                  const OptTensor& h_out_) {
@@ -853,9 +862,8 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x_, const Tensor&
   if (out.defined()) {
     check_state(out, x_, D, "h_out");
     expect(out.scalar_type() == at::kFloat && out.is_contiguous(), "h_out must be contiguous float32");
-    // (each value is read where it is written, so the whole of h or nothing of it)
-    const char *to = static_cast<const char*>(out.data_ptr()), *from = h.defined() ? static_cast<const char*>(h.data_ptr()) : nullptr;
-    expect(!from || to == from || to + out.nbytes() <= from || from + h.nbytes() <= to, "h_out overlaps h and is not h");
+    expect(in_place_or_apart(out, h), "h_out overlaps h and is not h");
+    for (const Tensor& t : {x, f, i}) expect(in_place_or_apart(out, t), "h_out overlaps x or a gate and is not it");
   } else {
     out = floats({B, D}, x);
   }

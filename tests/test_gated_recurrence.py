@@ -702,3 +702,20 @@ def test_training_converts_its_operands_once():
     with torch.no_grad():
         plain = allocations(x)
     assert allocations(x.detach().requires_grad_()) == plain + 1
+
+
+@pytest.mark.gpu
+def test_a_step_refuses_halves():
+    import fairseq_apollo_b200 as M
+    f, state = torch.randn(2, 8, device="cuda"), torch.randn(2, 8, device="cuda")
+    whole = torch.randn(3, 8, device="cuda")
+    for args in ((whole[:2], f, None), (f, whole[:2], None), (f, f, whole[:2]), (whole[1:2].expand(2, 8), f, None),
+                 (whole[1:].t().reshape(-1)[:16].view(2, 8).expand(2, 8), f, whole[:2])):
+        with pytest.raises(ValueError, match="overlaps"):
+            M.ops.gated_recurrence_step(*args, state, h_out=whole[1:])
+    half = whole.view(torch.bfloat16)[1:, :8]   # (the same memory in another type)
+    with pytest.raises(ValueError, match="overlaps"):
+        M.ops.gated_recurrence_step(half, half, None, state, h_out=whole[1:])
+    x = torch.randn(2, 8, device="cuda")
+    want = M.ops.gated_recurrence_step(x, f, None, state)[1]
+    assert torch.equal(M.ops.gated_recurrence_step(x, f, None, state, h_out=x)[1], want)   # x itself, value for value
