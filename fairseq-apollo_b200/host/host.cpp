@@ -864,6 +864,7 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x_, const Tensor&
     expect(out.scalar_type() == at::kFloat && out.is_contiguous(), "h_out must be contiguous float32");
     expect(in_place_or_apart(out, h), "h_out overlaps h and is not h");
     for (const Tensor& t : {x, f, i}) expect(in_place_or_apart(out, t), "h_out overlaps x or a gate and is not it");
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();   // (a graph that has saved it must not use the new values)
   } else {
     out = floats({B, D}, x);
   }

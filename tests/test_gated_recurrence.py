@@ -719,3 +719,19 @@ def test_a_step_refuses_halves():
     x = torch.randn(2, 8, device="cuda")
     want = M.ops.gated_recurrence_step(x, f, None, state)[1]
     assert torch.equal(M.ops.gated_recurrence_step(x, f, None, state, h_out=x)[1], want)   # x itself, value for value
+
+
+@pytest.mark.gpu
+def test_a_step_in_place_tells_graphs():
+    import fairseq_apollo_b200 as M
+    f = torch.randn(2, 8, device="cuda")
+    p = torch.ones(2, 8, device="cuda", requires_grad=True)
+    state = torch.randn(2, 8, device="cuda")
+    z = (p * state).sum()   # (keeps the state for p's gradient)
+    M.ops.gated_recurrence_step(f, f, None, state, h_out=state)
+    with pytest.raises(RuntimeError, match="modified"):
+        z.backward()
+    with torch.inference_mode():
+        s = torch.zeros(2, 8, device="cuda")
+        assert M.ops.gated_recurrence_step(f, f, None, s, h_out=s)[1].data_ptr() == s.data_ptr()
+    M.ops.gated_recurrence_step(f, f, None, s, h_out=s)
