@@ -998,17 +998,13 @@ Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
   if (vec * es == 16 && size % vec == 0) {
     // Held in one pass where eight blocks hold a sequence's steps of a tile of 64 bytes or more, and all of the call are on the device
     // at once (B = 7, L = 314, D = 768, 16 groups forward and backward 8.6 and 13.9 us, in two passes 10.6 and 17.6; in several
-    // waves, which load and compute by turns, B = 32, L = 1024, D = 1024 backward 97 us against 75); wider tiles as long as no
-    // further block is needed for them and the device stays full.
+    // waves, which load and compute by turns, B = 32, L = 1024, D = 1024 backward 97 us against 75).
     const int places = bwd ? kHeldBack / 2 : kHeld;
     auto lanes_of = [&](int ng) { return kThreads / (ng * size / vec); };
     auto blocks_of = [&](int ng) { return (L + places * lanes_of(ng) - 1) / (places * lanes_of(ng)); };
     int ng = 1;
     while (ng < G && ng * size * es < kHeldRow) ++ng;
     if (ng * size <= kThreads * vec && blocks_of(ng) <= 8 && (long long)B * ((G + ng - 1) / ng) * blocks_of(ng) <= 3 * 148) {
-      while (2 * ng <= G && 2 * ng * size <= kThreads * vec && blocks_of(2 * ng) == blocks_of(ng) &&
-             (long long)B * ((G + 2 * ng - 1) / (2 * ng)) * blocks_of(ng) >= 3 * 148)
-        ng *= 2;
       p.ng = ng, p.tiles = (G + ng - 1) / ng, p.runs = blocks_of(ng), p.held = true;
       p.steps = (L + p.runs - 1) / p.runs;
       return p;
