@@ -154,6 +154,8 @@ struct Sums {
 };
 // behind it the ring, or what is held; a forward pass of one entry to a vector needs an eighth of the arrays
 constexpr int kPlaces = (sizeof(Sums) + 15) / 16 * 16, kFewer = kPlaces - 2 * kThreads * 7 * (int)sizeof(float);
+// Groups of a held tile at most: a cluster's joined statistics, three values to a group, go to what there is of the arrays then.
+constexpr int kHeldGroups = 2 * kThreads / 3;
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -988,7 +990,9 @@ struct Plan {
   int ng, tiles, steps, runs;
   bool held;   // in one pass, the runs of a sequence a cluster
 };
-constexpr int kHeldRow = 64;   // bytes of a row of a held tile at least
+// Bytes of a row of a held tile at least.  A group has 16 or more of them, and a tile takes no more groups than make them up.
+constexpr int kHeldRow = 64;
+static_assert(kHeldRow / 16 <= kHeldGroups, "a held tile's groups have their places");
 
 Plan plan_of(int dtype, int B, int L, int D, int G, int vec, bool bwd) {
   const int es = elem_size(dtype), size = D / G, arrays = bwd ? 2 : 1, blocks = (bwd ? 3 : 4) * 148;   // (all at once on the device)
