@@ -463,3 +463,30 @@ def test_norm_then_recurrence(dtype):
     assert float((y.detach().cpu().to(F64) - ref).norm() / ref.norm()) < tol
     for g, v in zip(grads, want):
         assert float((g.cpu().to(F64) - v).norm() / v.norm()) < 2 * tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2, 700, 514, 2), (3, 1100, 771, 3), (1, 600, 4104, 1), (2, 530, 2600, 2)])
+def test_groups_wider_than_a_block_over_long_sequences(shape, dtype):
+    """groups of 257 channels and more, padded: runs of 64 values of a thread are joined many times over"""
+    import fairseq_apollo_b200 as M
+    for pad, activation in (("any", "silu"), ("right", "silu"), (None, None)):
+        args = inputs(*shape[:3], dtype, shape[1], pad)
+        check_all(run_all(M, *args, shape[3], activation), *args, shape[3], activation)
+
+
+@pytest.mark.gpu
+def test_wide_groups_off_the_boundaries():
+    """300 channels to a group fit a tile on whole vectors, and take the wide form on odd 16-bit addresses"""
+    import fairseq_apollo_b200 as M
+    for dtype in DTYPES:
+        x, dy, w, c, mask = inputs(2, 400, 600, dtype, 3, "any")
+
+        def odd(t):
+            wide = torch.full(t.shape[:-1] + (t.shape[-1] + 3,), 7.0, dtype=t.dtype, device=t.device)
+            wide[..., 1:601] = t
+            return wide[..., 1:601]
+
+        for shape in (lambda t: t, odd):
+            check_all(run_all(M, x, dy, w, c, mask, 2, "silu", shape), x, dy, w, c, mask, 2, "silu")
