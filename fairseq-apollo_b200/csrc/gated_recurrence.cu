@@ -51,7 +51,7 @@ namespace mega {
 
 namespace {
 
-constexpr int kW = 8;        // segments (warps) of a block: two blocks of 128 registers a thread fit a multiprocessor
+constexpr int kW = 8;        // segments (warps) of a block: two blocks of 128 registers a thread fit a multiprocessor (kResident)
 constexpr int kC = 64;       // channels of a tile: two to a lane, for packed arithmetic; a row is 128 or 256 bytes
 constexpr int kStages = 2;   // tiles of a warp's ring (one is worked on while 64 KB a multiprocessor are on their way)
 
@@ -69,12 +69,17 @@ struct RecArgs {
 };
 
 // Steps of a segment: what h_loc and A of every step (the backward: leak, state and, with an input gate, its two factors) leave of
-// 128 registers; fp32 tiles would not fit the shared memory of two blocks otherwise.  The forward saves the states that the
-// backward's segments start from.
+// 128 registers; fp32 tiles would not fit the shared memory of two blocks otherwise (the backward with an input gate does not with 8
+// either).  The forward saves the states that the backward's segments start from.
 template <typename T, bool kGate>
 constexpr int kBackSteps = sizeof(T) == 4 || kGate ? 8 : 16;
 template <typename T>
 constexpr int kForwardSteps = sizeof(T) == 4 ? 8 : 16;
+// Blocks on a multiprocessor.  The fp32 backward with an input gate has 128 KB of tiles to a block: one, which may have all registers.
+template <typename T, bool kGate, bool kBack>
+constexpr int kResident = kBack && kGate && sizeof(T) == 4 ? 1 : 2;
+template <typename T, bool kGate, bool kBack>
+constexpr int kRingBytes = kW * kStages * ((kGate ? 3 : 2) + (kBack ? 1 : 0)) * (kBack ? kBackSteps<T, kGate> : kForwardSteps<T>) * kC * (int)sizeof(T);
 
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
@@ -381,6 +386,12 @@ struct Post {
   uint64_t bar[2];
   unsigned odd;   // lanes of the cluster (in its first block) that have seen values that are not finite
 };
+// (of a multiprocessor's 228 KB of shared memory a block takes 1 KB besides)
+template <typename T, bool kGate, bool kBack>
+constexpr bool fits() {
+  constexpr int block = kRingBytes<T, kGate, kBack> + (int)sizeof(Post) + 1024;
+  return kResident<T, kGate, kBack> == (2 * block <= (228 << 10) ? 2 : 1);
+}
 
 // Every warp's map -> the state that enters each; `carry` is the state that enters the whole stride, then the next one (in a block
 // by itself: in the last warp alone, the others find it here in the next round).  kDir > 0: in the order of warps and ranks, else
@@ -660,9 +671,10 @@ __device__ __noinline__ f32x2 backward_again(const RecArgs& a, char* ring, int b
 
 // ---- forward ---------------------------------------------------------------------------------
 template <typename T, bool kGate, int kMode, bool kSerial>
-__global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(const __grid_constant__ RecArgs a) {
+__global__ void __launch_bounds__(kW * 32, kResident<T, kGate, false>) rec_fwd_kernel(const __grid_constant__ RecArgs a) {
   constexpr int kS = kForwardSteps<T>, kSave = kBackSteps<T, kGate>, kOps = kGate ? 3 : 2;
   using Op = Tile<T, kS, kMode>;
+  static_assert(fits<T, kGate, false>(), "as many blocks as cluster_of reckons with");
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
   constexpr bool kFour = kMode == 16 && sizeof(T) == 2;   // (the other forms and the backward have no registers left for it)
   extern __shared__ __align__(16) char smem[];
@@ -829,11 +841,11 @@ __global__ void __launch_bounds__(kW * 32, 2) rec_fwd_kernel(const __grid_consta
 }
 
 // ---- backward --------------------------------------------------------------------------------
-// (fp32 with an input gate: a block's 145 KB of shared memory leave a multiprocessor no second one, so it may have all registers)
 template <typename T, bool kGate, int kMode, bool kSerial>
-__global__ void __launch_bounds__(kW * 32, sizeof(T) == 4 && kGate ? 1 : 2) rec_bwd_kernel(const __grid_constant__ RecArgs a) {
+__global__ void __launch_bounds__(kW * 32, kResident<T, kGate, true>) rec_bwd_kernel(const __grid_constant__ RecArgs a) {
   constexpr int kS = kBackSteps<T, kGate>, kOps = kGate ? 4 : 3;
   using Op = Tile<T, kS, kMode>;
+  static_assert(fits<T, kGate, true>(), "as many blocks as cluster_of reckons with");
   constexpr bool kPair = kMode == 16 || (kMode == 4 && sizeof(T) == 2);
   extern __shared__ __align__(16) char smem[];
   __shared__ Post post;
@@ -1082,10 +1094,11 @@ int mode_of(int es, std::initializer_list<Operand> in, std::initializer_list<Ope
 
 // Blocks to a cluster, 0 for serial warps: what is predicted to take the least time.  A round takes two blocks on a multiprocessor about 2.4 us and one
 // block 1.6 (bf16 forward; the other forms' ratios are alike), a cluster's exchange some more; a launch is rounds and one to begin
-// with, in as many waves as it has blocks for (the device holds that many clusters at once).  Measured, bf16 forward, clusters of
-// 1, 2, 4, 8: B = 8, L = 4096, D = 1024 56, 49, 54, 61 us; B = 1, L = 65536, D = 2048 791, 498, 262, 190; B = 8, L = 4096,
-// D = 2048 74, 91, 103, 120.
-int cluster_of(int tiles, int B, int L, int steps) {
+// with, in as many waves as it has blocks for (the device holds that many clusters at once; half where a multiprocessor holds one
+// block, which then always runs by itself: kResident).  Measured, bf16 forward, clusters of 1, 2, 4, 8: B = 8, L = 4096, D = 1024
+// 51, 46, 51, 60 us; B = 1, L = 65536, D = 2048 739, 486, 249, 178; B = 8, L = 4096, D = 2048 72, 88, 98, 113; fp32 backward with an
+// input gate (one block): B = 2, L = 8192, D = 1024 325, 193, 103, 164; B = 20, L = 1000, D = 320 45, 56, 62, 70.
+int cluster_of(int tiles, int B, int L, int steps, int resident) {
   const int forced = g_options[OPT_REC_CLUSTER].load(std::memory_order_relaxed);
   if (forced == 1 || forced == 2 || forced == 4 || forced == 8) return forced;
   const long long units = (long long)tiles * B;
@@ -1095,17 +1108,18 @@ int cluster_of(int tiles, int B, int L, int steps) {
     double round;
   };
   constexpr Form kForms[] = {{1, 296, 1.}, {2, 296, 1.2}, {4, 284, 1.25}, {8, 264, 1.3}};
+  auto waves_of = [&](long long n, long long slots) {   // the last one takes less where one block runs by itself
+    if (resident == 1) return (double)((n + slots / 2 - 1) / (slots / 2));
+    const long long last = n % slots;
+    return (double)(n / slots) + (last == 0 ? 0. : last <= slots / 2 ? 1.6 / 2.4 : 1.);
+  };
   int best = 1;
   double least = 1e300;
   for (const Form& f : kForms) {
-    const long long blocks = (long long)tiles * B * f.size, last = blocks % f.slots;
-    const double waves = (double)(blocks / f.slots) + (last == 0 ? 0. : last <= f.slots / 2 ? 1.6 / 2.4 : 1.);
-    const double cost = waves * ((L + f.size * kW * steps - 1) / (f.size * kW * steps) + 1) * f.round;
+    const double cost = waves_of(units * f.size, f.slots) * ((L + f.size * kW * steps - 1) / (f.size * kW * steps) + 1) * f.round;
     if (cost < least * 0.999) least = cost, best = f.size;
   }
-  const long long slots = 296 * kW, last = units % slots;
-  const double waves = (double)(units / slots) + (last == 0 ? 0. : last <= slots / 2 ? 1.6 / 2.4 : 1.);
-  return waves * ((L + steps - 1) / steps + 1) < least ? 0 : best;
+  return waves_of(units, 296 * kW) * ((L + steps - 1) / steps + 1) < least ? 0 : best;
 }
 
 template <typename Kernel>
@@ -1134,8 +1148,9 @@ void launch_rec(Kernel kernel, int tiles, int B, int cluster, size_t smem, cudaS
 
 template <typename T, bool kGate, int kMode>
 void run_mode(bool bwd, int B, RecArgs a, cudaStream_t s) {
-  const int steps = bwd ? kBackSteps<T, kGate> : kForwardSteps<T>, tiles = (a.D + kC - 1) / kC, cluster = cluster_of(tiles, B, a.L, steps);
-  const size_t smem = size_t(kW) * kStages * ((kGate ? 3 : 2) + (bwd ? 1 : 0)) * steps * kC * sizeof(T);
+  const int steps = bwd ? kBackSteps<T, kGate> : kForwardSteps<T>, tiles = (a.D + kC - 1) / kC;
+  const int cluster = cluster_of(tiles, B, a.L, steps, bwd ? kResident<T, kGate, true> : kResident<T, kGate, false>);
+  const size_t smem = bwd ? kRingBytes<T, kGate, true> : kRingBytes<T, kGate, false>;
   a.tiles = tiles, a.units = tiles * B;
   if (cluster == 0)
     launch_rec(bwd ? rec_bwd_kernel<T, kGate, kMode, true> : rec_fwd_kernel<T, kGate, kMode, true>, tiles, B, 0, smem, s, a);

@@ -735,3 +735,25 @@ def test_a_step_in_place_tells_graphs():
         s = torch.zeros(2, 8, device="cuda")
         assert M.ops.gated_recurrence_step(f, f, None, s, h_out=s)[1].data_ptr() == s.data_ptr()
     M.ops.gated_recurrence_step(f, f, None, s, h_out=s)
+
+
+@pytest.mark.gpu
+def test_the_split_reckons_with_the_blocks_that_fit():
+    """the fp32 backward with an input gate has a multiprocessor for each of its blocks: 100 sequences' tiles by blocks by themselves"""
+    import fairseq_apollo_b200 as M
+    from fairseq_apollo_b200 import _lib
+    r = inputs(20, 1000, 320, torch.float32, True, 1)
+    leaves = [cuda(r[k]).requires_grad_() for k in ("x", "f", "i", "h_in")]
+    y = M.gated_recurrence(*leaves[:3], h_in=leaves[3])
+    dy = cuda(r["dy"])
+
+    def backward(cluster):
+        _lib.set_option(8, cluster)
+        try:
+            return torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        finally:
+            _lib.set_option(8, 0)
+
+    chosen, one, four = backward(0), backward(1), backward(4)
+    assert any(not torch.equal(a, b) for a, b in zip(one, four))   # (maps are joined in another order)
+    assert all(torch.equal(a, b) for a, b in zip(chosen, one))
