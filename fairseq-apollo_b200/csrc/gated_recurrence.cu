@@ -5,9 +5,9 @@
 // written with the leak l where a gate stands open (f >> 0): it is far below the spacing of floats next to 1, and a decay 1 - l would
 // round it to a few bits, the same way at every step.  Where a gate is closed (f << 0) it is the decay k that is small, and 1 - l
 // has few of its bits, or none: there h = x + k (h - x), and the gradient of f, k l times the rest, has k as it is.  fp32 calls take the
-// smaller of l and k at every step (gate_side2); 16-bit calls l alone, and walk a segment with the sides when one of its gates is
-// closed that far (the sides for all segments: B = 64, L = 1024, D = 2048 bf16 forward 150 us against 137, backward 292 against 231;
-// both walks where every segment has such a gate: B = 8, L = 4096, D = 2048 forward 156 us against 74, backward 335 against 122).
+// smaller of l and k at every step (gate_side2); 16-bit calls l alone, and the sides in segments where a gate is closed that far, which
+// the warp looks at first (bf16, the sides in all segments: B = 8, L = 4096, D = 2048 forward 90 us against 74, backward 158 against 124;
+// B = 1, L = 65536 216 against 185 and 385 against 304).
 //
 // A run of steps maps the state that enters it linearly to the one that leaves, h -> h_loc + A h (h_loc: from a zero state,
 // A: the product of the decays), and such maps compose, so the time axis is split: a warp takes 64 channels (two to a lane) of
@@ -143,12 +143,11 @@ __device__ __forceinline__ f32x2 minus_leak2(f32x2 f) {
   return minus_sigmoid2<T, 1>(f);
 }
 // Whether every gate is held by the smaller of its sides.  In 16-bit types that is left to segments with a gate so far closed that
-// 1 - l loses what a 16-bit value shows of the decay (LeastGate).
+// 1 - l loses what a 16-bit value shows of the decay (any_closed).
 template <typename T>
 constexpr bool kSides = sizeof(T) == 4;
-// The least of the gates' arguments that a lane has seen.  Below kLeast the decay is less than 1 / 400 (fp16: 1 / 50), and 1 - l, off by
-// 4 x 2^-24 absolutely, by more than 2^-13 of it (2^-16), a sixteenth of the type's half step: such a segment is walked again with
-// the sides.
+// The least of the gates' arguments that a lane has seen.  1 - l is off by 3 x 2^-24 absolutely (the sum 1 + e and the reciprocal):
+// above kLeast by at most 2^-13.7 of the decay (fp16: 2^-15.2), a twenty-sixth (a ninth) of the type's half step.
 template <typename T>
 struct LeastGate {   // (fp32: none)
   __device__ __forceinline__ void see(const T*) {}
@@ -163,7 +162,7 @@ struct LeastGate<__nv_bfloat16> {
 };
 template <>
 struct LeastGate<__half> {
-  static constexpr float kLeast = -4.f;
+  static constexpr float kLeast = -5.f;
   __half2 v = __floats2half2_rn(0.f, 0.f);
   __device__ __forceinline__ void see(const __half* p) { v = __hmin2(v, *reinterpret_cast<const __half2*>(p)); }
   __device__ __forceinline__ bool closed() const { return fminf(__low2float(v), __high2float(v)) < kLeast; }
@@ -346,6 +345,24 @@ __device__ __forceinline__ unsigned flags_of(unsigned byte) {
   return __ballot_sync(0xffffffffu, byte != 0);
 }
 
+// whether a gate of the warp's segment is closed that far; padded steps do not count
+template <typename T, int kS>
+__device__ __forceinline__ bool any_closed(const T* f, unsigned flags) {
+  if constexpr (kSides<T>) {
+    return false;
+  } else {
+    LeastGate<T> least;
+    if ((flags & 0xffffu) == 0) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) least.see(f + s * kC);
+    } else {
+#pragma unroll 1
+      for (int s = 0; s < kS; ++s)
+        if (!((flags >> s) & 1u)) least.see(f + s * kC);
+    }
+    return __any_sync(0xffffffffu, least.closed());
+  }
+}
 template <int kS>
 __device__ __forceinline__ bool all_padded(unsigned flags) {
   return (flags & ((1u << kS) - 1u)) == (1u << kS) - 1u;
@@ -730,7 +747,7 @@ __global__ void __launch_bounds__(kW * 32, kResident<T, kGate, false>) rec_fwd_k
     const T* op = reinterpret_cast<const T*>(ring + (k % kStages) * (kOps * Op::kBytes)) + 2 * lane;
     Map loc[kS];
     f32x2 h = pack2(0.f, 0.f), A = pack2(1.f, 1.f);
-    LeastGate<T> least;
+    const bool closed = (flags & 0xffffu) == 0 && any_closed<T, kS>(op + kS * kC, 0u);   // (padded ones take the sides in any case)
     auto step = [&](int s, auto sides) {
       const T* fs = op + kS * kC + s * kC;
       const f32x2 xv = two(op + s * kC);
@@ -741,34 +758,38 @@ __global__ void __launch_bounds__(kW * 32, kResident<T, kGate, false>) rec_fwd_k
         h = kGate ? fma2(in, xv, pass(c, open, h)) : fma2(c, sub2(h, xv), either(open, h, xv));
         A = pass(c, open, A);
       } else {
-        least.see(fs);
         const f32x2 nl = minus_leak2<T>(two(fs));
         h = kGate ? fma2(in, xv, fma2(nl, h, h)) : fma2(nl, sub2(h, xv), h);
         A = fma2(nl, A, A);
       }
     };
     constexpr std::bool_constant<kSides<T>> usual;
-    auto by_step = [&](auto sides) {   // padded steps among them
+    auto by_step = [&] {   // with the gates' sides, padded steps among them
       h = pack2(0.f, 0.f), A = pack2(1.f, 1.f);
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         if ((flags >> (16 + s)) & 1u) odd = seen(odd, h), h = pack2(0.f, 0.f), A = minus_zero();
         if (!((flags >> s) & 1u)) {
           const f32x2 before = A;
-          step(s, sides);
+          step(s, std::true_type{});
           if (before == minus_zero()) A = minus_zero();
         }
         loc[s] = {A, h};
       }
     };
-    bool walk = false;   // with the gates' sides
-    if (flags == 0) {
+    if (flags == 0 && !closed) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         step(s, usual);
         loc[s] = {A, h};
       }
-    } else if (only_resets(flags)) {
+    } else if (!kSides<T> && flags == 0) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        step(s, std::true_type{});
+        loc[s] = {A, h};
+      }
+    } else if (only_resets(flags) && !closed) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         odd = seen(odd, h);
@@ -779,12 +800,9 @@ __global__ void __launch_bounds__(kW * 32, kResident<T, kGate, false>) rec_fwd_k
       }
     } else if (idle<kS>(flags)) {
       loc[kS - 1] = {A, h};
-    } else if (!kSides<T>) {
-      by_step(usual);
     } else {
-      walk = true;
+      by_step();
     }
-    if (walk || least.closed()) by_step(std::true_type{});
     f32x2 in;
     if (kSerial) {
       in = carry;
@@ -907,7 +925,7 @@ __global__ void __launch_bounds__(kW * 32, kResident<T, kGate, true>) rec_bwd_ke
     const T* gy = op + 2 * kS * kC;
     // c: minus the leak, with `sides` the smaller side of the gate; v: h_{t-1} - x, with an input gate h_{t-1}
     f32x2 c[kS], v[kS], gate[kGate ? kS : 1], slope[kGate ? kS : 1];
-    LeastGate<T> least;
+    const bool closed = any_closed<T, kS>(op + kS * kC, flags);
     auto state_step = [&](int s, auto sides) {
       const T* fs = op + kS * kC + s * kC;
       const f32x2 xv = two(op + s * kC);
@@ -918,7 +936,6 @@ __global__ void __launch_bounds__(kW * 32, kResident<T, kGate, true>) rec_bwd_ke
         const f32x2 open = open_bits(c[s]);
         h = kGate ? fma2(gate[s], xv, pass(c[s], open, h)) : fma2(c[s], v[s], either(open, h, xv));
       } else {
-        least.see(fs);
         c[s] = minus_leak2<T>(two(fs));
         h = kGate ? fma2(gate[s], xv, fma2(c[s], h, h)) : fma2(c[s], v[s], h);
       }
@@ -956,13 +973,17 @@ __global__ void __launch_bounds__(kW * 32, kResident<T, kGate, true>) rec_bwd_ke
         if ((flags >> (16 + s)) & 1u) odd = seen(odd, m.h), m = {minus_zero(), pack2(0.f, 0.f)};
       }
     };
-    bool walk = false;   // with the gates' sides
-    if (flags == 0) {
+    if (flags == 0 && !closed) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) state_step(s, usual);
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) grad_step(s, usual);
-    } else if (only_resets(flags)) {
+    } else if (!kSides<T> && flags == 0) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) state_step(s, std::true_type{});
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) grad_step(s, std::true_type{});
+    } else if (only_resets(flags) && !closed) {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         odd = seen(odd, h);
@@ -976,13 +997,12 @@ __global__ void __launch_bounds__(kW * 32, kResident<T, kGate, true>) rec_bwd_ke
         m.h = cut_at(flags, s) ? pack2(0.f, 0.f) : m.h;
         m.a = cut_from(flags, s) ? minus_zero() : m.a;
       }
-    } else if (!kSides<T> && !idle<kS>(flags)) {
-      by_step(usual);
-    } else {
-      walk = !idle<kS>(flags);
+    } else if (!idle<kS>(flags)) {
+      if (!closed)
+        by_step(usual);
+      else if constexpr (!kSides<T>)
+        by_step(std::true_type{});
     }
-    walk = walk || least.closed();
-    if (walk) by_step(std::true_type{});
     f32x2 q;
     if (kSerial) {
       q = carry;
@@ -1015,10 +1035,13 @@ __global__ void __launch_bounds__(kW * 32, kResident<T, kGate, true>) rec_bwd_ke
       put<kPair>(ft + s * a.dfl, of, count);
       if (kGate) put<kPair>(it + s * a.dil, oi, count);
     };
-    if (flags == 0 && whole && !walk) {
+    if (flags == 0 && whole && !closed) {
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) out_step(s, usual, false, 2);
-    } else if (only_resets(flags) && whole && !walk) {
+    } else if (!kSides<T> && flags == 0 && whole) {
+#pragma unroll
+      for (int s = kS - 1; s >= 0; --s) out_step(s, std::true_type{}, false, 2);
+    } else if (only_resets(flags) && whole && !closed) {
 #pragma unroll
       for (int s = kS - 1; s >= 0; --s) {
         out_step(s, usual, false, 2);
