@@ -28,16 +28,19 @@
 // large values is no larger than they are.  h - x of such values overflows, an infinity less its leak is NaN, and so is one times a
 // product of decays that has underflowed: all of them mark the values behind them as not finite.  Each lane keeps what it has seen
 // of that (a product with 0 a round); where it has, one warp goes through the tile's steps in order at the end, and what had come out
-// not finite is replaced (0.5 us a step forward and 0.9 backward, until all is NaN: joining infinite maps as they come cost calls that
+// not finite is replaced (0.5 us a step forward and 1 backward, until all is NaN: joining infinite maps as they come cost calls that
 // have none 3 to 12 %).
-// Bound: HBM where the blocks fill the device (B = 64, L = 1024, D = 2048 bf16: forward 135 us, backward 230, 0.91 and 0.89 of the
+//
+// Bound: HBM where the blocks fill the device (B = 64, L = 1024, D = 2048 bf16: forward 134 us, backward 224, 0.92 and 0.91 of the
 // measured copy rate over 3 and 5 arrays).  With fewer it is the rounds: a multiprocessor takes some 1.2 us for a block's tile, of
 // which the special-function operations of the gates are 0.55 and its instructions 0.6, and an exchange through a cluster adds 0.3
-// to 0.7 (B = 8, L = 4096, D = 2048 75 and 128 us; B = 1, L = 65536, D = 2048 190 and 305, 0.64 and 0.67).  Masks cost 2 % more.
-// What was tried there and no faster: leaks of the next tile taken while a block waits (203 and 347 us, registers); stages of the
-// gates' operations batched over 4, 8 and 16 rows (210, 210, 205); three stages of the ring (198); segments of 8 steps and three
-// blocks to a multiprocessor (255); blocks of four warps (better where there are four for each multiprocessor and more, worse
-// backward); clusters spread over the multiprocessors by preference.
+// to 0.7 (B = 8, L = 4096, D = 2048 74 and 124 us; B = 1, L = 65536, D = 2048 184 and 304, 0.67 and 0.67).  Resets cost 3 to 4 % more.
+// What was tried there, beside 190 and 305 us at the larger then, and no faster: leaks of the next tile taken while a block waits (203
+// and 347, registers); stages of the gates' operations batched over 4, 8 and 16 rows (210, 210, 205); three stages of the ring (198);
+// segments of 8 steps and three blocks to a multiprocessor (255); blocks of four warps (better where there are four for each
+// multiprocessor and more, worse backward); clusters spread over the multiprocessors by preference.
+// Of 128 registers the 16-byte forms spill 8 bytes a thread at most, the 4-byte ones 16; rows of 16-bit values on odd addresses, which
+// come through registers, up to 144 backward and 80 forward (B = 32, L = 2000, D = 1001 346 us backward, D = 1000 176).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -332,7 +335,7 @@ struct Tile {
 
 // The padding (bits 0 ..) and resets (bits 16 ..) of a segment, one byte to a lane; steps behind the end are padded.  The byte is asked
 // for a round before flags_of() looks at it, and nothing may look at it earlier: a test beside the load, which the compiler makes when
-// it can, waits for memory in every round (B = 8, L = 4096, D = 2048 with resets: forward 89 us, backward 141).
+// it can, waits for memory in every round (B = 8, L = 4096, D = 2048 with resets: forward 89 us, backward 141, without 76 and 127).
 __device__ __forceinline__ unsigned flag_byte(const RecArgs& a, int b, int t0, int steps, int lane) {
   const int s = lane & 15, t = t0 + s;
   const unsigned char* mask = lane < 16 ? a.pad : a.reset;
@@ -1119,8 +1122,8 @@ int mode_of(int es, std::initializer_list<Operand> in, std::initializer_list<Ope
 // block 1.6 (bf16 forward; the other forms' ratios are alike), a cluster's exchange some more; a launch is rounds and one to begin
 // with, in as many waves as it has blocks for (the device holds that many clusters at once; half where a multiprocessor holds one
 // block, which then always runs by itself: kResident).  Measured, bf16 forward, clusters of 1, 2, 4, 8: B = 8, L = 4096, D = 1024
-// 51, 46, 51, 60 us; B = 1, L = 65536, D = 2048 739, 486, 249, 178; B = 8, L = 4096, D = 2048 72, 88, 98, 113; fp32 backward with an
-// input gate (one block): B = 2, L = 8192, D = 1024 325, 193, 103, 164; B = 20, L = 1000, D = 320 45, 56, 62, 70.
+// 54, 47, 53, 60 us; B = 1, L = 65536, D = 2048 771, 504, 258, 184; B = 8, L = 4096, D = 2048 74, 91, 101, 115; fp32 backward with an
+// input gate (one block): B = 2, L = 8192, D = 1024 323, 193, 103, 164; B = 20, L = 1000, D = 320 45, 56, 62, 70.
 int cluster_of(int tiles, int B, int L, int steps, int resident) {
   const int forced = g_options[OPT_REC_CLUSTER].load(std::memory_order_relaxed);
   if (forced == 1 || forced == 2 || forced == 4 || forced == 8) return forced;

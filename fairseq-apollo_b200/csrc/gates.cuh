@@ -16,7 +16,7 @@ __device__ __forceinline__ float within(float v, float most) {
 // 16-bit types: as 2^(v / ln 2) with the product rounded once, relative error (2 + |v|) 2^-23.  fp32: the product's rounding error
 // r and the constant's own are taken along, 2^(p + r) = 2^p (1 + r ln 2), which leaves the approximation's 2^-22 whatever v is;
 // expf and the division cost three times as many instructions (gates are most of what a step of the recurrence computes: B = 16,
-// L = 2048, D = 1024 forward 86 us with them, 72 without).  There v is held within 88, where e^v is finite and r means something.
+// L = 2048, D = 1024 forward 82 us with them, 67 without).  There v is held within 88, where e^v is finite and r means something.
 template <typename T, int kSign>
 __device__ __forceinline__ f32x2 exp_pair(f32x2 v) {
   constexpr float kLog = kSign * 1.4426950408889634f;   // 1 / ln 2 in fp32; what is missing of it times ln 2 below

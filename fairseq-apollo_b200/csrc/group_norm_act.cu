@@ -15,7 +15,8 @@
 // saves it little, as its 16 special-function operations to a vector take as long (16 x 4096 x 512 bf16, 32 groups, forward: 17 us
 // for the first pass, 26 for the second, which takes 24 of its 67 MB from DRAM, 25 for a copy; 6 x 32768 x 1024 206 us, 0.90 of the
 // measured copy rate over the three arrays).  Calls in pieces that fit L2 were slower by their launches (6 x 32768 x 1024 forward 231
-// us against 206, backward 446 against 324; a call that fits as it is takes the same).
+// us against 206, backward 446 against 324; a call that fits as it is takes the same).  Of the kernels only the sums of 16-bit groups
+// that share a vector spill registers (44 bytes a thread).
 //
 // Statistics: a thread adds up d = x - p and d^2 with p the first value of its run.  p being one of the n values, the squares about
 // it are at most n + 1 times those about the mean, so n <= kRun bounds what their difference loses; such entries are then joined by

@@ -7,7 +7,6 @@ caller's ``incremental_state``, one token at a time or whole sequences.
 from typing import Dict, Optional
 
 import torch
-import torch.nn.functional as F
 from torch import Tensor, nn
 
 from .. import functions, ops
