@@ -281,3 +281,54 @@ def test_values_next_to_the_largest(dtype):
         y, h = M.gated_recurrence(cuda(x), cuda(f), cuda(i), h_in=cuda(h_in), want_state=True)
         close(h, want["h"], "h")
         close(M.ops.gated_recurrence_step(cuda(x[:, 0]), cuda(f[:, 0]), cuda(i[:, 0]), cuda(h_in))[1], want["h"], "h")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinite_values_in_other_memory_orders(dtype, gate):
+    """rows on odd addresses, columns of wider rows, time first, channels not adjacent"""
+    import fairseq_apollo_b200 as M
+
+    def odd_columns(t):
+        wide = torch.full(t.shape[:-1] + (t.shape[-1] + 9,), 7.0, dtype=t.dtype, device=t.device)
+        wide[..., 5:5 + t.shape[-1]] = t
+        return wide[..., 5:5 + t.shape[-1]]
+
+    for D in (64, 65):
+        for L, kw in ((300, {"pad": "right"}), (90, {"reset": "docs"})):
+            r = odd_values(3, L, D, dtype, gate, D + L, "all", **kw)
+            plain = run_all(M, r, False)
+            check_odd(plain, r)
+            for shape in (odd_columns, lambda t: t.transpose(0, 1).contiguous().transpose(0, 1),
+                          lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)):
+                got = run_all(M, r, False, shape)
+                for k in plain:
+                    assert torch.equal(plain[k].nan_to_num(3.0), got[k].nan_to_num(3.0)), k
+
+
+@pytest.mark.gpu
+def test_infinite_values_replayed():
+    """captured, replayed with an infinity in the captured tensors and without again"""
+    import fairseq_apollo_b200 as M
+    r = inputs(2, 900, 64, torch.bfloat16, False, 6, None, "docs")
+    x, f, h, cut = (cuda(r[k]) for k in ("x", "f", "h_in", "reset"))
+
+    def call():
+        with torch.no_grad():
+            return M.gated_recurrence(x, f, reset_mask=cut, h_in=h, want_state=True)
+
+    clean = call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    keep = x.clone()
+    for value in (float("inf"), None, float("nan"), None):
+        x.copy_(keep)
+        if value is not None:
+            x[0, 10, 3] = value
+        graph.replay()
+        torch.cuda.synchronize()
+        want = clean if value is None else call()
+        assert all(torch.equal(a.nan_to_num(3.0), b.nan_to_num(3.0)) for a, b in zip(got, want))
+        assert (value is None) == bool(torch.isfinite(got[0]).all())
