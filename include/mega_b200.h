@@ -624,7 +624,8 @@ MEGA_API int mega_block_cache_fill(const void* k, int64_t ksb, int64_t ksl, cons
  * step whose byte of pad_mask is set leaves the state as it is (after the reset, when both are set), gives y = 0, and
  * what lies there in x, f, i is not used.  A state that is not finite reaches no step behind a reset; until then an infinite
  * one stays, as does an infinite x or gradient, however little of it a gate lets through, and two infinities of opposite
- * sign make a NaN.  A NaN stays.  The decay and the leak are held to their last places on either side of a gate.
+ * sign make a NaN.  A NaN stays.  The decay keeps its last places where a gate is nearly closed, the leak where it is nearly
+ * open (in the 16-bit types to a ninth of half a step of theirs).
  *
  * x, f, i, y (and the gradients) are (B, L, D) with contiguous channels; the strides of the other two axes are free, 0
  * and negative ones among them for what is read, and outputs do not overlap one another or an input.  Masks are (B, L)
