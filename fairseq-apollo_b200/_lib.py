@@ -27,6 +27,15 @@ class BlockStepArgs(ctypes.Structure):
                 + [("norm_eps", c_d), ("qk_eps", c_d), ("cap", c_l), ("pos", ctypes.c_int32), ("qk_dtype", ctypes.c_int32)])
 
 
+class DecayedAttentionArgs(ctypes.Structure):
+    """mega_decayed_attention_args of include/mega_b200.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "gate_dtype", "B", "L", "H", "K", "V")] + [("flags", ctypes.c_uint32), ("scale", c_d)]
+                + [(n, c_p) for n in ("q", "k", "v", "f")] + [(n, c_l * 3) for n in ("qs", "ks", "vs", "fs")]
+                + [(n, c_p) for n in ("pad_mask", "reset_mask", "h_in", "h_out", "y")] + [("ys", c_l * 3), ("dy", c_p), ("gs", c_l * 3)]
+                + [(n, c_p) for n in ("dh_out", "dh_in", "dq", "dk", "dv", "df")] + [(n, c_l * 3) for n in ("dqs", "dks", "dvs", "dfs")]
+                + [("work", c_p)])
+
+
 # name -> argument types, in the order of include/mega_b200.h
 SIGNATURES = {
     "mega_ema_coeffs": [c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_p, c_p, c_p, c_p],
@@ -92,6 +101,11 @@ SIGNATURES = {
     "mega_gated_recurrence_step": [c_p] * 4 + [c_i] * 3 + [c_l] * 4 + [c_p] * 3,
     "mega_group_norm_fwd": [c_p] * 2 + [c_i] * 4 + [c_l] * 4 + [c_p] * 3 + [c_i, c_d, c_u] + [c_p] * 5,
     "mega_group_norm_bwd": [c_p] * 3 + [c_i] * 4 + [c_l] * 6 + [c_p] * 3 + [c_i, c_u] + [c_p] * 7,
+    "mega_decayed_attention_fwd": [c_p, c_p],
+    "mega_decayed_attention_bwd": [c_p, c_p],
+    "mega_decayed_attention_step": [c_p, c_p],
+    "mega_rms_norm_fwd": [c_p] * 4 + [c_i] * 4 + [c_l] * 8 + [c_p, c_i, c_d, c_p],
+    "mega_rms_norm_bwd": [c_p] * 4 + [c_i] * 4 + [c_l] * 8 + [c_p, c_i, c_d] + [c_p] * 3,
     "mega_set_option": [c_i, c_i],
     "mega_debug_device_error": [ctypes.POINTER(c_i), c_i],
 }
@@ -102,6 +116,8 @@ OTHER = {
     "mega_block_step_work": ([c_i, c_i, c_i, c_i, c_i, c_l], c_l),
     "mega_gated_recurrence_segment": ([c_i, c_i], c_i),
     "mega_group_norm_work": ([c_i] * 6, c_l),
+    "mega_decayed_attention_work": ([c_p, c_i], c_l),
+    "mega_rms_norm_work": ([c_i] * 5, c_l),
     "mega_launch_count": ([], ctypes.c_uint64),
     "mega_debug_last_kernel": ([], ctypes.c_char_p),
 }

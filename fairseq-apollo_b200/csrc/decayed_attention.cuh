@@ -1,0 +1,117 @@
+// What the forms of linear attention with a decay for each head share (decayed_attention.cu has the mathematics).
+#pragma once
+#include "common.cuh"
+
+namespace mega {
+
+struct Operand {
+  const void* p;
+  long long sb, sl, sh;   // strides in elements; the last axis is contiguous
+  int d, vec;             // width; bytes of a piece that every row's start and width are multiples of
+};
+
+// One walk over the steps of every (sequence, head)
+struct Walk {
+  Operand q, k, v, x;     // queries, keys, values; x: what the outputs are multiplied with for the gates' gradient
+  void* out;
+  long long ob, ol, oh;
+  int piece;              // bytes of a piece of an output row that every row's start and width are multiples of
+  const void* f;
+  long long fb, fl, fh;
+  int f_dtype;
+  const uint8_t *pad, *reset;
+  const float* s_in;
+  float* s_out;
+  int s_row, s_col;       // strides of the states that come in and go out: (keys, values) of this walk
+  float2* dots;           // [tile][B H][L]: x . out of the part from the state that entered; the pairs' sum W of a step
+  void* anchors;          // [B H][chunk][tile] states that enter a chunk, in the activations' type (written, or read:)
+  float* through;         // [B H][chunk][part]: what passes the whole chunk
+  float *local, *factor;  // states that segments leave by themselves, and their decay
+  int B, L, H, tiles, chunks, per, segs;
+  float p_scale, o_scale, s_scale;
+  int rev, excl;
+};
+
+__device__ __forceinline__ float gate_value(const Walk& w, long long at) {
+  if (w.f_dtype == MEGA_F32) return __ldg(static_cast<const float*>(w.f) + at);
+  if (w.f_dtype == MEGA_BF16) return Elem<__nv_bfloat16>::ld(static_cast<const __nv_bfloat16*>(w.f) + at);
+  return Elem<__half>::ld(static_cast<const __half*>(w.f) + at);
+}
+
+// The gates of a chunk of 32 N steps, N steps of the walk to a lane
+template <int N>
+struct GateIn {
+  float f[N];
+  unsigned pad, reset;
+};
+template <int N>
+__device__ __forceinline__ int gate_row(const Walk& w, int lane, int i) {
+  const int p = N * lane + i;
+  return w.rev ? 32 * N - 1 - p : p;
+}
+template <int N>
+__device__ __forceinline__ GateIn<N> gates_fetch(const Walk& w, int b, int h, int tile, int lane) {
+  GateIn<N> g;
+  g.pad = (1u << N) - 1, g.reset = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    g.f[i] = 0.f;
+    const long long t = (long long)tile * (32 * N) + gate_row<N>(w, lane, i);
+    if (t >= w.L) continue;
+    g.f[i] = gate_value(w, b * w.fb + t * w.fl + h * w.fh);
+    if (!w.pad || !w.pad[b * (long long)w.L + t]) g.pad &= ~(1u << i);
+    if (w.reset && w.reset[b * (long long)w.L + t]) g.reset |= 1u << i;
+  }
+  return g;
+}
+// What they come to: running sum of log2 a (in 64 bits), resets so far, weight of a step in the state that leaves, and the weight of
+// the state that enters in it (0: a reset lies between).  A gate whose decay is below fp32's range counts as a reset.
+template <int N>
+struct GateOut {
+  double sum[N];
+  int count[N];
+  float weight[N], enter;
+  int total;
+  bool padded;
+};
+// log2 sigmoid(f), and whether that is no decay but a reset
+__device__ __forceinline__ double log2_gate(float f) {
+  return (double)(f < 0.f ? f - log1pf(expf(f)) : -log1pf(expf(-f))) * 1.4426950408889634;
+}
+__device__ __forceinline__ bool closed(double g) { return g < -149.; }
+template <int N>
+__device__ __forceinline__ GateOut<N> gates_scan(const Walk& w, const GateIn<N>& in, int lane) {
+  double s[N], sum = 0.;
+  int c[N], cnt = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s[i] = in.pad >> i & 1 ? 0. : log2_gate(in.f[i]);
+    c[i] = (in.reset >> i & 1) || closed(s[i]);
+    if (c[i]) s[i] = 0.;
+    sum += s[i], cnt += c[i];
+  }
+  double upto = sum;
+  int counted = cnt;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double u = __shfl_up_sync(~0u, upto, o);
+    const int v = __shfl_up_sync(~0u, counted, o);
+    if (lane >= o) upto += u, counted += v;
+  }
+  const double all = __shfl_sync(~0u, upto, 31);
+  GateOut<N> r;
+  r.total = __shfl_sync(~0u, counted, 31);
+  upto -= sum, counted -= cnt;   // (what lies before this lane's steps)
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (!w.excl) upto += s[i], counted += c[i];
+    r.sum[i] = upto, r.count[i] = counted;
+    r.weight[i] = counted == r.total && !(in.pad >> i & 1) ? w.s_scale * exp2f((float)(all - upto)) : 0.f;
+    if (w.excl) upto += s[i], counted += c[i];
+  }
+  r.enter = r.total ? 0.f : exp2f((float)all);
+  r.padded = __any_sync(~0u, in.pad != 0);
+  return r;
+}
+
+}  // namespace mega

@@ -60,3 +60,22 @@ def group_norm(x, weight, bias, num_groups, padding_mask, eps, activation):
     """y = act(GroupNorm(x)) from the module's parameters (effective scale weight + 1)."""
     fn = _lib.host().group_norm_train if needs_grad(x, weight, bias) else _lib.host().group_norm
     return fn(x, weight, bias, num_groups, padding_mask, eps, ops._silu(activation))
+
+
+def decayed_attention(q, k, v, forget, padding_mask=None, reset_mask=None, h_in=None, scale=1.0, want_state=False, reverse=False):
+    """ops.decayed_attention_fwd with gradients of q, k, v, forget and h_in (through y and through the state that leaves)."""
+    r = _lib.host().decayed_attention_train(q, k, v, forget, padding_mask, reset_mask, h_in, float(scale), want_state, reverse)
+    return tuple(r) if want_state else r[0]
+
+
+def decayed_attention_packed(z, num_heads, keys, padding_mask=None, reset_mask=None, h_in=None, scale=1.0, want_state=False, reverse=False):
+    """decayed_attention on z (B, L, H (2 K + V + 1)): queries, keys, values and gates of all heads side by side, as one projection
+    leaves them; z's gradient is written in place of its parts."""
+    r = _lib.host().decayed_attention_packed(z, num_heads, keys, padding_mask, reset_mask, h_in, float(scale), want_state, reverse)
+    return tuple(r) if want_state else r[0]
+
+
+def rms_norm(x, weight, residual=None, num_groups=1, eps=1e-5):
+    """ops.rms_norm_fwd with gradients of x, the residual and weight."""
+    r = _lib.host().rms_norm_train(x, weight, residual, int(num_groups), float(eps))
+    return r[0] if residual is None else tuple(r)

@@ -1094,6 +1094,315 @@ Tensor group_norm_train(const Tensor& x, const Tensor& weight, const Tensor& bia
   return GnFn::apply(x, weight, bias, groups, mask, eps, silu);
 }
 
+// ------------------------------------------------------------- linear attention with a decay for each head
+struct Att {
+  Tensor q, k, v, f, pad, reset, h_in;
+  mega_decayed_attention_args a;
+};
+void put(int64_t* to, const Tensor& t, int64_t first) {   // strides of the axes in front of the last one
+  for (int64_t i = 0; i < 3; ++i) to[i] = t.stride(first + i);
+}
+// q, k (..., H, K), v (..., H, V), f (..., H) of one type and device (the gates' type may be float32); `lead`: axes in front of the heads
+void check_att(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& f, int64_t lead) {
+  on_cuda(q, k, v, f);
+  dtype_of(q);
+  expect(q.dim() == lead + 2 && v.dim() == lead + 2,
+         lead == 2 ? "q, k and v must be (batch, length, heads, width)" : "q, k and v must be (batch, heads, width)");
+  if (k.scalar_type() != q.scalar_type()) throw py::type_error("k must have q's type");
+  expect(k.device() == q.device(), "k must be on q's device");
+  expect(k.sizes() == q.sizes(), "k must have q's shape");
+  if (v.scalar_type() != q.scalar_type()) throw py::type_error("v must have q's type");
+  if (f.scalar_type() != q.scalar_type() && f.scalar_type() != at::kFloat) throw py::type_error("the gates must have q's type or be float32");
+  if (v.device() != q.device() || f.device() != q.device()) throw py::value_error("v and the gates must be on q's device");
+  expect(v.sizes().slice(0, lead + 1) == q.sizes().slice(0, lead + 1), "v must have q's batch, length and heads");
+  expect(f.sizes() == q.sizes().slice(0, lead + 1), "the gates must have q's shape without its width");
+  expect(q.size(-1) >= 1 && v.size(-1) >= 1 && q.size(-1) <= MEGA_ATT_MOST && v.size(-1) <= MEGA_ATT_MOST,
+         "heads have 1 to 256 keys and values");
+}
+void check_att_state(const Tensor& h, const Tensor& q, const Tensor& v, const char* what) {
+  if (!h.defined()) return;
+  if (h.device() != q.device()) throw py::value_error(std::string(what) + " must be on q's device");
+  if (!at::isFloatingType(h.scalar_type())) throw py::type_error(std::string(what) + " must be a floating-point tensor");
+  expect(h.dim() == 4 && h.size(0) == q.size(0) && h.size(1) == q.size(-2) && h.size(2) == q.size(-1) && h.size(3) == v.size(-1),
+         "a state must be (batch, heads, keys, values)");
+}
+// gates of (heads), the same at every step, as (batch, length, heads)
+Tensor gates_of(const Tensor& f, const Tensor& q) { return f.dim() == 1 && q.dim() >= 3 ? f.expand(q.sizes().slice(0, q.dim() - 1)) : f; }
+Att att_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& f, const Tensor& pad, const Tensor& reset, const Tensor& h_in,
+             double scale, bool reverse) {
+  check_att(q, k, v, f, 2);
+  on_cuda(pad, reset, h_in);
+  check_att_state(h_in, q, v, "h_in");
+  Att r = {channels(q.detach()), channels(k.detach()), channels(v.detach()), f.detach(), mask_on(pad, q, "padding_mask"),
+           mask_on(reset, q, "reset_mask"), f32c(h_in), {}};
+  mega_decayed_attention_args& a = r.a;
+  a.dtype = dtype_of(q), a.gate_dtype = dtype_of(f);
+  a.B = extent(q.size(0)), a.L = extent(q.size(1)), a.H = extent(q.size(2)), a.K = (int)q.size(3), a.V = (int)v.size(3);
+  a.flags = reverse ? MEGA_ATT_REVERSE : 0u;
+  a.scale = scale;
+  a.q = r.q.data_ptr(), a.k = r.k.data_ptr(), a.v = r.v.data_ptr(), a.f = r.f.data_ptr();
+  put(a.qs, r.q, 0), put(a.ks, r.k, 0), put(a.vs, r.v, 0), put(a.fs, r.f, 0);
+  a.pad_mask = ptr<uint8_t>(r.pad), a.reset_mask = ptr<uint8_t>(r.reset);
+  a.h_in = fptr(r.h_in);
+  return r;
+}
+Tensor att_work(const mega_decayed_attention_args& a, int backward, const Tensor& like) {
+  const int64_t n = mega_decayed_attention_work(&a, backward);
+  return n ? at::empty({n}, at::TensorOptions().dtype(at::kByte).device(like.device())) : Tensor();
+}
+void run_att(Att& r, const Tensor& y, const Tensor& h_out, const Where& w) {
+  r.a.y = y.data_ptr();
+  put(r.a.ys, y, 0);
+  r.a.h_out = fptr(h_out);
+  const Tensor work = att_work(r.a, 0, y);
+  r.a.work = ptr(work);
+  check(mega_decayed_attention_fwd(&r.a, w.stream), "decayed_attention_fwd");
+}
+Tensor att_state(const Tensor& q, const Tensor& v) { return floats({q.size(0), q.size(-2), q.size(-1), v.size(-1)}, q); }
+
+// (y, state behind the last step or None)
+std::tuple<Tensor, OptTensor> decayed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& f, const OptTensor& pad,
+                                                const OptTensor& reset, const OptTensor& h_in, double scale, bool want_state, bool reverse) {
+  Att r = att_args(q, k, v, gates_of(f, q), given(pad), given(reset), given(h_in), scale, reverse);
+  const Where w(q);
+  const Tensor y = rec_like(v);
+  Tensor h = want_state ? att_state(q, v) : Tensor();
+  if (v.numel() == 0) {   // (no step: the state stays)
+    if (h.defined()) r.h_in.defined() ? h.copy_(r.h_in) : h.zero_();
+  } else {
+    run_att(r, y, h, w);
+  }
+  if (!want_state) return {y, std::nullopt};
+  return {y, h};
+}
+
+// whether any value of t lies where `out` (contiguous) has one
+bool apart(const Tensor& out, const Tensor& t) {
+  if (!t.defined() || t.numel() == 0 || out.numel() == 0) return true;
+  const char *to = static_cast<const char*>(out.data_ptr()), *from = static_cast<const char*>(t.data_ptr());
+  int64_t low = 0, high = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) (t.stride(i) < 0 ? low : high) += (t.size(i) - 1) * t.stride(i);
+  return to + out.nbytes() <= from + low * t.element_size() || from + (high + 1) * t.element_size() <= to;
+}
+
+// one step: q, k (B, H, K), v (B, H, V), f (B, H) -> (y, h'); h' is `h_out` where given, which may be h
+std::tuple<Tensor, Tensor> decayed_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& f_, const OptTensor& h_,
+                                                  double scale, const OptTensor& h_out_) {
+  const Tensor f = gates_of(f_, q_);
+  check_att(q_, k_, v_, f, 1);
+  on_cuda(given(h_), given(h_out_));
+  check_att_state(given(h_), q_, v_, "h");
+  const Where w(q_);
+  const Tensor q = channels(q_), k = channels(k_), v = channels(v_), h = f32c(given(h_));
+  Tensor y = at::empty(v.sizes(), v.options().requires_grad(false)), out = given(h_out_);
+  if (out.defined()) {
+    check_att_state(out, q_, v_, "h_out");
+    expect(out.scalar_type() == at::kFloat && out.is_contiguous(), "h_out must be contiguous float32");
+    expect(!h.defined() || out.data_ptr() == h.data_ptr() || apart(out, h), "h_out overlaps h and is not h");
+    for (const Tensor& t : {q, k, v, f}) expect(apart(out, t), "h_out overlaps q, k, v or the gates");
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();   // (a graph that has saved it must not use the new values)
+  } else {
+    out = att_state(q, v);
+  }
+  if (v.numel()) {
+    mega_decayed_attention_args a = {};
+    a.dtype = dtype_of(q), a.gate_dtype = dtype_of(f);
+    a.B = extent(q.size(0)), a.L = 1, a.H = extent(q.size(1)), a.K = (int)q.size(2), a.V = (int)v.size(2);
+    a.scale = scale;
+    a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.f = f.data_ptr();
+    auto strides = [](int64_t* to, const Tensor& t) { to[0] = t.stride(0), to[1] = 0, to[2] = t.stride(1); };
+    strides(a.qs, q), strides(a.ks, k), strides(a.vs, v), strides(a.fs, f), strides(a.ys, y);
+    a.y = y.data_ptr(), a.h_in = fptr(h), a.h_out = fptr(out);
+    check(mega_decayed_attention_step(&a, w.stream), "decayed_attention_step");
+  }
+  return {y, out};
+}
+
+// Separate operands, or one tensor z (B, L, H (2 K + V + 1)) that holds q, k, v and the gates side by side, whose gradient then comes
+// as one tensor too.
+struct AttParts {
+  Tensor q, k, v, f;
+  AttParts(const Tensor& z, int64_t heads, int64_t keys) {
+    const int64_t kd = heads * keys, vd = z.size(2) - 2 * kd - heads;
+    q = part(z, 0, kd, heads), k = part(z, kd, kd, heads), v = part(z, 2 * kd, vd, heads), f = z.narrow(2, 2 * kd + vd, heads);
+  }
+  static Tensor part(const Tensor& z, int64_t from, int64_t n, int64_t heads) {
+    return z.narrow(2, from, n).unflatten(2, {heads, n / heads});
+  }
+};
+class AttFn : public torch::autograd::Function<AttFn> {
+ public:
+  static variable_list forward(AutogradContext* ctx, Tensor q, OptTensor k, OptTensor v, OptTensor f, OptTensor pad, OptTensor reset,
+                               OptTensor h_in, double scale, bool want_state, bool reverse, int64_t heads, int64_t keys) {
+    Att r;
+    if (heads) {
+      const AttParts p(q.detach(), heads, keys);
+      r = att_args(p.q, p.k, p.v, p.f, given(pad), given(reset), given(h_in), scale, reverse);
+    } else {
+      r = att_args(q, *k, *v, *f, given(pad), given(reset), given(h_in), scale, reverse);
+    }
+    const Where w(q);
+    Tensor y = rec_like(r.v), h = want_state ? att_state(r.q, r.v) : Tensor();
+    run_att(r, y, h, w);
+    ctx->set_materialize_grads(false);
+    const Tensor state = given(h_in);
+    const bool same = state.defined() && r.h_in.data_ptr() == state.data_ptr();
+    ctx->save_for_backward({q, given(k), given(v), given(f), r.pad, r.reset, same ? state : r.h_in});
+    ctx->saved_data["state"] = state.defined() ? (int64_t)state.scalar_type() : (int64_t)-1;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["reverse"] = reverse;
+    ctx->saved_data["heads"] = heads;
+    ctx->saved_data["keys"] = keys;
+    if (!want_state) return {y};
+    return {y, h};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order();
+    const auto s = ctx->get_saved_variables();
+    const int64_t heads = ctx->saved_data["heads"].toInt(), keys = ctx->saved_data["keys"].toInt();
+    const int64_t state = ctx->saved_data["state"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const bool reverse = ctx->saved_data["reverse"].toBool();
+    const Where w(s[0]);
+    Att r;
+    Tensor dz, dq, dk, dv, df;
+    if (heads) {
+      const AttParts p(s[0].detach(), heads, keys);
+      r = att_args(p.q, p.k, p.v, p.f, s[4], s[5], s[6], scale, reverse);
+      dz = at::empty(s[0].sizes(), s[0].options().requires_grad(false));
+      const AttParts d(dz, heads, keys);
+      dq = d.q, dk = d.k, dv = d.v, df = d.f;
+    } else {
+      r = att_args(s[0], s[1], s[2], s[3], s[4], s[5], s[6], scale, reverse);
+      dq = rec_like(r.q), dk = rec_like(r.k), dv = rec_like(r.v), df = at::empty(r.f.sizes(), r.f.options().requires_grad(false));
+    }
+    const Tensor dy = grads[0].defined() ? rec_grad(grads[0], r.v) : at::zeros(r.v.sizes(), r.v.options());
+    const Tensor dh_out = grads.size() > 1 && grads[1].defined() ? f32c(grads[1]) : Tensor();
+    Tensor dh_in = state >= 0 ? att_state(r.q, r.v) : Tensor();
+    mega_decayed_attention_args& a = r.a;
+    a.dy = dy.data_ptr(), a.dq = dq.data_ptr(), a.dk = dk.data_ptr(), a.dv = dv.data_ptr(), a.df = df.data_ptr();
+    put(a.gs, dy, 0), put(a.dqs, dq, 0), put(a.dks, dk, 0), put(a.dvs, dv, 0), put(a.dfs, df, 0);
+    a.dh_out = fptr(dh_out), a.dh_in = fptr(dh_in);
+    const Tensor work = att_work(a, 1, dy);
+    a.work = ptr(work);
+    check(mega_decayed_attention_bwd(&a, w.stream), "decayed_attention_bwd");
+    if (dh_in.defined()) dh_in = dh_in.to((at::ScalarType)state);
+    const Tensor no;
+    if (heads) return {dz, no, no, no, no, no, dh_in, no, no, no, no, no};
+    return {dq, dk, dv, df, no, no, dh_in, no, no, no, no, no};
+  }
+};
+// (y, h) or (y,); differentiable
+variable_list decayed_attention_train(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& f_, const OptTensor& pad,
+                                      const OptTensor& reset, const OptTensor& h_in, double scale, bool want_state, bool reverse) {
+  on_cuda(q, k, v, f_);
+  const Tensor f = gates_of(f_, q);
+  if (q.numel() == 0 || v.numel() == 0) {   // (else AttFn checks them, and converts what it has to once)
+    att_args(q, k, v, f, given(pad), given(reset), given(h_in), scale, reverse);
+    variable_list r = {v * ((q * k).sum(-1, true) * f.unsqueeze(-1)).to(v.scalar_type())};   // (no values, but gradients of that shape)
+    if (want_state) r.push_back(h_in.has_value() ? h_in->to(at::kFloat, false, true) : att_state(q, v).zero_());
+    return r;
+  }
+  return AttFn::apply(q, OptTensor(k), OptTensor(v), OptTensor(f), pad, reset, h_in, scale, want_state, reverse, (int64_t)0, (int64_t)0);
+}
+variable_list decayed_attention_packed(const Tensor& z, int64_t heads, int64_t keys, const OptTensor& pad, const OptTensor& reset,
+                                       const OptTensor& h_in, double scale, bool want_state, bool reverse) {
+  on_cuda(z);
+  expect(z.dim() == 3 && heads >= 1 && keys >= 1 && (z.size(2) - heads * (2 * keys + 1)) > 0 && (z.size(2) - heads * (2 * keys + 1)) % heads == 0,
+         "the packed operand must be (batch, length, heads (2 keys + values + 1))");
+  if (z.numel() == 0) {
+    const AttParts p(z, heads, keys);
+    return decayed_attention_train(p.q, p.k, p.v, p.f, pad, reset, h_in, scale, want_state, reverse);
+  }
+  return AttFn::apply(z, OptTensor(), OptTensor(), OptTensor(), pad, reset, h_in, scale, want_state, reverse, heads, keys);
+}
+
+// -------------------------------------------------------------------- root-mean-square norm with a residual
+struct Rms {
+  Tensor x, res, w;
+  int B, L, D, G;
+};
+Rms rms_args(const Tensor& x, const Tensor& weight, const Tensor& res, int64_t groups) {
+  on_cuda(x, weight, res);
+  dtype_of(x);
+  expect(x.dim() >= 2, "x must be (batch, ..., channels)");
+  same_kind(res, x, "the residual");
+  const int64_t d = x.size(-1);
+  expect(groups >= 1 && d % groups == 0, "num_groups must divide the channels");
+  expect_numel(weight, d, "weight");
+  if (!at::isFloatingType(weight.scalar_type())) throw py::type_error("weight must be a floating-point tensor");
+  if (weight.device() != x.device()) throw py::value_error("weight must be on x's device");
+  Rms r;
+  if (x.numel() == 0) return r;
+  r.x = gn_rows(x.detach());
+  if (res.defined()) r.res = gn_rows(res.detach());
+  r.w = gn_param(weight.detach());
+  r.B = extent(r.x.size(0)), r.L = extent(r.x.size(1)), r.D = extent(d), r.G = extent(groups);
+  return r;
+}
+// y, and r with a residual
+std::pair<Tensor, Tensor> run_rms(const Tensor& x, const Rms& r, double eps, const Where& w) {
+  auto [out, y] = gn_like(x, r.x);
+  Tensor total, sum;
+  if (r.res.defined()) std::tie(total, sum) = gn_like(x, r.x);
+  check(mega_rms_norm_fwd(r.x.data_ptr(), ptr(r.res), y.data_ptr(), ptr(sum), dtype_of(r.x), r.B, r.L, r.D, STRIDES2(r.x), STRIDES2(r.res),
+                          STRIDES2(y), STRIDES2(sum), fptr(r.w), r.G, eps, w.stream), "rms_norm_fwd");
+  return {out, total};
+}
+std::tuple<Tensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight, const OptTensor& res, int64_t groups, double eps) {
+  const Rms r = rms_args(x, weight, given(res), groups);
+  const bool two = res.has_value();
+  if (x.numel() == 0) return {fresh(x), two ? OptTensor(fresh(x)) : std::nullopt};
+  const Where w(x);
+  auto [y, sum] = run_rms(x, r, eps, w);
+  return {y, two ? OptTensor(sum) : std::nullopt};
+}
+class RmsFn : public torch::autograd::Function<RmsFn> {
+ public:
+  static variable_list forward(AutogradContext* ctx, Tensor x, Tensor weight, OptTensor res, int64_t groups, double eps) {
+    const Rms r = rms_args(x, weight, given(res), groups);
+    const Where w(x);
+    auto [y, sum] = run_rms(x, r, eps, w);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({sum.defined() ? sum : x, weight});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["residual"] = sum.defined();
+    if (!sum.defined()) return {y};
+    return {y, sum};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order();
+    const auto s = ctx->get_saved_variables();
+    const Rms r = rms_args(s[0], s[1], Tensor(), ctx->saved_data["groups"].toInt());
+    const Where w(s[0]);
+    const int dt = dtype_of(r.x);
+    auto rows = [&](const Tensor& g) { return g.defined() ? gn_rows(g.scalar_type() == r.x.scalar_type() ? g : g.to(r.x.scalar_type())) : Tensor(); };
+    Tensor dy = rows(grads[0]);
+    const Tensor dr = grads.size() > 1 ? rows(grads[1]) : Tensor();
+    if (!dy.defined()) dy = at::zeros(r.x.sizes(), r.x.options());
+    auto [out, dx] = gn_like(s[0], r.x);
+    Tensor dw = floats({r.D}, r.x);
+    const Tensor work = bytes_of(mega_rms_norm_work(dt, r.B, r.L, r.D, r.G), r.x);
+    check(mega_rms_norm_bwd(dy.data_ptr(), ptr(dr), r.x.data_ptr(), dx.data_ptr(), dt, r.B, r.L, r.D, STRIDES2(dy), STRIDES2(dr), STRIDES2(r.x),
+                            STRIDES2(dx), fptr(r.w), r.G, ctx->saved_data["eps"].toDouble(), fptr(dw), work.data_ptr(), w.stream), "rms_norm_bwd");
+    const Tensor& weight = s[1];
+    Tensor g = weight.dim() == 1 ? dw : dw.view(weight.sizes());
+    if (weight.scalar_type() != at::kFloat) g = g.to(weight.scalar_type());
+    return {out, g, ctx->saved_data["residual"].toBool() ? out : Tensor(), Tensor(), Tensor()};
+  }
+};
+variable_list rms_norm_train(const Tensor& x, const Tensor& weight, const OptTensor& res, int64_t groups, double eps) {
+  if (x.numel() == 0) {   // (no values, but gradients of that shape)
+    rms_args(x, weight, given(res), groups);
+    const Tensor total = res.has_value() ? x + *res : x;
+    const Tensor y = (total * weight.view({-1})).to(x.scalar_type());
+    return res.has_value() ? variable_list{y, total} : variable_list{y};
+  }
+  return RmsFn::apply(x, weight, res, groups, eps);
+}
+
 Tensor softmax_fwd(const Tensor& x, bool causal) {
   on_cuda(x);
   const Where w(x);
@@ -1736,6 +2045,12 @@ PYBIND11_MODULE(_mega_host, m) {
   m.def("gated_recurrence_step", &gated_recurrence_step);
   m.def("gated_recurrence_train", &gated_recurrence_train);
   m.def("gated_recurrence_packed", &gated_recurrence_packed);
+  m.def("decayed_attention", &decayed_attention);
+  m.def("decayed_attention_step", &decayed_attention_step);
+  m.def("decayed_attention_train", &decayed_attention_train);
+  m.def("decayed_attention_packed", &decayed_attention_packed);
+  m.def("rms_norm", &rms_norm);
+  m.def("rms_norm_train", &rms_norm_train);
   m.def("group_norm", &group_norm);
   m.def("group_norm_fwd", &group_norm_fwd);
   m.def("group_norm_train", &group_norm_train);

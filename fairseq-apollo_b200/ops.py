@@ -535,6 +535,38 @@ def gated_recurrence_step(x, forget, input_gate=None, h=None, h_out=None):
     return _lib.host().gated_recurrence_step(x, forget, input_gate, h, h_out)
 
 
+# ------------------------------------- linear attention with a decay for each head
+def decayed_attention_fwd(q, k, v, forget, padding_mask=None, reset_mask=None, h_in=None, scale=1.0, want_state=False, reverse=False):
+    """S_t = a_t S_{t-1} + k_t v_t^T, y_t = scale S_t^T q_t with a = sigmoid(forget), one state S (K, V) per sequence and head, over the
+    steps of q, k (B, L, H, K), v (B, L, H, V) (1 to 256 keys and values), forget (B, L, H) or, the same at every step, (H).  q, k and v
+    share a dtype, forget has it too or is float32; strides are free (column slices, time-major memory, heads that share keys by
+    ``expand``), a copy is made where the last axis is not contiguous.
+    padding_mask (B, L), non-zero = padded: the state stays as it is, y = 0.  reset_mask (B, L), non-zero: the step starts from a
+    zero state (the first step of a document in a packed sequence).  h_in (B, H, K, V): the state that comes in.
+    In 16-bit types pairs' weights and the state are rounded to that type where they enter matrix products (a state beyond fp16's
+    range then is infinite); sums and the state itself are fp32.  A value that is not finite at a step that is not padded may reach
+    every output of its sequence and head.
+    ``reverse`` walks from the last step to the first.
+    Returns y like v, and the state behind the walk's last step (B, H, K, V) fp32 when ``want_state``."""
+    y, h = _lib.host().decayed_attention(q, k, v, forget, padding_mask, reset_mask, h_in, float(scale), want_state, reverse)
+    return (y, h) if want_state else y
+
+
+def decayed_attention_step(q, k, v, forget, h=None, scale=1.0, h_out=None):
+    """One step: q, k (B, H, K), v (B, H, V), forget (B, H) or (H), h (B, H, K, V) the state (None: zero) -> (y like v, h' (B, H, K, V)
+    fp32).  ``h_out``: the contiguous fp32 tensor that takes h': ``h`` itself for an update in place, or memory that overlaps neither it
+    nor q, k, v and the gates.  It counts as changed in place."""
+    return _lib.host().decayed_attention_step(q, k, v, forget, h, float(scale), h_out)
+
+
+# -------------------------------------------- root-mean-square norm with a residual
+def rms_norm_fwd(x, weight, residual=None, num_groups=1, eps=1e-5):
+    """r = x + residual, rounded to x's type, y = r / sqrt(mean(r^2) + eps) * (1 + weight) for x (B, ..., D): the mean over each group of
+    D / num_groups adjacent channels.  Returns y, or (y, r) with a residual (of x's shape and dtype)."""
+    y, r = _lib.host().rms_norm(x, weight, residual, int(num_groups), float(eps))
+    return y if residual is None else (y, r)
+
+
 # ------------------------------------------------------ group norm with an activation
 def group_norm_fwd(x, gamma, beta, num_groups, padding_mask=None, eps=1e-5, activation=None, offset=False):
     """Group norm of x (B, ..., D), channels last: mean and variance of a group of D / num_groups adjacent channels over all

@@ -677,6 +677,72 @@ MEGA_API int mega_group_norm_bwd(const void* dy, const void* x, void* dx, int dt
                         const uint8_t* pad_mask, int num_groups, unsigned flags, const int64_t* count, const float* mean,
                         const float* rstd, float* dgamma, float* dbeta, void* work, mega_stream_t stream);
 
+/*
+ * ---- Linear attention with a decay for each head -----------------------------------------------
+ * One state S (K, V) per sequence and head, q, k (B, L, H, K), v (B, L, H, V), f (B, L, H):
+ *   S_t = a_t S_{t-1} + k_t v_t^T      y_t = scale S_t^T q_t      a = sigmoid(f)
+ * A step whose byte of reset_mask is set starts from a zero state; a step whose byte of pad_mask is set leaves the state as it
+ * is (after the reset, when both are set), gives y = 0, and what lies there in q, k, v, f, dy is not used.  MEGA_ATT_REVERSE walks
+ * from the last step to the first.  A value of q, k, v that is not finite at a step that is not padded may reach every output of its
+ * sequence and head.
+ *
+ * Strides are in elements, (sequence, step, head), the last axis is contiguous; those of what is read are free, 0 and negative
+ * ones among them, outputs overlap neither one another nor an input.  q, k, v, y, dy and their gradients are of `dtype`, f and df
+ * of `gate_dtype`: MEGA_F32 or `dtype`.  Masks are (B, L) uint8.  h_in, h_out, dh_out, dh_in are (B, H, K, V) fp32, contiguous; either
+ * may be NULL (a NULL h_in or dh_out is zero), h_out may be h_in, dh_in may be dh_out.  K and V are at most MEGA_ATT_MOST
+ * (MEGA_ERR_UNSUPPORTED).
+ * `work`: device memory of mega_decayed_attention_work() bytes, 16-byte aligned, used by this call alone until it is done (may be
+ * NULL where that is 0).
+ *
+ * mega_decayed_attention_fwd: y, h_out.
+ * mega_decayed_attention_bwd: from q, k, v, f, h_in, dy and dh_out the gradients dq, dk, dv, df (0 at padded steps) and dh_in.
+ * mega_decayed_attention_step: one step of every sequence (L = 1, the second stride of each operand is not used, no masks): y, h_out.
+ * In 16-bit types the products' operands (pairs' weights, the state) are rounded to that type, sums and the state are fp32.
+ */
+#define MEGA_ATT_REVERSE 1u
+#define MEGA_ATT_MOST 256
+typedef struct {
+  int32_t dtype, gate_dtype, B, L, H, K, V;
+  uint32_t flags;
+  double scale;
+  const void *q, *k, *v, *f;
+  int64_t qs[3], ks[3], vs[3], fs[3];
+  const uint8_t *pad_mask, *reset_mask;
+  const float* h_in;
+  float* h_out;
+  void* y;
+  int64_t ys[3];
+  const void* dy;
+  int64_t gs[3];
+  const float* dh_out;
+  float* dh_in;
+  void *dq, *dk, *dv, *df;
+  int64_t dqs[3], dks[3], dvs[3], dfs[3];
+  void* work;
+} mega_decayed_attention_args;
+MEGA_API int64_t mega_decayed_attention_work(const mega_decayed_attention_args* args, int backward);
+MEGA_API int mega_decayed_attention_fwd(const mega_decayed_attention_args* args, mega_stream_t stream);
+MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_args* args, mega_stream_t stream);
+MEGA_API int mega_decayed_attention_step(const mega_decayed_attention_args* args, mega_stream_t stream);
+
+/*
+ * ---- Root-mean-square norm with a residual -----------------------------------------------------
+ * Rows of D contiguous channels in num_groups groups of D / num_groups adjacent ones: r = x + residual, rounded to the activations'
+ * type (residual == NULL: r = x), y = r / sqrt(mean(r^2) + eps) * (1 + weight), the mean over a group.  Operands are (B, L, D),
+ * strides of the first two axes free; weight (D) fp32.
+ * mega_rms_norm_fwd: y, and r where `sum` is not NULL (it is required with a residual).
+ * mega_rms_norm_bwd: from dy, dr (r's own gradient, NULL: zero) and r the gradient dx of x, which is the residual's too, and dweight
+ * (D) fp32, summed over rows in a fixed order.  `work`: device memory of mega_rms_norm_work() bytes, 16-byte aligned, used by this
+ * call alone until it is done.  At most 65535 groups and 2^20 channels (MEGA_ERR_UNSUPPORTED).
+ */
+MEGA_API int64_t mega_rms_norm_work(int dtype, int B, int L, int D, int num_groups);
+MEGA_API int mega_rms_norm_fwd(const void* x, const void* residual, void* y, void* sum, int dtype, int B, int L, int D, int64_t xsb,
+                      int64_t xsl, int64_t rsb, int64_t rsl, int64_t ysb, int64_t ysl, int64_t ssb, int64_t ssl, const float* weight,
+                      int num_groups, double eps, mega_stream_t stream);
+MEGA_API int mega_rms_norm_bwd(const void* dy, const void* dr, const void* r, void* dx, int dtype, int B, int L, int D, int64_t gsb,
+                      int64_t gsl, int64_t rgsb, int64_t rgsl, int64_t rsb, int64_t rsl, int64_t dsb, int64_t dsl, const float* weight,
+                      int num_groups, double eps, float* dweight, void* work, mega_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
