@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
 
     if constexpr (kOut) {
       // ---- the state that enters: written by the walk of dq, and multiplied with the gradient of the one that leaves by that of dk
-      if (kDots && gt.enter != 0.f) {
+      if (kDots && gt.enter > (kDots == 1 ? 0.f : kLeast)) {
         T* a = static_cast<T*>(w.anchors) + slot(((long long)bh * w.chunks + tile_of(c)) * w.tiles + tile);
         if (kDots == 1) each_state([&](float& v, int r, int cc) { Elem<T>::st(a + r * VT + cc, v); });
         else {
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
       if (kDots == 2 && tid == 0) {
         float sum = 0.f;
         for (int i = 0; i < kWarps; ++i) sum += sh.sums[i];
-        w.through[((long long)bh * w.chunks + tile_of(c)) * w.tiles + tile] = gt.enter == 0.f ? 0.f : gt.enter * sum;
+        w.through[((long long)bh * w.chunks + tile_of(c)) * w.tiles + tile] = gt.enter > kLeast ? gt.enter * sum : 0.f;
       }
     }
 
@@ -641,13 +641,15 @@ int value_tile(int keys) { return key_tile(keys) == 256 ? 32 : 64; }
 // How a walk is cut: into tiles of values, and, where (sequence, head, tile)s do not fill the device, the time axis into segments,
 // whose states are found first at the price of a second pass over keys and values.
 struct Plan {
+  bool tc;
   int tiles, chunks, per, segs;
   size_t local, factor, anchors, through;   // floats
 };
-Plan plan_of(int dtype, int B, int L, int H, int keys, int values) {
+Plan plan_of(bool tc, int dtype, int B, int L, int H, int keys, int values) {
   Plan p;
-  const int c = kC, vt = value_tile(keys);
-  const long long places = 2 * 148;
+  p.tc = tc;
+  const int c = tc ? kTcChunk : kC, vt = tc ? (values <= 64 ? 64 : 128) : value_tile(keys);
+  const long long places = tc ? 148 : 2 * 148;
   p.chunks = (L + c - 1) / c;
   p.tiles = (values + vt - 1) / vt;
   const long long blocks = (long long)B * H * p.tiles;
@@ -662,9 +664,10 @@ Plan plan_of(int dtype, int B, int L, int H, int keys, int values) {
   p.local = even(n * p.tiles * keys * vt);
   p.factor = even(n);
   p.anchors = even(bh * p.chunks * p.tiles * keys * vt * elem_size(dtype) / 4 + 1);
-  p.through = even(bh * p.chunks * p.tiles);
+  p.through = even(bh * p.chunks * std::max(p.tiles, kTcParts));
   return p;
 }
+bool tc_heads(const mega_decayed_attention_args& a) { return a.dtype != MEGA_F32 && a.K <= kTcMost && a.V <= kTcMost; }
 
 template <typename T, int KD, int VT, int STAGES>
 void run_walk(const Walk& w, int dots, void* stream) {
@@ -691,6 +694,7 @@ int run(int dtype, Walk& w, const Plan& p, int dots, float* work, void* stream) 
   if ((long long)p.tiles * w.B * w.H * p.segs > 0x7fffffffLL) return MEGA_ERR_UNSUPPORTED;
   w.local = work, w.factor = work + p.local;
   w.piece = vec_of(w.out, w.ob, w.ol, w.oh, w.v.d, elem_size(dtype), 32);
+  if (p.tc) return tc_walk(dtype, w, dots, stream);
   MEGA_DISPATCH_DTYPE(dtype, run_keys<T>(w, dots, stream));
   return MEGA_OK;
 }
@@ -719,20 +723,22 @@ struct BackPlan {
   Plan dq, dk, dv;
   size_t walk, dots, all;   // floats
 };
-BackPlan back_plan(const mega_decayed_attention_args& a) {
+BackPlan back_plan(const mega_decayed_attention_args& a, bool tc) {
   BackPlan p;
-  p.dq = p.dk = plan_of(a.dtype, a.B, a.L, a.H, a.V, a.K);
-  p.dv = plan_of(a.dtype, a.B, a.L, a.H, a.K, a.V);
+  p.dq = p.dk = plan_of(tc, a.dtype, a.B, a.L, a.H, a.V, a.K);
+  p.dv = plan_of(tc, a.dtype, a.B, a.L, a.H, a.K, a.V);
   p.walk = std::max(p.dq.local + p.dq.factor, p.dv.local + p.dv.factor);
   p.dots = ((size_t)a.B * a.H * p.dq.tiles * a.L * 2 + 3) / 4 * 4;
   p.all = p.walk + 2 * p.dots + p.dq.anchors + p.dq.through;
   return p;
 }
-size_t forward_floats(const mega_decayed_attention_args& a) {
-  const Plan p = plan_of(a.dtype, a.B, a.L, a.H, a.K, a.V);
+// (whether the tensor memory's form takes a call depends on its memory too: room for either)
+size_t forward_floats(const mega_decayed_attention_args& a, bool tc) {
+  const Plan p = plan_of(tc, a.dtype, a.B, a.L, a.H, a.K, a.V);
   return p.local + p.factor;
 }
 }  // namespace
+cudaError_t decayed_attention_read_device_error(int* v, bool reset) { return tc_read_device_error(v, reset); }
 }  // namespace mega
 
 using namespace mega;
@@ -740,7 +746,8 @@ using namespace mega;
 extern "C" MEGA_API int64_t mega_decayed_attention_work(const mega_decayed_attention_args* a, int backward) {
   if (!a || !valid_dtype(a->dtype) || a->B <= 0 || a->L <= 0 || a->H <= 0 || a->K <= 0 || a->V <= 0 || a->K > MEGA_ATT_MOST || a->V > MEGA_ATT_MOST)
     return 0;
-  size_t n = backward ? back_plan(*a).all : forward_floats(*a);
+  size_t n = backward ? back_plan(*a, false).all : forward_floats(*a, false);
+  if (tc_heads(*a)) n = std::max(n, backward ? back_plan(*a, true).all : forward_floats(*a, true));
   return (int64_t)(n * sizeof(float));
 }
 
@@ -751,7 +758,7 @@ extern "C" MEGA_API int mega_decayed_attention_fwd(const mega_decayed_attention_
   const int size = elem_size(a->dtype);
   Walk w = base(*a);
   w.q = operand(a->q, a->qs, a->K, size), w.k = operand(a->k, a->ks, a->K, size), w.v = operand(a->v, a->vs, a->V, size);
-  const Plan p = plan_of(a->dtype, a->B, a->L, a->H, a->K, a->V);
+  const Plan p = plan_of(tc_takes(a->dtype, w), a->dtype, a->B, a->L, a->H, a->K, a->V);
   if (p.segs > 1 && !a->work) return MEGA_ERR_NULL;
   if (a->work && !aligned_to(a->work, 16)) return MEGA_ERR_ALIGN;
   w.out = a->y, w.ob = a->ys[0], w.ol = a->ys[1], w.oh = a->ys[2];
@@ -772,7 +779,7 @@ extern "C" MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_
                 dy = operand(a->dy, a->gs, a->V, size);
   Walk w = base(*a);
   w.q = dy, w.k = v, w.v = k, w.x = q;
-  const BackPlan p = back_plan(*a);
+  const BackPlan p = back_plan(*a, tc_takes(a->dtype, w));
   float* at = static_cast<float*>(a->work);
   auto take = [&](size_t n) { float* r = at; at += n; return r; };
   float* walk = take(p.walk);
@@ -804,9 +811,10 @@ extern "C" MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_
   rc = run(a->dtype, w, p.dv, 0, walk, stream);
   if (rc) return rc;
 
-  const GateGrad gg = {forward, dots_q, dots_k, through, p.dq.tiles, p.dk.tiles, p.dk.tiles, a->df, a->dfs[0], a->dfs[1],
+  const GateGrad gg = {forward, dots_q, dots_k, through, p.dq.tiles, p.dk.tiles, p.dk.tc ? kTcParts : p.dk.tiles, a->df, a->dfs[0], a->dfs[1],
                        a->dfs[2]};
   const dim3 grid((unsigned)(((long long)a->B * a->H * forward.chunks + 3) / 4));
-  launch(gate_grad_kernel<kC / 32>, grid, dim3(128), 0, stream, gg);
+  if (p.dk.tc) launch(gate_grad_kernel<kTcChunk / 32>, grid, dim3(128), 0, stream, gg);
+  else launch(gate_grad_kernel<kC / 32>, grid, dim3(128), 0, stream, gg);
   return check_launch("decayed_attention_bwd");
 }

@@ -32,6 +32,10 @@ struct Walk {
   int rev, excl;
 };
 
+// The walk of dq leaves a chunk's state where its weight in the next one is above zero; that of dk, whose sum of the same gates may round
+// otherwise, reads it where the weight is well above.
+constexpr float kLeast = 1e-35f;
+
 __device__ __forceinline__ float gate_value(const Walk& w, long long at) {
   if (w.f_dtype == MEGA_F32) return __ldg(static_cast<const float*>(w.f) + at);
   if (w.f_dtype == MEGA_BF16) return Elem<__nv_bfloat16>::ld(static_cast<const __nv_bfloat16*>(w.f) + at);
@@ -113,5 +117,12 @@ __device__ __forceinline__ GateOut<N> gates_scan(const Walk& w, const GateIn<N>&
   r.padded = __any_sync(~0u, in.pad != 0);
   return r;
 }
+
+// The form on tcgen05 products (decayed_attention_tc.cu): 16-bit activations, heads of at most 128 keys and values
+constexpr int kTcChunk = 128, kTcMost = 128, kTcParts = 8;
+bool tc_takes(int dtype, const Walk& w);
+int tc_walk(int dtype, const Walk& w, int dots, void* stream);
+cudaError_t tc_read_device_error(int* v, bool reset);
+cudaError_t decayed_attention_read_device_error(int* v, bool reset);
 
 }  // namespace mega
