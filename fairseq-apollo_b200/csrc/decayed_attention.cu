@@ -228,8 +228,9 @@ __device__ __forceinline__ void gates_put(const Walk& w, Gates& o, const GateIn<
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = gate_row<2>(w, lane, i);
-    o.hi[row] = (float)r.sum[i];
-    o.lo[row] = (float)(r.sum[i] - (double)o.hi[row]);
+    o.hi[row] = gate_sum(r.sum[i]);   // (finite)
+    o.lo[row] = gate_sum(r.sum[i] - (long long)(o.hi[row] * 0x1p40f));
+    o.hi[row] += r.bad;
     o.count[row] = r.count[i];
     o.weight[row] = r.weight[i];
     o.pad[row] = in.pad >> i & 1;
@@ -631,8 +632,11 @@ int vec_of(const void* p, long long sb, long long sl, long long sh, int d, int s
   }
   return size;
 }
-Operand operand(const void* p, const int64_t* s, int d, int size) {
-  return {p, s[0], s[1], s[2], d, vec_of(p, s[0], s[1], s[2], d, size, 16)};
+// (of an axis with one place the stride is not used)
+Operand operand(const mega_decayed_attention_args& a, const void* p, const int64_t* s, int d) {
+  Operand o = {p, a.B > 1 ? s[0] : 0, a.L > 1 ? s[1] : 0, a.H > 1 ? s[2] : 0, d, 0};
+  o.vec = vec_of(p, o.sb, o.sl, o.sh, d, elem_size(a.dtype), 16);
+  return o;
 }
 
 int key_tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -755,9 +759,8 @@ extern "C" MEGA_API int mega_decayed_attention_fwd(const mega_decayed_attention_
   const int bad = check_args(a);
   if (bad) return bad;
   if (!a->y) return MEGA_ERR_NULL;
-  const int size = elem_size(a->dtype);
   Walk w = base(*a);
-  w.q = operand(a->q, a->qs, a->K, size), w.k = operand(a->k, a->ks, a->K, size), w.v = operand(a->v, a->vs, a->V, size);
+  w.q = operand(*a, a->q, a->qs, a->K), w.k = operand(*a, a->k, a->ks, a->K), w.v = operand(*a, a->v, a->vs, a->V);
   const Plan p = plan_of(tc_takes(a->dtype, w), a->dtype, a->B, a->L, a->H, a->K, a->V);
   if (p.segs > 1 && !a->work) return MEGA_ERR_NULL;
   if (a->work && !aligned_to(a->work, 16)) return MEGA_ERR_ALIGN;
@@ -774,9 +777,8 @@ extern "C" MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_
   if (bad) return bad;
   if (!a->dy || !a->dq || !a->dk || !a->dv || !a->df || !a->work) return MEGA_ERR_NULL;
   if (!aligned_to(a->work, 16)) return MEGA_ERR_ALIGN;
-  const int size = elem_size(a->dtype);
-  const Operand q = operand(a->q, a->qs, a->K, size), k = operand(a->k, a->ks, a->K, size), v = operand(a->v, a->vs, a->V, size),
-                dy = operand(a->dy, a->gs, a->V, size);
+  const Operand q = operand(*a, a->q, a->qs, a->K), k = operand(*a, a->k, a->ks, a->K), v = operand(*a, a->v, a->vs, a->V),
+                dy = operand(*a, a->dy, a->gs, a->V);
   Walk w = base(*a);
   w.q = dy, w.k = v, w.v = k, w.x = q;
   const BackPlan p = back_plan(*a, tc_takes(a->dtype, w));

@@ -68,41 +68,43 @@ __device__ __forceinline__ GateIn<N> gates_fetch(const Walk& w, int b, int h, in
   }
   return g;
 }
-// What they come to: running sum of log2 a (in 64 bits), resets so far, weight of a step in the state that leaves, and the weight of
+// What they come to: running sum of log2 a (whole numbers of 2^-40: their order does not matter, so both directions agree), resets so far, weight of a step in the state that leaves, and the weight of
 // the state that enters in it (0: a reset lies between).  A gate whose decay is below fp32's range counts as a reset.
 template <int N>
 struct GateOut {
-  double sum[N];
+  long long sum[N];
   int count[N];
-  float weight[N], enter;
+  float weight[N], enter, bad;   // bad: what the sums have to be given besides, 0 or NaN
   int total;
   bool padded;
 };
 // log2 sigmoid(f), and whether that is no decay but a reset
-__device__ __forceinline__ double log2_gate(float f) {
-  return (double)(f < 0.f ? f - log1pf(expf(f)) : -log1pf(expf(-f))) * 1.4426950408889634;
-}
-__device__ __forceinline__ bool closed(double g) { return g < -149.; }
+__device__ __forceinline__ float log2_gate(float f) { return (f < 0.f ? f - log1pf(expf(f)) : -log1pf(expf(-f))) * 1.44269504f; }
+__device__ __forceinline__ bool closed(float g) { return g < -149.f; }
+__device__ __forceinline__ float gate_sum(long long s) { return (float)s * 0x1p-40f; }
 template <int N>
 __device__ __forceinline__ GateOut<N> gates_scan(const Walk& w, const GateIn<N>& in, int lane) {
-  double s[N], sum = 0.;
+  long long s[N], sum = 0;
   int c[N], cnt = 0;
+  bool nan = false;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    s[i] = in.pad >> i & 1 ? 0. : log2_gate(in.f[i]);
-    c[i] = (in.reset >> i & 1) || closed(s[i]);
-    if (c[i]) s[i] = 0.;
+    const float g = in.pad >> i & 1 ? 0.f : log2_gate(in.f[i]);
+    c[i] = (in.reset >> i & 1) || closed(g);
+    nan = nan || g != g;
+    s[i] = c[i] ? 0 : (long long)(g * 0x1p40f);
     sum += s[i], cnt += c[i];
   }
-  double upto = sum;
+  long long upto = sum;
   int counted = cnt;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double u = __shfl_up_sync(~0u, upto, o);
+    const long long u = __shfl_up_sync(~0u, upto, o);
     const int v = __shfl_up_sync(~0u, counted, o);
     if (lane >= o) upto += u, counted += v;
   }
-  const double all = __shfl_sync(~0u, upto, 31);
+  const float bad = __any_sync(~0u, nan) ? __int_as_float(0x7fffffff) : 0.f;   // (a gate that is NaN: the whole chunk is)
+  const long long all = __shfl_sync(~0u, upto, 31);
   GateOut<N> r;
   r.total = __shfl_sync(~0u, counted, 31);
   upto -= sum, counted -= cnt;   // (what lies before this lane's steps)
@@ -110,10 +112,11 @@ __device__ __forceinline__ GateOut<N> gates_scan(const Walk& w, const GateIn<N>&
   for (int i = 0; i < N; ++i) {
     if (!w.excl) upto += s[i], counted += c[i];
     r.sum[i] = upto, r.count[i] = counted;
-    r.weight[i] = counted == r.total && !(in.pad >> i & 1) ? w.s_scale * exp2f((float)(all - upto)) : 0.f;
+    r.weight[i] = counted == r.total && !(in.pad >> i & 1) ? w.s_scale * exp2f(gate_sum(all - upto) + bad) : 0.f;
     if (w.excl) upto += s[i], counted += c[i];
   }
-  r.enter = r.total ? 0.f : exp2f((float)all);
+  r.enter = r.total ? 0.f : exp2f(gate_sum(all) + bad);
+  r.bad = bad;
   r.padded = __any_sync(~0u, in.pad != 0);
   return r;
 }

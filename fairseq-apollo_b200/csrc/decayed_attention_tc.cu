@@ -8,12 +8,13 @@
 //   O2 = (weighted pairs) V
 // and y = e O1 + O2 with a row's factor e.  For the gates' gradient also X V^T, in O2's place before it.
 // Roles: four warps of pairs and outputs (a thread has a row of the chunk), four or eight of weights and state (a thread has a step's
-// keys, then a row of the state, whose fp32 values stay in its registers), three that load, one that issues products.  All exchange over
+// keys, then a row of the state, whose fp32 values stay in its registers), one that loads, one for the gates, one for padded steps, one that issues products.  All exchange over
 // mbarriers.
 //
-// Operands lie as planes of 16 bytes along keys or values, rows one after another: eight rows of a plane are a core matrix, so the same
-// memory serves with either axis as the contraction, a thread that owns a row reads and writes without bank conflicts, and so do loads
-// by cp.async of 8 rows x 64 bytes.  (cp.async and not TMA: any alignment down to 4 bytes, and padded rows arrive as zeros.)
+// Activations lie as TMA leaves them (columns of 64, rows of 128 bytes, swizzled), what the threads write as planes of 16 bytes along
+// keys or values, rows one after another.  Both serve with either axis as the contraction, and a thread that owns a row reads and
+// writes it without bank conflicts.  (Loads by cp.async, three warps of them, took 140 cycles each and held up every other access to
+// shared memory: 213 us where this takes LATER, 8 x 4096 x 16 heads of 64.)
 //
 // The state is accumulated by each chunk's own sum, which is then added in fp32: a long chain inside the tensor cores' accumulator
 // would be cut off, not rounded, thousands of times.
@@ -37,13 +38,14 @@ struct TcGates {
   int total;                   // resets
   int pad_[2];
 };
+// barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it
 enum { kQFull, kQEmpty, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kXFull = kVEmpty + 2, kXEmpty, kGFull, kGEmpty = kGFull + 2,
-       kPDone = kGEmpty + 2, kPReady, kODone, kORead, kSReady, kDsDone, kWReady, kLoFree, kW2Ready, kBars };
+       kPDone = kGEmpty + 2, kPReady, kODone, kORead, kSReady, kDsDone, kWReady, kLoFree, kW2Ready, kQRaw, kKRaw, kVRaw = kKRaw + 2, kXRaw = kVRaw + 2, kBars };
 
 // kOut: outputs; else the state that a segment leaves by itself.  kDots: sums for the gates' gradient (1: walk of dq, 2: of dk).
 template <typename T, int KD, int VD, bool kOut, int kDots>
 struct Lay {
-  static constexpr int kTk = KD / 8 * kPlane, kTv = VD / 8 * kPlane, kTs = VD / 8 * KD * 16;
+  static constexpr int kTk = KD * kC * 2, kTv = VD * kC * 2, kTs = VD / 8 * KD * 16;
   static constexpr int kPieces = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
   // with heads of 128 x 128 there is no room for the third piece: it takes the second's place when that has been used
   static constexpr bool kSeq = kOut && KD == 128 && VD == 128 && kPieces == 3;
@@ -53,7 +55,7 @@ struct Lay {
   // (a product over 128 rows of 64 keys reads on into what follows: no piece and no tile of keys is last)
   static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 && !kSeq ? kTk : 0), kOffV = kOffK + 2 * kTk,
                        kOffQ = kOffV + kVStages * kTv, kOffX = kOffQ + (kOut ? kTk : 0), kOffS = kOffX + (kDots ? kTv : 0),
-                       kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kEnd = kOffBar + kBars * 8 + 16;
+                       kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8, kEnd = kOffSlot + 16;
   static_assert(kEnd <= 227 * 1024, "shared memory");
   static_assert(sizeof(TcGates) % 16 == 0, "gates");
 };
@@ -121,58 +123,50 @@ __device__ __forceinline__ void umma_tm(uint32_t d, uint32_t a, uint64_t b, uint
                "r"(id), "r"((uint32_t)onto)
                : "memory");
 }
-// operands whose contraction runs along the planes (16 bytes: 8 places), or over the rows
-__device__ __forceinline__ uint64_t along(uint32_t at, uint32_t plane) { return umma_desc(at, plane, 128); }
+// planes whose contraction runs over the rows
 __device__ __forceinline__ uint64_t over(uint32_t at, uint32_t plane) { return umma_desc(at, 128, plane); }
 
-// ------------------------------------------------------------------------------------------------------- loads
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool there) {
-  const int n = there ? BYTES : 0;   // (0: zeros)
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(n) : "memory");
+// columns of 64: rows whose contraction runs along them, or over the rows
+constexpr int kBox = 64 * kC * 2;
+__device__ __forceinline__ uint64_t tile_desc(uint32_t at) {
+  return (uint64_t)((at >> 4) & 0x3fffu) | ((uint64_t)(kBox >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// a tile by one warp: 8 rows x 64 bytes at a time; rows behind the last one and padded ones become zeros
-template <int D, int VEC>
-__device__ __forceinline__ void load_rows(uint32_t to, const char* from, long long row_bytes, int rows, int bytes, const uint32_t (&pad)[4], int lane) {
-  const int r8 = lane & 7, c4 = lane >> 3;
+constexpr int kAlong(int k) { return (k / 4 * kBox + k % 4 * 32) / 16; }   // of 16 places
+constexpr int kOver(int k) { return k * 2048 / 16; }
+// 16 bytes of a row
+__device__ __forceinline__ uint32_t piece_of(int row, int c) { return c / 8 * kBox + row * 128 + ((c ^ row) & 7) * 16; }
+
+struct Maps {
+  CUtensorMap q, k, v, x;
+};
+__device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap* m, int c, int t, int h, int b, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
+               "l"(reinterpret_cast<uint64_t>(m)), "r"(c), "r"(t), "r"(h), "r"(b), "r"(bar)
+               : "memory");
+}
+// 128 steps of an operand; rows behind the last one and columns it does not have become zeros.  An axis whose stride is 0 has one place.
+template <int D>
+__device__ __forceinline__ void load_tile(uint32_t to, const CUtensorMap* m, const Operand& o, int t0, int h, int b, uint32_t bar) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(D * kC * 2) : "memory");
 #pragma unroll
-  for (int g = 0; g < kC / 8; ++g) {
-    const int r = g * 8 + r8;
-    const bool there = r < rows && !(pad[g >> 2] >> (r & 31) & 1);
-    const char* src = from + (there ? r : 0) * row_bytes;
-#pragma unroll
-    for (int c = 0; c < D / 8; c += 4)
-#pragma unroll
-      for (int s = 0; s < 16; s += VEC) {
-        const int at = (c + c4) * 16 + s;
-        if (at < bytes) copy_async<VEC>(to + (c + c4) * kPlane + r * 16 + s, src + at, there);
-      }
-  }
+  for (int c = 0; c < D; c += 64) tma_load_4d(to + c / 64 * kBox, m, c, t0, o.sh ? h : 0, o.sb ? b : 0, bar);
 }
 template <int D>
-__device__ __forceinline__ void load_tile(uint32_t to, const Operand& o, const char* base, long long t0, int rows, const uint32_t (&pad)[4], int lane) {
-  const char* from = base + t0 * o.sl * 2;
-  if (o.vec == 16) load_rows<D, 16>(to, from, o.sl * 2, rows, o.d * 2, pad, lane);
-  else if (o.vec == 8) load_rows<D, 8>(to, from, o.sl * 2, rows, o.d * 2, pad, lane);
-  else load_rows<D, 4>(to, from, o.sl * 2, rows, o.d * 2, pad, lane);
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int LEFT>
-__device__ __forceinline__ void landed(uint32_t bar) {   // (and visible to the tensor cores)
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-  fence_proxy_async();
-  arrive(bar);
+__device__ __forceinline__ void clear_rows(uint32_t at, const uint32_t (&pad)[4], int lane) {
+#pragma unroll 1
+  for (int k = 0; k < 4; ++k)
+    if (pad[k] >> lane & 1)
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) sts16(at + piece_of(32 * k + lane, c), make_uint4(0, 0, 0, 0));
 }
 
 template <typename T, int KD, int VD, bool kOut, int kDots>
-__global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_kernel(const __grid_constant__ Walk w) {
+__global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_kernel(const __grid_constant__ Walk w, const __grid_constant__ Maps maps) {
   using L = Lay<T, KD, VD, kOut, kDots>;
   constexpr int kStateWarps = L::kState, kHalves = kStateWarps / 4, kStateThreads = 32 * kStateWarps;
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int gone_;
-  __shared__ uint32_t tm_slot;
-  volatile int* gone = &gone_;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  int* const slot_ = reinterpret_cast<int*>(smem + L::kOffSlot);   // where tensor memory lies; whether a wait has given up
+  volatile int* gone = slot_ + 1;
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H), b = bh / w.H, h = bh % w.H;
@@ -185,24 +179,22 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   auto gates = [&](int n) -> TcGates& { return reinterpret_cast<TcGates*>(smem + L::kOffG)[n & 1]; };
 
   if (tid == 0) {
-    gone_ = 0;
+    *gone = 0;
     auto init = [&](int i, uint32_t count) { mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, count); };
-    for (int i : {(int)kQFull, (int)kKFull, kKFull + 1, (int)kVFull, kVFull + 1, (int)kXFull, (int)kGFull, kGFull + 1}) init(i, 32);
+    for (int i : {(int)kQFull, (int)kKFull, kKFull + 1, (int)kVFull, kVFull + 1, (int)kXFull, (int)kQRaw, (int)kKRaw, kKRaw + 1, (int)kVRaw, kVRaw + 1, (int)kXRaw})
+      init(i, 1);
+    for (int i : {(int)kGFull, kGFull + 1}) init(i, 32);
     for (int i : {(int)kQEmpty, (int)kKEmpty, kKEmpty + 1, (int)kVEmpty, kVEmpty + 1, (int)kPDone, (int)kODone, (int)kDsDone, (int)kLoFree}) init(i, 1);
     for (int i : {(int)kXEmpty, (int)kPReady, (int)kORead}) init(i, 128);
     for (int i : {(int)kSReady, (int)kWReady, (int)kW2Ready}) init(i, kStateThreads);
     for (int i : {(int)kGEmpty, kGEmpty + 1}) init(i, kStateThreads + (kOut ? 128 : 0));
     mbar_fence_init();
   }
-  if (w.k.d < KD || w.v.d < VD) {   // (columns that no load writes)
-    for (int i = tid; i < L::kOffG / 16; i += L::kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-    fence_proxy_async();
-  }
-  if (warp == 0) tm_alloc(smem_u32(&tm_slot), kOut ? 512 : 128);
+  if (warp == 0) tm_alloc(smem_u32(slot_), kOut ? 512 : 128);
   tm_before();
   __syncthreads();
   tm_after();
-  const uint32_t tm = tm_slot;
+  const uint32_t tm = *reinterpret_cast<volatile uint32_t*>(slot_);
   constexpr uint32_t kCs = kOut ? kColS : 0;
 
   if (warp < 4) {
@@ -290,7 +282,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           if constexpr (kDots != 0) {
 #pragma unroll
             for (int m = 0; m < 32; m += 8) {
-              const uint4 u = lds16(base + L::kOffX + (c + m) / 8 * kPlane + i * 16);
+              const uint4 u = lds16(base + L::kOffX + piece_of(i, (c + m) / 8));
               const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
@@ -377,7 +369,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       uint4 last[L::kSeq ? kPlanes : 1];
 #pragma unroll
       for (int c = 0; c < kPlanes; ++c) {
-        const uint32_t at = (half * kPlanes + c) * kPlane + row * 16, key = base + L::kOffK + (n & 1) * L::kTk + at;
+        const uint32_t at = (half * kPlanes + c) * kPlane + row * 16, key = base + L::kOffK + (n & 1) * L::kTk + piece_of(row, half * kPlanes + c);
         const uint4 u = lds16(key);
         const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
         uint32_t piece[3][4];
@@ -470,60 +462,78 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       for (int c = 0; c < 64; ++c)
         if (col0 + c < w.v.d) w.s_out[s_at + (long long)(col0 + c) * w.s_col] = st[c];
     }
-  } else if (warp < 4 + kStateWarps + 3) {
+  } else if (warp == 4 + kStateWarps) {
     // ================================================================================ loads
-    const int lw = warp - 4 - kStateWarps;
-    const char* qp = static_cast<const char*>(w.q.p) + (b * w.q.sb + h * w.q.sh) * 2;
-    const char* kp = static_cast<const char*>(w.k.p) + (b * w.k.sb + h * w.k.sh) * 2;
-    const char* vp = static_cast<const char*>(w.v.p) + (b * w.v.sb + h * w.v.sh) * 2;
-    const char* xp = static_cast<const char*>(w.x.p) + (b * w.x.sb + h * w.x.sh) * 2;
-    GateIn<4> ahead;
-    if (lw == 0) ahead = gates_fetch<4>(w, b, h, tile_of(0), lane);
-    for (int n = 0; n < chunks; ++n) {
-      const long long t0 = (long long)tile_of(n) * kC;
-      const int rows = (int)min((long long)kC, w.L - t0);
-      uint32_t pad[4] = {0, 0, 0, 0};
-      if (w.pad) {
-        const uint8_t* m = w.pad + (long long)b * w.L + t0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) pad[k] = __ballot_sync(~0u, 32 * k + lane < rows && m[32 * k + lane]);
-      }
-      if (lw == 0) {
-        const GateIn<4> in = ahead;
-        if (n + 1 < chunks) ahead = gates_fetch<4>(w, b, h, tile_of(n + 1), lane);
+    if (umma_elect()) {
+      constexpr int kS = L::kVStages;
+      const bool raw = w.pad != nullptr;
+      for (int n = 0; n < chunks; ++n) {
+        const int t0 = tile_of(n) * kC, stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
+        if (n > 1) wait(kKEmpty + (n & 1), ((n >> 1) - 1) & 1);
+        load_tile<KD>(base + L::kOffK + (n & 1) * L::kTk, &maps.k, w.k, t0, h, b, bar((raw ? kKRaw : kKFull) + (n & 1)));
+        auto values = [&]() {
+          if (use) wait(kVEmpty + stage, (use - 1) & 1);
+          load_tile<VD>(base + L::kOffV + stage * L::kTv, &maps.v, w.v, t0, h, b, bar((raw ? kVRaw : kVFull) + stage));
+        };
+        if (kS == 2) values();
         if (kOut) {
           if (n) wait(kQEmpty, (n - 1) & 1);
-          load_tile<KD>(base + L::kOffQ, w.q, qp, t0, rows, pad, lane);
+          load_tile<KD>(base + L::kOffQ, &maps.q, w.q, t0, h, b, bar(raw ? kQRaw : kQFull));
         }
-        if (n > 1) wait(kGEmpty + (n & 1), ((n >> 1) - 1) & 1);
-        const GateOut<4> r = gates_scan<4>(w, in, lane);
-        TcGates& g = gates(n);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int at = gate_row<4>(w, lane, k);
-          g.sum[at] = (float)r.sum[k], g.weight[at] = r.weight[k], g.count[at] = (uint8_t)r.count[k];
-        }
-        if (lane == 0) g.enter = r.enter, g.total = r.total;
-        __syncwarp();
-        arrive(bar(kGFull + (n & 1)));
-        if (kOut) landed<0>(bar(kQFull));
-      } else if (lw == 1) {
-        if (n > 1) wait(kKEmpty + (n & 1), ((n >> 1) - 1) & 1);
-        load_tile<KD>(base + L::kOffK + (n & 1) * L::kTk, w.k, kp, t0, rows, pad, lane);
-        landed<0>(bar(kKFull + (n & 1)));
-      } else {
-        constexpr int kS = L::kVStages;
-        const int stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
-        if (use) wait(kVEmpty + stage, (use - 1) & 1);
-        load_tile<VD>(base + L::kOffV + stage * L::kTv, w.v, vp, t0, rows, pad, lane);
         if (kDots) {
           if (n) wait(kXEmpty, (n - 1) & 1);
-          load_tile<VD>(base + L::kOffX, w.x, xp, t0, rows, pad, lane);
-          landed<1>(bar(kVFull + stage));
-          landed<0>(bar(kXFull));
-        } else {
-          landed<0>(bar(kVFull + stage));
+          load_tile<VD>(base + L::kOffX, &maps.x, w.x, t0, h, b, bar(raw ? kXRaw : kXFull));
         }
+        if (kS == 1) values();
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5 + kStateWarps) {
+    // ================================================================================ gates
+    GateIn<4> ahead = gates_fetch<4>(w, b, h, tile_of(0), lane);
+    for (int n = 0; n < chunks; ++n) {
+      const GateIn<4> in = ahead;
+      if (n + 1 < chunks) ahead = gates_fetch<4>(w, b, h, tile_of(n + 1), lane);
+      if (n > 1) wait(kGEmpty + (n & 1), ((n >> 1) - 1) & 1);
+      const GateOut<4> r = gates_scan<4>(w, in, lane);
+      TcGates& g = gates(n);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int at = gate_row<4>(w, lane, k);
+        g.sum[at] = gate_sum(r.sum[k]) + r.bad, g.weight[at] = r.weight[k], g.count[at] = (uint8_t)r.count[k];
+      }
+      if (lane == 0) g.enter = r.enter, g.total = r.total;
+      __syncwarp();
+      arrive(bar(kGFull + (n & 1)));
+    }
+  } else if (warp == 6 + kStateWarps) {
+    // ================================================================================ padded steps: whatever lies there becomes zeros
+    if (w.pad) {
+      for (int n = 0; n < chunks; ++n) {
+        const int t0 = tile_of(n) * kC, rows = min(kC, w.L - t0);
+        constexpr int kS = L::kVStages;
+        const int stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
+        const uint8_t* m = w.pad + (long long)b * w.L + t0;
+        uint32_t pad[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pad[k] = __ballot_sync(~0u, 32 * k + lane < rows && m[32 * k + lane]);
+        const bool any = (pad[0] | pad[1] | pad[2] | pad[3]) != 0;
+        auto pass = [&](auto width, uint32_t at, int from, int to, uint32_t parity) {
+          wait(from, parity);
+          if (any) {
+            clear_rows<decltype(width)::value>(at, pad, lane);
+            fence_proxy_async();
+          }
+          __syncwarp();
+          if (lane == 0) arrive(bar(to));
+        };
+        using Keys = std::integral_constant<int, KD>;
+        using Values = std::integral_constant<int, VD>;
+        pass(Keys(), base + L::kOffK + (n & 1) * L::kTk, kKRaw + (n & 1), kKFull + (n & 1), n >> 1 & 1);
+        if (kOut) pass(Keys(), base + L::kOffQ, kQRaw, kQFull, n & 1);
+        if (kDots && kS == 1) pass(Values(), base + L::kOffX, kXRaw, kXFull, n & 1);
+        pass(Values(), base + L::kOffV + stage * L::kTv, kVRaw + stage, kVFull + stage, use & 1);
+        if (kDots && kS == 2) pass(Values(), base + L::kOffX, kXRaw, kXFull, n & 1);
       }
     }
   } else {
@@ -531,12 +541,12 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     if (umma_elect()) {
     constexpr uint32_t kPairs = idesc<T>(128, false, false), kRows = idesc<T>(VD, false, true), kBoth = idesc<T>(VD, true, true);
     constexpr int kS = L::kVStages;
-    const uint64_t q = along(base + L::kOffQ, kPlane), s = over(base + L::kOffS, KD * 16), x = along(base + L::kOffX, kPlane);
+    const uint64_t q = tile_desc(base + L::kOffQ), s = over(base + L::kOffS, KD * 16), x = tile_desc(base + L::kOffX);
     const uint64_t lo = over(base + L::kOffLo, kPlane), lo2 = over(base + L::kOffLo2, kPlane);
     for (int n = 0; n < chunks; ++n) {
       const int stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
       const uint32_t key = base + L::kOffK + (n & 1) * L::kTk, val = base + L::kOffV + stage * L::kTv;
-      const uint64_t k_along = along(key, kPlane), k_over = over(key, kPlane), v_along = along(val, kPlane), v_over = over(val, kPlane);
+      const uint64_t kt = tile_desc(key), vt = tile_desc(val);
       if constexpr (kOut) {
         wait(kQFull, n & 1);
         wait(kKFull + (n & 1), n >> 1 & 1);
@@ -547,16 +557,16 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         }
         tm_after();
 #pragma unroll
-        for (int k = 0; k < KD / 16; ++k) umma(tm + kColP, q + k * (2 * kPlane / 16), k_along + k * (2 * kPlane / 16), kPairs, k > 0);
+        for (int k = 0; k < KD / 16; ++k) umma(tm + kColP, q + kAlong(k), kt + kAlong(k), kPairs, k > 0);
         if (kDots)
 #pragma unroll
-          for (int k = 0; k < VD / 16; ++k) umma(tm + kColO2, x + k * (2 * kPlane / 16), v_along + k * (2 * kPlane / 16), kPairs, k > 0);
+          for (int k = 0; k < VD / 16; ++k) umma(tm + kColO2, x + kAlong(k), vt + kAlong(k), kPairs, k > 0);
         umma_commit(bar(kPDone));
         wait(kSReady, n & 1);
         if (!kDots && n) wait(kORead, (n - 1) & 1);
         tm_after();
 #pragma unroll
-        for (int k = 0; k < KD / 16; ++k) umma(tm + kColO1, q + k * (2 * kPlane / 16), s + k * 16, kRows, k > 0);
+        for (int k = 0; k < KD / 16; ++k) umma(tm + kColO1, q + kAlong(k), s + k * 16, kRows, k > 0);
         umma_commit(bar(kQEmpty));
       }
       wait(kWReady, n & 1);
@@ -564,11 +574,11 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       tm_after();
       if constexpr (L::kPieces == 3 && !L::kSeq)
 #pragma unroll
-        for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo2 + k * 16, v_over + k * 16, kBoth, k > 0);
+        for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo2 + k * 16, vt + kOver(k), kBoth, k > 0);
 #pragma unroll
-      for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo + k * 16, v_over + k * 16, kBoth, k > 0 || (L::kPieces == 3 && !L::kSeq));
+      for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo + k * 16, vt + kOver(k), kBoth, k > 0 || (L::kPieces == 3 && !L::kSeq));
 #pragma unroll
-      for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, k_over + k * 16, v_over + k * 16, kBoth, true);
+      for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, kt + kOver(k), vt + kOver(k), kBoth, true);
       if constexpr (L::kSeq) umma_commit(bar(kLoFree));
       else {
         umma_commit(bar(kDsDone));
@@ -578,14 +588,14 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         wait(kPReady, n & 1);
         tm_after();
 #pragma unroll
-        for (int k = 0; k < kC / 16; ++k) umma_tm(tm + kColO2, tm + kColP + k * 8, v_over + k * 16, kRows, k > 0);
+        for (int k = 0; k < kC / 16; ++k) umma_tm(tm + kColO2, tm + kColP + k * 8, vt + kOver(k), kRows, k > 0);
         umma_commit(bar(kODone));
       }
       if constexpr (L::kSeq) {
         wait(kW2Ready, n & 1);
         tm_after();
 #pragma unroll
-        for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo + k * 16, v_over + k * 16, kBoth, true);
+        for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo + k * 16, vt + kOver(k), kBoth, true);
         umma_commit(bar(kDsDone));
         umma_commit(bar(kKEmpty + (n & 1)));
       }
@@ -604,11 +614,11 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
 }
 
 template <typename T, int KD, int VD>
-void run(const Walk& w, int dots, void* stream) {
+void run(const Walk& w, const Maps& maps, int dots, void* stream) {
   const long long blocks = (long long)w.B * w.H;
   auto go = [&](auto kernel, auto lay, long long n) {
     using L = decltype(lay);
-    launch(kernel, dim3((unsigned)n), dim3(L::kThreads), L::kEnd, stream, w);
+    launch(kernel, dim3((unsigned)n), dim3(L::kThreads), L::kEnd, stream, w, maps);
   };
   if (w.segs > 1) go(tc_kernel<T, KD, VD, false, 0>, Lay<T, KD, VD, false, 0>(), blocks * (w.segs - 1));
   if (dots == 0) go(tc_kernel<T, KD, VD, true, 0>, Lay<T, KD, VD, true, 0>(), blocks * w.segs);
@@ -616,20 +626,35 @@ void run(const Walk& w, int dots, void* stream) {
   else go(tc_kernel<T, KD, VD, true, 2>, Lay<T, KD, VD, true, 2>(), blocks * w.segs);
 }
 template <typename T>
-void pick(const Walk& w, int dots, void* stream) {
-  if (w.k.d <= 64) w.v.d <= 64 ? run<T, 64, 64>(w, dots, stream) : run<T, 64, 128>(w, dots, stream);
-  else w.v.d <= 64 ? run<T, 128, 64>(w, dots, stream) : run<T, 128, 128>(w, dots, stream);
+void pick(const Walk& w, const Maps& m, int dots, void* stream) {
+  if (w.k.d <= 64) w.v.d <= 64 ? run<T, 64, 64>(w, m, dots, stream) : run<T, 64, 128>(w, m, dots, stream);
+  else w.v.d <= 64 ? run<T, 128, 64>(w, m, dots, stream) : run<T, 128, 128>(w, m, dots, stream);
+}
+
+// (width, step, head, sequence) of an operand; false where TMA cannot address it
+bool map_of(CUtensorMap* m, int dtype, const Operand& o, const Walk& w) {
+  auto place = [](int n, long long stride) { return (uint64_t)(stride ? n : 1); };
+  auto step = [](long long stride) { return stride ? stride : 8; };
+  return make_tensor_map_4d(m, dtype, o.p, o.d, w.L, place(w.H, o.sh), place(w.B, o.sb), step(o.sl), step(o.sh), step(o.sb), 64, kC);
+}
+bool maps_of(Maps* m, int dtype, const Walk& w) {
+  if (!map_of(&m->q, dtype, w.q, w) || !map_of(&m->k, dtype, w.k, w) || !map_of(&m->v, dtype, w.v, w)) return false;
+  if (!w.x.p) m->x = m->v;
+  return !w.x.p || map_of(&m->x, dtype, w.x, w);
 }
 }  // namespace
 
 bool tc_takes(int dtype, const Walk& w) {
   if (dtype == MEGA_F32 || g_options[OPT_DISABLE_MMA].load()) return false;
   for (const Operand* o : {&w.q, &w.k, &w.v, &w.x})
-    if (o->p && (o->d > kTcMost || o->vec < 4)) return false;
-  return true;
+    if (o->p && (o->d > kTcMost || o->vec < 16 || o->sl < 0 || o->sh < 0 || o->sb < 0 || (o->sl == 0 && w.L > 1))) return false;
+  Maps m;   // (what the driver refuses is known before a plan is made)
+  return maps_of(&m, dtype, w);
 }
 int tc_walk(int dtype, const Walk& w, int dots, void* stream) {
-  dtype == MEGA_BF16 ? pick<__nv_bfloat16>(w, dots, stream) : pick<__half>(w, dots, stream);
+  Maps m;
+  if (!maps_of(&m, dtype, w)) return MEGA_ERR_UNSUPPORTED;
+  dtype == MEGA_BF16 ? pick<__nv_bfloat16>(w, m, dots, stream) : pick<__half>(w, m, dots, stream);
   g_last_kernel.store("decayed_attention_tc", std::memory_order_relaxed);
   return MEGA_OK;
 }

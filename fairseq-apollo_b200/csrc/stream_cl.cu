@@ -61,6 +61,25 @@ bool make_tensor_map_3d(CUtensorMap* out, int dtype, const void* base, uint64_t 
   return r == CUDA_SUCCESS;
 }
 
+bool make_tensor_map_4d(CUtensorMap* out, int dtype, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2, uint64_t dim3,
+                        int64_t stride1, int64_t stride2, int64_t stride3, uint32_t box0, uint32_t box1) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || !aligned_to(base, 16)) return false;
+  const int es = elem_size(dtype);
+  for (int64_t s : {stride1, stride2, stride3})
+    if (s <= 0 || s * es % 16 != 0 || s * es >= (int64_t)1 << 40) return false;
+  if ((uint64_t)box0 * es % 16 != 0 || box0 > 256 || box1 > 256) return false;
+  CUtensorMapDataType dt = dtype == MEGA_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                           : dtype == MEGA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  cuuint64_t dims[4] = {dim0, dim1, dim2, dim3};
+  cuuint64_t strides[3] = {(cuuint64_t)stride1 * es, (cuuint64_t)stride2 * es, (cuuint64_t)stride3 * es};
+  cuuint32_t box[4] = {box0, box1, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(out, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // ---------------------------------------------------------------------------
 // kernel
 // ---------------------------------------------------------------------------

@@ -16,6 +16,10 @@ bool make_tensor_map_3d(CUtensorMap* out, int dtype, const void* base, uint64_t 
                         uint64_t dim2, int64_t stride1_elems, int64_t stride2_elems, uint32_t box0,
                         uint32_t box1, uint32_t box2, CUtensorMapSwizzle swizzle);
 
+// The same with four axes (positive strides), boxes of box0 x box1 and 128-byte swizzle.
+bool make_tensor_map_4d(CUtensorMap* out, int dtype, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2, uint64_t dim3,
+                        int64_t stride1_elems, int64_t stride2_elems, int64_t stride3_elems, uint32_t box0, uint32_t box1);
+
 // Device-side error word of this translation unit (device code is not linked across files):
 // set when a bounded wait gives up, which is never expected in normal operation.
 static __device__ int g_device_error = 0;
