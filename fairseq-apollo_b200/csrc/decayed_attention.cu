@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
   };
   if (kDots) fetch_x(from);
   fetch(from, 0);
-  if (warp == 0) gates_put(w, sh.g[from & 1], gates_fetch<2>(w, b, h, tile_of(from), lane), lane);
+  if (warp == 0) gates_put(w, sh.g[from & 1], gates_fetch<T, 2>(w, b, h, tile_of(from), lane), lane);
 
   for (int c = from; c < to; ++c) {
     const int stage = STAGES == 2 ? (c - from) & 1 : 0;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
     }
     GateIn<2> next;
     if (STAGES == 2 && c + 1 < to) fetch(c + 1, stage ^ 1);
-    if (warp == 0 && c + 1 < to) next = gates_fetch<2>(w, b, h, tile_of(c + 1), lane);
+    if (warp == 0 && c + 1 < to) next = gates_fetch<T, 2>(w, b, h, tile_of(c + 1), lane);
 
     if constexpr (kOut) {
       // ---- the state that enters: written by the walk of dq, and multiplied with the gradient of the one that leaves by that of dk
@@ -569,7 +569,7 @@ struct GateGrad {
   long long db, dl, dh;
 };
 // a warp to a chunk of 32 N steps of a head
-template <int N>
+template <typename T, int N>
 __global__ void __launch_bounds__(128) gate_grad_kernel(const GateGrad a) {
   const Walk& w = a.w;
   const int lane = threadIdx.x & 31;
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(128) gate_grad_kernel(const GateGrad a) {
   if (at >= bhs * w.chunks) return;
   const long long bh = at / w.chunks;
   const int tile = (int)(at % w.chunks), b = (int)(bh / w.H), h = (int)(bh % w.H);
-  const GateIn<N> in = gates_fetch<N>(w, b, h, tile, lane);
+  const GateIn<N> in = gates_fetch<T, N>(w, b, h, tile, lane);
   float through = 0.f;
   for (int i = 0; i < a.parts; ++i) through += a.through[at * a.parts + i];
   float ends[N], kept[N], behind = 0.f, before = 0.f;   // pairs and reads that end at a step; what a step leaves behind the chunk
@@ -617,8 +617,7 @@ __global__ void __launch_bounds__(128) gate_grad_kernel(const GateGrad a) {
     const float v = (in.pad >> i & 1) || (in.reset >> i & 1) || closed(log2_gate(in.f[i])) ? 0.f : da * gate_of<float>(in.f[i]).c;
     const long long to = b * a.db + t * a.dl + h * a.dh;
     if (w.f_dtype == MEGA_F32) static_cast<float*>(a.df)[to] = v;
-    else if (w.f_dtype == MEGA_BF16) static_cast<__nv_bfloat16*>(a.df)[to] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(a.df)[to] = __float2half_rn(v);
+    else Elem<T>::st(static_cast<T*>(a.df) + to, v);
   }
 }
 }  // namespace
@@ -647,7 +646,7 @@ int value_tile(int keys) { return key_tile(keys) == 256 ? 32 : 64; }
 struct Plan {
   bool tc;
   int tiles, chunks, per, segs;
-  size_t local, factor, anchors, through;   // floats
+  size_t local, factor, gates, anchors, through;   // floats
 };
 Plan plan_of(bool tc, int dtype, int B, int L, int H, int keys, int values) {
   Plan p;
@@ -667,6 +666,7 @@ Plan plan_of(bool tc, int dtype, int B, int L, int H, int keys, int values) {
   auto even = [](size_t n) { return (n + 3) / 4 * 4; };
   p.local = even(n * p.tiles * keys * vt);
   p.factor = even(n);
+  p.gates = tc ? bh * p.chunks * (kTcGates / 4) : 0;
   p.anchors = even(bh * p.chunks * p.tiles * keys * vt * elem_size(dtype) / 4 + 1);
   p.through = even(bh * p.chunks * std::max(p.tiles, kTcParts));
   return p;
@@ -692,12 +692,11 @@ void run_keys(const Walk& w, int dots, void* stream) {
     default: return run_walk<T, 256, 32, sizeof(T) == 4 ? 1 : 2>(w, dots, stream);
   }
 }
-// `work`: the plan's local states and factors
+// `work`: the plan's local states, factors and gates
 int run(int dtype, Walk& w, const Plan& p, int dots, float* work, void* stream) {
   w.tiles = p.tiles, w.per = p.per, w.segs = p.segs, w.chunks = p.chunks;
   if ((long long)p.tiles * w.B * w.H * p.segs > 0x7fffffffLL) return MEGA_ERR_UNSUPPORTED;
-  w.local = work, w.factor = work + p.local;
-  w.piece = vec_of(w.out, w.ob, w.ol, w.oh, w.v.d, elem_size(dtype), 32);
+  w.gates = work, w.local = work + p.gates, w.factor = w.local + p.local;
   if (p.tc) return tc_walk(dtype, w, dots, stream);
   MEGA_DISPATCH_DTYPE(dtype, run_keys<T>(w, dots, stream));
   return MEGA_OK;
@@ -716,6 +715,10 @@ int check_args(const mega_decayed_attention_args* a) {
   if (!aligned_to(a->f, elem_size(a->gate_dtype)) || !aligned_to(a->df, elem_size(a->gate_dtype))) return MEGA_ERR_ALIGN;
   return MEGA_OK;
 }
+void put_out(Walk& w, const mega_decayed_attention_args& a, void* p, const int64_t* s) {
+  w.out = p, w.ob = s[0], w.ol = s[1], w.oh = s[2];
+  w.piece = vec_of(p, a.B > 1 ? s[0] : 0, a.L > 1 ? s[1] : 0, a.H > 1 ? s[2] : 0, w.v.d, elem_size(a.dtype), 32);
+}
 Walk base(const mega_decayed_attention_args& a) {
   Walk w = {};
   w.f = a.f, w.fb = a.fs[0], w.fl = a.fs[1], w.fh = a.fs[2], w.f_dtype = a.gate_dtype;
@@ -731,15 +734,15 @@ BackPlan back_plan(const mega_decayed_attention_args& a, bool tc) {
   BackPlan p;
   p.dq = p.dk = plan_of(tc, a.dtype, a.B, a.L, a.H, a.V, a.K);
   p.dv = plan_of(tc, a.dtype, a.B, a.L, a.H, a.K, a.V);
-  p.walk = std::max(p.dq.local + p.dq.factor, p.dv.local + p.dv.factor);
-  p.dots = ((size_t)a.B * a.H * p.dq.tiles * a.L * 2 + 3) / 4 * 4;
+  p.walk = std::max(p.dq.local + p.dq.factor, p.dv.local + p.dv.factor) + p.dq.gates;
+  p.dots = ((size_t)a.B * a.H * (tc ? kTcDots : p.dq.tiles) * a.L * 2 + 3) / 4 * 4;
   p.all = p.walk + 2 * p.dots + p.dq.anchors + p.dq.through;
   return p;
 }
 // (whether the tensor memory's form takes a call depends on its memory too: room for either)
 size_t forward_floats(const mega_decayed_attention_args& a, bool tc) {
   const Plan p = plan_of(tc, a.dtype, a.B, a.L, a.H, a.K, a.V);
-  return p.local + p.factor;
+  return p.local + p.factor + p.gates;
 }
 }  // namespace
 cudaError_t decayed_attention_read_device_error(int* v, bool reset) { return tc_read_device_error(v, reset); }
@@ -761,10 +764,10 @@ extern "C" MEGA_API int mega_decayed_attention_fwd(const mega_decayed_attention_
   if (!a->y) return MEGA_ERR_NULL;
   Walk w = base(*a);
   w.q = operand(*a, a->q, a->qs, a->K), w.k = operand(*a, a->k, a->ks, a->K), w.v = operand(*a, a->v, a->vs, a->V);
+  put_out(w, *a, a->y, a->ys);
   const Plan p = plan_of(tc_takes(a->dtype, w), a->dtype, a->B, a->L, a->H, a->K, a->V);
-  if (p.segs > 1 && !a->work) return MEGA_ERR_NULL;
+  if (p.local + p.factor + p.gates && !a->work) return MEGA_ERR_NULL;
   if (a->work && !aligned_to(a->work, 16)) return MEGA_ERR_ALIGN;
-  w.out = a->y, w.ob = a->ys[0], w.ol = a->ys[1], w.oh = a->ys[2];
   w.s_in = a->h_in, w.s_out = a->h_out, w.s_row = a->V, w.s_col = 1;
   w.p_scale = w.o_scale = (float)a->scale, w.s_scale = 1.f;
   w.rev = (a->flags & MEGA_ATT_REVERSE) != 0;
@@ -781,14 +784,17 @@ extern "C" MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_
                 dy = operand(*a, a->dy, a->gs, a->V);
   Walk w = base(*a);
   w.q = dy, w.k = v, w.v = k, w.x = q;
-  const BackPlan p = back_plan(*a, tc_takes(a->dtype, w));
+  put_out(w, *a, a->dq, a->dqs);
+  Walk wk = base(*a), wv = base(*a);
+  wk.q = v, wk.k = dy, wk.v = q, wk.x = k, wv.q = k, wv.k = q, wv.v = dy;
+  put_out(wk, *a, a->dk, a->dks), put_out(wv, *a, a->dv, a->dvs);
+  const BackPlan p = back_plan(*a, tc_takes(a->dtype, w) && tc_takes(a->dtype, wk) && tc_takes(a->dtype, wv));
   float* at = static_cast<float*>(a->work);
   auto take = [&](size_t n) { float* r = at; at += n; return r; };
   float* walk = take(p.walk);
   float2 *dots_q = reinterpret_cast<float2*>(take(p.dots)), *dots_k = reinterpret_cast<float2*>(take(p.dots));
   float *anchors = take(p.dq.anchors), *through = take(p.dq.through);
   const bool rev = (a->flags & MEGA_ATT_REVERSE) != 0;
-  w.out = a->dq, w.ob = a->dqs[0], w.ol = a->dqs[1], w.oh = a->dqs[2];
   w.s_in = a->h_in, w.s_row = 1, w.s_col = a->V;
   w.p_scale = w.o_scale = (float)a->scale, w.s_scale = 1.f;
   w.rev = rev;
@@ -797,26 +803,26 @@ extern "C" MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_
   if (rc) return rc;
   const Walk forward = w;
 
-  w = base(*a);
-  w.q = v, w.k = dy, w.v = q, w.x = k;
-  w.out = a->dk, w.ob = a->dks[0], w.ol = a->dks[1], w.oh = a->dks[2];
-  w.s_in = a->dh_out, w.s_out = a->dh_in, w.s_row = 1, w.s_col = a->V;
-  w.p_scale = w.s_scale = (float)a->scale, w.o_scale = 1.f;
-  w.rev = !rev, w.excl = 1;
-  w.dots = dots_k, w.anchors = anchors, w.through = through;
-  rc = run(a->dtype, w, p.dk, 2, walk, stream);
+  wk.s_in = a->dh_out, wk.s_out = a->dh_in, wk.s_row = 1, wk.s_col = a->V;
+  wk.p_scale = wk.s_scale = (float)a->scale, wk.o_scale = 1.f;
+  wk.rev = !rev, wk.excl = 1;
+  wk.dots = dots_k, wk.anchors = anchors, wk.through = through;
+  rc = run(a->dtype, wk, p.dk, 2, walk, stream);
   if (rc) return rc;
 
-  w.q = k, w.k = q, w.v = dy;
-  w.out = a->dv, w.ob = a->dvs[0], w.ol = a->dvs[1], w.oh = a->dvs[2];
-  w.s_out = nullptr, w.s_row = a->V, w.s_col = 1;
-  rc = run(a->dtype, w, p.dv, 0, walk, stream);
+  wv.s_in = a->dh_out, wv.s_row = a->V, wv.s_col = 1;
+  wv.p_scale = wv.s_scale = (float)a->scale, wv.o_scale = 1.f;
+  wv.rev = !rev, wv.excl = 1, wv.gates_there = 1;   // (those of the walk before, in the same place)
+  rc = run(a->dtype, wv, p.dv, 0, walk, stream);
   if (rc) return rc;
 
-  const GateGrad gg = {forward, dots_q, dots_k, through, p.dq.tiles, p.dk.tiles, p.dk.tc ? kTcParts : p.dk.tiles, a->df, a->dfs[0], a->dfs[1],
+  const int tiles = p.dk.tc ? kTcDots : p.dk.tiles;
+  const GateGrad gg = {forward, dots_q, dots_k, through, tiles, tiles, p.dk.tc ? kTcParts : p.dk.tiles, a->df, a->dfs[0], a->dfs[1],
                        a->dfs[2]};
   const dim3 grid((unsigned)(((long long)a->B * a->H * forward.chunks + 3) / 4));
-  if (p.dk.tc) launch(gate_grad_kernel<kTcChunk / 32>, grid, dim3(128), 0, stream, gg);
-  else launch(gate_grad_kernel<kC / 32>, grid, dim3(128), 0, stream, gg);
+  MEGA_DISPATCH_DTYPE(a->dtype, {
+    if (p.dk.tc) launch(gate_grad_kernel<T, kTcChunk / 32>, grid, dim3(128), 0, stream, gg);
+    else launch(gate_grad_kernel<T, kC / 32>, grid, dim3(128), 0, stream, gg);
+  });
   return check_launch("decayed_attention_bwd");
 }

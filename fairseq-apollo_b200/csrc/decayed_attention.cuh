@@ -26,6 +26,8 @@ struct Walk {
   float2* dots;           // [tile][B H][L]: x . out of the part from the state that entered; the pairs' sum W of a step
   void* anchors;          // [B H][chunk][tile] states that enter a chunk, in the activations' type (written, or read:)
   float* through;         // [B H][chunk][part]: what passes the whole chunk
+  void* gates;            // [B H][chunk]: what the tensor memory's form reads of the gates
+  int gates_there;        // (an earlier walk has left them)
   float *local, *factor;  // states that segments leave by themselves, and their decay
   int B, L, H, tiles, chunks, per, segs;
   float p_scale, o_scale, s_scale;
@@ -36,10 +38,10 @@ struct Walk {
 // otherwise, reads it where the weight is well above.
 constexpr float kLeast = 1e-35f;
 
+// (gates are of the activations' type or fp32)
+template <typename T>
 __device__ __forceinline__ float gate_value(const Walk& w, long long at) {
-  if (w.f_dtype == MEGA_F32) return __ldg(static_cast<const float*>(w.f) + at);
-  if (w.f_dtype == MEGA_BF16) return Elem<__nv_bfloat16>::ld(static_cast<const __nv_bfloat16*>(w.f) + at);
-  return Elem<__half>::ld(static_cast<const __half*>(w.f) + at);
+  return w.f_dtype == MEGA_F32 ? __ldg(static_cast<const float*>(w.f) + at) : Elem<T>::ld(static_cast<const T*>(w.f) + at);
 }
 
 // The gates of a chunk of 32 N steps, N steps of the walk to a lane
@@ -53,7 +55,7 @@ __device__ __forceinline__ int gate_row(const Walk& w, int lane, int i) {
   const int p = N * lane + i;
   return w.rev ? 32 * N - 1 - p : p;
 }
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ GateIn<N> gates_fetch(const Walk& w, int b, int h, int tile, int lane) {
   GateIn<N> g;
   g.pad = (1u << N) - 1, g.reset = 0;
@@ -62,7 +64,7 @@ __device__ __forceinline__ GateIn<N> gates_fetch(const Walk& w, int b, int h, in
     g.f[i] = 0.f;
     const long long t = (long long)tile * (32 * N) + gate_row<N>(w, lane, i);
     if (t >= w.L) continue;
-    g.f[i] = gate_value(w, b * w.fb + t * w.fl + h * w.fh);
+    g.f[i] = gate_value<T>(w, b * w.fb + t * w.fl + h * w.fh);
     if (!w.pad || !w.pad[b * (long long)w.L + t]) g.pad &= ~(1u << i);
     if (w.reset && w.reset[b * (long long)w.L + t]) g.reset |= 1u << i;
   }
@@ -72,14 +74,14 @@ __device__ __forceinline__ GateIn<N> gates_fetch(const Walk& w, int b, int h, in
 // the state that enters in it (0: a reset lies between).  A gate whose decay is below fp32's range counts as a reset.
 template <int N>
 struct GateOut {
-  long long sum[N];
+  long long sum[N], all;
   int count[N];
   float weight[N], enter, bad;   // bad: what the sums have to be given besides, 0 or NaN
   int total;
   bool padded;
 };
 // log2 sigmoid(f), and whether that is no decay but a reset
-__device__ __forceinline__ float log2_gate(float f) { return (f < 0.f ? f - log1pf(expf(f)) : -log1pf(expf(-f))) * 1.44269504f; }
+__device__ __forceinline__ float log2_gate(float f) { return (fminf(f, 0.f) - log1pf(expf(-fabsf(f)))) * 1.44269504f; }
 __device__ __forceinline__ bool closed(float g) { return g < -149.f; }
 __device__ __forceinline__ float gate_sum(long long s) { return (float)s * 0x1p-40f; }
 template <int N>
@@ -106,6 +108,7 @@ __device__ __forceinline__ GateOut<N> gates_scan(const Walk& w, const GateIn<N>&
   const float bad = __any_sync(~0u, nan) ? __int_as_float(0x7fffffff) : 0.f;   // (a gate that is NaN: the whole chunk is)
   const long long all = __shfl_sync(~0u, upto, 31);
   GateOut<N> r;
+  r.all = all;
   r.total = __shfl_sync(~0u, counted, 31);
   upto -= sum, counted -= cnt;   // (what lies before this lane's steps)
 #pragma unroll
@@ -122,7 +125,7 @@ __device__ __forceinline__ GateOut<N> gates_scan(const Walk& w, const GateIn<N>&
 }
 
 // The form on tcgen05 products (decayed_attention_tc.cu): 16-bit activations, heads of at most 128 keys and values
-constexpr int kTcChunk = 128, kTcMost = 128, kTcParts = 8;
+constexpr int kTcChunk = 128, kTcMost = 128, kTcParts = 8, kTcDots = 2, kTcGates = 1200;   // shares of Walk::through and Walk::dots
 bool tc_takes(int dtype, const Walk& w);
 int tc_walk(int dtype, const Walk& w, int dots, void* stream);
 cudaError_t tc_read_device_error(int* v, bool reset);

@@ -7,9 +7,9 @@
 //   dS = (w K)^T V                  w K in pieces of 8 (bf16, three) or 11 (fp16, two) bits, the first in K's place
 //   O2 = (weighted pairs) V
 // and y = e O1 + O2 with a row's factor e.  For the gates' gradient also X V^T, in O2's place before it.
-// Roles: four warps of pairs and outputs (a thread has a row of the chunk), four or eight of weights and state (a thread has a step's
-// keys, then a row of the state, whose fp32 values stay in its registers), one that loads, one for the gates, one for padded steps, one that issues products.  All exchange over
-// mbarriers.
+// Roles: eight warps of pairs and outputs (a thread has half of a row of the chunk), eight of weights and state (a thread has half of a
+// step's keys, then half of a row of the state, whose fp32 values stay in its registers), one that loads, one for
+// padded steps, one that issues products.  All exchange over mbarriers.
 //
 // Activations lie as TMA leaves them (columns of 64, rows of 128 bytes, swizzled), what the threads write as planes of 16 bytes along
 // keys or values, rows one after another.  Both serve with either axis as the contraction, and a thread that owns a row reads and
@@ -18,8 +18,9 @@
 //
 // The state is accumulated by each chunk's own sum, which is then added in fp32: a long chain inside the tensor cores' accumulator
 // would be cut off, not rounded, thousands of times.
-#include <algorithm>
+#include <mutex>
 #include <type_traits>
+#include <unordered_map>
 
 #include "common.cuh"
 #include "decayed_attention.cuh"
@@ -31,29 +32,81 @@ namespace {
 
 constexpr int kC = kTcChunk, kPlane = kC * 16;
 
+// What the gates of a chunk come to.  A pair's weight 2^(sum_i - sum_j) is one factor of j, from there to the last step of its 32, and
+// one of i, from that step on; so is a step's weight in the state that leaves.  Only where the first factor gets too small, or a reset
+// lies among those 32 steps, pairs inside them need a power of two each.
 struct TcGates {
-  float sum[kC], weight[kC];   // running sum of log2 a; weight of a step in the state that leaves
-  uint8_t count[kC];           // resets so far
-  float enter;                 // weight of the state that enters in the one that leaves
-  int total;                   // resets
-  int pad_[2];
+  float sum[kC];      // running sum of log2 a
+  float col[kC];      // weight of a step at the last of its 32 (0: a reset lies between)
+  uint8_t count[kC];  // resets so far
+  float leave[4];     // weight of the last of 32 steps in the state that leaves
+  uint32_t pad[4];    // padded steps
+  float enter;        // weight of the state that enters in the one that leaves
+  uint8_t apart[4];   // whether resets lie among 32 steps, or their decay is out of range
+  uint32_t padded, pad_;
 };
+static_assert(sizeof(TcGates) == kTcGates, "gates");
+__device__ __forceinline__ int last_of(const Walk& w, int block) { return 32 * block + (w.rev ? 0 : 31); }
+
+// They are found before the walk, a warp to a chunk: a warp of the walk itself took 3000 cycles for one and its loads as many again,
+// which was most of a chunk's time.
+template <typename T>
+__global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ Walk w) {
+  const int lane = threadIdx.x & 31;
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  pdl_next();   // (the walk waits for this kernel's end where it reads the gates)
+  if (at >= (long long)w.B * w.H * w.chunks) return;
+  const int bh = (int)(at / w.chunks), tile = (int)(at % w.chunks);
+  const GateIn<4> in = gates_fetch<T, 4>(w, bh / w.H, bh % w.H, tile, lane);
+  const GateOut<4> r = gates_scan<4>(w, in, lane);
+  TcGates& g = static_cast<TcGates*>(w.gates)[at];
+  // (eight lanes hold 32 steps; the last of them in the order of the walk is the last one's)
+  const long long end = __shfl_sync(~0u, r.sum[3], lane | 7);
+  const int there = __shfl_sync(~0u, r.count[3], lane | 7);
+  unsigned mask = 0;   // of this lane's rows in their word
+  float sum[4], col[4];
+  uint8_t count[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int to = w.rev ? 3 - k : k;   // rows ascend
+    sum[to] = gate_sum(r.sum[k]) + r.bad, count[to] = (uint8_t)r.count[k];
+    col[to] = r.count[k] == there && !(in.pad >> k & 1) ? exp2f(gate_sum(end - r.sum[k]) + r.bad) : 0.f;
+    mask |= (in.pad >> k & 1) << to;
+  }
+  const int row = w.rev ? kC - 4 - 4 * lane : 4 * lane, word = row / 32;
+  *reinterpret_cast<float4*>(g.sum + row) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+  *reinterpret_cast<float4*>(g.col + row) = make_float4(col[0], col[1], col[2], col[3]);
+  *reinterpret_cast<uchar4*>(g.count + row) = make_uchar4(count[0], count[1], count[2], count[3]);
+  const unsigned lanes = 0xffu << (lane & 24);
+  const bool reset = __any_sync(lanes, r.count[0] != there || r.count[1] != there || r.count[2] != there);
+  const bool far = __any_sync(lanes, gate_sum(end - r.sum[0]) < -100.f);
+  mask = __reduce_or_sync(lanes, mask << (row & 31));
+  if ((lane & 7) == 7) {
+    g.apart[word] = reset || far;
+    g.leave[word] = there == r.total ? w.s_scale * exp2f(gate_sum(r.all - end) + r.bad) : 0.f;
+    g.pad[word] = mask;
+  }
+  if (lane == 0) g.enter = r.enter, g.padded = r.padded;
+}
+
 // barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it
 enum { kQFull, kQEmpty, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kXFull = kVEmpty + 2, kXEmpty, kGFull, kGEmpty = kGFull + 2,
-       kPDone = kGEmpty + 2, kPReady, kODone, kORead, kSReady, kDsDone, kWReady, kLoFree, kW2Ready, kQRaw, kKRaw, kVRaw = kKRaw + 2, kXRaw = kVRaw + 2, kBars };
+       kPDone = kGEmpty + 2, kPReady, kODone, kORead, kSReady, kDsDone, kWReady, kQRaw, kKRaw, kVRaw = kKRaw + 2, kXRaw = kVRaw + 2, kBars };
 
 // kOut: outputs; else the state that a segment leaves by itself.  kDots: sums for the gates' gradient (1: walk of dq, 2: of dk).
 template <typename T, int KD, int VD, bool kOut, int kDots>
 struct Lay {
   static constexpr int kTk = KD * kC * 2, kTv = VD * kC * 2, kTs = VD / 8 * KD * 16;
-  static constexpr int kPieces = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
-  // with heads of 128 x 128 there is no room for the third piece: it takes the second's place when that has been used
-  static constexpr bool kSeq = kOut && KD == 128 && VD == 128 && kPieces == 3;
-  static constexpr int kVStages = kOut && kDots && KD == 128 && VD == 128 ? 1 : 2;
-  static constexpr int kState = VD == 128 ? 8 : 4;                       // warps of weights and state
-  static constexpr int kThreads = 32 * (4 + kState + 4);
-  // (a product over 128 rows of 64 keys reads on into what follows: no piece and no tile of keys is last)
-  static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 && !kSeq ? kTk : 0), kOffV = kOffK + 2 * kTk,
+  static constexpr bool kBig = KD == 128 && VD == 128 && kOut;   // heads of 128 x 128: shared memory holds seven of their tiles
+  // pieces of weighted keys; beside x there is no room for a third one (which matters to no output but the gradient of the state)
+  static constexpr int kPieces = std::is_same<T, __nv_bfloat16>::value && !(kBig && kDots) ? 3 : 2;
+  static constexpr int kVStages = kBig && (kDots || kPieces == 3) ? 1 : 2;
+  static constexpr int kThreads = 640;   // 8 warps of pairs and outputs, 8 of weights and state, loads, padding, products, and one that rests
+  // Registers of a thread: 96 at launch, 20 warps; where the state takes 64 of them its eight warps have 128, the first eight 88 and
+  // the last four 48: 2 x 88 + 2 x 128 + 48 for each four warps, as at launch (5 x 96).
+  static constexpr int kRegs = 96;
+  static constexpr bool kMove = VD == 128;
+  static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 ? kTk : 0), kOffV = kOffK + 2 * kTk,
                        kOffQ = kOffV + kVStages * kTv, kOffX = kOffQ + (kOut ? kTk : 0), kOffS = kOffX + (kDots ? kTv : 0),
                        kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8, kEnd = kOffSlot + 16;
   static_assert(kEnd <= 227 * 1024, "shared memory");
@@ -68,17 +121,15 @@ __device__ __forceinline__ bool tried(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// A wait that gives up (after some seconds: never expected) raises `gone`; from then on no wait lasts, and everything runs out on
-// whatever the buffers hold.
-__device__ __noinline__ void wait_long(uint32_t bar, uint32_t parity, volatile int* gone) {
-  const long long start = clock64();
-  while (!*gone) {
-    if (tried(bar, parity)) return;
-    if (clock64() - start > 4000000000LL) {
-      g_device_error = 1;
-      *gone = 1;
+// A wait that gives up (after seconds: never expected) raises `gone`; from then on no wait lasts, and everything runs out on whatever the
+// buffers hold.  (Short: the roles' loops together are to stay in the instruction cache.)
+__device__ __forceinline__ void wait_for(uint32_t bar, uint32_t parity, volatile int* gone) {
+#pragma unroll 1
+  for (int i = 0; !tried(bar, parity); ++i)
+    if (i > 1 << 24 || *gone) {   // (a try itself lasts a fraction of a microsecond)
+      g_device_error = *gone = 1;
+      break;
     }
-  }
 }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ float ex2(float v) {
@@ -98,6 +149,14 @@ __device__ __forceinline__ float2 unpack(uint32_t v) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
   else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
+__device__ __forceinline__ void tm_ld16(uint32_t at, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+        "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(at)
+      : "memory");
+}
 template <int N>
 __device__ __forceinline__ void loaded(float (&v)[N]) {   // (the registers of a load from tensor memory, once it has been waited for)
 #pragma unroll
@@ -112,11 +171,32 @@ __device__ __forceinline__ void sts16(uint32_t at, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// w v as 16-bit pieces that add up to it.  bf16 (three): the upper, middle and lower eight bits, cut off, which is exact; fp16 (two): what
+// rounding leaves is the second.
+template <typename T, int PIECES>
+__device__ __forceinline__ void split(float2 v, float w, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+  v.x *= w, v.y *= w;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    auto upper = [](float f) { return __uint_as_float(__float_as_uint(f) & 0xffff0000u); };
+    auto both = [](float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); };
+    p0 = both(v.x, v.y);
+    v.x -= upper(v.x), v.y -= upper(v.y);
+    p1 = PIECES == 2 ? pack<T>(v.x, v.y) : both(v.x, v.y);
+    v.x -= upper(v.x), v.y -= upper(v.y);
+    p2 = both(v.x, v.y);
+  } else {
+    p0 = pack<T>(v.x, v.y);
+    const float2 r = unpack<T>(p0);
+    p1 = pack<T>(v.x - r.x, v.y - r.y);
+    p2 = 0;
+  }
+}
+
 // Products, all over k = 16 places at a time.  d = or += a b; A in shared or tensor memory.
 template <typename T>
-__host__ __device__ constexpr uint32_t idesc(int n, bool a_mn, bool b_mn) {
+__host__ __device__ constexpr uint32_t idesc(int n, bool a_mn, bool b_mn, int m) {
   const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  return (1u << 4) | (type << 7) | (type << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+  return (1u << 4) | (type << 7) | (type << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ void umma_tm(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool onto) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
@@ -151,19 +231,17 @@ __device__ __forceinline__ void load_tile(uint32_t to, const CUtensorMap* m, con
 #pragma unroll
   for (int c = 0; c < D; c += 64) tma_load_4d(to + c / 64 * kBox, m, c, t0, o.sh ? h : 0, o.sb ? b : 0, bar);
 }
-template <int D>
-__device__ __forceinline__ void clear_rows(uint32_t at, const uint32_t (&pad)[4], int lane) {
-#pragma unroll 1
+__device__ __forceinline__ void clear_rows(uint32_t at, int planes, const uint32_t (&pad)[4], int lane) {
+#pragma unroll
   for (int k = 0; k < 4; ++k)
     if (pad[k] >> lane & 1)
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) sts16(at + piece_of(32 * k + lane, c), make_uint4(0, 0, 0, 0));
+#pragma unroll 1
+      for (int c = 0; c < planes; ++c) sts16(at + piece_of(32 * k + lane, c), make_uint4(0, 0, 0, 0));
 }
 
 template <typename T, int KD, int VD, bool kOut, int kDots>
 __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_kernel(const __grid_constant__ Walk w, const __grid_constant__ Maps maps) {
   using L = Lay<T, KD, VD, kOut, kDots>;
-  constexpr int kStateWarps = L::kState, kHalves = kStateWarps / 4, kStateThreads = 32 * kStateWarps;
   extern __shared__ __align__(1024) unsigned char smem[];
   int* const slot_ = reinterpret_cast<int*>(smem + L::kOffSlot);   // where tensor memory lies; whether a wait has given up
   volatile int* gone = slot_ + 1;
@@ -172,93 +250,115 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H), b = bh / w.H, h = bh % w.H;
   const int first = seg * w.per, chunks = min(w.per, w.chunks - first);   // in the order of the walk
   auto bar = [&](int i) { return base + L::kOffBar + i * 8; };
-  auto wait = [&](int i, uint32_t parity) {
-    if (!tried(bar(i), parity)) wait_long(bar(i), parity, gone);
-  };
+  auto wait = [&](int i, uint32_t parity) { wait_for(bar(i), parity, gone); };
   auto tile_of = [&](int n) { return w.rev ? w.chunks - 1 - first - n : first + n; };
   auto gates = [&](int n) -> TcGates& { return reinterpret_cast<TcGates*>(smem + L::kOffG)[n & 1]; };
 
   if (tid == 0) {
     *gone = 0;
     auto init = [&](int i, uint32_t count) { mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, count); };
-    for (int i : {(int)kQFull, (int)kKFull, kKFull + 1, (int)kVFull, kVFull + 1, (int)kXFull, (int)kQRaw, (int)kKRaw, kKRaw + 1, (int)kVRaw, kVRaw + 1, (int)kXRaw})
+    for (int i : {(int)kQFull, (int)kKFull, kKFull + 1, (int)kVFull, kVFull + 1, (int)kXFull, (int)kGFull, kGFull + 1, (int)kQRaw, (int)kKRaw, kKRaw + 1, (int)kVRaw, kVRaw + 1, (int)kXRaw})
       init(i, 1);
-    for (int i : {(int)kGFull, kGFull + 1}) init(i, 32);
-    for (int i : {(int)kQEmpty, (int)kKEmpty, kKEmpty + 1, (int)kVEmpty, kVEmpty + 1, (int)kPDone, (int)kODone, (int)kDsDone, (int)kLoFree}) init(i, 1);
-    for (int i : {(int)kXEmpty, (int)kPReady, (int)kORead}) init(i, 128);
-    for (int i : {(int)kSReady, (int)kWReady, (int)kW2Ready}) init(i, kStateThreads);
-    for (int i : {(int)kGEmpty, kGEmpty + 1}) init(i, kStateThreads + (kOut ? 128 : 0));
+    for (int i : {(int)kQEmpty, (int)kKEmpty, kKEmpty + 1, (int)kVEmpty, kVEmpty + 1, (int)kPDone, (int)kODone, (int)kDsDone}) init(i, 1);
+    for (int i : {(int)kXEmpty, (int)kPReady, (int)kORead, (int)kSReady, (int)kWReady}) init(i, 256);
+    for (int i : {(int)kGEmpty, kGEmpty + 1}) init(i, (kOut ? 512 : 256) + (w.pad ? 32 : 0));
     mbar_fence_init();
+  }
+  if (warp == 16 && umma_elect()) {
+    prefetch_tensormap(&maps.k), prefetch_tensormap(&maps.v);
+    if (kOut) prefetch_tensormap(&maps.q);
+    if (kDots) prefetch_tensormap(&maps.x);
   }
   if (warp == 0) tm_alloc(smem_u32(slot_), kOut ? 512 : 128);
   tm_before();
   __syncthreads();
   tm_after();
+  pdl_wait();   // (all that comes before on the stream)
   const uint32_t tm = *reinterpret_cast<volatile uint32_t*>(slot_);
   constexpr uint32_t kCs = kOut ? kColS : 0;
 
-  if (warp < 4) {
+  if constexpr (L::kMove) {   // (the four warps that do little leave registers to those that hold the state)
+    if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    else if (warp >= 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
+  if (warp < 8) {
     // ================================================================================ pairs and outputs
     if constexpr (kOut) {
-      const int i = warp * 32 + lane;
-      const uint32_t quarter = tm + ((uint32_t)(warp * 32) << 16);
+      const int rb = warp & 3, half = warp >> 2, i = rb * 32 + lane;   // a row, and half of its pairs and of its outputs
+      const uint32_t quarter = tm + ((uint32_t)(rb * 32) << 16);
       for (int n = 0; n < chunks; ++n) {
         const TcGates& g = gates(n);
         const long long t = (long long)tile_of(n) * kC + i;
         wait(kGFull + (n & 1), n >> 1 & 1);
         const float gi = g.sum[i];
         const int ci = g.count[i];
-        const bool resets = g.total != 0;
         float inner = 0.f, read = 0.f;
         wait(kPDone, n & 1);
         tm_after();
-        auto block = [&](int jb, auto diagonal, auto counted) {
-          constexpr bool kDiag = decltype(diagonal)::value, kCount = decltype(counted)::value;
-          float v[32], x[kDots ? 32 : 1];
-          tm_ld32(quarter + kColP + 32 * jb, v);
-          if constexpr (kDots != 0) tm_ld32(quarter + kColO2 + 32 * jb, x);
-          tm_wait_ld();
-          loaded(v);
-          if constexpr (kDots != 0) loaded(x);
+        const int from = max(w.rev ? rb : 0, 2 * half), to = min(w.rev ? 3 : rb, 2 * half + 1);   // blocks of 32 steps that these rows see
+        auto put = [&](int jb, const float (&v)[32]) {
           uint32_t word[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 gj = *reinterpret_cast<const float4*>(g.sum + 32 * jb + j);
-            uchar4 cj;
-            if (kCount) cj = *reinterpret_cast<const uchar4*>(g.count + 32 * jb + j);
-            const float gg[4] = {gj.x, gj.y, gj.z, gj.w};
-            const unsigned char cc[4] = {cj.x, cj.y, cj.z, cj.w};
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              bool on = true;
-              if (kDiag) on = w.rev ? j + m >= lane : j + m <= lane;
-              if (kCount) on = on && cc[m] == ci;
-              float p = v[j + m] * (w.p_scale * ex2(fminf(gi - gg[m], 0.f)));
-              if (kDiag || kCount) p = on ? p : 0.f;
-              v[j + m] = p;
-              if constexpr (kDots != 0) {
-                if (kDiag || kCount) inner += on && !(kDiag && j + m == lane) ? p * x[j + m] : 0.f;
-                else inner += p * x[j + m];
-              }
-            }
-            word[j / 2] = pack<T>(v[j], v[j + 1]), word[j / 2 + 1] = pack<T>(v[j + 2], v[j + 3]);
-          }
-          tm_st8(quarter + kColP + 16 * jb, word);
-          tm_st8(quarter + kColP + 16 * jb + 8, word + 8);
+          for (int j = 0; j < 16; ++j) word[j] = pack<T>(v[2 * j], v[2 * j + 1]);
+          const uint32_t to = quarter + kColP + 64 * half + 16 * (jb & 1);   // (in the place of pairs that this warp has read)
+          tm_st8(to, word);
+          tm_st8(to + 8, word + 8);
         };
-#pragma unroll 1
-        for (int jb = 0; jb < 4; ++jb) {
-          if (w.rev ? jb < warp : jb > warp) {
-            uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            tm_st8(quarter + kColP + 16 * jb, zero);
-            tm_st8(quarter + kColP + 16 * jb + 8, zero);
-          } else if (resets) {
-            if (jb == warp) block(jb, std::true_type(), std::true_type());
-            else block(jb, std::false_type(), std::true_type());
-          } else {
-            if (jb == warp) block(jb, std::true_type(), std::false_type());
-            else block(jb, std::false_type(), std::false_type());
+        auto block = [&](int jb, float (&v)[32]) {
+          // (one factor above one and one below where the row lies inside the 32 steps: their product is what counts, while both are in range)
+          const int end = last_of(w, jb);
+          if (jb != rb || !g.apart[jb]) {
+            const float f = g.count[end] == ci ? w.p_scale * ex2(gi - g.sum[end]) : 0.f;
+            const f32x2 ff = pack2(f, f);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 c = *reinterpret_cast<const float4*>(g.col + 32 * jb + j);
+              unpack2(mul2(pack2(v[j], v[j + 1]), mul2(ff, pack2(c.x, c.y))), v[j], v[j + 1]);
+              unpack2(mul2(pack2(v[j + 2], v[j + 3]), mul2(ff, pack2(c.z, c.w))), v[j + 2], v[j + 3]);
+            }
+          } else {   // resets among these steps, or a decay by more than 2^-100: a power of two for each pair
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float p = v[j] * (w.p_scale * ex2(fminf(gi - g.sum[32 * jb + j], 0.f)));
+              v[j] = g.count[32 * jb + j] == ci ? p : 0.f;
+            }
           }
+          if (jb == rb) {
+            const uint32_t seen = w.rev ? ~0u << lane : ~0u >> (31 - lane);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = seen & (1u << j) ? v[j] : 0.f;
+          }
+          put(jb, v);
+          if constexpr (kDots != 0) {
+            // the pairs' sum, without the step by itself
+#pragma unroll
+            for (int k = 0; k < 32; k += 16) {
+              float x[16];
+              tm_ld16(quarter + kColO2 + 32 * jb + k, x);
+              tm_wait_ld();
+              loaded(x);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) inner += jb == rb && lane == k + j ? 0.f : v[k + j] * x[j];
+            }
+          }
+        };
+        {
+#pragma unroll 1
+          for (int jb = from; jb <= to; ++jb) {
+            float v[32];
+            tm_ld32(quarter + kColP + 32 * jb, v);
+            tm_wait_ld();
+            loaded(v);
+            block(jb, v);
+          }
+          const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+          for (int jb = 2 * half; jb < 2 * half + 2; ++jb)
+            if (jb < from || jb > to) {
+              tm_st8(quarter + kColP + 64 * half + 16 * (jb & 1), zero);
+              tm_st8(quarter + kColP + 64 * half + 16 * (jb & 1) + 8, zero);
+            }
         }
         tm_wait_st();
         tm_before();
@@ -270,30 +370,36 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         tm_after();
         char* row = static_cast<char*>(w.out) + (b * w.ob + h * w.oh + t * w.ol) * 2;
 #pragma unroll 1
-        for (int c = 0; c < VD; c += 32) {
+        for (int c = half * (VD / 2); c < (half + 1) * (VD / 2); c += 32) {
           float o[32], p[32];
           tm_ld32(quarter + kColO1 + c, o);
           tm_ld32(quarter + kColO2 + c, p);
+          uint4 u[kDots ? 4 : 1];
+          if constexpr (kDots != 0)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) u[m] = lds16(base + L::kOffX + piece_of(i, c / 8 + m));
           tm_wait_ld();
           loaded(o);
           loaded(p);
-#pragma unroll
-          for (int m = 0; m < 32; ++m) o[m] *= e;
-          if constexpr (kDots != 0) {
-#pragma unroll
-            for (int m = 0; m < 32; m += 8) {
-              const uint4 u = lds16(base + L::kOffX + piece_of(i, (c + m) / 8));
-              const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 x = unpack<T>(uu[k]);
-                read += o[m + 2 * k] * x.x + o[m + 2 * k + 1] * x.y;
-              }
-            }
-          }
           uint32_t word[16];
+          const f32x2 ee = pack2(e, e);
 #pragma unroll
-          for (int m = 0; m < 16; ++m) word[m] = pack<T>(o[2 * m] + p[2 * m], o[2 * m + 1] + p[2 * m + 1]);
+          for (int m = 0; m < 16; ++m) {
+            f32x2 y;
+            if constexpr (kDots != 0) {
+              const f32x2 own = mul2(ee, pack2(o[2 * m], o[2 * m + 1]));
+              const uint32_t uu[4] = {u[m / 4].x, u[m / 4].y, u[m / 4].z, u[m / 4].w};
+              const float2 x = unpack<T>(uu[m & 3]);
+              unpack2(own, o[2 * m], o[2 * m + 1]);
+              read += o[2 * m] * x.x + o[2 * m + 1] * x.y;
+              y = add2(own, pack2(p[2 * m], p[2 * m + 1]));
+            } else {
+              y = fma2(ee, pack2(o[2 * m], o[2 * m + 1]), pack2(p[2 * m], p[2 * m + 1]));
+            }
+            float lo, hi;
+            unpack2(y, lo, hi);
+            word[m] = pack<T>(lo, hi);
+          }
           if (t < w.L) {
             if (w.piece == 32) {
 #pragma unroll
@@ -302,14 +408,10 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
                   asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(row + (c + 2 * m) * 2), "r"(word[m]),
                                "r"(word[m + 1]), "r"(word[m + 2]), "r"(word[m + 3]), "r"(word[m + 4]), "r"(word[m + 5]), "r"(word[m + 6]), "r"(word[m + 7])
                                : "memory");
-            } else if (w.piece == 16) {
+            } else {
 #pragma unroll
               for (int m = 0; m < 16; m += 4)
                 if (c + 2 * m < w.v.d) *reinterpret_cast<uint4*>(row + (c + 2 * m) * 2) = make_uint4(word[m], word[m + 1], word[m + 2], word[m + 3]);
-            } else {
-#pragma unroll
-              for (int m = 0; m < 32; ++m)
-                if (c + m < w.v.d) *reinterpret_cast<unsigned short*>(row + (c + m) * 2) = (unsigned short)(word[m / 2] >> (16 * (m & 1)));
             }
           }
         }
@@ -317,31 +419,40 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         arrive(bar(kORead));
         if (kDots) {
           arrive(bar(kXEmpty));
-          if (t < w.L) w.dots[(long long)bh * w.L + t] = make_float2(read, inner);
+          if (t < w.L) w.dots[((long long)half * w.B * w.H + bh) * w.L + t] = make_float2(read, inner);
         }
         arrive(bar(kGEmpty + (n & 1)));
       }
     }
-  } else if (warp < 4 + kStateWarps) {
+  } else if (warp < 16) {
     // ================================================================================ weights and state
-    const int sw = warp - 4, row = (sw & 3) * 32 + lane, half = sw >> 2;   // a step, or a key; half: of the planes of keys, of the values
+    constexpr int kCols = VD / 2, kPlanes = KD / 16;
+    const int sw = warp - 8, step = (sw & 3) * 32 + lane, half = sw >> 2;   // a step; half: of the planes of keys, of the values
     const uint32_t quarter = tm + ((uint32_t)((sw & 3) * 32) << 16);
-    const bool holds = (sw & 3) * 32 < KD;   // (of 64 keys two warps have none)
-    constexpr int kPlanes = KD / 8 / kHalves;
-    const int col0 = half * 64;
-    float st[64];
+    // a key's row of the state: of 64, the tensor cores leave 16 in each warp's lanes
+    const int row = KD == 128 ? step : (sw & 3) * 16 + (lane & 15);
+    const int col0 = half * kCols;
+    float st[kCols];
     const long long s_at = (long long)bh * w.k.d * w.v.d + (long long)row * w.s_row;
     auto slot = [&](long long at) { return (at * w.k.d + row) * VD + col0; };   // a row of a state in the workspace
-    const bool mine = holds && row < w.k.d;
+    const bool holds = KD == 128 || lane < 16, mine = holds && row < w.k.d;
 #pragma unroll
-    for (int c = 0; c < 64; ++c) st[c] = kOut && mine && w.s_in && col0 + c < w.v.d ? w.s_in[s_at + (long long)(col0 + c) * w.s_col] : 0.f;
+    for (int c = 0; c < kCols; ++c) st[c] = 0.f;
+    if (kOut && mine && w.s_in) {
+      const float* p = w.s_in + s_at + (long long)col0 * w.s_col;
+#pragma unroll
+      for (int c0 = 0; c0 < kCols; c0 += 8)   // (values come in eights)
+        if (col0 + c0 < w.v.d)
+#pragma unroll
+          for (int c = c0; c < c0 + 8; ++c, p += w.s_col) st[c] = *p;
+    }
     if (kOut)
       for (int p = 0; p < seg; ++p) {
         const float fac = w.factor[(long long)p * w.B * w.H + bh];
         const float* l = w.local + slot((long long)p * w.B * w.H + bh);
         if (mine)
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
+          for (int c = 0; c < kCols; c += 4) {
             const float4 u = *reinterpret_cast<const float4*>(l + c);
             const float uu[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -352,7 +463,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     auto state_out = [&]() {
       if (holds)
 #pragma unroll
-        for (int c = 0; c < 64; c += 8)
+        for (int c = 0; c < kCols; c += 8)
           sts16(base + L::kOffS + (col0 + c) / 8 * (KD * 16) + row * 16,
                 make_uint4(pack<T>(st[c], st[c + 1]), pack<T>(st[c + 2], st[c + 3]), pack<T>(st[c + 4], st[c + 5]), pack<T>(st[c + 6], st[c + 7])));
       fence_proxy_async();
@@ -365,31 +476,24 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       wait(kGFull + (n & 1), n >> 1 & 1);
       wait(kKFull + (n & 1), n >> 1 & 1);
       if (kOut) wait(kPDone, n & 1);   // (the pairs' product has read the keys)
-      const float wt = g.weight[row], enter = g.enter;
-      uint4 last[L::kSeq ? kPlanes : 1];
+      const float wt = g.col[step] * g.leave[step >> 5], enter = g.enter;
+      constexpr int kAt = VD == 128 ? 2 : 4;   // (planes at a time: reads first, as none may pass a write)
+#pragma unroll 1
+      for (int c0 = 0; c0 < kPlanes; c0 += kAt) {
+        const uint32_t keys = base + L::kOffK + (n & 1) * L::kTk;
+        uint4 u[kAt];
 #pragma unroll
-      for (int c = 0; c < kPlanes; ++c) {
-        const uint32_t at = (half * kPlanes + c) * kPlane + row * 16, key = base + L::kOffK + (n & 1) * L::kTk + piece_of(row, half * kPlanes + c);
-        const uint4 u = lds16(key);
-        const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
-        uint32_t piece[3][4];
+        for (int c = 0; c < kAt; ++c) u[c] = lds16(keys + piece_of(step, half * kPlanes + c0 + c));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float2 v = unpack<T>(uu[k]);
-          v.x *= wt, v.y *= wt;
+        for (int c = 0; c < kAt; ++c) {
+          uint32_t piece[3][4];
+          const uint32_t uu[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
 #pragma unroll
-          for (int p = 0; p < L::kPieces; ++p) {
-            piece[p][k] = pack<T>(v.x, v.y);
-            const float2 r = unpack<T>(piece[p][k]);
-            v.x -= r.x, v.y -= r.y;
-          }
-        }
-        sts16(key, make_uint4(piece[0][0], piece[0][1], piece[0][2], piece[0][3]));
-        sts16(base + L::kOffLo + at, make_uint4(piece[1][0], piece[1][1], piece[1][2], piece[1][3]));
-        if constexpr (L::kPieces == 3) {
-          const uint4 v = make_uint4(piece[2][0], piece[2][1], piece[2][2], piece[2][3]);
-          if constexpr (L::kSeq) last[c] = v;
-          else sts16(base + L::kOffLo2 + at, v);
+          for (int k = 0; k < 4; ++k) split<T, L::kPieces>(unpack<T>(uu[k]), wt, piece[0][k], piece[1][k], piece[2][k]);
+          const int at = half * kPlanes + c0 + c;
+          sts16(keys + piece_of(step, at), make_uint4(piece[0][0], piece[0][1], piece[0][2], piece[0][3]));
+          sts16(base + L::kOffLo + at * kPlane + step * 16, make_uint4(piece[1][0], piece[1][1], piece[1][2], piece[1][3]));
+          if constexpr (L::kPieces == 3) sts16(base + L::kOffLo2 + at * kPlane + step * 16, make_uint4(piece[2][0], piece[2][1], piece[2][2], piece[2][3]));
         }
       }
       fence_proxy_async();
@@ -400,14 +504,14 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         if (kDots == 1) {
           if (mine && enter != 0.f)
 #pragma unroll
-            for (int c = 0; c < 64; c += 8)
+            for (int c = 0; c < kCols; c += 8)
               *reinterpret_cast<uint4*>(a + c) =
                   make_uint4(pack<T>(st[c], st[c + 1]), pack<T>(st[c + 2], st[c + 3]), pack<T>(st[c + 4], st[c + 5]), pack<T>(st[c + 6], st[c + 7]));
         } else {
           float s = 0.f;
           if (mine && enter > kLeast)
 #pragma unroll
-            for (int c = 0; c < 64; c += 8) {
+            for (int c = 0; c < kCols; c += 8) {
               const uint4 u = *reinterpret_cast<const uint4*>(a + c);
               const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -421,28 +525,25 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           if (lane == 0) {
             float* to = w.through + ((long long)bh * w.chunks + tile_of(n)) * kTcParts;
             to[sw] = enter > kLeast ? enter * s : 0.f;
-            if (kStateWarps < kTcParts) to[sw + 4] = 0.f;
           }
         }
       }
-      if constexpr (L::kSeq) {
-        wait(kLoFree, n & 1);
-#pragma unroll
-        for (int c = 0; c < kPlanes; ++c) sts16(base + L::kOffLo + (half * kPlanes + c) * kPlane + row * 16, last[c]);
-        fence_proxy_async();
-        arrive(bar(kW2Ready));
-      }
       wait(kDsDone, n & 1);
       tm_after();
-      if (holds) {
+      {
+        if (enter == 0.f)   // (not a factor: what is forgotten may be infinite)
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          float v[32];
-          tm_ld32(quarter + kCs + col0 + c, v);
+          for (int c = 0; c < kCols; ++c) st[c] = 0.f;
+        const f32x2 ee = pack2(enter, enter);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 16) {
+          float v[16];
+          tm_ld16(quarter + kCs + col0 + c, v);
           tm_wait_ld();
           loaded(v);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) st[c + k] = (enter == 0.f ? 0.f : enter * st[c + k]) + v[k];
+          for (int k = 0; k < 16; k += 2)
+            unpack2(fma2(ee, pack2(st[c + k], st[c + k + 1]), pack2(v[k], v[k + 1])), st[c + k], st[c + k + 1]);
         }
         tm_before();
       }
@@ -454,21 +555,28 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       if (mine) {
         float* l = w.local + slot((long long)seg * w.B * w.H + bh);
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) *reinterpret_cast<float4*>(l + c) = make_float4(st[c], st[c + 1], st[c + 2], st[c + 3]);
+        for (int c = 0; c < kCols; c += 4) *reinterpret_cast<float4*>(l + c) = make_float4(st[c], st[c + 1], st[c + 2], st[c + 3]);
       }
       if (sw == 0 && lane == 0) w.factor[(long long)seg * w.B * w.H + bh] = decay;
     } else if (w.s_out && first + chunks == w.chunks && mine) {
+      float* p = w.s_out + s_at + (long long)col0 * w.s_col;
 #pragma unroll
-      for (int c = 0; c < 64; ++c)
-        if (col0 + c < w.v.d) w.s_out[s_at + (long long)(col0 + c) * w.s_col] = st[c];
+      for (int c0 = 0; c0 < kCols; c0 += 8)
+        if (col0 + c0 < w.v.d)
+#pragma unroll
+          for (int c = c0; c < c0 + 8; ++c, p += w.s_col) *p = st[c];
     }
-  } else if (warp == 4 + kStateWarps) {
+  } else if (warp == 16) {
     // ================================================================================ loads
     if (umma_elect()) {
       constexpr int kS = L::kVStages;
       const bool raw = w.pad != nullptr;
       for (int n = 0; n < chunks; ++n) {
         const int t0 = tile_of(n) * kC, stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
+        if (n > 1) wait(kGEmpty + (n & 1), ((n >> 1) - 1) & 1);
+        mbar_expect_tx(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1), sizeof(TcGates));
+        bulk_load_1d(&gates(n), static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks + tile_of(n), sizeof(TcGates),
+                     reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1));
         if (n > 1) wait(kKEmpty + (n & 1), ((n >> 1) - 1) & 1);
         load_tile<KD>(base + L::kOffK + (n & 1) * L::kTk, &maps.k, w.k, t0, h, b, bar((raw ? kKRaw : kKFull) + (n & 1)));
         auto values = [&]() {
@@ -488,58 +596,38 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       }
     }
     __syncwarp();
-  } else if (warp == 5 + kStateWarps) {
-    // ================================================================================ gates
-    GateIn<4> ahead = gates_fetch<4>(w, b, h, tile_of(0), lane);
-    for (int n = 0; n < chunks; ++n) {
-      const GateIn<4> in = ahead;
-      if (n + 1 < chunks) ahead = gates_fetch<4>(w, b, h, tile_of(n + 1), lane);
-      if (n > 1) wait(kGEmpty + (n & 1), ((n >> 1) - 1) & 1);
-      const GateOut<4> r = gates_scan<4>(w, in, lane);
-      TcGates& g = gates(n);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int at = gate_row<4>(w, lane, k);
-        g.sum[at] = gate_sum(r.sum[k]) + r.bad, g.weight[at] = r.weight[k], g.count[at] = (uint8_t)r.count[k];
-      }
-      if (lane == 0) g.enter = r.enter, g.total = r.total;
-      __syncwarp();
-      arrive(bar(kGFull + (n & 1)));
-    }
-  } else if (warp == 6 + kStateWarps) {
+  } else if (warp == 17) {
     // ================================================================================ padded steps: whatever lies there becomes zeros
     if (w.pad) {
       for (int n = 0; n < chunks; ++n) {
-        const int t0 = tile_of(n) * kC, rows = min(kC, w.L - t0);
         constexpr int kS = L::kVStages;
         const int stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
-        const uint8_t* m = w.pad + (long long)b * w.L + t0;
-        uint32_t pad[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) pad[k] = __ballot_sync(~0u, 32 * k + lane < rows && m[32 * k + lane]);
-        const bool any = (pad[0] | pad[1] | pad[2] | pad[3]) != 0;
-        auto pass = [&](auto width, uint32_t at, int from, int to, uint32_t parity) {
-          wait(from, parity);
+        const TcGates& g = gates(n);
+        wait(kGFull + (n & 1), n >> 1 & 1);
+        const uint32_t pad[4] = {g.pad[0], g.pad[1], g.pad[2], g.pad[3]};
+        const bool any = g.padded;
+        arrive(bar(kGEmpty + (n & 1)));
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {   // keys, queries, values, x (and x before values where those have one place)
+          const int what = k < 2 ? k : kS == 1 ? 5 - k : k;
+          if ((what == 1 && !kOut) || (what == 3 && !kDots)) continue;
+          const int raw = what == 0 ? kKRaw + (n & 1) : what == 1 ? kQRaw : what == 2 ? kVRaw + stage : kXRaw;
+          const int full = what == 0 ? kKFull + (n & 1) : what == 1 ? kQFull : what == 2 ? kVFull + stage : kXFull;
+          const uint32_t at = base + (what == 0 ? L::kOffK + (n & 1) * L::kTk : what == 1 ? L::kOffQ : what == 2 ? L::kOffV + stage * L::kTv : L::kOffX);
+          wait(raw, what == 0 ? n >> 1 & 1 : what == 2 ? use & 1 : n & 1);
           if (any) {
-            clear_rows<decltype(width)::value>(at, pad, lane);
+            clear_rows(at, what < 2 ? KD / 8 : VD / 8, pad, lane);
             fence_proxy_async();
           }
           __syncwarp();
-          if (lane == 0) arrive(bar(to));
-        };
-        using Keys = std::integral_constant<int, KD>;
-        using Values = std::integral_constant<int, VD>;
-        pass(Keys(), base + L::kOffK + (n & 1) * L::kTk, kKRaw + (n & 1), kKFull + (n & 1), n >> 1 & 1);
-        if (kOut) pass(Keys(), base + L::kOffQ, kQRaw, kQFull, n & 1);
-        if (kDots && kS == 1) pass(Values(), base + L::kOffX, kXRaw, kXFull, n & 1);
-        pass(Values(), base + L::kOffV + stage * L::kTv, kVRaw + stage, kVFull + stage, use & 1);
-        if (kDots && kS == 2) pass(Values(), base + L::kOffX, kXRaw, kXFull, n & 1);
+          if (lane == 0) arrive(bar(full));
+        }
       }
     }
-  } else {
+  } else if (warp == 18) {
     // ================================================================================ products
     if (umma_elect()) {
-    constexpr uint32_t kPairs = idesc<T>(128, false, false), kRows = idesc<T>(VD, false, true), kBoth = idesc<T>(VD, true, true);
+    constexpr uint32_t kPairs = idesc<T>(128, false, false, 128), kRows = idesc<T>(VD, false, true, 128);
     constexpr int kS = L::kVStages;
     const uint64_t q = tile_desc(base + L::kOffQ), s = over(base + L::kOffS, KD * 16), x = tile_desc(base + L::kOffX);
     const uint64_t lo = over(base + L::kOffLo, kPlane), lo2 = over(base + L::kOffLo2, kPlane);
@@ -556,48 +644,38 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           if (n) wait(kORead, (n - 1) & 1);
         }
         tm_after();
-#pragma unroll
+#pragma unroll 2
         for (int k = 0; k < KD / 16; ++k) umma(tm + kColP, q + kAlong(k), kt + kAlong(k), kPairs, k > 0);
         if (kDots)
-#pragma unroll
+#pragma unroll 2
           for (int k = 0; k < VD / 16; ++k) umma(tm + kColO2, x + kAlong(k), vt + kAlong(k), kPairs, k > 0);
         umma_commit(bar(kPDone));
         wait(kSReady, n & 1);
         if (!kDots && n) wait(kORead, (n - 1) & 1);
         tm_after();
-#pragma unroll
+#pragma unroll 2
         for (int k = 0; k < KD / 16; ++k) umma(tm + kColO1, q + kAlong(k), s + k * 16, kRows, k > 0);
         umma_commit(bar(kQEmpty));
       }
       wait(kWReady, n & 1);
       wait(kVFull + stage, use & 1);
       tm_after();
-      if constexpr (L::kPieces == 3 && !L::kSeq)
-#pragma unroll
+      constexpr uint32_t kBoth = idesc<T>(VD, true, true, KD);
+      if constexpr (L::kPieces == 3)
+#pragma unroll 2
         for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo2 + k * 16, vt + kOver(k), kBoth, k > 0);
-#pragma unroll
-      for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo + k * 16, vt + kOver(k), kBoth, k > 0 || (L::kPieces == 3 && !L::kSeq));
-#pragma unroll
+#pragma unroll 2
+      for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo + k * 16, vt + kOver(k), kBoth, k > 0 || L::kPieces == 3);
+#pragma unroll 2
       for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, kt + kOver(k), vt + kOver(k), kBoth, true);
-      if constexpr (L::kSeq) umma_commit(bar(kLoFree));
-      else {
-        umma_commit(bar(kDsDone));
-        umma_commit(bar(kKEmpty + (n & 1)));
-      }
+      umma_commit(bar(kDsDone));
+      umma_commit(bar(kKEmpty + (n & 1)));
       if constexpr (kOut) {
         wait(kPReady, n & 1);
         tm_after();
-#pragma unroll
-        for (int k = 0; k < kC / 16; ++k) umma_tm(tm + kColO2, tm + kColP + k * 8, vt + kOver(k), kRows, k > 0);
+#pragma unroll 2
+        for (int k = 0; k < kC / 16; ++k) umma_tm(tm + kColO2, tm + kColP + k / 4 * 64 + k % 4 * 8, vt + kOver(k), kRows, k > 0);
         umma_commit(bar(kODone));
-      }
-      if constexpr (L::kSeq) {
-        wait(kW2Ready, n & 1);
-        tm_after();
-#pragma unroll
-        for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo + k * 16, vt + kOver(k), kBoth, true);
-        umma_commit(bar(kDsDone));
-        umma_commit(bar(kKEmpty + (n & 1)));
       }
       umma_commit(bar(kVEmpty + stage));
     }
@@ -613,22 +691,38 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   if (warp == 0) tm_free(tm, kOut ? 512 : 128);
 }
 
+// Whether the compiler gave a kernel the registers that its warps share out among themselves: with fewer they would wait for good.
+bool has_registers(const void* kernel, int regs) {
+  static std::mutex mutex;
+  static std::unordered_map<const void*, int> have;
+  std::lock_guard<std::mutex> lock(mutex);
+  int& n = have[kernel];
+  if (!n) {
+    cudaFuncAttributes a;
+    n = cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : -1;
+  }
+  return n >= regs;
+}
 template <typename T, int KD, int VD>
-void run(const Walk& w, const Maps& maps, int dots, void* stream) {
+bool run(const Walk& w, const Maps& maps, int dots, void* stream) {
   const long long blocks = (long long)w.B * w.H;
   auto go = [&](auto kernel, auto lay, long long n) {
     using L = decltype(lay);
-    launch(kernel, dim3((unsigned)n), dim3(L::kThreads), L::kEnd, stream, w, maps);
+    if (L::kMove && !has_registers(reinterpret_cast<const void*>(+kernel), L::kRegs)) return false;
+    launch_after(kernel, dim3((unsigned)n), dim3(L::kThreads), L::kEnd, stream, w, maps);
+    return true;
   };
-  if (w.segs > 1) go(tc_kernel<T, KD, VD, false, 0>, Lay<T, KD, VD, false, 0>(), blocks * (w.segs - 1));
-  if (dots == 0) go(tc_kernel<T, KD, VD, true, 0>, Lay<T, KD, VD, true, 0>(), blocks * w.segs);
-  else if (dots == 1) go(tc_kernel<T, KD, VD, true, 1>, Lay<T, KD, VD, true, 1>(), blocks * w.segs);
-  else go(tc_kernel<T, KD, VD, true, 2>, Lay<T, KD, VD, true, 2>(), blocks * w.segs);
+  if (!w.gates_there)
+    launch(tc_gates_kernel<T>, dim3((unsigned)((blocks * w.chunks + 3) / 4)), dim3(128), 0, stream, w);
+  if (w.segs > 1 && !go(tc_kernel<T, KD, VD, false, 0>, Lay<T, KD, VD, false, 0>(), blocks * (w.segs - 1))) return false;
+  if (dots == 0) return go(tc_kernel<T, KD, VD, true, 0>, Lay<T, KD, VD, true, 0>(), blocks * w.segs);
+  if (dots == 1) return go(tc_kernel<T, KD, VD, true, 1>, Lay<T, KD, VD, true, 1>(), blocks * w.segs);
+  return go(tc_kernel<T, KD, VD, true, 2>, Lay<T, KD, VD, true, 2>(), blocks * w.segs);
 }
 template <typename T>
-void pick(const Walk& w, const Maps& m, int dots, void* stream) {
-  if (w.k.d <= 64) w.v.d <= 64 ? run<T, 64, 64>(w, m, dots, stream) : run<T, 64, 128>(w, m, dots, stream);
-  else w.v.d <= 64 ? run<T, 128, 64>(w, m, dots, stream) : run<T, 128, 128>(w, m, dots, stream);
+bool pick(const Walk& w, const Maps& m, int dots, void* stream) {
+  if (w.k.d <= 64) return w.v.d <= 64 ? run<T, 64, 64>(w, m, dots, stream) : run<T, 64, 128>(w, m, dots, stream);
+  return w.v.d <= 64 ? run<T, 128, 64>(w, m, dots, stream) : run<T, 128, 128>(w, m, dots, stream);
 }
 
 // (width, step, head, sequence) of an operand; false where TMA cannot address it
@@ -645,7 +739,7 @@ bool maps_of(Maps* m, int dtype, const Walk& w) {
 }  // namespace
 
 bool tc_takes(int dtype, const Walk& w) {
-  if (dtype == MEGA_F32 || g_options[OPT_DISABLE_MMA].load()) return false;
+  if (dtype == MEGA_F32 || g_options[OPT_DISABLE_MMA].load() || w.piece < 16) return false;
   for (const Operand* o : {&w.q, &w.k, &w.v, &w.x})
     if (o->p && (o->d > kTcMost || o->vec < 16 || o->sl < 0 || o->sh < 0 || o->sb < 0 || (o->sl == 0 && w.L > 1))) return false;
   Maps m;   // (what the driver refuses is known before a plan is made)
@@ -654,7 +748,7 @@ bool tc_takes(int dtype, const Walk& w) {
 int tc_walk(int dtype, const Walk& w, int dots, void* stream) {
   Maps m;
   if (!maps_of(&m, dtype, w)) return MEGA_ERR_UNSUPPORTED;
-  dtype == MEGA_BF16 ? pick<__nv_bfloat16>(w, m, dots, stream) : pick<__half>(w, m, dots, stream);
+  if (!(dtype == MEGA_BF16 ? pick<__nv_bfloat16>(w, m, dots, stream) : pick<__half>(w, m, dots, stream))) return MEGA_ERR_UNSUPPORTED;
   g_last_kernel.store("decayed_attention_tc", std::memory_order_relaxed);
   return MEGA_OK;
 }
