@@ -90,8 +90,9 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
 }
 
 // barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it
-enum { kQFull, kQEmpty, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kXFull = kVEmpty + 2, kXEmpty, kGFull, kGEmpty = kGFull + 2,
-       kPDone = kGEmpty + 2, kPReady, kODone, kORead, kSReady, kDsDone, kWReady, kQRaw, kKRaw, kVRaw = kKRaw + 2, kXRaw = kVRaw + 2, kBars };
+enum { kQFull, kQEmpty = kQFull + 3, kQRaw = kQEmpty + 3, kKFull = kQRaw + 3, kKEmpty = kKFull + 3, kKRaw = kKEmpty + 3, kVFull = kKRaw + 3,
+       kVEmpty = kVFull + 3, kVRaw = kVEmpty + 3, kXFull = kVRaw + 3, kXEmpty = kXFull + 2, kXRaw = kXEmpty + 2, kGFull = kXRaw + 2, kGEmpty = kGFull + 2,
+       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kORead, kSReady, kDsDone, kWReady, kBars };
 
 // kOut: outputs; else the state that a segment leaves by itself.  kDots: sums for the gates' gradient (1: walk of dq, 2: of dk).
 template <typename T, int KD, int VD, bool kOut, int kDots>
@@ -100,20 +101,26 @@ struct Lay {
   static constexpr bool kBig = KD == 128 && VD == 128 && kOut;   // heads of 128 x 128: shared memory holds seven of their tiles
   // pieces of weighted keys; beside x there is no room for a third one (which matters to no output but the gradient of the state)
   static constexpr int kPieces = std::is_same<T, __nv_bfloat16>::value && !(kBig && kDots) ? 3 : 2;
-  static constexpr int kVStages = kBig && (kDots || kPieces == 3) ? 1 : 2;
+  // places of each operand, as shared memory has room
+  static constexpr bool kSmall = KD == 64 && VD == 64;
+  static constexpr int kQs = kSmall ? 3 : KD == 64 ? (kDots ? 2 : 3) : 1, kKs = kSmall ? 3 : KD == 64 && !kDots ? 3 : 2,
+                       kVs = kSmall ? 3 : kBig && (kDots || kPieces == 3) ? 1 : 2, kXs = kSmall ? 2 : 1;
   static constexpr int kThreads = 640;   // 8 warps of pairs and outputs, 8 of weights and state, loads, padding, products, and one that rests
   // Registers of a thread: 96 at launch, 20 warps; where the state takes 64 of them its eight warps have 128, the first eight 88 and
   // the last four 48: 2 x 88 + 2 x 128 + 48 for each four warps, as at launch (5 x 96).
   static constexpr int kRegs = 96;
   static constexpr bool kMove = VD == 128;
-  static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 ? kTk : 0), kOffV = kOffK + 2 * kTk,
-                       kOffQ = kOffV + kVStages * kTv, kOffX = kOffQ + (kOut ? kTk : 0), kOffS = kOffX + (kDots ? kTv : 0),
+  static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 ? kTk : 0), kOffV = kOffK + kKs * kTk,
+                       kOffQ = kOffV + kVs * kTv, kOffX = kOffQ + (kOut ? kQs * kTk : 0), kOffS = kOffX + (kDots ? kXs * kTv : 0),
                        kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8, kEnd = kOffSlot + 16;
   static_assert(kEnd <= 227 * 1024, "shared memory");
+  // Columns of tensor memory.  Where they suffice pairs have two places: those of the next chunk are worked on while this one's outputs
+  // are on their way.
+  static constexpr bool kTwo = kOut && VD == 64 && !kDots;
+  static constexpr uint32_t kColO1 = kTwo ? 256 : 128, kColO2 = kTwo ? 320 : 256, kColS = kOut ? 384 : 0;
+  static __device__ __forceinline__ uint32_t col_p(int n) { return kTwo ? (n & 1) * 128 : 0; }
   static_assert(sizeof(TcGates) % 16 == 0, "gates");
 };
-// columns of tensor memory
-constexpr uint32_t kColP = 0, kColO1 = 128, kColO2 = 256, kColS = 384;
 
 __device__ __forceinline__ bool tried(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -157,6 +164,12 @@ __device__ __forceinline__ void tm_ld16(uint32_t at, float* v) {
       : "r"(at)
       : "memory");
 }
+// chunk n's place among S, and the parity of the barriers of its use of that place
+template <int S>
+struct Ring {
+  static __device__ __forceinline__ int place(int n) { return n % S; }
+  static __device__ __forceinline__ uint32_t parity(int n) { return n / S & 1; }
+};
 template <int N>
 __device__ __forceinline__ void loaded(float (&v)[N]) {   // (the registers of a load from tensor memory, once it has been waited for)
 #pragma unroll
@@ -242,6 +255,10 @@ __device__ __forceinline__ void clear_rows(uint32_t at, int planes, const uint32
 template <typename T, int KD, int VD, bool kOut, int kDots>
 __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_kernel(const __grid_constant__ Walk w, const __grid_constant__ Maps maps) {
   using L = Lay<T, KD, VD, kOut, kDots>;
+  using Qr = Ring<L::kQs>;
+  using Kr = Ring<L::kKs>;
+  using Vr = Ring<L::kVs>;
+  using Xr = Ring<L::kXs>;
   extern __shared__ __align__(1024) unsigned char smem[];
   int* const slot_ = reinterpret_cast<int*>(smem + L::kOffSlot);   // where tensor memory lies; whether a wait has given up
   volatile int* gone = slot_ + 1;
@@ -251,17 +268,21 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   const int first = seg * w.per, chunks = min(w.per, w.chunks - first);   // in the order of the walk
   auto bar = [&](int i) { return base + L::kOffBar + i * 8; };
   auto wait = [&](int i, uint32_t parity) { wait_for(bar(i), parity, gone); };
+  auto done = [&](int i) {   // (a warp arrives as one: barriers take their threads one after another)
+    __syncwarp();
+    if (lane == 0) arrive(bar(i));
+  };
   auto tile_of = [&](int n) { return w.rev ? w.chunks - 1 - first - n : first + n; };
   auto gates = [&](int n) -> TcGates& { return reinterpret_cast<TcGates*>(smem + L::kOffG)[n & 1]; };
 
   if (tid == 0) {
     *gone = 0;
-    auto init = [&](int i, uint32_t count) { mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, count); };
-    for (int i : {(int)kQFull, (int)kKFull, kKFull + 1, (int)kVFull, kVFull + 1, (int)kXFull, (int)kGFull, kGFull + 1, (int)kQRaw, (int)kKRaw, kKRaw + 1, (int)kVRaw, kVRaw + 1, (int)kXRaw})
-      init(i, 1);
-    for (int i : {(int)kQEmpty, (int)kKEmpty, kKEmpty + 1, (int)kVEmpty, kVEmpty + 1, (int)kPDone, (int)kODone, (int)kDsDone}) init(i, 1);
-    for (int i : {(int)kXEmpty, (int)kPReady, (int)kORead, (int)kSReady, (int)kWReady}) init(i, 256);
-    for (int i : {(int)kGEmpty, kGEmpty + 1}) init(i, (kOut ? 512 : 256) + (w.pad ? 32 : 0));
+#pragma unroll 1
+    for (int i = 0; i < kBars; ++i) {
+      const bool empty = i == kGEmpty || i == kGEmpty + 1;
+      const bool all = i == kXEmpty || i == kXEmpty + 1 || i == kPReady || i == kPReady + 1 || i == kORead || i == kSReady || i == kWReady;
+      mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, empty ? (kOut ? 16 : 8) + (w.pad ? 1 : 0) : all ? 8 : 1);
+    }
     mbar_fence_init();
   }
   if (warp == 16 && umma_elect()) {
@@ -275,7 +296,6 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   tm_after();
   pdl_wait();   // (all that comes before on the stream)
   const uint32_t tm = *reinterpret_cast<volatile uint32_t*>(slot_);
-  constexpr uint32_t kCs = kOut ? kColS : 0;
 
   if constexpr (L::kMove) {   // (the four warps that do little leave registers to those that hold the state)
     if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
@@ -287,35 +307,43 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     if constexpr (kOut) {
       const int rb = warp & 3, half = warp >> 2, i = rb * 32 + lane;   // a row, and half of its pairs and of its outputs
       const uint32_t quarter = tm + ((uint32_t)(rb * 32) << 16);
-      for (int n = 0; n < chunks; ++n) {
+      float inner = 0.f, e_next = 0.f;
+      auto pairs = [&](int n) {
         const TcGates& g = gates(n);
-        const long long t = (long long)tile_of(n) * kC + i;
         wait(kGFull + (n & 1), n >> 1 & 1);
         const float gi = g.sum[i];
         const int ci = g.count[i];
-        float inner = 0.f, read = 0.f;
-        wait(kPDone, n & 1);
+        inner = 0.f;
+        e_next = ci ? 0.f : w.o_scale * ex2(gi);
+        wait(kPDone + (n & 1), n >> 1 & 1);
         tm_after();
         const int from = max(w.rev ? rb : 0, 2 * half), to = min(w.rev ? 3 : rb, 2 * half + 1);   // blocks of 32 steps that these rows see
         auto put = [&](int jb, const float (&v)[32]) {
           uint32_t word[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) word[j] = pack<T>(v[2 * j], v[2 * j + 1]);
-          const uint32_t to = quarter + kColP + 64 * half + 16 * (jb & 1);   // (in the place of pairs that this warp has read)
+          const uint32_t to = quarter + L::col_p(n) + 64 * half + 16 * (jb & 1);   // (in the place of pairs that this warp has read)
           tm_st8(to, word);
           tm_st8(to + 8, word + 8);
         };
-        auto block = [&](int jb, float (&v)[32]) {
+        auto block = [&](int jb) {
+          float v[32];
+          tm_ld32(quarter + L::col_p(n) + 32 * jb, v);
           // (one factor above one and one below where the row lies inside the 32 steps: their product is what counts, while both are in range)
           const int end = last_of(w, jb);
-          if (jb != rb || !g.apart[jb]) {
-            const float f = g.count[end] == ci ? w.p_scale * ex2(gi - g.sum[end]) : 0.f;
-            const f32x2 ff = pack2(f, f);
+          const float f = g.count[end] == ci ? w.p_scale * ex2(gi - g.sum[end]) : 0.f;
+          const bool apart = jb == rb && g.apart[jb];
+          float4 c[8];
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 c = *reinterpret_cast<const float4*>(g.col + 32 * jb + j);
-              unpack2(mul2(pack2(v[j], v[j + 1]), mul2(ff, pack2(c.x, c.y))), v[j], v[j + 1]);
-              unpack2(mul2(pack2(v[j + 2], v[j + 3]), mul2(ff, pack2(c.z, c.w))), v[j + 2], v[j + 3]);
+          for (int j = 0; j < 8; ++j) c[j] = *reinterpret_cast<const float4*>(g.col + 32 * jb + 4 * j);
+          const f32x2 ff = pack2(f, f);
+          tm_wait_ld();
+          loaded(v);
+          if (!apart) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              unpack2(mul2(pack2(v[4 * j], v[4 * j + 1]), mul2(ff, pack2(c[j].x, c[j].y))), v[4 * j], v[4 * j + 1]);
+              unpack2(mul2(pack2(v[4 * j + 2], v[4 * j + 3]), mul2(ff, pack2(c[j].z, c[j].w))), v[4 * j + 2], v[4 * j + 3]);
             }
           } else {   // resets among these steps, or a decay by more than 2^-100: a power of two for each pair
 #pragma unroll
@@ -335,7 +363,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
 #pragma unroll
             for (int k = 0; k < 32; k += 16) {
               float x[16];
-              tm_ld16(quarter + kColO2 + 32 * jb + k, x);
+              tm_ld16(quarter + L::kColO2 + 32 * jb + k, x);
               tm_wait_ld();
               loaded(x);
 #pragma unroll
@@ -345,42 +373,43 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         };
         {
 #pragma unroll 1
-          for (int jb = from; jb <= to; ++jb) {
-            float v[32];
-            tm_ld32(quarter + kColP + 32 * jb, v);
-            tm_wait_ld();
-            loaded(v);
-            block(jb, v);
-          }
+          for (int jb = from; jb <= to; ++jb) block(jb);
           const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
           for (int jb = 2 * half; jb < 2 * half + 2; ++jb)
             if (jb < from || jb > to) {
-              tm_st8(quarter + kColP + 64 * half + 16 * (jb & 1), zero);
-              tm_st8(quarter + kColP + 64 * half + 16 * (jb & 1) + 8, zero);
+              tm_st8(quarter + L::col_p(n) + 64 * half + 16 * (jb & 1), zero);
+              tm_st8(quarter + L::col_p(n) + 64 * half + 16 * (jb & 1) + 8, zero);
             }
         }
+        done(kGEmpty + (n & 1));
         tm_wait_st();
         tm_before();
-        arrive(bar(kPReady));
-
-        const float e = ci ? 0.f : w.o_scale * ex2(gi);
-        if (kDots) wait(kXFull, n & 1);
+        done(kPReady + (n & 1));
+      };
+      auto outputs = [&](int n, float e) {
+        const long long t = (long long)tile_of(n) * kC + i;
+        float read = 0.f;
+        if (kDots) wait(kXFull + Xr::place(n), Xr::parity(n));
         wait(kODone, n & 1);
         tm_after();
         char* row = static_cast<char*>(w.out) + (b * w.ob + h * w.oh + t * w.ol) * 2;
 #pragma unroll 1
         for (int c = half * (VD / 2); c < (half + 1) * (VD / 2); c += 32) {
           float o[32], p[32];
-          tm_ld32(quarter + kColO1 + c, o);
-          tm_ld32(quarter + kColO2 + c, p);
+          tm_ld32(quarter + L::kColO1 + c, o);
+          tm_ld32(quarter + L::kColO2 + c, p);
           uint4 u[kDots ? 4 : 1];
           if constexpr (kDots != 0)
 #pragma unroll
-            for (int m = 0; m < 4; ++m) u[m] = lds16(base + L::kOffX + piece_of(i, c / 8 + m));
+            for (int m = 0; m < 4; ++m) u[m] = lds16(base + L::kOffX + Xr::place(n) * L::kTv + piece_of(i, c / 8 + m));
           tm_wait_ld();
           loaded(o);
           loaded(p);
+          if (c + 32 >= (half + 1) * (VD / 2)) {
+            tm_before();
+            done(kORead);
+          }
           uint32_t word[16];
           const f32x2 ee = pack2(e, e);
 #pragma unroll
@@ -415,13 +444,17 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
             }
           }
         }
-        tm_before();
-        arrive(bar(kORead));
         if (kDots) {
-          arrive(bar(kXEmpty));
+          done(kXEmpty + Xr::place(n));
           if (t < w.L) w.dots[((long long)half * w.B * w.H + bh) * w.L + t] = make_float2(read, inner);
         }
-        arrive(bar(kGEmpty + (n & 1)));
+      };
+      constexpr int kAhead = L::kTwo ? 1 : 0;
+#pragma unroll 1
+      for (int n = -kAhead; n < chunks; ++n) {
+        const float e_now = e_next;
+        if (n + kAhead < chunks) pairs(n + kAhead);
+        if (n >= 0) outputs(n, kAhead ? e_now : e_next);
       }
     }
   } else if (warp < 16) {
@@ -467,20 +500,20 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           sts16(base + L::kOffS + (col0 + c) / 8 * (KD * 16) + row * 16,
                 make_uint4(pack<T>(st[c], st[c + 1]), pack<T>(st[c + 2], st[c + 3]), pack<T>(st[c + 4], st[c + 5]), pack<T>(st[c + 6], st[c + 7])));
       fence_proxy_async();
-      arrive(bar(kSReady));
+      done(kSReady);
     };
     if (kOut) state_out();
     float decay = 1.f;
     for (int n = 0; n < chunks; ++n) {
       const TcGates& g = gates(n);
       wait(kGFull + (n & 1), n >> 1 & 1);
-      wait(kKFull + (n & 1), n >> 1 & 1);
-      if (kOut) wait(kPDone, n & 1);   // (the pairs' product has read the keys)
+      wait(kKFull + Kr::place(n), Kr::parity(n));
+      if (kOut) wait(kPDone + (n & 1), n >> 1 & 1);   // (the pairs' product has read the keys)
       const float wt = g.col[step] * g.leave[step >> 5], enter = g.enter;
-      constexpr int kAt = VD == 128 ? 2 : 4;   // (planes at a time: reads first, as none may pass a write)
+      constexpr int kAt = 2;   // (planes at a time: reads first, as none may pass a write)
 #pragma unroll 1
       for (int c0 = 0; c0 < kPlanes; c0 += kAt) {
-        const uint32_t keys = base + L::kOffK + (n & 1) * L::kTk;
+        const uint32_t keys = base + L::kOffK + Kr::place(n) * L::kTk;
         uint4 u[kAt];
 #pragma unroll
         for (int c = 0; c < kAt; ++c) u[c] = lds16(keys + piece_of(step, half * kPlanes + c0 + c));
@@ -497,7 +530,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         }
       }
       fence_proxy_async();
-      arrive(bar(kWReady));
+      done(kWReady);
       if constexpr (kDots != 0) {
         // the state that enters: left by the walk of dq, multiplied with the gradient of the one that leaves by that of dk
         T* a = static_cast<T*>(w.anchors) + slot((long long)bh * w.chunks + tile_of(n));
@@ -538,7 +571,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
 #pragma unroll
         for (int c = 0; c < kCols; c += 16) {
           float v[16];
-          tm_ld16(quarter + kCs + col0 + c, v);
+          tm_ld16(quarter + L::kColS + col0 + c, v);
           tm_wait_ld();
           loaded(v);
 #pragma unroll
@@ -548,7 +581,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         tm_before();
       }
       decay *= enter;
-      arrive(bar(kGEmpty + (n & 1)));
+      done(kGEmpty + (n & 1));
       if (kOut && n + 1 < chunks) state_out();
     }
     if (!kOut) {
@@ -569,30 +602,30 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   } else if (warp == 16) {
     // ================================================================================ loads
     if (umma_elect()) {
-      constexpr int kS = L::kVStages;
       const bool raw = w.pad != nullptr;
+#pragma unroll 1
       for (int n = 0; n < chunks; ++n) {
-        const int t0 = tile_of(n) * kC, stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
-        if (n > 1) wait(kGEmpty + (n & 1), ((n >> 1) - 1) & 1);
-        mbar_expect_tx(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1), sizeof(TcGates));
-        bulk_load_1d(&gates(n), static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks + tile_of(n), sizeof(TcGates),
-                     reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1));
-        if (n > 1) wait(kKEmpty + (n & 1), ((n >> 1) - 1) & 1);
-        load_tile<KD>(base + L::kOffK + (n & 1) * L::kTk, &maps.k, w.k, t0, h, b, bar((raw ? kKRaw : kKFull) + (n & 1)));
+        const int t0 = tile_of(n) * kC;
+        if (n >= L::kKs) wait(kKEmpty + Kr::place(n), Kr::parity(n) ^ 1);
+        load_tile<KD>(base + L::kOffK + Kr::place(n) * L::kTk, &maps.k, w.k, t0, h, b, bar((raw ? kKRaw : kKFull) + Kr::place(n)));
         auto values = [&]() {
-          if (use) wait(kVEmpty + stage, (use - 1) & 1);
-          load_tile<VD>(base + L::kOffV + stage * L::kTv, &maps.v, w.v, t0, h, b, bar((raw ? kVRaw : kVFull) + stage));
+          if (n >= L::kVs) wait(kVEmpty + Vr::place(n), Vr::parity(n) ^ 1);
+          load_tile<VD>(base + L::kOffV + Vr::place(n) * L::kTv, &maps.v, w.v, t0, h, b, bar((raw ? kVRaw : kVFull) + Vr::place(n)));
         };
-        if (kS == 2) values();
+        if (L::kVs > 1) values();
         if (kOut) {
-          if (n) wait(kQEmpty, (n - 1) & 1);
-          load_tile<KD>(base + L::kOffQ, &maps.q, w.q, t0, h, b, bar(raw ? kQRaw : kQFull));
+          if (n >= L::kQs) wait(kQEmpty + Qr::place(n), Qr::parity(n) ^ 1);
+          load_tile<KD>(base + L::kOffQ + Qr::place(n) * L::kTk, &maps.q, w.q, t0, h, b, bar((raw ? kQRaw : kQFull) + Qr::place(n)));
         }
+        if (n > 1) wait(kGEmpty + (n & 1), (n >> 1 & 1) ^ 1);
+        uint64_t* const got = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1);
+        mbar_expect_tx(got, sizeof(TcGates));
+        bulk_load_1d(&gates(n), static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks + tile_of(n), sizeof(TcGates), got);
         if (kDots) {
-          if (n) wait(kXEmpty, (n - 1) & 1);
-          load_tile<VD>(base + L::kOffX, &maps.x, w.x, t0, h, b, bar(raw ? kXRaw : kXFull));
+          if (n >= L::kXs) wait(kXEmpty + Xr::place(n), Xr::parity(n) ^ 1);
+          load_tile<VD>(base + L::kOffX + Xr::place(n) * L::kTv, &maps.x, w.x, t0, h, b, bar((raw ? kXRaw : kXFull) + Xr::place(n)));
         }
-        if (kS == 1) values();
+        if (L::kVs == 1) values();
       }
     }
     __syncwarp();
@@ -600,27 +633,25 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     // ================================================================================ padded steps: whatever lies there becomes zeros
     if (w.pad) {
       for (int n = 0; n < chunks; ++n) {
-        constexpr int kS = L::kVStages;
-        const int stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
         const TcGates& g = gates(n);
         wait(kGFull + (n & 1), n >> 1 & 1);
         const uint32_t pad[4] = {g.pad[0], g.pad[1], g.pad[2], g.pad[3]};
         const bool any = g.padded;
-        arrive(bar(kGEmpty + (n & 1)));
+        done(kGEmpty + (n & 1));
 #pragma unroll 1
         for (int k = 0; k < 4; ++k) {   // keys, queries, values, x (and x before values where those have one place)
-          const int what = k < 2 ? k : kS == 1 ? 5 - k : k;
+          const int what = k < 2 ? k : L::kVs == 1 ? 5 - k : k;
           if ((what == 1 && !kOut) || (what == 3 && !kDots)) continue;
-          const int raw = what == 0 ? kKRaw + (n & 1) : what == 1 ? kQRaw : what == 2 ? kVRaw + stage : kXRaw;
-          const int full = what == 0 ? kKFull + (n & 1) : what == 1 ? kQFull : what == 2 ? kVFull + stage : kXFull;
-          const uint32_t at = base + (what == 0 ? L::kOffK + (n & 1) * L::kTk : what == 1 ? L::kOffQ : what == 2 ? L::kOffV + stage * L::kTv : L::kOffX);
-          wait(raw, what == 0 ? n >> 1 & 1 : what == 2 ? use & 1 : n & 1);
+          const int place = what == 0 ? Kr::place(n) : what == 1 ? Qr::place(n) : what == 2 ? Vr::place(n) : Xr::place(n);
+          const int raw = (what == 0 ? kKRaw : what == 1 ? kQRaw : what == 2 ? kVRaw : kXRaw) + place;
+          const int full = (what == 0 ? kKFull : what == 1 ? kQFull : what == 2 ? kVFull : kXFull) + place;
+          const uint32_t at = base + (what == 0 ? L::kOffK : what == 1 ? L::kOffQ : what == 2 ? L::kOffV : L::kOffX) + place * (what < 2 ? L::kTk : L::kTv);
+          wait(raw, what == 0 ? Kr::parity(n) : what == 1 ? Qr::parity(n) : what == 2 ? Vr::parity(n) : Xr::parity(n));
           if (any) {
             clear_rows(at, what < 2 ? KD / 8 : VD / 8, pad, lane);
             fence_proxy_async();
           }
-          __syncwarp();
-          if (lane == 0) arrive(bar(full));
+          done(full);
         }
       }
     }
@@ -628,60 +659,69 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     // ================================================================================ products
     if (umma_elect()) {
     constexpr uint32_t kPairs = idesc<T>(128, false, false, 128), kRows = idesc<T>(VD, false, true, 128);
-    constexpr int kS = L::kVStages;
-    const uint64_t q = tile_desc(base + L::kOffQ), s = over(base + L::kOffS, KD * 16), x = tile_desc(base + L::kOffX);
+    const uint64_t s = over(base + L::kOffS, KD * 16);
     const uint64_t lo = over(base + L::kOffLo, kPlane), lo2 = over(base + L::kOffLo2, kPlane);
-    for (int n = 0; n < chunks; ++n) {
-      const int stage = kS == 2 ? n & 1 : 0, use = kS == 2 ? n >> 1 : n;
-      const uint32_t key = base + L::kOffK + (n & 1) * L::kTk, val = base + L::kOffV + stage * L::kTv;
-      const uint64_t kt = tile_desc(key), vt = tile_desc(val);
+    auto keys_of = [&](int n) { return tile_desc(base + L::kOffK + Kr::place(n) * L::kTk); };
+    auto queries_of = [&](int n) { return tile_desc(base + L::kOffQ + Qr::place(n) * L::kTk); };
+    auto values_of = [&](int n) { return tile_desc(base + L::kOffV + Vr::place(n) * L::kTv); };
+    auto pairs = [&](int n) {
+      wait(kQFull + Qr::place(n), Qr::parity(n));
+      wait(kKFull + Kr::place(n), Kr::parity(n));
+      if (kDots) {
+        wait(kXFull + Xr::place(n), Xr::parity(n));
+        wait(kVFull + Vr::place(n), Vr::parity(n));
+        if (n) wait(kORead, (n - 1) & 1);
+      }
+      tm_after();
+      const uint64_t q = queries_of(n), kt = keys_of(n);
+#pragma unroll 2
+      for (int k = 0; k < KD / 16; ++k) umma(tm + L::col_p(n), q + kAlong(k), kt + kAlong(k), kPairs, k > 0);
+      if (kDots) {
+        const uint64_t x = tile_desc(base + L::kOffX + Xr::place(n) * L::kTv), vt = values_of(n);
+#pragma unroll 2
+        for (int k = 0; k < VD / 16; ++k) umma(tm + L::kColO2, x + kAlong(k), vt + kAlong(k), kPairs, k > 0);
+      }
+      umma_commit(bar(kPDone + (n & 1)));
+    };
+    constexpr int kAhead = L::kTwo ? 1 : 0;
+#pragma unroll 1
+    for (int n = -kAhead; n < chunks; ++n) {
+      if (kOut && n + kAhead < chunks) pairs(n + kAhead);
+      if (n < 0) continue;
+      const uint64_t kt = keys_of(n), vt = values_of(n);
       if constexpr (kOut) {
-        wait(kQFull, n & 1);
-        wait(kKFull + (n & 1), n >> 1 & 1);
-        if (kDots) {
-          wait(kXFull, n & 1);
-          wait(kVFull + stage, use & 1);
-          if (n) wait(kORead, (n - 1) & 1);
-        }
-        tm_after();
-#pragma unroll 2
-        for (int k = 0; k < KD / 16; ++k) umma(tm + kColP, q + kAlong(k), kt + kAlong(k), kPairs, k > 0);
-        if (kDots)
-#pragma unroll 2
-          for (int k = 0; k < VD / 16; ++k) umma(tm + kColO2, x + kAlong(k), vt + kAlong(k), kPairs, k > 0);
-        umma_commit(bar(kPDone));
         wait(kSReady, n & 1);
         if (!kDots && n) wait(kORead, (n - 1) & 1);
         tm_after();
+        const uint64_t q = queries_of(n);
 #pragma unroll 2
-        for (int k = 0; k < KD / 16; ++k) umma(tm + kColO1, q + kAlong(k), s + k * 16, kRows, k > 0);
-        umma_commit(bar(kQEmpty));
+        for (int k = 0; k < KD / 16; ++k) umma(tm + L::kColO1, q + kAlong(k), s + k * 16, kRows, k > 0);
+        umma_commit(bar(kQEmpty + Qr::place(n)));
+        wait(kVFull + Vr::place(n), Vr::parity(n));
+        wait(kPReady + (n & 1), n >> 1 & 1);
+        tm_after();
+#pragma unroll 2
+        for (int k = 0; k < kC / 16; ++k) umma_tm(tm + L::kColO2, tm + L::col_p(n) + k / 4 * 64 + k % 4 * 8, vt + kOver(k), kRows, k > 0);
+        umma_commit(bar(kODone));
+      } else {
+        wait(kVFull + Vr::place(n), Vr::parity(n));
       }
       wait(kWReady, n & 1);
-      wait(kVFull + stage, use & 1);
       tm_after();
       constexpr uint32_t kBoth = idesc<T>(VD, true, true, KD);
       if constexpr (L::kPieces == 3)
 #pragma unroll 2
-        for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo2 + k * 16, vt + kOver(k), kBoth, k > 0);
+        for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, lo2 + k * 16, vt + kOver(k), kBoth, k > 0);
 #pragma unroll 2
-      for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, lo + k * 16, vt + kOver(k), kBoth, k > 0 || L::kPieces == 3);
+      for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, lo + k * 16, vt + kOver(k), kBoth, k > 0 || L::kPieces == 3);
 #pragma unroll 2
-      for (int k = 0; k < kC / 16; ++k) umma(tm + kCs, kt + kOver(k), vt + kOver(k), kBoth, true);
+      for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, kt + kOver(k), vt + kOver(k), kBoth, true);
       umma_commit(bar(kDsDone));
-      umma_commit(bar(kKEmpty + (n & 1)));
-      if constexpr (kOut) {
-        wait(kPReady, n & 1);
-        tm_after();
-#pragma unroll 2
-        for (int k = 0; k < kC / 16; ++k) umma_tm(tm + kColO2, tm + kColP + k / 4 * 64 + k % 4 * 8, vt + kOver(k), kRows, k > 0);
-        umma_commit(bar(kODone));
-      }
-      umma_commit(bar(kVEmpty + stage));
+      umma_commit(bar(kKEmpty + Kr::place(n)));
+      umma_commit(bar(kVEmpty + Vr::place(n)));
     }
     // (nothing of this block's products is on its way when it ends: the last of each kind has been waited for by the other roles, or is)
-    const int stage = kS == 2 ? (chunks - 1) & 1 : 0, use = kS == 2 ? (chunks - 1) >> 1 : chunks - 1;
-    wait(kVEmpty + stage, use & 1);
+    wait(kVEmpty + Vr::place(chunks - 1), Vr::parity(chunks - 1));
     }
     __syncwarp();
   }
