@@ -9,7 +9,8 @@
 // and y = e O1 + O2 with a row's factor e.  For the gates' gradient also X V^T, in O2's place before it.
 // Roles: eight warps of pairs and outputs (a thread has half of a row of the chunk), eight of weights and state (a thread has half of a
 // step's keys, then half of a row of the state, whose fp32 values stay in its registers), one that loads, one for
-// padded steps, one that issues products.  All exchange over mbarriers.
+// padded steps, and two that issue products: those of pairs, and those with the state (one warp for both takes longer to wait and to issue
+// than the tensor cores to compute).  All exchange over mbarriers.
 //
 // Activations lie as TMA leaves them (columns of 64, rows of 128 bytes, swizzled), what the threads write as planes of 16 bytes along
 // keys or values, rows one after another.  Both serve with either axis as the contraction, and a thread that owns a row reads and
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
 // barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it
 enum { kQFull, kQEmpty = kQFull + 3, kQRaw = kQEmpty + 3, kKFull = kQRaw + 3, kKEmpty = kKFull + 3, kKRaw = kKEmpty + 3, kVFull = kKRaw + 3,
        kVEmpty = kVFull + 3, kVRaw = kVEmpty + 3, kXFull = kVRaw + 3, kXEmpty = kXFull + 2, kXRaw = kXEmpty + 2, kGFull = kXRaw + 2, kGEmpty = kGFull + 2,
-       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kORead, kSReady, kDsDone, kWReady, kBars };
+       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead, kSReady, kDsDone, kWReady, kBars };
 
 // kOut: outputs; else the state that a segment leaves by itself.  kDots: sums for the gates' gradient (1: walk of dq, 2: of dk).
 template <typename T, int KD, int VD, bool kOut, int kDots>
@@ -105,7 +106,7 @@ struct Lay {
   static constexpr bool kSmall = KD == 64 && VD == 64;
   static constexpr int kQs = kSmall ? 3 : KD == 64 ? (kDots ? 2 : 3) : 1, kKs = kSmall ? 3 : KD == 64 && !kDots ? 3 : 2,
                        kVs = kSmall ? 3 : kBig && (kDots || kPieces == 3) ? 1 : 2, kXs = kSmall ? 2 : 1;
-  static constexpr int kThreads = 640;   // 8 warps of pairs and outputs, 8 of weights and state, loads, padding, products, and one that rests
+  static constexpr int kThreads = 640;   // 8 warps of pairs and outputs, 8 of weights and state, loads, padding, products (2)
   // Registers of a thread: 96 at launch, 20 warps; where the state takes 64 of them its eight warps have 128, the first eight 88 and
   // the last four 48: 2 x 88 + 2 x 128 + 48 for each four warps, as at launch (5 x 96).
   static constexpr int kRegs = 96;
@@ -281,7 +282,8 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     for (int i = 0; i < kBars; ++i) {
       const bool empty = i == kGEmpty || i == kGEmpty + 1;
       const bool all = i == kXEmpty || i == kXEmpty + 1 || i == kPReady || i == kPReady + 1 || i == kORead || i == kSReady || i == kWReady;
-      mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, empty ? (kOut ? 16 : 8) + (w.pad ? 1 : 0) : all ? 8 : 1);
+      const bool both = kOut && ((i >= kQEmpty && i < kQEmpty + 3) || (i >= kVEmpty && i < kVEmpty + 3));   // (two warps' products read it)
+      mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, both ? 2 : empty ? (kOut ? 16 : 8) + (w.pad ? 1 : 0) : all ? 8 : 1);
     }
     mbar_fence_init();
   }
@@ -392,6 +394,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         float read = 0.f;
         if (kDots) wait(kXFull + Xr::place(n), Xr::parity(n));
         wait(kODone, n & 1);
+        wait(kO1Done, n & 1);
         tm_after();
         char* row = static_cast<char*>(w.out) + (b * w.ob + h * w.oh + t * w.ol) * 2;
 #pragma unroll 1
@@ -656,72 +659,82 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       }
     }
   } else if (warp == 18) {
-    // ================================================================================ products
-    if (umma_elect()) {
-    constexpr uint32_t kPairs = idesc<T>(128, false, false, 128), kRows = idesc<T>(VD, false, true, 128);
-    const uint64_t s = over(base + L::kOffS, KD * 16);
-    const uint64_t lo = over(base + L::kOffLo, kPlane), lo2 = over(base + L::kOffLo2, kPlane);
-    auto keys_of = [&](int n) { return tile_desc(base + L::kOffK + Kr::place(n) * L::kTk); };
-    auto queries_of = [&](int n) { return tile_desc(base + L::kOffQ + Qr::place(n) * L::kTk); };
-    auto values_of = [&](int n) { return tile_desc(base + L::kOffV + Vr::place(n) * L::kTv); };
-    auto pairs = [&](int n) {
-      wait(kQFull + Qr::place(n), Qr::parity(n));
-      wait(kKFull + Kr::place(n), Kr::parity(n));
-      if (kDots) {
-        wait(kXFull + Xr::place(n), Xr::parity(n));
-        wait(kVFull + Vr::place(n), Vr::parity(n));
-        if (n) wait(kORead, (n - 1) & 1);
-      }
-      tm_after();
-      const uint64_t q = queries_of(n), kt = keys_of(n);
-#pragma unroll 2
-      for (int k = 0; k < KD / 16; ++k) umma(tm + L::col_p(n), q + kAlong(k), kt + kAlong(k), kPairs, k > 0);
-      if (kDots) {
-        const uint64_t x = tile_desc(base + L::kOffX + Xr::place(n) * L::kTv), vt = values_of(n);
-#pragma unroll 2
-        for (int k = 0; k < VD / 16; ++k) umma(tm + L::kColO2, x + kAlong(k), vt + kAlong(k), kPairs, k > 0);
-      }
-      umma_commit(bar(kPDone + (n & 1)));
-    };
-    constexpr int kAhead = L::kTwo ? 1 : 0;
+    // ================================================================================ products of pairs
+    if (kOut && umma_elect()) {
+      constexpr uint32_t kPairs = idesc<T>(128, false, false, 128), kRows = idesc<T>(VD, false, true, 128);
+      constexpr int kAhead = L::kTwo ? 1 : 0;
 #pragma unroll 1
-    for (int n = -kAhead; n < chunks; ++n) {
-      if (kOut && n + kAhead < chunks) pairs(n + kAhead);
-      if (n < 0) continue;
-      const uint64_t kt = keys_of(n), vt = values_of(n);
-      if constexpr (kOut) {
-        wait(kSReady, n & 1);
-        if (!kDots && n) wait(kORead, (n - 1) & 1);
-        tm_after();
-        const uint64_t q = queries_of(n);
-#pragma unroll 2
-        for (int k = 0; k < KD / 16; ++k) umma(tm + L::kColO1, q + kAlong(k), s + k * 16, kRows, k > 0);
-        umma_commit(bar(kQEmpty + Qr::place(n)));
-        wait(kVFull + Vr::place(n), Vr::parity(n));
+      for (int n = -kAhead; n < chunks; ++n) {
+        if (const int m = n + kAhead; m < chunks) {
+          wait(kQFull + Qr::place(m), Qr::parity(m));
+          wait(kKFull + Kr::place(m), Kr::parity(m));
+          if (kDots) {
+            wait(kXFull + Xr::place(m), Xr::parity(m));
+            wait(kVFull + Vr::place(m), Vr::parity(m));
+            if (m) wait(kORead, (m - 1) & 1);
+          }
+          tm_after();
+          const uint64_t q = tile_desc(base + L::kOffQ + Qr::place(m) * L::kTk), kt = tile_desc(base + L::kOffK + Kr::place(m) * L::kTk);
+#pragma unroll
+          for (int k = 0; k < KD / 16; ++k) umma(tm + L::col_p(m), q + kAlong(k), kt + kAlong(k), kPairs, k > 0);
+          if (kDots) {
+            const uint64_t x = tile_desc(base + L::kOffX + Xr::place(m) * L::kTv), vt = tile_desc(base + L::kOffV + Vr::place(m) * L::kTv);
+#pragma unroll
+            for (int k = 0; k < VD / 16; ++k) umma(tm + L::kColO2, x + kAlong(k), vt + kAlong(k), kPairs, k > 0);
+          }
+          umma_commit(bar(kPDone + (m & 1)));
+          umma_commit(bar(kQEmpty + Qr::place(m)));
+        }
+        if (n < 0) continue;
+        const uint64_t vt = tile_desc(base + L::kOffV + Vr::place(n) * L::kTv);
+        if (!kDots) {
+          wait(kVFull + Vr::place(n), Vr::parity(n));
+          if (n) wait(kORead, (n - 1) & 1);
+        }
         wait(kPReady + (n & 1), n >> 1 & 1);
         tm_after();
-#pragma unroll 2
+#pragma unroll
         for (int k = 0; k < kC / 16; ++k) umma_tm(tm + L::kColO2, tm + L::col_p(n) + k / 4 * 64 + k % 4 * 8, vt + kOver(k), kRows, k > 0);
         umma_commit(bar(kODone));
-      } else {
-        wait(kVFull + Vr::place(n), Vr::parity(n));
+        umma_commit(bar(kVEmpty + Vr::place(n)));
       }
-      wait(kWReady, n & 1);
-      tm_after();
-      constexpr uint32_t kBoth = idesc<T>(VD, true, true, KD);
-      if constexpr (L::kPieces == 3)
-#pragma unroll 2
-        for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, lo2 + k * 16, vt + kOver(k), kBoth, k > 0);
-#pragma unroll 2
-      for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, lo + k * 16, vt + kOver(k), kBoth, k > 0 || L::kPieces == 3);
-#pragma unroll 2
-      for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, kt + kOver(k), vt + kOver(k), kBoth, true);
-      umma_commit(bar(kDsDone));
-      umma_commit(bar(kKEmpty + Kr::place(n)));
-      umma_commit(bar(kVEmpty + Vr::place(n)));
     }
-    // (nothing of this block's products is on its way when it ends: the last of each kind has been waited for by the other roles, or is)
-    wait(kVEmpty + Vr::place(chunks - 1), Vr::parity(chunks - 1));
+    __syncwarp();
+  } else {
+    // ================================================================================ products of the state
+    if (umma_elect()) {
+      constexpr uint32_t kRows = idesc<T>(VD, false, true, 128), kBoth = idesc<T>(VD, true, true, KD);
+      const uint64_t s = over(base + L::kOffS, KD * 16), lo = over(base + L::kOffLo, kPlane), lo2 = over(base + L::kOffLo2, kPlane);
+#pragma unroll 1
+      for (int n = 0; n < chunks; ++n) {
+        if constexpr (kOut) {
+          wait(kQFull + Qr::place(n), Qr::parity(n));
+          wait(kSReady, n & 1);
+          if (n) wait(kORead, (n - 1) & 1);
+          tm_after();
+          const uint64_t q = tile_desc(base + L::kOffQ + Qr::place(n) * L::kTk);
+#pragma unroll
+          for (int k = 0; k < KD / 16; ++k) umma(tm + L::kColO1, q + kAlong(k), s + k * 16, kRows, k > 0);
+          umma_commit(bar(kO1Done));
+          umma_commit(bar(kQEmpty + Qr::place(n)));
+        }
+        wait(kVFull + Vr::place(n), Vr::parity(n));
+        wait(kWReady, n & 1);
+        tm_after();
+        const uint64_t kt = tile_desc(base + L::kOffK + Kr::place(n) * L::kTk), vt = tile_desc(base + L::kOffV + Vr::place(n) * L::kTv);
+        if constexpr (L::kPieces == 3)
+#pragma unroll
+          for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, lo2 + k * 16, vt + kOver(k), kBoth, k > 0);
+#pragma unroll
+        for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, lo + k * 16, vt + kOver(k), kBoth, k > 0 || L::kPieces == 3);
+#pragma unroll
+        for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, kt + kOver(k), vt + kOver(k), kBoth, true);
+        umma_commit(bar(kDsDone));
+        umma_commit(bar(kKEmpty + Kr::place(n)));
+        umma_commit(bar(kVEmpty + Vr::place(n)));
+      }
+      // (nothing of this block's products is on its way when it ends)
+      wait(kVEmpty + Vr::place(chunks - 1), Vr::parity(chunks - 1));
     }
     __syncwarp();
   }
