@@ -6,7 +6,8 @@
 //   O1 = Q S                        S: the state that enters, in shared memory
 //   dS = (w K)^T V                  w K in pieces of 8 (bf16, three) or 11 (fp16, two) bits, the first in K's place
 //   O2 = (weighted pairs) V
-// and y = e O1 + O2 with a row's factor e.  For the gates' gradient also X V^T, in O2's place before it.
+// and y = e O1 + O2 with a row's factor e.  The sums for the gates' gradient are those of x with e O1 and with O2: of the latter, taken from
+// the walks of dq and dk, the pairs on one side of a step cancel because both walks round the same weights the same way.
 // Roles: eight warps of pairs and outputs (a thread has half of a row of the chunk), eight of weights and state (a thread has half of a
 // step's keys, then half of a row of the state, whose fp32 values stay in its registers), one that loads, one for
 // padded steps, and two that issue products: those of pairs, and those with the state (one warp for both takes longer to wait and to issue
@@ -33,13 +34,14 @@ namespace {
 
 constexpr int kC = kTcChunk, kPlane = kC * 16;
 
-// What the gates of a chunk come to.  A pair's weight 2^(sum_i - sum_j) is one factor of j, from there to the last step of its 32, and
+// What the gates of a chunk come to.  A pair's weight is one factor of j, from there to the last step of its 32, and
 // one of i, from that step on; so is a step's weight in the state that leaves.  Only where the first factor gets too small, or a reset
 // lies among those 32 steps, pairs inside them need a power of two each.
 struct TcGates {
-  float sum[kC];      // running sum of log2 a
+  int rel[kC];        // running sum of log2 a beyond that at the last of a step's 32, in 2^-18 (at most 32 x 149)
   float col[kC];      // weight of a step at the last of its 32 (0: a reset lies between)
   uint8_t count[kC];  // resets so far
+  float base[4];      // running sum of log2 a at the last of 32 steps
   float leave[4];     // weight of the last of 32 steps in the state that leaves
   uint32_t pad[4];    // padded steps
   float enter;        // weight of the state that enters in the one that leaves
@@ -65,17 +67,18 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
   const long long end = __shfl_sync(~0u, r.sum[3], lane | 7);
   const int there = __shfl_sync(~0u, r.count[3], lane | 7);
   unsigned mask = 0;   // of this lane's rows in their word
-  float sum[4], col[4];
+  int rel[4];
+  float col[4];
   uint8_t count[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int to = w.rev ? 3 - k : k;   // rows ascend
-    sum[to] = gate_sum(r.sum[k]) + r.bad, count[to] = (uint8_t)r.count[k];
+    rel[to] = (int)((r.sum[k] - end) >> 22), count[to] = (uint8_t)r.count[k];
     col[to] = r.count[k] == there && !(in.pad >> k & 1) ? exp2f(gate_sum(end - r.sum[k]) + r.bad) : 0.f;
     mask |= (in.pad >> k & 1) << to;
   }
   const int row = w.rev ? kC - 4 - 4 * lane : 4 * lane, word = row / 32;
-  *reinterpret_cast<float4*>(g.sum + row) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+  *reinterpret_cast<int4*>(g.rel + row) = make_int4(rel[0], rel[1], rel[2], rel[3]);
   *reinterpret_cast<float4*>(g.col + row) = make_float4(col[0], col[1], col[2], col[3]);
   *reinterpret_cast<uchar4*>(g.count + row) = make_uchar4(count[0], count[1], count[2], count[3]);
   const unsigned lanes = 0xffu << (lane & 24);
@@ -84,6 +87,7 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
   mask = __reduce_or_sync(lanes, mask << (row & 31));
   if ((lane & 7) == 7) {
     g.apart[word] = reset || far;
+    g.base[word] = gate_sum(end) + r.bad;
     g.leave[word] = there == r.total ? w.s_scale * exp2f(gate_sum(r.all - end) + r.bad) : 0.f;
     g.pad[word] = mask;
   }
@@ -117,7 +121,7 @@ struct Lay {
   static_assert(kEnd <= 227 * 1024, "shared memory");
   // Columns of tensor memory.  Where they suffice pairs have two places: those of the next chunk are worked on while this one's outputs
   // are on their way.
-  static constexpr bool kTwo = kOut && VD == 64 && !kDots;
+  static constexpr bool kTwo = kOut && VD == 64;
   static constexpr uint32_t kColO1 = kTwo ? 256 : 128, kColO2 = kTwo ? 320 : 256, kColS = kOut ? 384 : 0;
   static __device__ __forceinline__ uint32_t col_p(int n) { return kTwo ? (n & 1) * 128 : 0; }
   static_assert(sizeof(TcGates) % 16 == 0, "gates");
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       const bool empty = i == kGEmpty || i == kGEmpty + 1;
       const bool all = i == kXEmpty || i == kXEmpty + 1 || i == kPReady || i == kPReady + 1 || i == kORead || i == kSReady || i == kWReady;
       const bool both = kOut && ((i >= kQEmpty && i < kQEmpty + 3) || (i >= kVEmpty && i < kVEmpty + 3));   // (two warps' products read it)
-      mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, both ? 2 : empty ? (kOut ? 16 : 8) + (w.pad ? 1 : 0) : all ? 8 : 1);
+      mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, both ? 2 : empty ? 16 + (w.pad ? 1 : 0) : all ? (!kOut && i == kWReady ? 16 : 8) : 1);
     }
     mbar_fence_init();
   }
@@ -304,18 +308,53 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     else if (warp >= 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   }
+  // w K in pieces, of a step's `count` planes from `from` on
+  auto weigh = [&](int n, int step, int from, int count) {
+    const TcGates& g = gates(n);
+    const float wt = g.col[step] * g.leave[step >> 5];
+    const uint32_t keys = base + L::kOffK + Kr::place(n) * L::kTk;
+#pragma unroll 1
+    for (int c0 = from; c0 < from + count; c0 += 2) {   // (two at a time: reads first, as none may pass a write)
+      uint4 u[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) u[c] = lds16(keys + piece_of(step, c0 + c));
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t piece[3][4];
+        const uint32_t uu[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) split<T, L::kPieces>(unpack<T>(uu[k]), wt, piece[0][k], piece[1][k], piece[2][k]);
+        const int at = c0 + c;
+        sts16(keys + piece_of(step, at), make_uint4(piece[0][0], piece[0][1], piece[0][2], piece[0][3]));
+        sts16(base + L::kOffLo + at * kPlane + step * 16, make_uint4(piece[1][0], piece[1][1], piece[1][2], piece[1][3]));
+        if constexpr (L::kPieces == 3) sts16(base + L::kOffLo2 + at * kPlane + step * 16, make_uint4(piece[2][0], piece[2][1], piece[2][2], piece[2][3]));
+      }
+    }
+    fence_proxy_async();
+    done(kWReady);
+  };
+
   if (warp < 8) {
     // ================================================================================ pairs and outputs
-    if constexpr (kOut) {
+    if constexpr (!kOut) {   // (none: the other half of the weighted keys)
+#pragma unroll 1
+      for (int n = 0; n < chunks; ++n) {
+        wait(kGFull + (n & 1), n >> 1 & 1);
+        wait(kKFull + Kr::place(n), Kr::parity(n));
+        if (n) wait(kDsDone, (n - 1) & 1);   // (the products have read the last chunk's)
+        weigh(n, (warp & 3) * 32 + lane, (warp >> 2) * (KD / 16) + KD / 32, KD / 32);
+        done(kGEmpty + (n & 1));
+      }
+    } else {
       const int rb = warp & 3, half = warp >> 2, i = rb * 32 + lane;   // a row, and half of its pairs and of its outputs
       const uint32_t quarter = tm + ((uint32_t)(rb * 32) << 16);
-      float inner = 0.f, e_next = 0.f;
+      float e_next = 0.f;
       auto pairs = [&](int n) {
         const TcGates& g = gates(n);
         wait(kGFull + (n & 1), n >> 1 & 1);
-        const float gi = g.sum[i];
+        const int ri = g.rel[i];
+        const float gi = g.base[rb] + 0x1p-18f * (float)ri;
         const int ci = g.count[i];
-        inner = 0.f;
         e_next = ci ? 0.f : w.o_scale * ex2(gi);
         wait(kPDone + (n & 1), n >> 1 & 1);
         tm_after();
@@ -333,7 +372,9 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           tm_ld32(quarter + L::col_p(n) + 32 * jb, v);
           // (one factor above one and one below where the row lies inside the 32 steps: their product is what counts, while both are in range)
           const int end = last_of(w, jb);
-          const float f = g.count[end] == ci ? w.p_scale * ex2(gi - g.sum[end]) : 0.f;
+          // (inside the 32 steps the row's factor is one over its own as a column: both walks' weights agree to two units, however large the sums)
+          const float col = g.col[i];
+          const float f = g.count[end] != ci || (jb == rb && col == 0.f) ? 0.f : jb == rb ? __fdividef(w.p_scale, col) : w.p_scale * ex2(gi - g.base[jb]);
           const bool apart = jb == rb && g.apart[jb];
           float4 c[8];
 #pragma unroll
@@ -341,6 +382,12 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           const f32x2 ff = pack2(f, f);
           tm_wait_ld();
           loaded(v);
+          // a step by itself has the same weight to the last bit in the walks of dq and dk, whose sums differ by it
+          float own = 0.f;
+          if constexpr (kDots != 0)
+            if (jb == rb)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) own = j == lane ? v[j] * w.p_scale : own;
           if (!apart) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -350,7 +397,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           } else {   // resets among these steps, or a decay by more than 2^-100: a power of two for each pair
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const float p = v[j] * (w.p_scale * ex2(fminf(gi - g.sum[32 * jb + j], 0.f)));
+              const float p = v[j] * (w.p_scale * ex2(0x1p-18f * (float)min(ri - g.rel[32 * jb + j], 0)));
               v[j] = g.count[32 * jb + j] == ci ? p : 0.f;
             }
           }
@@ -358,20 +405,11 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
             const uint32_t seen = w.rev ? ~0u << lane : ~0u >> (31 - lane);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = seen & (1u << j) ? v[j] : 0.f;
+            if constexpr (kDots != 0)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = j == lane ? own : v[j];
           }
           put(jb, v);
-          if constexpr (kDots != 0) {
-            // the pairs' sum, without the step by itself
-#pragma unroll
-            for (int k = 0; k < 32; k += 16) {
-              float x[16];
-              tm_ld16(quarter + L::kColO2 + 32 * jb + k, x);
-              tm_wait_ld();
-              loaded(x);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) inner += jb == rb && lane == k + j ? 0.f : v[k + j] * x[j];
-            }
-          }
         };
         {
 #pragma unroll 1
@@ -391,7 +429,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       };
       auto outputs = [&](int n, float e) {
         const long long t = (long long)tile_of(n) * kC + i;
-        float read = 0.f;
+        float read = 0.f, inner = 0.f;
         if (kDots) wait(kXFull + Xr::place(n), Xr::parity(n));
         wait(kODone, n & 1);
         wait(kO1Done, n & 1);
@@ -424,6 +462,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
               const float2 x = unpack<T>(uu[m & 3]);
               unpack2(own, o[2 * m], o[2 * m + 1]);
               read += o[2 * m] * x.x + o[2 * m + 1] * x.y;
+              inner += p[2 * m] * x.x + p[2 * m + 1] * x.y;
               y = add2(own, pack2(p[2 * m], p[2 * m + 1]));
             } else {
               y = fma2(ee, pack2(o[2 * m], o[2 * m + 1]), pack2(p[2 * m], p[2 * m + 1]));
@@ -512,28 +551,8 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       wait(kGFull + (n & 1), n >> 1 & 1);
       wait(kKFull + Kr::place(n), Kr::parity(n));
       if (kOut) wait(kPDone + (n & 1), n >> 1 & 1);   // (the pairs' product has read the keys)
-      const float wt = g.col[step] * g.leave[step >> 5], enter = g.enter;
-      constexpr int kAt = 2;   // (planes at a time: reads first, as none may pass a write)
-#pragma unroll 1
-      for (int c0 = 0; c0 < kPlanes; c0 += kAt) {
-        const uint32_t keys = base + L::kOffK + Kr::place(n) * L::kTk;
-        uint4 u[kAt];
-#pragma unroll
-        for (int c = 0; c < kAt; ++c) u[c] = lds16(keys + piece_of(step, half * kPlanes + c0 + c));
-#pragma unroll
-        for (int c = 0; c < kAt; ++c) {
-          uint32_t piece[3][4];
-          const uint32_t uu[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) split<T, L::kPieces>(unpack<T>(uu[k]), wt, piece[0][k], piece[1][k], piece[2][k]);
-          const int at = half * kPlanes + c0 + c;
-          sts16(keys + piece_of(step, at), make_uint4(piece[0][0], piece[0][1], piece[0][2], piece[0][3]));
-          sts16(base + L::kOffLo + at * kPlane + step * 16, make_uint4(piece[1][0], piece[1][1], piece[1][2], piece[1][3]));
-          if constexpr (L::kPieces == 3) sts16(base + L::kOffLo2 + at * kPlane + step * 16, make_uint4(piece[2][0], piece[2][1], piece[2][2], piece[2][3]));
-        }
-      }
-      fence_proxy_async();
-      done(kWReady);
+      const float enter = g.enter;
+      weigh(n, step, half * kPlanes, kOut ? kPlanes : kPlanes / 2);
       if constexpr (kDots != 0) {
         // the state that enters: left by the walk of dq, multiplied with the gradient of the one that leaves by that of dk
         T* a = static_cast<T*>(w.anchors) + slot((long long)bh * w.chunks + tile_of(n));
@@ -605,10 +624,13 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   } else if (warp == 16) {
     // ================================================================================ loads
     if (umma_elect()) {
-      const bool raw = w.pad != nullptr;
+      const TcGates* const table = static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks;
+      bool next = w.pad && table[tile_of(0)].padded;
 #pragma unroll 1
       for (int n = 0; n < chunks; ++n) {
         const int t0 = tile_of(n) * kC;
+        const bool raw = next;   // (the others' loads are seen as they land)
+        next = w.pad && n + 1 < chunks && table[tile_of(n + 1)].padded;
         if (n >= L::kKs) wait(kKEmpty + Kr::place(n), Kr::parity(n) ^ 1);
         load_tile<KD>(base + L::kOffK + Kr::place(n) * L::kTk, &maps.k, w.k, t0, h, b, bar((raw ? kKRaw : kKFull) + Kr::place(n)));
         auto values = [&]() {
@@ -623,7 +645,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         if (n > 1) wait(kGEmpty + (n & 1), (n >> 1 & 1) ^ 1);
         uint64_t* const got = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1);
         mbar_expect_tx(got, sizeof(TcGates));
-        bulk_load_1d(&gates(n), static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks + tile_of(n), sizeof(TcGates), got);
+        bulk_load_1d(&gates(n), table + tile_of(n), sizeof(TcGates), got);
         if (kDots) {
           if (n >= L::kXs) wait(kXEmpty + Xr::place(n), Xr::parity(n) ^ 1);
           load_tile<VD>(base + L::kOffX + Xr::place(n) * L::kTv, &maps.x, w.x, t0, h, b, bar((raw ? kXRaw : kXFull) + Xr::place(n)));
@@ -635,12 +657,14 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   } else if (warp == 17) {
     // ================================================================================ padded steps: whatever lies there becomes zeros
     if (w.pad) {
+      uint32_t used = 0;   // parity of each place's uses by chunks with padding
       for (int n = 0; n < chunks; ++n) {
         const TcGates& g = gates(n);
         wait(kGFull + (n & 1), n >> 1 & 1);
         const uint32_t pad[4] = {g.pad[0], g.pad[1], g.pad[2], g.pad[3]};
         const bool any = g.padded;
         done(kGEmpty + (n & 1));
+        if (!any) continue;
 #pragma unroll 1
         for (int k = 0; k < 4; ++k) {   // keys, queries, values, x (and x before values where those have one place)
           const int what = k < 2 ? k : L::kVs == 1 ? 5 - k : k;
@@ -649,11 +673,10 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           const int raw = (what == 0 ? kKRaw : what == 1 ? kQRaw : what == 2 ? kVRaw : kXRaw) + place;
           const int full = (what == 0 ? kKFull : what == 1 ? kQFull : what == 2 ? kVFull : kXFull) + place;
           const uint32_t at = base + (what == 0 ? L::kOffK : what == 1 ? L::kOffQ : what == 2 ? L::kOffV : L::kOffX) + place * (what < 2 ? L::kTk : L::kTv);
-          wait(raw, what == 0 ? Kr::parity(n) : what == 1 ? Qr::parity(n) : what == 2 ? Vr::parity(n) : Xr::parity(n));
-          if (any) {
-            clear_rows(at, what < 2 ? KD / 8 : VD / 8, pad, lane);
-            fence_proxy_async();
-          }
+          wait(raw, used >> (3 * what + place) & 1);
+          used ^= 1u << (3 * what + place);
+          clear_rows(at, what < 2 ? KD / 8 : VD / 8, pad, lane);
+          fence_proxy_async();
           done(full);
         }
       }
@@ -668,29 +691,17 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         if (const int m = n + kAhead; m < chunks) {
           wait(kQFull + Qr::place(m), Qr::parity(m));
           wait(kKFull + Kr::place(m), Kr::parity(m));
-          if (kDots) {
-            wait(kXFull + Xr::place(m), Xr::parity(m));
-            wait(kVFull + Vr::place(m), Vr::parity(m));
-            if (m) wait(kORead, (m - 1) & 1);
-          }
           tm_after();
           const uint64_t q = tile_desc(base + L::kOffQ + Qr::place(m) * L::kTk), kt = tile_desc(base + L::kOffK + Kr::place(m) * L::kTk);
 #pragma unroll
           for (int k = 0; k < KD / 16; ++k) umma(tm + L::col_p(m), q + kAlong(k), kt + kAlong(k), kPairs, k > 0);
-          if (kDots) {
-            const uint64_t x = tile_desc(base + L::kOffX + Xr::place(m) * L::kTv), vt = tile_desc(base + L::kOffV + Vr::place(m) * L::kTv);
-#pragma unroll
-            for (int k = 0; k < VD / 16; ++k) umma(tm + L::kColO2, x + kAlong(k), vt + kAlong(k), kPairs, k > 0);
-          }
           umma_commit(bar(kPDone + (m & 1)));
           umma_commit(bar(kQEmpty + Qr::place(m)));
         }
         if (n < 0) continue;
         const uint64_t vt = tile_desc(base + L::kOffV + Vr::place(n) * L::kTv);
-        if (!kDots) {
-          wait(kVFull + Vr::place(n), Vr::parity(n));
-          if (n) wait(kORead, (n - 1) & 1);
-        }
+        wait(kVFull + Vr::place(n), Vr::parity(n));
+        if (n) wait(kORead, (n - 1) & 1);
         wait(kPReady + (n & 1), n >> 1 & 1);
         tm_after();
 #pragma unroll
