@@ -46,7 +46,8 @@ struct TcGates {
   uint32_t pad[4];    // padded steps
   float enter;        // weight of the state that enters in the one that leaves
   uint8_t apart[4];   // whether resets lie among 32 steps, or their decay is out of range
-  uint32_t padded, pad_;
+  uint32_t padded;    // 0: no step is, 2: all are and none resets (which leaves the state as it is)
+  uint32_t pad_;
 };
 static_assert(sizeof(TcGates) == kTcGates, "gates");
 __device__ __forceinline__ int last_of(const Walk& w, int block) { return 32 * block + (w.rev ? 0 : 31); }
@@ -91,13 +92,14 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
     g.leave[word] = there == r.total ? w.s_scale * exp2f(gate_sum(r.all - end) + r.bad) : 0.f;
     g.pad[word] = mask;
   }
-  if (lane == 0) g.enter = r.enter, g.padded = r.padded;
+  const bool all = __all_sync(~0u, in.pad == 15u);
+  if (lane == 0) g.enter = r.enter, g.padded = !r.padded ? 0 : all && !r.total ? 2 : 1;
 }
 
 // barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it
 enum { kQFull, kQEmpty = kQFull + 3, kQRaw = kQEmpty + 3, kKFull = kQRaw + 3, kKEmpty = kKFull + 3, kKRaw = kKEmpty + 3, kVFull = kKRaw + 3,
        kVEmpty = kVFull + 3, kVRaw = kVEmpty + 3, kXFull = kVRaw + 3, kXEmpty = kXFull + 2, kXRaw = kXEmpty + 2, kGFull = kXRaw + 2, kGEmpty = kGFull + 2,
-       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead, kSReady, kDsDone, kWReady, kBars };
+       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead = kO1Done + 2, kSReady = kORead + 2, kDsDone, kWReady, kBars = kWReady + 2 };
 
 // kOut: outputs; else the state that a segment leaves by itself.  kDots: sums for the gates' gradient (1: walk of dq, 2: of dk).
 template <typename T, int KD, int VD, bool kOut, int kDots>
@@ -122,8 +124,9 @@ struct Lay {
   // Columns of tensor memory.  Where they suffice pairs have two places: those of the next chunk are worked on while this one's outputs
   // are on their way.
   static constexpr bool kTwo = kOut && VD == 64;
-  static constexpr uint32_t kColO1 = kTwo ? 256 : 128, kColO2 = kTwo ? 320 : 256, kColS = kOut ? 384 : 0;
+  static constexpr uint32_t kColO2 = kTwo ? 384 : 256, kColS = !kOut ? 0 : kTwo ? 448 : 384;
   static __device__ __forceinline__ uint32_t col_p(int n) { return kTwo ? (n & 1) * 128 : 0; }
+  static __device__ __forceinline__ uint32_t col_o1(int n) { return kTwo ? 256 + (n & 1) * 64 : 128; }
   static_assert(sizeof(TcGates) % 16 == 0, "gates");
 };
 
@@ -270,7 +273,8 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H), b = bh / w.H, h = bh % w.H;
-  const int first = seg * w.per, chunks = min(w.per, w.chunks - first);   // in the order of the walk
+  int first = seg * w.per, chunks = min(w.per, w.chunks - first);   // in the order of the walk
+  const bool ends = first + chunks == w.chunks;
   auto bar = [&](int i) { return base + L::kOffBar + i * 8; };
   auto wait = [&](int i, uint32_t parity) { wait_for(bar(i), parity, gone); };
   auto done = [&](int i) {   // (a warp arrives as one: barriers take their threads one after another)
@@ -285,9 +289,9 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
 #pragma unroll 1
     for (int i = 0; i < kBars; ++i) {
       const bool empty = i == kGEmpty || i == kGEmpty + 1;
-      const bool all = i == kXEmpty || i == kXEmpty + 1 || i == kPReady || i == kPReady + 1 || i == kORead || i == kSReady || i == kWReady;
+      const bool all = i == kXEmpty || i == kXEmpty + 1 || i == kPReady || i == kPReady + 1 || i == kORead || i == kORead + 1 || i == kSReady || i >= kWReady;
       const bool both = kOut && ((i >= kQEmpty && i < kQEmpty + 3) || (i >= kVEmpty && i < kVEmpty + 3));   // (two warps' products read it)
-      mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, both ? 2 : empty ? 16 + (w.pad ? 1 : 0) : all ? (!kOut && i == kWReady ? 16 : 8) : 1);
+      mbar_init(reinterpret_cast<uint64_t*>(smem + L::kOffBar) + i, both ? 2 : empty ? 16 + (w.pad ? 1 : 0) : all ? (!kOut && i >= kWReady ? 16 : 8) : 1);
     }
     mbar_fence_init();
   }
@@ -301,6 +305,30 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   __syncthreads();
   tm_after();
   pdl_wait();   // (all that comes before on the stream)
+  if (w.pad) {
+    // chunks of nothing but padding at either end of the segment are not walked
+    const TcGates* const table = static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks;
+    int* const range = slot_ + 2;
+    if (tid == 0) range[0] = chunks, range[1] = -1;
+    __syncthreads();
+    for (int n = tid; n < chunks; n += L::kThreads)
+      if (table[tile_of(n)].padded != 2) {
+        atomicMin(range, n);
+        atomicMax(range + 1, n);
+      }
+    __syncthreads();
+    const int low = range[0], high = range[1] + 1;
+    if constexpr (kOut) {
+      const int per_row = w.v.d / 8, all = chunks - max(high - low, 0);
+      for (long long k = tid; k < (long long)all * kC * per_row; k += L::kThreads) {
+        const int at = (int)(k / (kC * per_row)), n = at < low ? at : at + high - low, r = (int)(k / per_row % kC);
+        const long long t = (long long)tile_of(n) * kC + r;
+        if (t < w.L) *reinterpret_cast<uint4*>(static_cast<char*>(w.out) + (b * w.ob + h * w.oh + t * w.ol + k % per_row * 8) * 2) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (high > low) first += low, chunks = high - low;
+    else chunks = 0;
+  }
   const uint32_t tm = *reinterpret_cast<volatile uint32_t*>(slot_);
 
   if constexpr (L::kMove) {   // (the four warps that do little leave registers to those that hold the state)
@@ -331,7 +359,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       }
     }
     fence_proxy_async();
-    done(kWReady);
+    done(kWReady + (n & 1));
   };
 
   if (warp < 8) {
@@ -432,13 +460,13 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         float read = 0.f, inner = 0.f;
         if (kDots) wait(kXFull + Xr::place(n), Xr::parity(n));
         wait(kODone, n & 1);
-        wait(kO1Done, n & 1);
+        wait(kO1Done + (n & 1), n >> 1 & 1);
         tm_after();
         char* row = static_cast<char*>(w.out) + (b * w.ob + h * w.oh + t * w.ol) * 2;
 #pragma unroll 1
         for (int c = half * (VD / 2); c < (half + 1) * (VD / 2); c += 32) {
           float o[32], p[32];
-          tm_ld32(quarter + L::kColO1 + c, o);
+          tm_ld32(quarter + L::col_o1(n) + c, o);
           tm_ld32(quarter + L::kColO2 + c, p);
           uint4 u[kDots ? 4 : 1];
           if constexpr (kDots != 0)
@@ -449,7 +477,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           loaded(p);
           if (c + 32 >= (half + 1) * (VD / 2)) {
             tm_before();
-            done(kORead);
+            done(kORead + (n & 1));
           }
           uint32_t word[16];
           const f32x2 ee = pack2(e, e);
@@ -613,7 +641,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         for (int c = 0; c < kCols; c += 4) *reinterpret_cast<float4*>(l + c) = make_float4(st[c], st[c + 1], st[c + 2], st[c + 3]);
       }
       if (sw == 0 && lane == 0) w.factor[(long long)seg * w.B * w.H + bh] = decay;
-    } else if (w.s_out && first + chunks == w.chunks && mine) {
+    } else if (w.s_out && ends && mine) {
       float* p = w.s_out + s_at + (long long)col0 * w.s_col;
 #pragma unroll
       for (int c0 = 0; c0 < kCols; c0 += 8)
@@ -625,7 +653,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     // ================================================================================ loads
     if (umma_elect()) {
       const TcGates* const table = static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks;
-      bool next = w.pad && table[tile_of(0)].padded;
+      bool next = w.pad && chunks && table[tile_of(0)].padded;
 #pragma unroll 1
       for (int n = 0; n < chunks; ++n) {
         const int t0 = tile_of(n) * kC;
@@ -691,6 +719,8 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         if (const int m = n + kAhead; m < chunks) {
           wait(kQFull + Qr::place(m), Qr::parity(m));
           wait(kKFull + Kr::place(m), Kr::parity(m));
+          // (a barrier tells two phases apart: the warps of weights have seen these products of two chunks ago, not only those of pairs)
+          if (m > 1) wait(kWReady + (m & 1), (m >> 1 & 1) ^ 1);
           tm_after();
           const uint64_t q = tile_desc(base + L::kOffQ + Qr::place(m) * L::kTk), kt = tile_desc(base + L::kOffK + Kr::place(m) * L::kTk);
 #pragma unroll
@@ -701,7 +731,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         if (n < 0) continue;
         const uint64_t vt = tile_desc(base + L::kOffV + Vr::place(n) * L::kTv);
         wait(kVFull + Vr::place(n), Vr::parity(n));
-        if (n) wait(kORead, (n - 1) & 1);
+        if (n) wait(kORead + ((n - 1) & 1), (n - 1) >> 1 & 1);
         wait(kPReady + (n & 1), n >> 1 & 1);
         tm_after();
 #pragma unroll
@@ -721,16 +751,19 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         if constexpr (kOut) {
           wait(kQFull + Qr::place(n), Qr::parity(n));
           wait(kSReady, n & 1);
-          if (n) wait(kORead, (n - 1) & 1);
+          if (L::kTwo ? n > 1 : n > 0) {   // (the place is free)
+            const int m = L::kTwo ? n - 2 : n - 1;
+            wait(kORead + (m & 1), m >> 1 & 1);
+          }
           tm_after();
           const uint64_t q = tile_desc(base + L::kOffQ + Qr::place(n) * L::kTk);
 #pragma unroll
-          for (int k = 0; k < KD / 16; ++k) umma(tm + L::kColO1, q + kAlong(k), s + k * 16, kRows, k > 0);
-          umma_commit(bar(kO1Done));
+          for (int k = 0; k < KD / 16; ++k) umma(tm + L::col_o1(n), q + kAlong(k), s + k * 16, kRows, k > 0);
+          umma_commit(bar(kO1Done + (n & 1)));
           umma_commit(bar(kQEmpty + Qr::place(n)));
         }
         wait(kVFull + Vr::place(n), Vr::parity(n));
-        wait(kWReady, n & 1);
+        wait(kWReady + (n & 1), n >> 1 & 1);
         tm_after();
         const uint64_t kt = tile_desc(base + L::kOffK + Kr::place(n) * L::kTk), vt = tile_desc(base + L::kOffV + Vr::place(n) * L::kTv);
         if constexpr (L::kPieces == 3)
@@ -745,7 +778,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         umma_commit(bar(kVEmpty + Vr::place(n)));
       }
       // (nothing of this block's products is on its way when it ends)
-      wait(kVEmpty + Vr::place(chunks - 1), Vr::parity(chunks - 1));
+      if (chunks) wait(kVEmpty + Vr::place(chunks - 1), Vr::parity(chunks - 1));
     }
     __syncwarp();
   }

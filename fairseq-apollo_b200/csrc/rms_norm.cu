@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads) rms_fwd_kernel(const Rms a, int lane
 }
 
 template <typename T, int kRowWarps, int kHeld, bool kRes, bool kSplit>
-__global__ void __launch_bounds__(kThreads) rms_bwd_kernel(const Rms a, int lanes) {
+__global__ void __launch_bounds__(kThreads, kHeld <= 4 ? 2 : 1) rms_bwd_kernel(const Rms a, int lanes) {
   constexpr int kV = kVals<T>, kStep = 32 * kRowWarps;
   __shared__ float smem[4][kWarps];
   extern __shared__ float sums[];   // kRowWarps == 1: [kHeld * 32 * kV]
@@ -350,7 +350,7 @@ struct Layout {
   int row_warps, held, lanes, groups;
   bool split;
 };
-Layout layout_of(int size, int D, int groups) {
+Layout layout_of(int size, int D, int groups, bool back) {
   const int v = 16 / size, n = D / groups, gp = n / v;
   if (n % v || (groups > 1 && D % v)) return {0, 0, 32, 1, false};
   auto held = [&](int pieces, int per) {
@@ -358,9 +358,12 @@ Layout layout_of(int size, int D, int groups) {
     return need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need <= 8 ? 8 : 0;
   };
   const int all = D / v;
-  if (groups > 1 && gp <= 32 && (gp & (gp - 1)) == 0 && all <= 8 * 32) return {1, held(all, 32), gp, 1, true};
+  // The backward holds three arrays and a row's share of dw: beyond four pieces to a thread that leaves a block of eight warps to a
+  // multiprocessor, so there a row is a block's (2048 channels in 16 bits: one piece to a thread).
+  const int most = back ? 4 : 8;
+  if (groups > 1 && gp <= 32 && (gp & (gp - 1)) == 0 && all <= most * 32) return {1, held(all, 32), gp, 1, true};
   if (groups > 1 && gp < 16) return {0, 0, 32, 1, false};
-  if (gp <= 8 * 32) return {1, held(gp, 32), 32, groups, false};
+  if (gp <= most * 32) return {1, held(gp, 32), 32, groups, false};
   if (gp <= 8 * kThreads) return {kWarps, held(gp, kThreads), 32, groups, false};
   return {0, 0, 32, 1, false};
 }
@@ -402,7 +405,8 @@ void dispatch(const Rms& a, const Layout& l, bool back, int blocks, void* stream
       default: return go<T, 1, 8>(a, l, back, blocks, stream);
     }
   }
-  switch (l.held) {   // (a row that a warp cannot hold has more than one piece to a thread)
+  switch (l.held) {
+    case 1: return go<T, kWarps, 1>(a, l, back, blocks, stream);
     case 2: return go<T, kWarps, 2>(a, l, back, blocks, stream);
     case 4: return go<T, kWarps, 4>(a, l, back, blocks, stream);
     default: return go<T, kWarps, 8>(a, l, back, blocks, stream);
@@ -442,7 +446,7 @@ extern "C" MEGA_API int mega_rms_norm_fwd(const void* x, const void* residual, v
   Rms a = base(B, L, D, num_groups, weight, eps);
   a.x = x, a.res = residual, a.y = y, a.sum = sum;
   a.xb = xsb, a.xl = xsl, a.rb = rsb, a.rl = rsl, a.yb = ysb, a.yl = ysl, a.sb = ssb, a.sl = ssl;
-  const Layout l = layout_of(size, D, num_groups);
+  const Layout l = layout_of(size, D, num_groups, false);
   const bool wide = l.held && rows16(x, xsb, xsl, size) && rows16(y, ysb, ysl, size) && aligned_to(weight, 16) &&
                     (!residual || (rows16(residual, rsb, rsl, size) && rows16(sum, ssb, ssl, size)));
   if (wide) {
@@ -465,7 +469,7 @@ extern "C" MEGA_API int mega_rms_norm_bwd(const void* dy, const void* dr, const 
   Rms a = base(B, L, D, num_groups, weight, eps);
   a.x = r, a.dy = dy, a.dr = dr, a.y = dx, a.dw = static_cast<float*>(work);
   a.xb = rsb, a.xl = rsl, a.yb = dsb, a.yl = dsl, a.gb = gsb, a.gl = gsl, a.hb = rgsb, a.hl = rgsl;
-  const Layout l = layout_of(size, D, num_groups);
+  const Layout l = layout_of(size, D, num_groups, true);
   const bool wide = l.held && rows16(r, rsb, rsl, size) && rows16(dx, dsb, dsl, size) && rows16(dy, gsb, gsl, size) && aligned_to(weight, 16) &&
                     (!dr || rows16(dr, rgsb, rgsl, size));
   int blocks;

@@ -248,6 +248,25 @@ def test_long_sequences_in_segments(dtype, b, n, h, kd, vd, reverse):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kd,vd", [(64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("b,n,h", [(1, 2100, 16), (8, 1200, 16), (3, 640, 60)])
+def test_many_heads(kd, vd, b, n, h):
+    """enough heads to fill the device, or segments of several chunks: calls one after another, each head as if by itself, no wait given up"""
+    q, k, v, f, hin, dy, dh = _inputs("bf16", b, n, h, kd, vd, shift=4.0)
+    pad = torch.arange(n, device="cuda")[None] >= torch.randint(n // 3, n + 1, (b, 1), device="cuda")
+    outs = [run(q, k, v, f, hin, pad, None, 0.1, False, dy, dh) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    for other in outs[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(outs[0], other))
+    part = slice(h - 2, h)
+    cut = [t[:1, :, part] for t in (q, k, v, f)]
+    ref, bound = reference(*cut, hin[:1, part], pad[:1], None, 0.1, False, dy[:1, :, part], dh[:1, part])
+    got = [outs[0][i][:1, part] if i in (1, 6) else outs[0][i][:1, :, part] for i in range(7)]
+    check(got, ref, bound, torch.bfloat16, kd, vd)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_parts_of_a_sequence_and_single_steps(dtype):
     """a sequence in two calls and in steps is the sequence in one, and the running state may be written in place"""
