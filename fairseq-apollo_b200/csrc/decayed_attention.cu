@@ -14,6 +14,12 @@
 // q_i . dq_i and k_j . dk_j of the parts that come from states, the last is the product of both states, for which the walk of dq leaves
 // every chunk's state in the activations' type.  Nothing is carried from chunk to chunk, where roundings would pile up.
 //
+// This file: chunks of 64 steps on mma.sync, for fp32 (three products of TF32 pieces for each), heads of more than 128 keys or values, operands
+// that TMA cannot address, and short calls; everything else goes to the form on tcgen05 (decayed_attention_tc.cu).  A block of four warps
+// has 64 (32) values of a head; the state stays in its registers in fp32, the next chunk is on its way by cp.async.  What bounds it: the
+// rate of mma.sync with few warps to a multiprocessor (8 x 4096 x 16 heads of 64 in bf16 328 us, the time to move q, k, v, y is 41;
+// fp32, 4 x 2805 x 7 heads of 50 x 83, rows on 4- and 8-byte boundaries, 370 us for 13).
+//
 // Resets (and gates so closed that their decay is zero in fp32) are counted rather than summed: a pair with another count between
 // its steps has no weight.  Padded steps keep the state and have zeros for keys and values.
 #include <algorithm>
@@ -713,6 +719,10 @@ int check_args(const mega_decayed_attention_args* a) {
   for (const void* p : {a->q, a->k, a->v, (const void*)a->y, a->dy, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
     if (!aligned_to(p, size)) return MEGA_ERR_ALIGN;
   if (!aligned_to(a->f, elem_size(a->gate_dtype)) || !aligned_to(a->df, elem_size(a->gate_dtype))) return MEGA_ERR_ALIGN;
+  for (const float* p : {a->h_in, (const float*)a->h_out, a->dh_out, (const float*)a->dh_in})
+    if (!aligned_to(p, 4)) return MEGA_ERR_ALIGN;
+  const size_t state = (size_t)a->B * a->H * a->K * a->V;
+  if (overlap(a->h_in, a->h_out, state) || overlap(a->dh_out, a->dh_in, state)) return MEGA_ERR_UNSUPPORTED;
   return MEGA_OK;
 }
 void put_out(Walk& w, const mega_decayed_attention_args& a, void* p, const int64_t* s) {

@@ -16,7 +16,14 @@
 // Activations lie as TMA leaves them (columns of 64, rows of 128 bytes, swizzled), what the threads write as planes of 16 bytes along
 // keys or values, rows one after another.  Both serve with either axis as the contraction, and a thread that owns a row reads and
 // writes it without bank conflicts.  (Loads by cp.async, three warps of them, took 140 cycles each and held up every other access to
-// shared memory: 213 us where this takes LATER, 8 x 4096 x 16 heads of 64.)
+// shared memory: they were what bounded it: 209 us, by TMA 135, 8 x 4096 x 16 heads of 64.)
+//
+// Measured (8 sequences x 4096 steps x 16 heads in bf16, forward, no padding): heads of 64 89 us, 3.0 TB/s of q, k, v and y; of 128
+// 149 us, 3.6 TB/s; the products of chunks on mma.sync (decayed_attention.cu) 328 and 585 us.  What bounds it: a chunk of 64 x 64 heads
+// takes 4000 cycles, its loads 1300, its products 1900; 6500 warp instructions at 1.2 a cycle and the exchanges between roles (250 cycles
+// a wait) are the rest.  Heads of 128 also saturate shared memory: products read 350 KB of operands a chunk at 128 bytes a cycle, and
+// the pieces of keys are 100 KB more (two pieces instead of three: 138 us for 152).  Steps on the way: gates by a kernel before (123 -> 101
+// us at 64), two places for pairs (101 -> 91), products from two warps (91 -> 88).
 //
 // The state is accumulated by each chunk's own sum, which is then added in fp32: a long chain inside the tensor cores' accumulator
 // would be cut off, not rounded, thousands of times.
@@ -111,14 +118,16 @@ struct Lay {
   // places of each operand, as shared memory has room
   static constexpr bool kSmall = KD == 64 && VD == 64;
   static constexpr int kQs = kSmall ? 3 : KD == 64 ? (kDots ? 2 : 3) : 1, kKs = kSmall ? 3 : KD == 64 && !kDots ? 3 : 2,
-                       kVs = kSmall ? 3 : kBig && (kDots || kPieces == 3) ? 1 : 2, kXs = kSmall ? 2 : 1;
+                       kVs = kSmall ? 3 : kBig && kPieces == 3 ? 1 : 2, kXs = kSmall ? 2 : 1;
+  static constexpr bool kX = kDots && !kBig;   // x by way of shared memory; else each thread reads its half of a row itself (with one place
+                                               // for values instead, the walks of dq and dk took 235 us for 207, 8 x 4096 x 16 heads)
   static constexpr int kThreads = 640;   // 8 warps of pairs and outputs, 8 of weights and state, loads, padding, products (2)
   // Registers of a thread: 96 at launch, 20 warps; where the state takes 64 of them its eight warps have 128, the first eight 88 and
   // the last four 48: 2 x 88 + 2 x 128 + 48 for each four warps, as at launch (5 x 96).
   static constexpr int kRegs = 96;
   static constexpr bool kMove = VD == 128;
   static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 ? kTk : 0), kOffV = kOffK + kKs * kTk,
-                       kOffQ = kOffV + kVs * kTv, kOffX = kOffQ + (kOut ? kQs * kTk : 0), kOffS = kOffX + (kDots ? kXs * kTv : 0),
+                       kOffQ = kOffV + kVs * kTv, kOffX = kOffQ + (kOut ? kQs * kTk : 0), kOffS = kOffX + (kX ? kXs * kTv : 0),
                        kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8, kEnd = kOffSlot + 16;
   static_assert(kEnd <= 227 * 1024, "shared memory");
   // Columns of tensor memory.  Where they suffice pairs have two places: those of the next chunk are worked on while this one's outputs
@@ -178,6 +187,11 @@ struct Ring {
   static __device__ __forceinline__ int place(int n) { return n % S; }
   static __device__ __forceinline__ uint32_t parity(int n) { return n / S & 1; }
 };
+template <int N>
+__device__ __forceinline__ void tm_load(uint32_t at, float* v) {
+  if constexpr (N == 32) tm_ld32(at, v);
+  else tm_ld16(at, v);
+}
 template <int N>
 __device__ __forceinline__ void loaded(float (&v)[N]) {   // (the registers of a load from tensor memory, once it has been waited for)
 #pragma unroll
@@ -298,7 +312,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   if (warp == 16 && umma_elect()) {
     prefetch_tensormap(&maps.k), prefetch_tensormap(&maps.v);
     if (kOut) prefetch_tensormap(&maps.q);
-    if (kDots) prefetch_tensormap(&maps.x);
+    if (L::kX) prefetch_tensormap(&maps.x);
   }
   if (warp == 0) tm_alloc(smem_u32(slot_), kOut ? 512 : 128);
   tm_before();
@@ -374,9 +388,11 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         done(kGEmpty + (n & 1));
       }
     } else {
+      constexpr int kW = 32;   // columns at a time (sixteen take longer: 94 us for 86, 8 x 4096 x 16 heads of 64)
       const int rb = warp & 3, half = warp >> 2, i = rb * 32 + lane;   // a row, and half of its pairs and of its outputs
       const uint32_t quarter = tm + ((uint32_t)(rb * 32) << 16);
       float e_next = 0.f;
+      bool live = false;   // (read by the thread itself, x of a padded step must not count)
       auto pairs = [&](int n) {
         const TcGates& g = gates(n);
         wait(kGFull + (n & 1), n >> 1 & 1);
@@ -384,29 +400,22 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         const float gi = g.base[rb] + 0x1p-18f * (float)ri;
         const int ci = g.count[i];
         e_next = ci ? 0.f : w.o_scale * ex2(gi);
+        live = !(g.pad[rb] >> lane & 1);
         wait(kPDone + (n & 1), n >> 1 & 1);
         tm_after();
         const int from = max(w.rev ? rb : 0, 2 * half), to = min(w.rev ? 3 : rb, 2 * half + 1);   // blocks of 32 steps that these rows see
-        auto put = [&](int jb, const float (&v)[32]) {
-          uint32_t word[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) word[j] = pack<T>(v[2 * j], v[2 * j + 1]);
-          const uint32_t to = quarter + L::col_p(n) + 64 * half + 16 * (jb & 1);   // (in the place of pairs that this warp has read)
-          tm_st8(to, word);
-          tm_st8(to + 8, word + 8);
-        };
-        auto block = [&](int jb) {
-          float v[32];
-          tm_ld32(quarter + L::col_p(n) + 32 * jb, v);
-          // (one factor above one and one below where the row lies inside the 32 steps: their product is what counts, while both are in range)
-          const int end = last_of(w, jb);
-          // (inside the 32 steps the row's factor is one over its own as a column: both walks' weights agree to two units, however large the sums)
+        // kW pairs of a row
+        auto block = [&](int jb, int k) {
+          float v[kW];
+          tm_ld32(quarter + L::col_p(n) + 32 * jb + k, v);
+          // (one factor above one and one below where the row lies inside the 32 steps: their product is what counts, while both are in range.
+          // The row's is then one over its own as a column: both walks' weights agree to two units, however large the sums.)
+          const int end = last_of(w, jb), j0 = 32 * jb + k;
           const float col = g.col[i];
           const float f = g.count[end] != ci || (jb == rb && col == 0.f) ? 0.f : jb == rb ? __fdividef(w.p_scale, col) : w.p_scale * ex2(gi - g.base[jb]);
-          const bool apart = jb == rb && g.apart[jb];
-          float4 c[8];
+          float4 c[kW / 4];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) c[j] = *reinterpret_cast<const float4*>(g.col + 32 * jb + 4 * j);
+          for (int j = 0; j < kW / 4; ++j) c[j] = *reinterpret_cast<const float4*>(g.col + j0 + 4 * j);
           const f32x2 ff = pack2(f, f);
           tm_wait_ld();
           loaded(v);
@@ -415,33 +424,38 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           if constexpr (kDots != 0)
             if (jb == rb)
 #pragma unroll
-              for (int j = 0; j < 32; ++j) own = j == lane ? v[j] * w.p_scale : own;
-          if (!apart) {
+              for (int j = 0; j < kW; ++j) own = j == lane - k ? v[j] * w.p_scale : own;
+          if (jb != rb || !g.apart[jb]) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < kW / 4; ++j) {
               unpack2(mul2(pack2(v[4 * j], v[4 * j + 1]), mul2(ff, pack2(c[j].x, c[j].y))), v[4 * j], v[4 * j + 1]);
               unpack2(mul2(pack2(v[4 * j + 2], v[4 * j + 3]), mul2(ff, pack2(c[j].z, c[j].w))), v[4 * j + 2], v[4 * j + 3]);
             }
           } else {   // resets among these steps, or a decay by more than 2^-100: a power of two for each pair
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float p = v[j] * (w.p_scale * ex2(0x1p-18f * (float)min(ri - g.rel[32 * jb + j], 0)));
-              v[j] = g.count[32 * jb + j] == ci ? p : 0.f;
+            for (int j = 0; j < kW; ++j) {
+              const float p = v[j] * (w.p_scale * ex2(0x1p-18f * (float)min(ri - g.rel[j0 + j], 0)));
+              v[j] = g.count[j0 + j] == ci ? p : 0.f;
             }
           }
           if (jb == rb) {
-            const uint32_t seen = w.rev ? ~0u << lane : ~0u >> (31 - lane);
+            const uint32_t seen = (w.rev ? ~0u << lane : ~0u >> (31 - lane)) >> k;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = seen & (1u << j) ? v[j] : 0.f;
+            for (int j = 0; j < kW; ++j) v[j] = seen & (1u << j) ? v[j] : 0.f;
             if constexpr (kDots != 0)
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = j == lane ? own : v[j];
+              for (int j = 0; j < kW; ++j) v[j] = j == lane - k ? own : v[j];
           }
-          put(jb, v);
+          uint32_t word[kW / 2];
+#pragma unroll
+          for (int j = 0; j < kW / 2; ++j) word[j] = pack<T>(v[2 * j], v[2 * j + 1]);
+          const uint32_t to = quarter + L::col_p(n) + 64 * half + 16 * (jb & 1) + k / 2;   // (in the place of pairs that this warp has read)
+#pragma unroll
+          for (int j = 0; j < kW / 2; j += 8) tm_st8(to + j, word + j);
         };
         {
 #pragma unroll 1
-          for (int jb = from; jb <= to; ++jb) block(jb);
+          for (int j = 32 * from; j < 32 * to + 32; j += kW) block(j / 32, j % 32);
           const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
           for (int jb = 2 * half; jb < 2 * half + 2; ++jb)
@@ -458,31 +472,41 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       auto outputs = [&](int n, float e) {
         const long long t = (long long)tile_of(n) * kC + i;
         float read = 0.f, inner = 0.f;
-        if (kDots) wait(kXFull + Xr::place(n), Xr::parity(n));
+        constexpr int kUnroll = kDots && !L::kX ? 4 : 1, kHalf = VD / 2, kO = kDots && !L::kX ? 16 : kW;
+        uint4 xr[kDots && !L::kX ? kHalf / 8 : 1];
+        if constexpr (kDots && !L::kX) {
+          const T* xp = static_cast<const T*>(w.x.p) + b * w.x.sb + h * w.x.sh + t * w.x.sl + half * kHalf;
+#pragma unroll
+          for (int m = 0; m < kHalf / 8; ++m)
+            xr[m] = live && t < w.L && half * kHalf + 8 * m < w.x.d ? __ldg(reinterpret_cast<const uint4*>(xp) + m) : make_uint4(0, 0, 0, 0);
+        } else if (kDots) {
+          wait(kXFull + Xr::place(n), Xr::parity(n));
+        }
         wait(kODone, n & 1);
         wait(kO1Done + (n & 1), n >> 1 & 1);
         tm_after();
         char* row = static_cast<char*>(w.out) + (b * w.ob + h * w.oh + t * w.ol) * 2;
-#pragma unroll 1
-        for (int c = half * (VD / 2); c < (half + 1) * (VD / 2); c += 32) {
-          float o[32], p[32];
-          tm_ld32(quarter + L::col_o1(n) + c, o);
-          tm_ld32(quarter + L::kColO2 + c, p);
-          uint4 u[kDots ? 4 : 1];
+#pragma unroll kUnroll
+        for (int c0 = 0; c0 < kHalf; c0 += kO) {
+          const int c = half * kHalf + c0;
+          float o[kO], p[kO];
+          tm_load<kO>(quarter + L::col_o1(n) + c, o);
+          tm_load<kO>(quarter + L::kColO2 + c, p);
+          uint4 u[kDots ? kO / 8 : 1];
           if constexpr (kDots != 0)
 #pragma unroll
-            for (int m = 0; m < 4; ++m) u[m] = lds16(base + L::kOffX + Xr::place(n) * L::kTv + piece_of(i, c / 8 + m));
+            for (int m = 0; m < kO / 8; ++m) u[m] = kDots && !L::kX ? xr[kDots && !L::kX ? c0 / 8 + m : 0] : lds16(base + L::kOffX + Xr::place(n) * L::kTv + piece_of(i, c / 8 + m));
           tm_wait_ld();
           loaded(o);
           loaded(p);
-          if (c + 32 >= (half + 1) * (VD / 2)) {
+          if (c0 + kO >= kHalf) {
             tm_before();
             done(kORead + (n & 1));
           }
-          uint32_t word[16];
+          uint32_t word[kO / 2];
           const f32x2 ee = pack2(e, e);
 #pragma unroll
-          for (int m = 0; m < 16; ++m) {
+          for (int m = 0; m < kO / 2; ++m) {
             f32x2 y;
             if constexpr (kDots != 0) {
               const f32x2 own = mul2(ee, pack2(o[2 * m], o[2 * m + 1]));
@@ -502,20 +526,20 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           if (t < w.L) {
             if (w.piece == 32) {
 #pragma unroll
-              for (int m = 0; m < 16; m += 8)
+              for (int m = 0; m < kO / 2; m += 8)
                 if (c + 2 * m < w.v.d)
                   asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(row + (c + 2 * m) * 2), "r"(word[m]),
                                "r"(word[m + 1]), "r"(word[m + 2]), "r"(word[m + 3]), "r"(word[m + 4]), "r"(word[m + 5]), "r"(word[m + 6]), "r"(word[m + 7])
                                : "memory");
             } else {
 #pragma unroll
-              for (int m = 0; m < 16; m += 4)
+              for (int m = 0; m < kO / 2; m += 4)
                 if (c + 2 * m < w.v.d) *reinterpret_cast<uint4*>(row + (c + 2 * m) * 2) = make_uint4(word[m], word[m + 1], word[m + 2], word[m + 3]);
             }
           }
         }
         if (kDots) {
-          done(kXEmpty + Xr::place(n));
+          if (L::kX) done(kXEmpty + Xr::place(n));
           if (t < w.L) w.dots[((long long)half * w.B * w.H + bh) * w.L + t] = make_float2(read, inner);
         }
       };
@@ -674,7 +698,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         uint64_t* const got = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1);
         mbar_expect_tx(got, sizeof(TcGates));
         bulk_load_1d(&gates(n), table + tile_of(n), sizeof(TcGates), got);
-        if (kDots) {
+        if (L::kX) {
           if (n >= L::kXs) wait(kXEmpty + Xr::place(n), Xr::parity(n) ^ 1);
           load_tile<VD>(base + L::kOffX + Xr::place(n) * L::kTv, &maps.x, w.x, t0, h, b, bar((raw ? kXRaw : kXFull) + Xr::place(n)));
         }
@@ -696,7 +720,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
 #pragma unroll 1
         for (int k = 0; k < 4; ++k) {   // keys, queries, values, x (and x before values where those have one place)
           const int what = k < 2 ? k : L::kVs == 1 ? 5 - k : k;
-          if ((what == 1 && !kOut) || (what == 3 && !kDots)) continue;
+          if ((what == 1 && !kOut) || (what == 3 && !L::kX)) continue;
           const int place = what == 0 ? Kr::place(n) : what == 1 ? Qr::place(n) : what == 2 ? Vr::place(n) : Xr::place(n);
           const int raw = (what == 0 ? kKRaw : what == 1 ? kQRaw : what == 2 ? kVRaw : kXRaw) + place;
           const int full = (what == 0 ? kKFull : what == 1 ? kQFull : what == 2 ? kVFull : kXFull) + place;
@@ -836,6 +860,9 @@ bool maps_of(Maps* m, int dtype, const Walk& w) {
 }  // namespace
 
 bool tc_takes(int dtype, const Walk& w) {
+  // A call of up to 64 steps is half a chunk here and one of the other form: 72 us for 34, 64 sequences x 64 steps x 16 heads of 64, 18.6 for
+  // 12.1 with one sequence; at 300 steps it is 23 for 33, at 8 x 1024 33 for 91.
+  if (w.L <= kTcChunk / 2) return false;
   if (dtype == MEGA_F32 || g_options[OPT_DISABLE_MMA].load() || w.piece < 16) return false;
   for (const Operand* o : {&w.q, &w.k, &w.v, &w.x})
     if (o->p && (o->d > kTcMost || o->vec < 16 || o->sl < 0 || o->sh < 0 || o->sb < 0 || (o->sl == 0 && w.L > 1))) return false;

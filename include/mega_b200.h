@@ -689,7 +689,8 @@ MEGA_API int mega_group_norm_bwd(const void* dy, const void* x, void* dx, int dt
  * Strides are in elements, (sequence, step, head), the last axis is contiguous; those of what is read are free, 0 and negative
  * ones among them, outputs overlap neither one another nor an input.  q, k, v, y, dy and their gradients are of `dtype`, f and df
  * of `gate_dtype`: MEGA_F32 or `dtype`.  Masks are (B, L) uint8.  h_in, h_out, dh_out, dh_in are (B, H, K, V) fp32, contiguous; either
- * may be NULL (a NULL h_in or dh_out is zero), h_out may be h_in, dh_in may be dh_out.  K and V are at most MEGA_ATT_MOST
+ * may be NULL (a NULL h_in or dh_out is zero).  mega_decayed_attention_step may write h_out over h_in; elsewhere states that overlap are
+ * refused (MEGA_ERR_UNSUPPORTED: a segment of a sequence may still read the one while another has written the other).  K and V are at most MEGA_ATT_MOST
  * (MEGA_ERR_UNSUPPORTED).
  * `work`: device memory of mega_decayed_attention_work() bytes, 16-byte aligned, used by this call alone until it is done (may be
  * NULL where that is 0).

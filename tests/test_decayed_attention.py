@@ -524,6 +524,11 @@ def test_refusals_on_the_host():
         assert lib.mega_decayed_attention_fwd(ctypes.byref(a), None) == status, key
         setattr(a, key, good[key])
     assert lib.mega_decayed_attention_bwd(ctypes.byref(a), None) == 1
+    a.h_in = a.h_out = 64       # states that overlap: another segment may still read what one has written
+    assert lib.mega_decayed_attention_fwd(ctypes.byref(a), None) == 7
+    a.h_out = 66
+    assert lib.mega_decayed_attention_fwd(ctypes.byref(a), None) == 5
+    a.h_in = a.h_out = None
     assert lib.mega_decayed_attention_step(ctypes.byref(a), None) == 3
     a.L = 1
     assert lib.mega_decayed_attention_step(ctypes.byref(a), None) == 1
