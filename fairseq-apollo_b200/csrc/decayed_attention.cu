@@ -107,7 +107,7 @@ struct Mma {
     ldsm4t(r, smem_u32(s + (k0 + (lane & 15)) * ld + n0 + (lane >> 4) * 8));
     b[0].r[0] = r[0], b[0].r[1] = r[1], b[1].r[0] = r[2], b[1].r[1] = r[3];
   }
-  static __device__ __forceinline__ void go(float* c, const A& a, const B& b) { mma16(c, a.r, b.r, T()); }
+  static __device__ __forceinline__ void go(float* c, float*, const A& a, const B& b) { mma16(c, a.r, b.r, T()); }
   // results of 16 columns as A
   static __device__ __forceinline__ void from(A& a, const float (*c)[4]) {
     a.r[0] = pack<T>(c[0][0], c[0][1]), a.r[1] = pack<T>(c[0][2], c[0][3]);
@@ -166,9 +166,11 @@ struct Mma<float> {
 #pragma unroll
     for (int i = 0; i < 2; ++i) tf32_split(p[8 * i], b[i].h[0], b[i].l[0]), tf32_split(p[ld + 8 * i], b[i].h[1], b[i].l[1]);
   }
-  static __device__ __forceinline__ void go(float* c, const A& a, const B& b) {
-    mma8(c, a.l, b.h);
-    mma8(c, a.h, b.l);
+  // The products with a small piece have a sum of their own, x: the accumulator is cut off at each step, at the size of what it holds
+  // (4 x 2805 x 7 heads of 50 x 83: outputs 1.0e-6 from 64 bits with one sum, 3.7e-7 with two)
+  static __device__ __forceinline__ void go(float* c, float* x, const A& a, const B& b) {
+    mma8(x, a.l, b.h);
+    mma8(x, a.h, b.l);
     mma8(c, a.h, b.h);
   }
   static __device__ __forceinline__ void from(A& a, const float (*c)[4]) {
@@ -243,6 +245,26 @@ __device__ __forceinline__ void gates_put(const Walk& w, Gates& o, const GateIn<
   }
   if (lane == 0) o.enter = r.enter, o.padded = r.padded;
 }
+
+// A second sum beside `c` (fp32: see Mma<float>::go), which is added to it at the end; 16-bit types have none
+template <typename T, int N>
+struct Beside {
+  float x[sizeof(T) == 4 ? N : 1][4];
+  __device__ __forceinline__ Beside() {
+#pragma unroll
+    for (int n = 0; n < (sizeof(T) == 4 ? N : 1); ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][i] = 0.f;
+  }
+  __device__ __forceinline__ float* of(int n) { return x[sizeof(T) == 4 ? n : 0]; }
+  __device__ __forceinline__ void join(float (*c)[4]) {
+    if constexpr (sizeof(T) == 4)
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[n][i] += x[n][i];
+  }
+};
 
 template <typename T, int KD, int VT, int STAGES, bool kX>
 struct Shared {
@@ -387,24 +409,47 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
       for (int n = 0; n < kC / 8; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[n][i] = 0.f;
+      constexpr bool kApart = sizeof(T) == 4;   // (fp32: one after the other, as each has a second sum)
+      {
+        Beside<T, kN> small;
 #pragma unroll 4
-      for (int k0 = 0; k0 < KD; k0 += M::kStep) {
-        typename M::A a;
-        typename M::B bb[2];
-        M::a_rows(a, qs, kLk, warp * 16, k0, lane);
+        for (int k0 = 0; k0 < KD; k0 += M::kStep) {
+          typename M::A a;
+          typename M::B bb[2];
+          M::a_rows(a, qs, kLk, warp * 16, k0, lane);
 #pragma unroll
-        for (int n = 0; n < kN; n += 2) {
-          M::b_cols(bb, sh.s, kLv, n * 8, k0, lane);
-          M::go(o[n], a, bb[0]);
-          M::go(o[n + 1], a, bb[1]);
-        }
-#pragma unroll
-        for (int n = 0; n < kC / 8; n += 2)
-          if (w.rev ? n / 2 >= warp : n / 2 <= warp) {
-            M::b_rows(bb, ks, kLk, n * 8, k0, lane);
-            M::go(p[n], a, bb[0]);
-            M::go(p[n + 1], a, bb[1]);
+          for (int n = 0; n < kN; n += 2) {
+            M::b_cols(bb, sh.s, kLv, n * 8, k0, lane);
+            M::go(o[n], small.of(n), a, bb[0]);
+            M::go(o[n + 1], small.of(n + 1), a, bb[1]);
           }
+          if constexpr (!kApart)
+#pragma unroll
+            for (int n = 0; n < kC / 8; n += 2)
+              if (w.rev ? n / 2 >= warp : n / 2 <= warp) {
+                M::b_rows(bb, ks, kLk, n * 8, k0, lane);
+                M::go(p[n], nullptr, a, bb[0]);
+                M::go(p[n + 1], nullptr, a, bb[1]);
+              }
+        }
+        small.join(o);
+      }
+      if constexpr (kApart) {
+        Beside<T, kC / 8> small;
+#pragma unroll 2
+        for (int k0 = 0; k0 < KD; k0 += M::kStep) {
+          typename M::A a;
+          typename M::B bb[2];
+          M::a_rows(a, qs, kLk, warp * 16, k0, lane);
+#pragma unroll
+          for (int n = 0; n < kC / 8; n += 2)
+            if (w.rev ? n / 2 >= warp : n / 2 <= warp) {
+              M::b_rows(bb, ks, kLk, n * 8, k0, lane);
+              M::go(p[n], small.of(n), a, bb[0]);
+              M::go(p[n + 1], small.of(n + 1), a, bb[1]);
+            }
+        }
+        small.join(p);
       }
       const int i0 = warp * 16 + g, i1 = i0 + 8;
       const float h0 = gt.hi[i0], h1 = gt.hi[i1], l0 = gt.lo[i0], l1 = gt.lo[i1];
@@ -445,15 +490,17 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
             float p2[2][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) p2[0][i] = p2[1][i] = 0.f;
+            Beside<T, 2> small;
 #pragma unroll 2
             for (int k0 = 0; k0 < VT; k0 += M::kStep) {
               typename M::A a;
               typename M::B bb[2];
               M::a_rows(a, sh.x, kLv, warp * 16, k0, lane);
               M::b_rows(bb, vs, kLv, n * 8, k0, lane);
-              M::go(p2[0], a, bb[0]);
-              M::go(p2[1], a, bb[1]);
+              M::go(p2[0], small.of(0), a, bb[0]);
+              M::go(p2[1], small.of(1), a, bb[1]);
             }
+            small.join(p2);
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -472,6 +519,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
         if (t4 == 0 && t0 + i1 < w.L) d[i1] = make_float2(dot[1], dot[3]);
       }
       // ---- weighted pairs times values
+      Beside<T, kN> small;
 #pragma unroll
       for (int k0 = 0; k0 < kC; k0 += M::kStep)
         if (w.rev ? k0 / 16 >= warp : k0 / 16 <= warp) {
@@ -481,10 +529,11 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
 #pragma unroll
           for (int n = 0; n < kN; n += 2) {
             M::b_cols(bb, vs, kLv, n * 8, k0, lane);
-            M::go(o[n], a, bb[0]);
-            M::go(o[n + 1], a, bb[1]);
+            M::go(o[n], small.of(n), a, bb[0]);
+            M::go(o[n + 1], small.of(n + 1), a, bb[1]);
           }
         }
+      small.join(o);
       // ---- outputs
       T* op = static_cast<T*>(w.out) + b * w.ob + h * w.oh + tile * VT;
 #pragma unroll
@@ -528,6 +577,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
         for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) add[n][i] = 0.f;
+        Beside<T, kN> small;
 #pragma unroll
         for (int k0 = 0; k0 < kC; k0 += M::kStep) {
           typename M::A a[M::kPieces];
@@ -538,11 +588,12 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
             M::b_cols(bb, vs, kLv, n * 8, k0, lane);
 #pragma unroll
             for (int p = M::kPieces - 1; p >= 0; --p) {   // (small ones first)
-              M::go(add[n], a[p], bb[0]);
-              M::go(add[n + 1], a[p], bb[1]);
+              M::go(add[n], small.of(n), a[p], bb[0]);
+              M::go(add[n + 1], small.of(n + 1), a[p], bb[1]);
             }
           }
         }
+        small.join(add);
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -693,7 +744,7 @@ template <typename T>
 void run_keys(const Walk& w, int dots, void* stream) {
   switch (key_tile(w.k.d)) {
     case 32: return run_walk<T, 32, 64, 2>(w, dots, stream);
-    case 64: return run_walk<T, 64, 64, 2>(w, dots, stream);
+    case 64: return run_walk<T, 64, 64, sizeof(T) == 4 ? 1 : 2>(w, dots, stream);   // (ONE)
     case 128: return run_walk<T, 128, 64, 2>(w, dots, stream);
     default: return run_walk<T, 256, 32, sizeof(T) == 4 ? 1 : 2>(w, dots, stream);
   }
