@@ -18,7 +18,7 @@
 // that TMA cannot address, and short calls; everything else goes to the form on tcgen05 (decayed_attention_tc.cu).  A block of four warps
 // has 64 (32) values of a head; the state stays in its registers in fp32, the next chunk is on its way by cp.async.  What bounds it: the
 // rate of mma.sync with few warps to a multiprocessor (8 x 4096 x 16 heads of 64 in bf16 328 us, the time to move q, k, v, y is 41;
-// fp32, 4 x 2805 x 7 heads of 50 x 83, rows on 4- and 8-byte boundaries, 370 us for 13).
+// fp32, 4 x 2805 x 7 heads of 50 x 83, rows on 4- and 8-byte boundaries, 284 us for 13).
 //
 // Resets (and gates so closed that their decay is zero in fp32) are counted rather than summed: a pair with another count between
 // its steps has no weight.  Padded steps keep the state and have zeros for keys and values.
@@ -744,7 +744,7 @@ template <typename T>
 void run_keys(const Walk& w, int dots, void* stream) {
   switch (key_tile(w.k.d)) {
     case 32: return run_walk<T, 32, 64, 2>(w, dots, stream);
-    case 64: return run_walk<T, 64, 64, sizeof(T) == 4 ? 1 : 2>(w, dots, stream);   // (ONE)
+    case 64: return run_walk<T, 64, 64, sizeof(T) == 4 ? 1 : 2>(w, dots, stream);   // (fp32: one place, three blocks to a multiprocessor: 284 us for 381)
     case 128: return run_walk<T, 128, 64, 2>(w, dots, stream);
     default: return run_walk<T, 256, 32, sizeof(T) == 4 ? 1 : 2>(w, dots, stream);
   }
