@@ -447,7 +447,6 @@ def test_captured_calls():
 @pytest.mark.gpu
 def test_empty_calls():
     for b, n, h in ((0, 5, 2), (2, 0, 2), (2, 5, 0)):
-        q, v, f = (torch.randn(b, n, h, 8, device="cuda", requires_grad=True) for _ in range(2)).__iter__(), None, None
         q, v = [torch.randn(b, n, h, w, device="cuda", requires_grad=True) for w in (8, 4)]
         f = torch.randn(b, n, h, device="cuda", requires_grad=True)
         s = torch.randn(b, h, 8, 4, device="cuda", requires_grad=True)
