@@ -39,6 +39,15 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// A thread that has not called the runtime yet (an autograd thread's first backward, where all its memory comes from a cache) has no
+// current context, and this call of the driver's, unlike a launch, makes none: it fails, which would send the call to another form.
+template <typename... Args>
+static bool encode(EncodeTiledFn fn, Args... args) {
+  if (fn(args...) == CUDA_SUCCESS) return true;
+  int device;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && fn(args...) == CUDA_SUCCESS;
+}
+
 bool make_tensor_map_3d(CUtensorMap* out, int dtype, const void* base, uint64_t dim0, uint64_t dim1,
                         uint64_t dim2, int64_t stride1, int64_t stride2, uint32_t box0, uint32_t box1,
                         uint32_t box2, CUtensorMapSwizzle swizzle) {
@@ -56,9 +65,8 @@ bool make_tensor_map_3d(CUtensorMap* out, int dtype, const void* base, uint64_t 
   cuuint64_t strides[2] = {(cuuint64_t)stride1 * es, (cuuint64_t)stride2 * es};
   cuuint32_t box[3] = {box0, box1, box2};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(out, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode(fn, out, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 bool make_tensor_map_4d(CUtensorMap* out, int dtype, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2, uint64_t dim3,
@@ -76,8 +84,8 @@ bool make_tensor_map_4d(CUtensorMap* out, int dtype, const void* base, uint64_t 
   cuuint64_t strides[3] = {(cuuint64_t)stride1 * es, (cuuint64_t)stride2 * es, (cuuint64_t)stride3 * es};
   cuuint32_t box[4] = {box0, box1, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(out, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode(fn, out, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // ---------------------------------------------------------------------------

@@ -1,0 +1,61 @@
+"""Linear attention with a decay for each head where states, gradients or gates leave their usual range, and which form takes a call.
+
+Every test runs both forms of whole sequences (tcgen05, and mma.sync by way of the option that leaves the first one out), against the
+recurrence in 64 bits.  Tolerances are on norms: an elementwise bound adds up every share's largest error, under which a lost piece of
+an operand would not show.
+
+Outputs and gradients in 16-bit types have three roundings on their way (a pair's weight, the state that is read, the result), of which
+each is at most u = half a step of the value and together, independently of one another, sqrt(3) u / sqrt(3) = u in the mean square.
+fp16 below its normal range: half a step is 2^-25 whatever the value, for the result alone.
+
+States are fp32 sums: the products of a chunk cut their sum off up to 24 times (three pieces of eight groups of 16 steps) by at most
+2^-23 of a partial sum, half of that on average, of partial sums half as large on average: 24 * 2^-25 = 7e-7; a weight is a product of
+two powers of two and a sum of logarithms (8 * 2^-24 ln 2 + 2 * 2^-23 = 6e-7).  Together below 1.5e-6 (two pieces of bf16 keys, where
+there is room for no more: 2^-17 of a key besides).
+"""
+import threading
+
+import pytest
+import torch
+
+import fairseq_apollo_b200 as M
+from fairseq_apollo_b200 import _lib
+from test_decayed_attention import DT, _inputs, reference, run
+
+STATE = 1.5e-6
+HEADS = [(64, 64), (64, 128), (128, 64), (128, 128), (40, 24)]
+
+
+@pytest.fixture(params=["tcgen05", "mma"])
+def form(request):
+    _lib.set_option(1, int(request.param == "mma"))
+    yield request.param
+    _lib.set_option(1, 0)
+
+
+def near(got, ref, rel, step=0.0):
+    """|error| <= rel |ref| + step for every value, in the mean square"""
+    assert torch.isfinite(got).all()
+    err, allowed = float((got.detach().double() - ref).norm()), rel * float(ref.norm()) + step * ref.numel() ** 0.5
+    assert err <= allowed, (err / allowed, err / (float(ref.norm()) + 1e-300))
+
+
+@pytest.mark.gpu
+def test_a_thread_that_is_new_to_cuda_takes_the_same_form():
+    """a thread's first call, with all its memory from the allocator's cache (as an autograd thread's first backward may have it)"""
+    q, k, v, f, hin, _, _ = _inputs("bf16", 2, 300, 2, 64, 64)
+    _lib.set_option(1, 0)
+    with torch.no_grad():
+        want = M.decayed_attention(q, k, v, f, h_in=hin)
+        assert _lib.last_kernel() == "decayed_attention_tc"
+        M.decayed_attention(q, k, v, f, h_in=hin)   # (all sizes are in the cache then)
+    got = []
+
+    def first():
+        with torch.no_grad():
+            got.append(M.decayed_attention(q, k, v, f, h_in=hin))
+        got.append(_lib.last_kernel())
+    thread = threading.Thread(target=first)
+    thread.start()
+    thread.join()
+    assert got[1] == "decayed_attention_tc" and torch.equal(got[0], want)
