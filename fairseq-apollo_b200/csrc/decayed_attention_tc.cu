@@ -399,8 +399,8 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         const int ri = g.rel[i];
         const float gi = g.base[rb] + 0x1p-18f * (float)ri;
         const int ci = g.count[i];
-        e_next = ci ? 0.f : w.o_scale * ex2(gi);
         live = !(g.pad[rb] >> lane & 1);
+        e_next = ci || !live ? 0.f : w.o_scale * ex2(gi);
         wait(kPDone + (n & 1), n >> 1 & 1);
         tm_after();
         const int from = max(w.rev ? rb : 0, 2 * half), to = min(w.rev ? 3 : rb, 2 * half + 1);   // blocks of 32 steps that these rows see
@@ -486,6 +486,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         wait(kO1Done + (n & 1), n >> 1 & 1);
         tm_after();
         char* row = static_cast<char*>(w.out) + (b * w.ob + h * w.oh + t * w.ol) * 2;
+        const bool apart = __any_sync(~0u, e == 0.f);   // rows that read nothing of the state (which may be infinite: no factor)
 #pragma unroll kUnroll
         for (int c0 = 0; c0 < kHalf; c0 += kO) {
           const int c = half * kHalf + c0;
@@ -499,6 +500,9 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           tm_wait_ld();
           loaded(o);
           loaded(p);
+          if (apart)
+#pragma unroll
+            for (int m = 0; m < kO; ++m) o[m] = e == 0.f ? 0.f : o[m];
           if (c0 + kO >= kHalf) {
             tm_before();
             done(kORead + (n & 1));

@@ -59,3 +59,32 @@ def test_a_thread_that_is_new_to_cuda_takes_the_same_form():
     thread.start()
     thread.join()
     assert got[1] == "decayed_attention_tc" and torch.equal(got[0], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kd,vd", [("bf16", 64, 64), ("fp16", 64, 128), ("fp16", 128, 128), ("bf16", 128, 128), ("fp32", 64, 40)])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_states_that_are_not_finite_reach_what_reads_them_alone(form, dtype, kd, vd, reverse, value):
+    """a state that comes in reaches no step behind a reset and no padded step, the gradient of the one that leaves none before it"""
+    b, n, h = 2, 300, 2
+    q, k, v, f, hin, dy, dh = _inputs(dtype, b, n, h, kd, vd)
+    at = torch.arange(n, device="cuda")
+    at = (n - 1 - at if reverse else at)[None].expand(b, n)   # steps in the order of the walk
+    reset, pad = at == 30, ((at >= 5) & (at < 10)) | ((at >= 40) & (at < 60)) | ((at >= 130) & (at < 150))
+    before, behind = at < 30, at >= 30
+
+    def call(hin, dh):
+        return run(q, k, v, f, hin, pad, reset, 0.1, reverse, dy, dh)
+    odd = torch.full_like(hin, value)
+    want, got = call(torch.zeros_like(hin), dh), call(odd, dh)
+    assert torch.equal(got[0][behind], want[0][behind]) and float(got[0][pad].detach().abs().max()) == 0 and torch.equal(got[1], want[1])
+    for i in (2, 3, 4, 5):
+        assert torch.equal(got[i][behind], want[i][behind]), i
+        assert float(got[i][pad].abs().max()) == 0, i
+    assert torch.equal(got[6], want[6])
+    want, got = call(hin, torch.zeros_like(dh)), call(hin, odd)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2]) and torch.equal(got[6], want[6])
+    for i in (3, 4, 5):
+        assert torch.equal(got[i][before], want[i][before]), i
+        assert float(got[i][pad].abs().max()) == 0, i
