@@ -710,7 +710,7 @@ Plan plan_of(bool tc, int dtype, int B, int L, int H, int keys, int values) {
   p.tc = tc;
   const int c = tc ? kTcChunk : kC, vt = tc ? (values <= 64 ? 64 : 128) : value_tile(keys);
   const long long places = tc ? 148 : 2 * 148;
-  p.chunks = (L + c - 1) / c;
+  p.chunks = (L - 1) / c + 1;   // (L may be the largest there is)
   p.tiles = (values + vt - 1) / vt;
   const long long blocks = (long long)B * H * p.tiles;
   p.per = p.chunks;

@@ -13,6 +13,7 @@ States are fp32 sums: the products of a chunk cut their sum off up to 24 times (
 two powers of two and a sum of logarithms (8 * 2^-24 ln 2 + 2 * 2^-23 = 6e-7).  Together below 1.5e-6 (two pieces of bf16 keys, where
 there is room for no more: 2^-17 of a key besides).
 """
+import ctypes
 import threading
 
 import pytest
@@ -88,3 +89,16 @@ def test_states_that_are_not_finite_reach_what_reads_them_alone(form, dtype, kd,
     for i in (3, 4, 5):
         assert torch.equal(got[i][before], want[i][before]), i
         assert float(got[i][pad].abs().max()) == 0, i
+
+
+def test_the_longest_sequences_have_their_chunks_counted():
+    lib, a = _lib.lib(), _lib.DecayedAttentionArgs()
+    for key, value in dict(dtype=1, gate_dtype=1, B=1, H=1, K=8, V=8).items():
+        setattr(a, key, value)
+    for backward in (0, 1):
+        sizes = []
+        for length in (2 ** 31 - 256, 2 ** 31 - 1):
+            a.L = length
+            sizes.append(lib.mega_decayed_attention_work(ctypes.byref(a), backward))
+        # (a forward call has the gates of 2^24 chunks of 128 steps, 1216 bytes each)
+        assert 2 ** 24 * 1024 < sizes[0] <= sizes[1] < 1.01 * sizes[0], sizes
