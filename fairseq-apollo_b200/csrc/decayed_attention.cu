@@ -114,9 +114,10 @@ struct Mma {
     a.r[2] = pack<T>(c[1][0], c[1][1]), a.r[3] = pack<T>(c[1][2], c[1][3]);
   }
   // A = (w k)^T, rows m0.. of the keys, places of the steps k0..  The state is to keep fp32's places: the product w k goes in as pieces
-  // of 8 bits (bf16: three, 24 bits) or 11 (fp16: two, 22; a piece below fp16's normal range is a multiple of 2^-24).
+  // of 8 bits (bf16: three, 24 bits) or 11 (fp16: two, 22; scaled by `up`).
   static constexpr int kPieces = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
-  static __device__ __forceinline__ void a_weighted(A* p, const T* s, int ld, int m0, int k0, const float* w, int lane) {
+  template <typename F>
+  static __device__ __forceinline__ void each_weighted(const T* s, int ld, int m0, int k0, const float* w, int lane, F&& fn) {
     uint32_t r[4];
     ldsm4t(r, smem_u32(s + (k0 + (lane & 7) + (lane >> 4) * 8) * ld + m0 + ((lane >> 3) & 1) * 8));
     const int t = lane & 3;
@@ -126,13 +127,27 @@ struct Mma {
       float2 v = unpack<T>(r[i]);
       const float2 u = i < 2 ? w0 : w1;
       v.x *= u.x, v.y *= u.y;
+      fn(i, v);
+    }
+  }
+  // the exponent of the largest one of 16 keys and the chunk's steps
+  static __device__ __forceinline__ int largest(const T* s, int ld, int m0, const float* w, int lane) {
+    float most = 0.f;
+#pragma unroll
+    for (int k0 = 0; k0 < kC; k0 += kStep)
+      each_weighted(s, ld, m0, k0, w, lane, [&](int, const float2& v) { most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))); });
+    return (int)(__reduce_max_sync(~0u, __float_as_uint(most)) >> 23);
+  }
+  static __device__ __forceinline__ void a_weighted(A* p, const T* s, int ld, int m0, int k0, const float* w, float up, int lane) {
+    each_weighted(s, ld, m0, k0, w, lane, [&](int i, float2 v) {
+      if constexpr (kScaled<T>) v.x *= up, v.y *= up;
 #pragma unroll
       for (int n = 0; n < kPieces; ++n) {
         p[n].r[i] = pack<T>(v.x, v.y);
         const float2 h = unpack<T>(p[n].r[i]);
         v.x -= h.x, v.y -= h.y;
       }
-    }
+    });
   }
 };
 __device__ __forceinline__ void tf32_split(float v, uint32_t& hi, uint32_t& lo) {
@@ -178,7 +193,7 @@ struct Mma<float> {
     tf32_split(c[0][1], a.h[2], a.l[2]), tf32_split(c[0][3], a.h[3], a.l[3]);
   }
   static constexpr int kPieces = 1;   // (of 22 bits, as all operands)
-  static __device__ __forceinline__ void a_weighted(A* p, const float* s, int ld, int m0, int k0, const float* w, int lane) {
+  static __device__ __forceinline__ void a_weighted(A* p, const float* s, int ld, int m0, int k0, const float* w, float, int lane) {
     A& hi = *p;
     const int t = lane & 3;
     const float* f = s + (k0 + 2 * t) * ld + m0 + (lane >> 2);
@@ -578,11 +593,13 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) add[n][i] = 0.f;
         Beside<T, kN> small;
+        int up = 0;
+        if constexpr (kScaled<T>) up = scale_of(M::largest(ks, kLk, (warp * kM + m) * 16, gt.weight, lane));
 #pragma unroll
         for (int k0 = 0; k0 < kC; k0 += M::kStep) {
           typename M::A a[M::kPieces];
           typename M::B bb[2];
-          M::a_weighted(a, ks, kLk, (warp * kM + m) * 16, k0, gt.weight, lane);
+          M::a_weighted(a, ks, kLk, (warp * kM + m) * 16, k0, gt.weight, two_to(up), lane);
 #pragma unroll
           for (int n = 0; n < kN; n += 2) {
             M::b_cols(bb, vs, kLv, n * 8, k0, lane);
@@ -597,7 +614,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) st[m][n][i] = (e == 0.f ? 0.f : e * st[m][n][i]) + add[n][i];
+          for (int i = 0; i < 4; ++i) st[m][n][i] = (e == 0.f ? 0.f : e * st[m][n][i]) + (kScaled<T> ? two_to(-up) : 1.f) * add[n][i];
         if (kOut) state_to_shared<T, VT>(sh.s, kLv, (warp * kM + m) * 16, st[m], lane);
       }
     }

@@ -1,5 +1,7 @@
 // What the forms of linear attention with a decay for each head share (decayed_attention.cu has the mathematics).
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mega {
@@ -37,6 +39,15 @@ struct Walk {
 // The walk of dq leaves a chunk's state where its weight in the next one is above zero; that of dk, whose sum of the same gates may round
 // otherwise, reads it where the weight is well above.
 constexpr float kLeast = 1e-35f;
+
+// fp16 has five bits of exponent: what is rounded to it on the way to a product is first multiplied with a power of two that brings the
+// largest value to 2^14 or above, and the product's fp32 sum with its inverse.  (Weighted keys as they are would be multiples of 2^-24:
+// the state of gradients of 1e-3 was off by 7e-4, of 1e-5 by 6e-2.)  bf16 has fp32's exponents.
+template <typename T>
+constexpr bool kScaled = std::is_same<T, __half>::value;
+// the power, from the biased exponent of the largest value; what is not finite stays as it is
+__device__ __forceinline__ int scale_of(int exponent) { return exponent == 255 ? 0 : min(141 - exponent, 100); }
+__device__ __forceinline__ float two_to(int n) { return __int_as_float((127 + n) << 23); }
 
 // (gates are of the activations' type or fp32)
 template <typename T>

@@ -128,7 +128,8 @@ struct Lay {
   static constexpr bool kMove = VD == 128;
   static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 ? kTk : 0), kOffV = kOffK + kKs * kTk,
                        kOffQ = kOffV + kVs * kTv, kOffX = kOffQ + (kOut ? kQs * kTk : 0), kOffS = kOffX + (kX ? kXs * kTv : 0),
-                       kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8, kEnd = kOffSlot + 16;
+                       kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8,
+                       kOffMost = kOffSlot + 16, kEnd = kOffMost + (kScaled<T> ? 32 : 0);
   static_assert(kEnd <= 227 * 1024, "shared memory");
   // Columns of tensor memory.  Where they suffice pairs have two places: those of the next chunk are worked on while this one's outputs
   // are on their way.
@@ -156,6 +157,9 @@ __device__ __forceinline__ void wait_for(uint32_t bar, uint32_t parity, volatile
     }
 }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// `THREADS` threads, whole warps, meet
+template <int ID, int THREADS>
+__device__ __forceinline__ void named_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(THREADS) : "memory"); }
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -350,10 +354,34 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     else if (warp >= 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   }
-  // w K in pieces, of a step's `count` planes from `from` on
-  auto weigh = [&](int n, int step, int from, int count) {
+  // fp16: the power of two that w K of a chunk is multiplied with, from `count` planes of a step in each thread.  The warps of weights
+  // meet for it, each with a byte for its exponent: two sets of them in turn, as a warp may be at the next chunk while another still reads.
+  // (Reading the keys once more and meeting costs 856 -> 924 us, training of 2 x 16384 x 16 heads of 64 x 128.)
+  auto keys_scale = [&](int n, int step, int from, int count) {
     const TcGates& g = gates(n);
-    const float wt = g.col[step] * g.leave[step >> 5];
+    const uint32_t keys = base + L::kOffK + Kr::place(n) * L::kTk;
+    __half2 top = __float2half2_rn(0.f);
+#pragma unroll 2
+    for (int c = from; c < from + count; ++c) {
+      const uint4 u = lds16(keys + piece_of(step, c));
+      const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&uu[k])));
+    }
+    const float most = fmaxf(__low2float(top), __high2float(top)) * fabsf(g.col[step] * g.leave[step >> 5]);
+    constexpr int kMeet = kOut ? 8 : 16;
+    volatile unsigned char* const of = smem + L::kOffMost + (n & 1) * kMeet;
+    const unsigned own = __reduce_max_sync(~0u, __float_as_uint(most)) >> 23;
+    if (lane == 0) of[warp & (kMeet - 1)] = (unsigned char)own;
+    __syncwarp();
+    named_sync<1, 32 * kMeet>();
+    return scale_of((int)__reduce_max_sync(~0u, (unsigned)of[lane & (kMeet - 1)]));
+  };
+  // w K in pieces, of a step's `count` planes from `from` on
+  auto weigh = [&](int n, int step, int from, int count, int up) {
+    const TcGates& g = gates(n);
+    float wt = g.col[step] * g.leave[step >> 5];
+    if constexpr (kScaled<T>) wt *= two_to(up);
     const uint32_t keys = base + L::kOffK + Kr::place(n) * L::kTk;
 #pragma unroll 1
     for (int c0 = from; c0 < from + count; c0 += 2) {   // (two at a time: reads first, as none may pass a write)
@@ -379,12 +407,15 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   if (warp < 8) {
     // ================================================================================ pairs and outputs
     if constexpr (!kOut) {   // (none: the other half of the weighted keys)
+      const int step = (warp & 3) * 32 + lane, from = (warp >> 2) * (KD / 16) + KD / 32;
+      int up = 0;
 #pragma unroll 1
       for (int n = 0; n < chunks; ++n) {
         wait(kGFull + (n & 1), n >> 1 & 1);
         wait(kKFull + Kr::place(n), Kr::parity(n));
         if (n) wait(kDsDone, (n - 1) & 1);   // (the products have read the last chunk's)
-        weigh(n, (warp & 3) * 32 + lane, (warp >> 2) * (KD / 16) + KD / 32, KD / 32);
+        if constexpr (kScaled<T>) up = keys_scale(n, step, from, KD / 32);
+        weigh(n, step, from, KD / 32, up);
         done(kGEmpty + (n & 1));
       }
     } else {
@@ -602,13 +633,16 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     };
     if (kOut) state_out();
     float decay = 1.f;
+    constexpr int kMine = kOut ? kPlanes : kPlanes / 2;
+    int up = 0;
     for (int n = 0; n < chunks; ++n) {
       const TcGates& g = gates(n);
       wait(kGFull + (n & 1), n >> 1 & 1);
       wait(kKFull + Kr::place(n), Kr::parity(n));
+      if constexpr (kScaled<T>) up = keys_scale(n, step, half * kPlanes, kMine);
       if (kOut) wait(kPDone + (n & 1), n >> 1 & 1);   // (the pairs' product has read the keys)
       const float enter = g.enter;
-      weigh(n, step, half * kPlanes, kOut ? kPlanes : kPlanes / 2);
+      weigh(n, step, half * kPlanes, kMine, up);
       if constexpr (kDots != 0) {
         // the state that enters: left by the walk of dq, multiplied with the gradient of the one that leaves by that of dk
         T* a = static_cast<T*>(w.anchors) + slot((long long)bh * w.chunks + tile_of(n));
@@ -645,7 +679,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         if (enter == 0.f)   // (not a factor: what is forgotten may be infinite)
 #pragma unroll
           for (int c = 0; c < kCols; ++c) st[c] = 0.f;
-        const f32x2 ee = pack2(enter, enter);
+        const f32x2 ee = pack2(enter, enter), unit = pack2(two_to(-up), two_to(-up));
 #pragma unroll
         for (int c = 0; c < kCols; c += 16) {
           float v[16];
@@ -653,8 +687,11 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           tm_wait_ld();
           loaded(v);
 #pragma unroll
-          for (int k = 0; k < 16; k += 2)
-            unpack2(fma2(ee, pack2(st[c + k], st[c + k + 1]), pack2(v[k], v[k + 1])), st[c + k], st[c + k + 1]);
+          for (int k = 0; k < 16; k += 2) {
+            f32x2 sum = pack2(v[k], v[k + 1]);
+            if constexpr (kScaled<T>) sum = mul2(unit, sum);
+            unpack2(fma2(ee, pack2(st[c + k], st[c + k + 1]), sum), st[c + k], st[c + k + 1]);
+          }
         }
         tm_before();
       }

@@ -91,6 +91,42 @@ def test_states_that_are_not_finite_reach_what_reads_them_alone(form, dtype, kd,
         assert float(got[i][pad].abs().max()) == 0, i
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kd,vd", HEADS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, 1e-5])
+def test_states_and_their_gradients_keep_fp32_places(form, dtype, kd, vd, size):
+    """weighted keys are held in pieces whose places suffice however small the gradients are"""
+    q, k, v, f, hin, dy, dh = _inputs(dtype, 2, 300, 2, kd, vd)
+    dy, dh = (dy.float() * size).to(DT[dtype]), dh * size
+    kw = dict(hin=hin, scale=kd ** -0.5, dy=dy, dh=dh)
+    ref, _ = reference(q, k, v, f, **kw)
+    got = run(q, k, v, f, **kw)
+    near(got[1], ref[1], STATE)
+    two = dtype == "bf16" and form == "tcgen05" and kd > 64 and vd > 64
+    near(got[6], ref[6], STATE + (2.0 ** -17 if two else 0.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,n,h", [(5, 700, 16), (1, 2100, 16)])
+@pytest.mark.parametrize("kd,vd", HEADS[:4])
+def test_fp16_over_many_chunks(form, kd, vd, b, n, h):
+    """blocks that walk several chunks, with and without segments; gradients of 1e-4"""
+    q, k, v, f, hin, dy, dh = _inputs("fp16", b, n, h, kd, vd, shift=4.0, gate_dtype=torch.float32)
+    dy, dh = (dy.float() * 1e-4).half(), dh * 1e-4
+    pad = torch.arange(n, device="cuda")[None].expand(b, n) >= n - 150
+    got = run(q, k, v, f, hin, pad, None, 0.1, False, dy, dh)
+    again = run(q, k, v, f, hin, pad, None, 0.1, False, dy, dh)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0 and all(torch.equal(x, y) for x, y in zip(got, again))
+    part = slice(h - 2, h)
+    ref, _ = reference(*(t[:1, :, part] for t in (q, k, v, f)), hin[:1, part], pad[:1], None, 0.1, False, dy[:1, :, part], dh[:1, part])
+    got = [got[i][:1, part] if i in (1, 6) else got[i][:1, :, part] for i in range(7)]
+    near(got[1], ref[1], STATE)
+    near(got[6], ref[6], STATE)
+    near(got[0], ref[0], 2.0 ** -11)
+
+
 def test_the_longest_sequences_have_their_chunks_counted():
     lib, a = _lib.lib(), _lib.DecayedAttentionArgs()
     for key, value in dict(dtype=1, gate_dtype=1, B=1, H=1, K=8, V=8).items():
