@@ -288,19 +288,20 @@ struct Shared {
   T s[KD * kLv];
   T x[kX ? kC * kLv : 8];
   Gates g[2];
-  float sums[kWarps];
+  float sums[kWarps], tops[kWarps];
 };
 
 // A state's value in the products: rounded to their type (the state itself stays in fp32 registers; of the three roundings on the way
 // to an output it is the one of the share that comes from before the chunk)
 template <typename T, int VT>
-__device__ __forceinline__ void state_to_shared(T* s, int ld, int row0, const float (*acc)[4], int lane) {
+__device__ __forceinline__ void state_to_shared(T* s, int ld, int row0, const float (*acc)[4], float up, int lane) {
 #pragma unroll
   for (int n = 0; n < VT / 8; ++n)
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       T* p = s + (row0 + (lane >> 2) + 8 * hf) * ld + n * 8 + 2 * (lane & 3);
       if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(acc[n][2 * hf], acc[n][2 * hf + 1]);
+      else if constexpr (kScaled<T>) *reinterpret_cast<uint32_t*>(p) = pack<T>(up * acc[n][2 * hf], up * acc[n][2 * hf + 1]);
       else *reinterpret_cast<uint32_t*>(p) = pack<T>(acc[n][2 * hf], acc[n][2 * hf + 1]);
     }
 }
@@ -355,10 +356,32 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
       const float* l = w.local + slot(((long long)p * w.B * w.H + bh) * w.tiles + tile);
       each_state([&](float& v, int r, int c) { v = (fac == 0.f ? 0.f : fac * v) + l[r * VT + c]; });
     }
+  }
+  int scale = 0;   // fp16: of the state in shared memory, a power of two
+  // the state that enters the next chunk, where all that it is multiplied with finds it
+  auto state_out = [&]() {
+    if constexpr (kScaled<T>) {
+      float top = 0.f;
+      if (holds)
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(st[m][n][i]));
+      const unsigned bits = __reduce_max_sync(~0u, __float_as_uint(top));
+      if (lane == 0) sh.tops[warp] = __uint_as_float(bits);
+      __syncthreads();
+      unsigned most = 0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) most = max(most, __float_as_uint(sh.tops[i]));
+      scale = scale_of((int)(most >> 23));
+    }
     if (holds)
 #pragma unroll
-      for (int m = 0; m < kM; ++m) state_to_shared<T, VT>(sh.s, kLv, (warp * kM + m) * 16, st[m], lane);
-  }
+      for (int m = 0; m < kM; ++m) state_to_shared<T, VT>(sh.s, kLv, (warp * kM + m) * 16, st[m], two_to(scale), lane);
+  };
+  if (kOut) state_out();
   float decay = 1.f;   // of the segment so far
 
   auto tile_of = [&](int c) { return w.rev ? w.chunks - 1 - c : c; };
@@ -405,7 +428,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
       // ---- the state that enters: written by the walk of dq, and multiplied with the gradient of the one that leaves by that of dk
       if (kDots && gt.enter > (kDots == 1 ? 0.f : kLeast)) {
         T* a = static_cast<T*>(w.anchors) + slot(((long long)bh * w.chunks + tile_of(c)) * w.tiles + tile);
-        if (kDots == 1) each_state([&](float& v, int r, int cc) { Elem<T>::st(a + r * VT + cc, v); });
+        if (kDots == 1) each_state([&](float& v, int r, int cc) { Elem<T>::st(a + r * VT + cc, kScaled<T> ? two_to(scale) * v : v); });
         else {
           float sum = 0.f;
           each_state([&](float& v, int r, int cc) { sum += v * Elem<T>::ld(a + r * VT + cc); });
@@ -470,7 +493,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
       const float h0 = gt.hi[i0], h1 = gt.hi[i1], l0 = gt.lo[i0], l1 = gt.lo[i1];
       // (a padded step has no pairs and reads no state: -1 resets)
       const int c0 = gt.pad[i0] ? -1 : gt.count[i0], c1 = gt.pad[i1] ? -1 : gt.count[i1];
-      const float e0 = w.o_scale * exp2f(h0), e1 = w.o_scale * exp2f(h1);
+      const float unit = kScaled<T> ? two_to(-scale) : 1.f, e0 = w.o_scale * exp2f(h0) * unit, e1 = w.o_scale * exp2f(h1) * unit;
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         o[n][0] = c0 ? 0.f : e0 * o[n][0], o[n][1] = c0 ? 0.f : e0 * o[n][1];
@@ -573,10 +596,15 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
       }
       __syncthreads();   // (the state in shared memory, and x, have been read)
       if (kDots && c + 1 < to) fetch_x(c + 1);
-      if (kDots == 2 && tid == 0) {
-        float sum = 0.f;
-        for (int i = 0; i < kWarps; ++i) sum += sh.sums[i];
-        w.through[((long long)bh * w.chunks + tile_of(c)) * w.tiles + tile] = gt.enter > kLeast ? gt.enter * sum : 0.f;
+      if (kDots && tid == 0) {
+        const long long at = ((long long)bh * w.chunks + tile_of(c)) * w.tiles + tile;
+        if (kScaled<T> && kDots == 1) w.units[at] = unit;
+        if (kDots == 2) {
+          float sum = 0.f;
+          for (int i = 0; i < kWarps; ++i) sum += sh.sums[i];
+          if (kScaled<T> && gt.enter > kLeast) sum *= w.units[at];
+          w.through[at] = gt.enter > kLeast ? gt.enter * sum : 0.f;
+        }
       }
     }
 
@@ -615,9 +643,10 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
         for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) st[m][n][i] = (e == 0.f ? 0.f : e * st[m][n][i]) + (kScaled<T> ? two_to(-up) : 1.f) * add[n][i];
-        if (kOut) state_to_shared<T, VT>(sh.s, kLv, (warp * kM + m) * 16, st[m], lane);
+        if (kOut && !kScaled<T>) state_to_shared<T, VT>(sh.s, kLv, (warp * kM + m) * 16, st[m], 1.f, lane);
       }
     }
+    if constexpr (kOut && kScaled<T>) state_out();
     if (STAGES == 1 && c + 1 < to) {
       __syncthreads();
       fetch(c + 1, 0);
@@ -720,7 +749,7 @@ int value_tile(int keys) { return key_tile(keys) == 256 ? 32 : 64; }
 struct Plan {
   bool tc;
   int tiles, chunks, per, segs;
-  size_t local, factor, gates, anchors, through;   // floats
+  size_t local, factor, gates, anchors, units, through;   // floats
 };
 Plan plan_of(bool tc, int dtype, int B, int L, int H, int keys, int values) {
   Plan p;
@@ -742,6 +771,7 @@ Plan plan_of(bool tc, int dtype, int B, int L, int H, int keys, int values) {
   p.factor = even(n);
   p.gates = tc ? bh * p.chunks * (kTcGates / 4) : 0;
   p.anchors = even(bh * p.chunks * p.tiles * keys * vt * elem_size(dtype) / 4 + 1);
+  p.units = dtype == MEGA_F16 ? even(bh * p.chunks * p.tiles) : 0;
   p.through = even(bh * p.chunks * std::max(p.tiles, kTcParts));
   return p;
 }
@@ -814,7 +844,7 @@ BackPlan back_plan(const mega_decayed_attention_args& a, bool tc) {
   p.dv = plan_of(tc, a.dtype, a.B, a.L, a.H, a.K, a.V);
   p.walk = std::max(p.dq.local + p.dq.factor, p.dv.local + p.dv.factor) + p.dq.gates;
   p.dots = ((size_t)a.B * a.H * (tc ? kTcDots : p.dq.tiles) * a.L * 2 + 3) / 4 * 4;
-  p.all = p.walk + 2 * p.dots + p.dq.anchors + p.dq.through;
+  p.all = p.walk + 2 * p.dots + p.dq.anchors + p.dq.units + p.dq.through;
   return p;
 }
 // (whether the tensor memory's form takes a call depends on its memory too: room for either)
@@ -871,12 +901,12 @@ extern "C" MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_
   auto take = [&](size_t n) { float* r = at; at += n; return r; };
   float* walk = take(p.walk);
   float2 *dots_q = reinterpret_cast<float2*>(take(p.dots)), *dots_k = reinterpret_cast<float2*>(take(p.dots));
-  float *anchors = take(p.dq.anchors), *through = take(p.dq.through);
+  float *anchors = take(p.dq.anchors), *units = take(p.dq.units), *through = take(p.dq.through);
   const bool rev = (a->flags & MEGA_ATT_REVERSE) != 0;
   w.s_in = a->h_in, w.s_row = 1, w.s_col = a->V;
   w.p_scale = w.o_scale = (float)a->scale, w.s_scale = 1.f;
   w.rev = rev;
-  w.dots = dots_q, w.anchors = anchors;
+  w.dots = dots_q, w.anchors = anchors, w.units = units;
   int rc = run(a->dtype, w, p.dq, 1, walk, stream);
   if (rc) return rc;
   const Walk forward = w;
@@ -884,7 +914,7 @@ extern "C" MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_
   wk.s_in = a->dh_out, wk.s_out = a->dh_in, wk.s_row = 1, wk.s_col = a->V;
   wk.p_scale = wk.s_scale = (float)a->scale, wk.o_scale = 1.f;
   wk.rev = !rev, wk.excl = 1;
-  wk.dots = dots_k, wk.anchors = anchors, wk.through = through;
+  wk.dots = dots_k, wk.anchors = anchors, wk.units = units, wk.through = through;
   rc = run(a->dtype, wk, p.dk, 2, walk, stream);
   if (rc) return rc;
 

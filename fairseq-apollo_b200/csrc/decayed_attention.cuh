@@ -27,6 +27,7 @@ struct Walk {
   int s_row, s_col;       // strides of the states that come in and go out: (keys, values) of this walk
   float2* dots;           // [tile][B H][L]: x . out of the part from the state that entered; the pairs' sum W of a step
   void* anchors;          // [B H][chunk][tile] states that enter a chunk, in the activations' type (written, or read:)
+  float* units;           // [B H][chunk][tile]: fp16: what those states are to be multiplied with
   float* through;         // [B H][chunk][part]: what passes the whole chunk
   void* gates;            // [B H][chunk]: what the tensor memory's form reads of the gates
   int gates_there;        // (an earlier walk has left them)

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
 // barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it
 enum { kQFull, kQEmpty = kQFull + 3, kQRaw = kQEmpty + 3, kKFull = kQRaw + 3, kKEmpty = kKFull + 3, kKRaw = kKEmpty + 3, kVFull = kKRaw + 3,
        kVEmpty = kVFull + 3, kVRaw = kVEmpty + 3, kXFull = kVRaw + 3, kXEmpty = kXFull + 2, kXRaw = kXEmpty + 2, kGFull = kXRaw + 2, kGEmpty = kGFull + 2,
-       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead = kO1Done + 2, kSReady = kORead + 2, kDsDone, kWReady, kBars = kWReady + 2 };
+       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead = kO1Done + 2, kSReady = kORead + 2, kDsDone, kUnit, kWReady = kUnit + 4, kBars = kWReady + 2 };
 
 // kOut: outputs; else the state that a segment leaves by itself.  kDots: sums for the gates' gradient (1: walk of dq, 2: of dk).
 template <typename T, int KD, int VD, bool kOut, int kDots>
@@ -129,7 +129,7 @@ struct Lay {
   static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 ? kTk : 0), kOffV = kOffK + kKs * kTk,
                        kOffQ = kOffV + kVs * kTv, kOffX = kOffQ + (kOut ? kQs * kTk : 0), kOffS = kOffX + (kX ? kXs * kTv : 0),
                        kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8,
-                       kOffMost = kOffSlot + 16, kEnd = kOffMost + (kScaled<T> ? 32 : 0);
+                       kOffMost = kOffSlot + 16, kOffUnit = kOffMost + 32, kEnd = kOffMost + (kScaled<T> ? 48 : 0);
   static_assert(kEnd <= 227 * 1024, "shared memory");
   // Columns of tensor memory.  Where they suffice pairs have two places: those of the next chunk are worked on while this one's outputs
   // are on their way.
@@ -354,10 +354,14 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     else if (warp >= 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   }
-  // fp16: the power of two that w K of a chunk is multiplied with, from `count` planes of a step in each thread.  The warps of weights
-  // meet for it, each with a byte for its exponent: two sets of them in turn, as a warp may be at the next chunk while another still reads.
-  // (Reading the keys once more and meeting costs 856 -> 924 us, training of 2 x 16384 x 16 heads of 64 x 128.)
-  auto keys_scale = [&](int n, int step, int from, int count) {
+  // fp16: the powers of two that w K of a chunk, from `count` planes of a step in each thread, and the state that enters it, whose largest
+  // value in this thread is `held`, are multiplied with.  The warps of weights meet for them, each with a byte for its exponents: two sets of
+  // them in turn, as a warp may be at the next chunk while another still reads.
+  // (Reading the keys once more and meeting costs 856 -> 924 us, training of 2 x 16384 x 16 heads of 64 x 128; the state's scale 9 more.)
+  struct Scales {
+    int keys, state;
+  };
+  auto scales = [&](int n, int step, int from, int count, float held) {
     const TcGates& g = gates(n);
     const uint32_t keys = base + L::kOffK + Kr::place(n) * L::kTk;
     __half2 top = __float2half2_rn(0.f);
@@ -370,12 +374,20 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     }
     const float most = fmaxf(__low2float(top), __high2float(top)) * fabsf(g.col[step] * g.leave[step >> 5]);
     constexpr int kMeet = kOut ? 8 : 16;
-    volatile unsigned char* const of = smem + L::kOffMost + (n & 1) * kMeet;
+    volatile unsigned char* const of = smem + L::kOffMost + (n & 1) * 16;
     const unsigned own = __reduce_max_sync(~0u, __float_as_uint(most)) >> 23;
-    if (lane == 0) of[warp & (kMeet - 1)] = (unsigned char)own;
+    const unsigned ours = kOut ? __reduce_max_sync(~0u, __float_as_uint(held)) >> 23 : 0;
+    if (lane == 0) {
+      of[warp & (kMeet - 1)] = (unsigned char)own;
+      if (kOut) of[8 + (warp & 7)] = (unsigned char)ours;
+    }
     __syncwarp();
     named_sync<1, 32 * kMeet>();
-    return scale_of((int)__reduce_max_sync(~0u, (unsigned)of[lane & (kMeet - 1)]));
+    const unsigned got = of[lane & 15];   // (16 keys' exponents, or eight and eight states')
+    Scales r;
+    r.keys = scale_of((int)__reduce_max_sync(~0u, !kOut || (lane & 8) == 0 ? got : 0u));
+    r.state = kOut ? scale_of((int)__reduce_max_sync(~0u, lane & 8 ? got : 0u)) : 0;
+    return r;
   };
   // w K in pieces, of a step's `count` planes from `from` on
   auto weigh = [&](int n, int step, int from, int count, int up) {
@@ -414,7 +426,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         wait(kGFull + (n & 1), n >> 1 & 1);
         wait(kKFull + Kr::place(n), Kr::parity(n));
         if (n) wait(kDsDone, (n - 1) & 1);   // (the products have read the last chunk's)
-        if constexpr (kScaled<T>) up = keys_scale(n, step, from, KD / 32);
+        if constexpr (kScaled<T>) up = scales(n, step, from, KD / 32, 0.f).keys;
         weigh(n, step, from, KD / 32, up);
         done(kGEmpty + (n & 1));
       }
@@ -516,6 +528,11 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         wait(kODone, n & 1);
         wait(kO1Done + (n & 1), n >> 1 & 1);
         tm_after();
+        if constexpr (kScaled<T>) {
+          // (four places: the next state but one waits for these outputs to be read)
+          wait(kUnit + (n & 3), n >> 2 & 1);
+          e *= two_to(113 - (int)*(volatile unsigned char*)(smem + L::kOffUnit + (n & 3)));
+        }
         char* row = static_cast<char*>(w.out) + (b * w.ob + h * w.oh + t * w.ol) * 2;
         const bool apart = __any_sync(~0u, e == 0.f);   // rows that read nothing of the state (which may be infinite: no factor)
 #pragma unroll kUnroll
@@ -621,17 +638,22 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
             for (int k = 0; k < 4; ++k) st[c + k] = (fac == 0.f ? 0.f : fac * st[c + k]) + uu[k];
           }
       }
-    // the state as an operand: rounded to 16 bits (the state itself is not)
+    // eight values of the state as an operand: rounded to 16 bits (the state itself is not), fp16 after a scale
+    float scale = 1.f;
+    auto eight = [&](int c) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = kScaled<T> ? st[c + k] * scale : st[c + k];
+      return make_uint4(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]), pack<T>(v[4], v[5]), pack<T>(v[6], v[7]));
+    };
     auto state_out = [&]() {
       if (holds)
 #pragma unroll
-        for (int c = 0; c < kCols; c += 8)
-          sts16(base + L::kOffS + (col0 + c) / 8 * (KD * 16) + row * 16,
-                make_uint4(pack<T>(st[c], st[c + 1]), pack<T>(st[c + 2], st[c + 3]), pack<T>(st[c + 4], st[c + 5]), pack<T>(st[c + 6], st[c + 7])));
+        for (int c = 0; c < kCols; c += 8) sts16(base + L::kOffS + (col0 + c) / 8 * (KD * 16) + row * 16, eight(c));
       fence_proxy_async();
       done(kSReady);
     };
-    if (kOut) state_out();
+    if (kOut && !kScaled<T>) state_out();
     float decay = 1.f;
     constexpr int kMine = kOut ? kPlanes : kPlanes / 2;
     int up = 0;
@@ -639,7 +661,22 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       const TcGates& g = gates(n);
       wait(kGFull + (n & 1), n >> 1 & 1);
       wait(kKFull + Kr::place(n), Kr::parity(n));
-      if constexpr (kScaled<T>) up = keys_scale(n, step, half * kPlanes, kMine);
+      if constexpr (kScaled<T>) {
+        float held = 0.f;
+        if (kOut && holds)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) held = fmaxf(held, fabsf(st[c]));
+        const Scales r = scales(n, step, half * kPlanes, kMine, held);
+        up = r.keys, scale = two_to(r.state);
+        if constexpr (kOut) {
+          if (sw == 0 && lane == 0) {
+            smem[L::kOffUnit + (n & 3)] = (unsigned char)(r.state + 113);
+            arrive(bar(kUnit + (n & 3)));
+            if (kDots == 1) w.units[(long long)bh * w.chunks + tile_of(n)] = two_to(-r.state);
+          }
+          state_out();
+        }
+      }
       if (kOut) wait(kPDone + (n & 1), n >> 1 & 1);   // (the pairs' product has read the keys)
       const float enter = g.enter;
       weigh(n, step, half * kPlanes, kMine, up);
@@ -650,8 +687,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           if (mine && enter != 0.f)
 #pragma unroll
             for (int c = 0; c < kCols; c += 8)
-              *reinterpret_cast<uint4*>(a + c) =
-                  make_uint4(pack<T>(st[c], st[c + 1]), pack<T>(st[c + 2], st[c + 3]), pack<T>(st[c + 4], st[c + 5]), pack<T>(st[c + 6], st[c + 7]));
+              *reinterpret_cast<uint4*>(a + c) = eight(c);
         } else {
           float s = 0.f;
           if (mine && enter > kLeast)
@@ -668,8 +704,9 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
 #pragma unroll
           for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
           if (lane == 0) {
-            float* to = w.through + ((long long)bh * w.chunks + tile_of(n)) * kTcParts;
-            to[sw] = enter > kLeast ? enter * s : 0.f;
+            const long long at = (long long)bh * w.chunks + tile_of(n);
+            if (kScaled<T> && enter > kLeast) s *= w.units[at];
+            w.through[at * kTcParts + sw] = enter > kLeast ? enter * s : 0.f;
           }
         }
       }
@@ -697,7 +734,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       }
       decay *= enter;
       done(kGEmpty + (n & 1));
-      if (kOut && n + 1 < chunks) state_out();
+      if (kOut && !kScaled<T> && n + 1 < chunks) state_out();
     }
     if (!kOut) {
       if (mine) {

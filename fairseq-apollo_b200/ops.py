@@ -543,8 +543,8 @@ def decayed_attention_fwd(q, k, v, forget, padding_mask=None, reset_mask=None, h
     ``expand``), a copy is made where the last axis is not contiguous.
     padding_mask (B, L), non-zero = padded: the state stays as it is, y = 0.  reset_mask (B, L), non-zero: the step starts from a
     zero state (the first step of a document in a packed sequence).  h_in (B, H, K, V): the state that comes in.
-    In 16-bit types pairs' weights and the state are rounded to that type where they enter matrix products (a state beyond fp16's
-    range then is infinite); sums and the state itself are fp32.  A value that is not finite at a step that is not padded may reach
+    In 16-bit types pairs' weights and the state are rounded to that type where they enter matrix products (in fp16 a state of any size,
+    by a power of two); sums and the state itself are fp32.  A value that is not finite at a step that is not padded may reach
     every output of its sequence and head.
     ``reverse`` walks from the last step to the first.
     Returns y like v, and the state behind the walk's last step (B, H, K, V) fp32 when ``want_state``."""

@@ -34,10 +34,10 @@ def form(request):
     _lib.set_option(1, 0)
 
 
-def near(got, ref, rel, step=0.0):
-    """|error| <= rel |ref| + step for every value, in the mean square"""
+def near(got, ref, rel, step=0.0, size=None):
+    """|error| <= rel |ref| (or another size) + step for every value, in the mean square"""
     assert torch.isfinite(got).all()
-    err, allowed = float((got.detach().double() - ref).norm()), rel * float(ref.norm()) + step * ref.numel() ** 0.5
+    err, allowed = float((got.detach().double() - ref).norm()), rel * float((ref if size is None else size).norm()) + step * ref.numel() ** 0.5
     assert err <= allowed, (err / allowed, err / (float(ref.norm()) + 1e-300))
 
 
@@ -125,6 +125,44 @@ def test_fp16_over_many_chunks(form, kd, vd, b, n, h):
     near(got[1], ref[1], STATE)
     near(got[6], ref[6], STATE)
     near(got[0], ref[0], 2.0 ** -11)
+
+
+def gate_sizes(q, k, v, f, hin, scale, dy, dh):
+    """d log a_t = a_t <R_t, S_{t-1}> adds up one product for every key and value, with roundings of their own: off by at most u in the
+    mean square (three of them) of the products' norm, which may be larger than their sum.  Those norms, times the gates' slope."""
+    q, k, v, f, s, dy, r = (t.double() for t in (q, k, v, f, hin, dy, dh))
+    a, states, out = torch.sigmoid(f)[..., None, None], [], [None] * q.shape[1]
+    for t in range(q.shape[1]):
+        states.append(s)
+        s = a[:, t] * s + k[:, t, :, :, None] * v[:, t, :, None, :]
+    for t in reversed(range(q.shape[1])):
+        r = r + scale * q[:, t, :, :, None] * dy[:, t, :, None, :]
+        out[t] = (a[:, t] * r * states[t]).square().sum((-1, -2)).sqrt()
+        r = a[:, t] * r
+    return torch.stack(out, 1) * torch.sigmoid(-f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kd,vd", HEADS)
+@pytest.mark.parametrize("size", [5e5, 1.0, 1e-4])
+def test_fp16_reads_states_of_any_size(form, kd, vd, size):
+    """states beyond fp16's range, and below its normal one, beside outputs inside it: keys and values that add next to nothing, and
+    queries that bring the outputs back to their usual size"""
+    q, k, v, f, hin, dy, dh = _inputs("fp16", 2, 300, 2, kd, vd, gate_dtype=torch.float32, shift=5.0)
+    unit = 2.0 ** -10 if size > 1 else 1.0
+    q, dy = (t * (unit if size > 1 else 16.0) for t in (q, dy))
+    k, v = ((t.float() * (unit if size > 1 else size ** 0.5)).half() for t in (k, v))
+    hin, dh = hin * size, dh * size
+    kw = dict(hin=hin, scale=kd ** -0.5, dy=dy, dh=dh)
+    ref, _ = reference(q, k, v, f, **kw)
+    assert all(float(ref[i].abs().max()) < 65504 for i in (0, 2, 3, 4))
+    got = run(q, k, v, f, **kw)
+    u = 2.0 ** -11
+    for i in (0, 2, 3, 4):
+        near(got[i], ref[i], u, 2.0 ** -25)
+    near(got[5], ref[5], u, size=gate_sizes(q, k, v, f, **kw))
+    near(got[1], ref[1], STATE)
+    near(got[6], ref[6], STATE)
 
 
 def test_the_longest_sequences_have_their_chunks_counted():
