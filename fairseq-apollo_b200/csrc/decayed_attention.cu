@@ -556,6 +556,26 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
         if (t4 == 0 && t0 + i0 < w.L) d[i0] = make_float2(dot[0], dot[2]);
         if (t4 == 0 && t0 + i1 < w.L) d[i1] = make_float2(dot[1], dot[3]);
       }
+      // fp16: a power of two for a row's pairs, which its outputs have until they are done
+      float back0 = 1.f, back1 = 1.f;
+      if constexpr (kScaled<T>) {
+        float top0 = 0.f, top1 = 0.f;
+#pragma unroll
+        for (int n = 0; n < kC / 8; ++n)
+          if (w.rev ? n / 2 >= warp : n / 2 <= warp)
+            top0 = fmaxf(top0, fmaxf(fabsf(p[n][0]), fabsf(p[n][1]))), top1 = fmaxf(top1, fmaxf(fabsf(p[n][2]), fabsf(p[n][3])));
+#pragma unroll
+        for (int i = 1; i <= 2; i <<= 1) top0 = fmaxf(top0, __shfl_xor_sync(~0u, top0, i)), top1 = fmaxf(top1, __shfl_xor_sync(~0u, top1, i));
+        // (at most 2^60: the share of the state is in the same sum)
+        const int up0 = min(scale_of(__float_as_int(top0) >> 23), 60), up1 = min(scale_of(__float_as_int(top1) >> 23), 60);
+        const float f0 = two_to(up0), f1 = two_to(up1);
+        back0 = two_to(-up0), back1 = two_to(-up1);
+#pragma unroll
+        for (int n = 0; n < kC / 8; ++n)
+          if (w.rev ? n / 2 >= warp : n / 2 <= warp) p[n][0] *= f0, p[n][1] *= f0, p[n][2] *= f1, p[n][3] *= f1;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) o[n][0] *= f0, o[n][1] *= f0, o[n][2] *= f1, o[n][3] *= f1;
+      }
       // ---- weighted pairs times values
       Beside<T, kN> small;
 #pragma unroll
@@ -582,7 +602,8 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
           const int cc = n * 8 + 2 * t4;
-          const float u = o[n][2 * hf], v = o[n][2 * hf + 1];
+          const float back = hf ? back1 : back0, u = kScaled<T> ? back * o[n][2 * hf] : o[n][2 * hf],
+                      v = kScaled<T> ? back * o[n][2 * hf + 1] : o[n][2 * hf + 1];
           if (w.piece >= 2 * (int)sizeof(T)) {
             if (cc < dv) {
               if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(row + cc) = make_float2(u, v);

@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
   *reinterpret_cast<uchar4*>(g.count + row) = make_uchar4(count[0], count[1], count[2], count[3]);
   const unsigned lanes = 0xffu << (lane & 24);
   const bool reset = __any_sync(lanes, r.count[0] != there || r.count[1] != there || r.count[2] != there);
-  const bool far = __any_sync(lanes, gate_sum(end - r.sum[0]) < -100.f);
+  const bool far = __any_sync(lanes, gate_sum(end - r.sum[0]) < (kScaled<T> ? -60.f : -100.f));   // (fp16: besides a scale of up to 2^40)
   mask = __reduce_or_sync(lanes, mask << (row & 31));
   if ((lane & 7) == 7) {
     g.apart[word] = reset || far;
@@ -126,14 +126,14 @@ struct Lay {
   // the last four 48: 2 x 88 + 2 x 128 + 48 for each four warps, as at launch (5 x 96).
   static constexpr int kRegs = 96;
   static constexpr bool kMove = VD == 128;
-  static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 ? kTk : 0), kOffV = kOffK + kKs * kTk,
-                       kOffQ = kOffV + kVs * kTv, kOffX = kOffQ + (kOut ? kQs * kTk : 0), kOffS = kOffX + (kX ? kXs * kTv : 0),
-                       kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8,
-                       kOffMost = kOffSlot + 16, kOffUnit = kOffMost + 32, kEnd = kOffMost + (kScaled<T> ? 48 : 0);
-  static_assert(kEnd <= 227 * 1024, "shared memory");
   // Columns of tensor memory.  Where they suffice pairs have two places: those of the next chunk are worked on while this one's outputs
   // are on their way.
   static constexpr bool kTwo = kOut && VD == 64;
+  static constexpr int kOffLo = 0, kOffLo2 = kOffLo + kTk, kOffK = kOffLo2 + (kPieces == 3 ? kTk : 0), kOffV = kOffK + kKs * kTk,
+                       kOffQ = kOffV + kVs * kTv, kOffX = kOffQ + (kOut ? kQs * kTk : 0), kOffS = kOffX + (kX ? kXs * kTv : 0),
+                       kOffG = kOffS + (kOut ? kTs : 0), kOffBar = kOffG + 2 * (int)sizeof(TcGates), kOffSlot = kOffBar + kBars * 8,
+                       kOffMost = kOffSlot + 16, kOffUnit = kOffMost + 32, kOffPairs = kOffUnit + 4, kEnd = kOffMost + (!kScaled<T> ? 0 : kTwo ? 64 : 48);
+  static_assert(kEnd <= 227 * 1024, "shared memory");
   static constexpr uint32_t kColO2 = kTwo ? 384 : 256, kColS = !kOut ? 0 : kTwo ? 448 : 384;
   static __device__ __forceinline__ uint32_t col_p(int n) { return kTwo ? (n & 1) * 128 : 0; }
   static __device__ __forceinline__ uint32_t col_o1(int n) { return kTwo ? 256 + (n & 1) * 64 : 128; }
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       constexpr int kW = 32;   // columns at a time (sixteen take longer: 94 us for 86, 8 x 4096 x 16 heads of 64)
       const int rb = warp & 3, half = warp >> 2, i = rb * 32 + lane;   // a row, and half of its pairs and of its outputs
       const uint32_t quarter = tm + ((uint32_t)(rb * 32) << 16);
-      float e_next = 0.f;
+      float e_next = 0.f, unit_next = 1.f;
       bool live = false;   // (read by the thread itself, x of a padded step must not count)
       auto pairs = [&](int n) {
         const TcGates& g = gates(n);
@@ -447,6 +447,28 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         wait(kPDone + (n & 1), n >> 1 & 1);
         tm_after();
         const int from = max(w.rev ? rb : 0, 2 * half), to = min(w.rev ? 3 : rb, 2 * half + 1);   // blocks of 32 steps that these rows see
+        float p_scale = w.p_scale;
+        if constexpr (kScaled<T>) {
+          // fp16: a power of two for all pairs of the chunk, from the largest one before its weight (at most 2^40: a row's factor may be 2^60).
+          // Two sets of bytes in turn where the next chunk's pairs may be under way while another warp still reads.
+          float top = 0.f;
+#pragma unroll 1
+          for (int jb = from; jb <= to; ++jb) {
+            float v[32];
+            tm_ld32(quarter + L::col_p(n) + 32 * jb, v);
+            tm_wait_ld();
+            loaded(v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) top = fmaxf(top, fabsf(v[j]));
+          }
+          const unsigned own = __reduce_max_sync(~0u, __float_as_uint(top * fabsf(p_scale))) >> 23;
+          volatile unsigned char* const of = smem + L::kOffPairs + (L::kTwo ? (n & 1) * 8 : 0);
+          if (lane == 0) of[warp] = (unsigned char)own;
+          __syncwarp();
+          named_sync<2, 256>();
+          const int up = min(scale_of((int)__reduce_max_sync(~0u, (unsigned)of[lane & 7])), 40);
+          p_scale *= two_to(up), unit_next = two_to(-up);
+        }
         // kW pairs of a row
         auto block = [&](int jb, int k) {
           float v[kW];
@@ -455,7 +477,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           // The row's is then one over its own as a column: both walks' weights agree to two units, however large the sums.)
           const int end = last_of(w, jb), j0 = 32 * jb + k;
           const float col = g.col[i];
-          const float f = g.count[end] != ci || (jb == rb && col == 0.f) ? 0.f : jb == rb ? __fdividef(w.p_scale, col) : w.p_scale * ex2(gi - g.base[jb]);
+          const float f = g.count[end] != ci || (jb == rb && col == 0.f) ? 0.f : jb == rb ? __fdividef(p_scale, col) : p_scale * ex2(gi - g.base[jb]);
           float4 c[kW / 4];
 #pragma unroll
           for (int j = 0; j < kW / 4; ++j) c[j] = *reinterpret_cast<const float4*>(g.col + j0 + 4 * j);
@@ -467,7 +489,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           if constexpr (kDots != 0)
             if (jb == rb)
 #pragma unroll
-              for (int j = 0; j < kW; ++j) own = j == lane - k ? v[j] * w.p_scale : own;
+              for (int j = 0; j < kW; ++j) own = j == lane - k ? v[j] * p_scale : own;
           if (jb != rb || !g.apart[jb]) {
 #pragma unroll
             for (int j = 0; j < kW / 4; ++j) {
@@ -477,7 +499,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           } else {   // resets among these steps, or a decay by more than 2^-100: a power of two for each pair
 #pragma unroll
             for (int j = 0; j < kW; ++j) {
-              const float p = v[j] * (w.p_scale * ex2(0x1p-18f * (float)min(ri - g.rel[j0 + j], 0)));
+              const float p = v[j] * (p_scale * ex2(0x1p-18f * (float)min(ri - g.rel[j0 + j], 0)));
               v[j] = g.count[j0 + j] == ci ? p : 0.f;
             }
           }
@@ -512,7 +534,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         tm_before();
         done(kPReady + (n & 1));
       };
-      auto outputs = [&](int n, float e) {
+      auto outputs = [&](int n, float e, float unit) {   // unit: what the pairs' share is to be multiplied with
         const long long t = (long long)tile_of(n) * kC + i;
         float read = 0.f, inner = 0.f;
         constexpr int kUnroll = kDots && !L::kX ? 4 : 1, kHalf = VD / 2, kO = kDots && !L::kX ? 16 : kW;
@@ -557,6 +579,9 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           }
           uint32_t word[kO / 2];
           const f32x2 ee = pack2(e, e);
+          if constexpr (kScaled<T>)
+#pragma unroll
+            for (int m = 0; m < kO / 2; ++m) unpack2(mul2(pack2(unit, unit), pack2(p[2 * m], p[2 * m + 1])), p[2 * m], p[2 * m + 1]);
 #pragma unroll
           for (int m = 0; m < kO / 2; ++m) {
             f32x2 y;
@@ -598,9 +623,9 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
       constexpr int kAhead = L::kTwo ? 1 : 0;
 #pragma unroll 1
       for (int n = -kAhead; n < chunks; ++n) {
-        const float e_now = e_next;
+        const float e_now = e_next, unit_now = unit_next;
         if (n + kAhead < chunks) pairs(n + kAhead);
-        if (n >= 0) outputs(n, kAhead ? e_now : e_next);
+        if (n >= 0) outputs(n, kAhead ? e_now : e_next, kAhead ? unit_now : unit_next);
       }
     }
   } else if (warp < 16) {

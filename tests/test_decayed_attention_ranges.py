@@ -165,6 +165,38 @@ def test_fp16_reads_states_of_any_size(form, kd, vd, size):
     near(got[6], ref[6], STATE)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kd,vd", HEADS)
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, 1e-5])
+def test_fp16_gradients_of_any_size(form, kd, vd, size):
+    q, k, v, f, hin, dy, dh = _inputs("fp16", 2, 300, 2, kd, vd, gate_dtype=torch.float32)
+    dy, dh = (dy.float() * size).half(), dh * size
+    kw = dict(hin=hin, scale=kd ** -0.5, dy=dy, dh=dh)
+    ref, _ = reference(q, k, v, f, **kw)
+    got = run(q, k, v, f, **kw)
+    u = 2.0 ** -11
+    for i in (2, 3, 4):
+        near(got[i], ref[i], u, 2.0 ** -25)
+    near(got[5], ref[5], u, size=gate_sizes(q, k, v, f, **kw))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kd,vd", HEADS)
+def test_fp16_pairs_of_any_size(form, kd, vd):
+    """products of queries and keys beyond fp16's range, beside values so small that the outputs are not"""
+    q, k, v, f, hin, dy, dh = _inputs("fp16", 2, 300, 2, kd, vd, gate_dtype=torch.float32)
+    q, k, v, dy = q * 256, k * 256, v * 2.0 ** -10, dy * 2.0 ** -10
+    kw = dict(hin=hin * 0.1, scale=1.0, dy=dy, dh=dh)
+    ref, _ = reference(q, k, v, f, **kw)
+    assert float(torch.einsum("blhk,blhk->blh", q.double(), k.double()).abs().max()) > 1e5
+    assert all(float(ref[i].abs().max()) < 65504 for i in (0, 2, 3, 4))
+    got = run(q, k, v, f, **kw)
+    u = 2.0 ** -11
+    for i in (0, 2, 3, 4):
+        near(got[i], ref[i], u, 2.0 ** -25)
+    near(got[5], ref[5], u, size=gate_sizes(q, k, v, f, **kw))
+
+
 def test_the_longest_sequences_have_their_chunks_counted():
     lib, a = _lib.lib(), _lib.DecayedAttentionArgs()
     for key, value in dict(dtype=1, gate_dtype=1, B=1, H=1, K=8, V=8).items():
