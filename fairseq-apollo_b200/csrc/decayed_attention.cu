@@ -506,8 +506,7 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const Walk w) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = n * 8 + 2 * t4 + (i & 1), r = i < 2 ? i0 : i1;
-            float d = (i < 2 ? h0 : h1) - gt.hi[j];
-            if (sizeof(T) == 4) d += (i < 2 ? l0 : l1) - gt.lo[j];
+            const float d = (i < 2 ? h0 : h1) - gt.hi[j] + ((i < 2 ? l0 : l1) - gt.lo[j]);   // (sums of some thousands lie behind closed gates)
             const bool on = (w.rev ? j >= r : j <= r) && gt.count[j] == (i < 2 ? c0 : c1);
             p[n][i] = on ? p[n][i] * (w.p_scale * exp2f(fminf(d, 0.f))) : 0.f;
           }

@@ -137,7 +137,7 @@ __device__ __forceinline__ GateOut<N> gates_scan(const Walk& w, const GateIn<N>&
 }
 
 // The form on tcgen05 products (decayed_attention_tc.cu): 16-bit activations, heads of at most 128 keys and values
-constexpr int kTcChunk = 128, kTcMost = 128, kTcParts = 8, kTcDots = 2, kTcGates = 1216;   // shares of Walk::through and Walk::dots
+constexpr int kTcChunk = 128, kTcMost = 128, kTcParts = 8, kTcDots = 2, kTcGates = 1280;   // shares of Walk::through and Walk::dots
 bool tc_takes(int dtype, const Walk& w);
 int tc_walk(int dtype, const Walk& w, int dots, void* stream);
 cudaError_t tc_read_device_error(int* v, bool reset);

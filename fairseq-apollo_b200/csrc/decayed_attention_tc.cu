@@ -49,6 +49,7 @@ struct TcGates {
   float col[kC];      // weight of a step at the last of its 32 (0: a reset lies between)
   uint8_t count[kC];  // resets so far
   float base[4];      // running sum of log2 a at the last of 32 steps
+  float between[4][4];   // [i][j]: running sum from the last of the 32 steps j to that of i (a difference of sums of thousands, as whole numbers)
   float leave[4];     // weight of the last of 32 steps in the state that leaves
   uint32_t pad[4];    // padded steps
   float enter;        // weight of the state that enters in the one that leaves
@@ -93,7 +94,11 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
   const bool reset = __any_sync(lanes, r.count[0] != there || r.count[1] != there || r.count[2] != there);
   const bool far = __any_sync(lanes, gate_sum(end - r.sum[0]) < (kScaled<T> ? -60.f : -100.f));   // (fp16: besides a scale of up to 2^40)
   mask = __reduce_or_sync(lanes, mask << (row & 31));
+  float gap[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) gap[k] = gate_sum(end - __shfl_sync(~0u, end, 8 * (w.rev ? 3 - k : k))) + r.bad;   // (rows ascend)
   if ((lane & 7) == 7) {
+    *reinterpret_cast<float4*>(g.between[word]) = make_float4(gap[0], gap[1], gap[2], gap[3]);
     g.apart[word] = reset || far;
     g.base[word] = gate_sum(end) + r.bad;
     g.leave[word] = there == r.total ? w.s_scale * exp2f(gate_sum(r.all - end) + r.bad) : 0.f;
@@ -477,7 +482,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           // The row's is then one over its own as a column: both walks' weights agree to two units, however large the sums.)
           const int end = last_of(w, jb), j0 = 32 * jb + k;
           const float col = g.col[i];
-          const float f = g.count[end] != ci || (jb == rb && col == 0.f) ? 0.f : jb == rb ? __fdividef(p_scale, col) : p_scale * ex2(gi - g.base[jb]);
+          const float f = g.count[end] != ci || (jb == rb && col == 0.f) ? 0.f : jb == rb ? __fdividef(p_scale, col) : p_scale * ex2(g.between[rb][jb] + 0x1p-18f * (float)ri);
           float4 c[kW / 4];
 #pragma unroll
           for (int j = 0; j < kW / 4; ++j) c[j] = *reinterpret_cast<const float4*>(g.col + j0 + 4 * j);
