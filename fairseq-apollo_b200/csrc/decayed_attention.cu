@@ -952,5 +952,6 @@ extern "C" MEGA_API int mega_decayed_attention_bwd(const mega_decayed_attention_
     if (p.dk.tc) launch(gate_grad_kernel<T, kTcChunk / 32>, grid, dim3(128), 0, stream, gg);
     else launch(gate_grad_kernel<T, kC / 32>, grid, dim3(128), 0, stream, gg);
   });
+  if (p.dk.tc) g_last_kernel.store("decayed_attention_tc", std::memory_order_relaxed);   // (of the walks; the gates' gradient has one form)
   return check_launch("decayed_attention_bwd");
 }

@@ -27,9 +27,8 @@
 //
 // The state is accumulated by each chunk's own sum, which is then added in fp32: a long chain inside the tensor cores' accumulator
 // would be cut off, not rounded, thousands of times.
-#include <mutex>
+#include <atomic>
 #include <type_traits>
-#include <unordered_map>
 
 #include "common.cuh"
 #include "decayed_attention.cuh"
@@ -922,36 +921,47 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
 
 // Whether the compiler gave a kernel the registers that its warps share out among themselves: with fewer they would wait for good.
 bool has_registers(const void* kernel, int regs) {
-  static std::mutex mutex;
-  static std::unordered_map<const void*, int> have;
-  std::lock_guard<std::mutex> lock(mutex);
-  int& n = have[kernel];
-  if (!n) {
-    cudaFuncAttributes a;
-    n = cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : -1;
-  }
-  return n >= regs;
+  cudaFuncAttributes a;
+  if (cudaFuncGetAttributes(&a, kernel) == cudaSuccess) return a.numRegs >= regs;
+  cudaGetLastError();
+  return false;
 }
+// The kernels of a walk whose keys and values are padded to KD and VD
 template <typename T, int KD, int VD>
-bool run(const Walk& w, const Maps& maps, int dots, void* stream) {
-  const long long blocks = (long long)w.B * w.H;
-  auto go = [&](auto kernel, auto lay, long long n) {
-    using L = decltype(lay);
-    if (L::kMove && !has_registers(reinterpret_cast<const void*>(+kernel), L::kRegs)) return false;
-    launch_after(kernel, dim3((unsigned)n), dim3(L::kThreads), L::kEnd, stream, w, maps);
-    return true;
+struct Width {
+  template <bool kOut, int kDots>
+  static bool takes() {
+    using L = Lay<T, KD, VD, kOut, kDots>;
+    return !L::kMove || has_registers(reinterpret_cast<const void*>(+tc_kernel<T, KD, VD, kOut, kDots>), L::kRegs);
+  }
+  static bool takes_all() {
+    static std::atomic<bool> known{false};   // (asked until they do: it costs microseconds)
+    if (!known.load(std::memory_order_relaxed) && takes<false, 0>() && takes<true, 0>() && takes<true, 1>() && takes<true, 2>()) known.store(true);
+    return known.load(std::memory_order_relaxed);
+  }
+  template <bool kOut, int kDots>
+  static void go(const Walk& w, const Maps& maps, long long n, void* stream) {
+    using L = Lay<T, KD, VD, kOut, kDots>;
+    launch_after(tc_kernel<T, KD, VD, kOut, kDots>, dim3((unsigned)n), dim3(L::kThreads), L::kEnd, stream, w, maps);
+  }
+  static void run(const Walk& w, const Maps& maps, int dots, void* stream) {
+    const long long blocks = (long long)w.B * w.H;
+    if (!w.gates_there) launch(tc_gates_kernel<T>, dim3((unsigned)((blocks * w.chunks + 3) / 4)), dim3(128), 0, stream, w);
+    if (w.segs > 1) go<false, 0>(w, maps, blocks * (w.segs - 1), stream);
+    if (dots == 0) go<true, 0>(w, maps, blocks * w.segs, stream);
+    else if (dots == 1) go<true, 1>(w, maps, blocks * w.segs, stream);
+    else go<true, 2>(w, maps, blocks * w.segs, stream);
+  }
+};
+// fn(Width) for a walk's widths
+template <typename F>
+auto with_width(int dtype, const Walk& w, F&& fn) {
+  auto widths = [&](auto zero) {
+    using T = decltype(zero);
+    if (w.k.d <= 64) return w.v.d <= 64 ? fn(Width<T, 64, 64>()) : fn(Width<T, 64, 128>());
+    return w.v.d <= 64 ? fn(Width<T, 128, 64>()) : fn(Width<T, 128, 128>());
   };
-  if (!w.gates_there)
-    launch(tc_gates_kernel<T>, dim3((unsigned)((blocks * w.chunks + 3) / 4)), dim3(128), 0, stream, w);
-  if (w.segs > 1 && !go(tc_kernel<T, KD, VD, false, 0>, Lay<T, KD, VD, false, 0>(), blocks * (w.segs - 1))) return false;
-  if (dots == 0) return go(tc_kernel<T, KD, VD, true, 0>, Lay<T, KD, VD, true, 0>(), blocks * w.segs);
-  if (dots == 1) return go(tc_kernel<T, KD, VD, true, 1>, Lay<T, KD, VD, true, 1>(), blocks * w.segs);
-  return go(tc_kernel<T, KD, VD, true, 2>, Lay<T, KD, VD, true, 2>(), blocks * w.segs);
-}
-template <typename T>
-bool pick(const Walk& w, const Maps& m, int dots, void* stream) {
-  if (w.k.d <= 64) return w.v.d <= 64 ? run<T, 64, 64>(w, m, dots, stream) : run<T, 64, 128>(w, m, dots, stream);
-  return w.v.d <= 64 ? run<T, 128, 64>(w, m, dots, stream) : run<T, 128, 128>(w, m, dots, stream);
+  return dtype == MEGA_BF16 ? widths(__nv_bfloat16()) : widths(__half());
 }
 
 // (width, step, head, sequence) of an operand; false where TMA cannot address it
@@ -974,13 +984,13 @@ bool tc_takes(int dtype, const Walk& w) {
   if (dtype == MEGA_F32 || g_options[OPT_DISABLE_MMA].load() || w.piece < 16) return false;
   for (const Operand* o : {&w.q, &w.k, &w.v, &w.x})
     if (o->p && (o->d > kTcMost || o->vec < 16 || o->sl < 0 || o->sh < 0 || o->sb < 0 || (o->sl == 0 && w.L > 1))) return false;
-  Maps m;   // (what the driver refuses is known before a plan is made)
-  return maps_of(&m, dtype, w);
+  Maps m;   // (what the driver refuses, or the compiler did not give, is known before a plan is made)
+  return maps_of(&m, dtype, w) && with_width(dtype, w, [](auto width) { return width.takes_all(); });
 }
 int tc_walk(int dtype, const Walk& w, int dots, void* stream) {
   Maps m;
   if (!maps_of(&m, dtype, w)) return MEGA_ERR_UNSUPPORTED;
-  if (!(dtype == MEGA_BF16 ? pick<__nv_bfloat16>(w, m, dots, stream) : pick<__half>(w, m, dots, stream))) return MEGA_ERR_UNSUPPORTED;
+  with_width(dtype, w, [&](auto width) { width.run(w, m, dots, stream); });
   g_last_kernel.store("decayed_attention_tc", std::memory_order_relaxed);
   return MEGA_OK;
 }

@@ -21,7 +21,7 @@ import torch
 
 import fairseq_apollo_b200 as M
 from fairseq_apollo_b200 import _lib
-from test_decayed_attention import DT, _inputs, reference, run
+from test_decayed_attention import DT, _inputs, both, reference, run
 
 STATE = 1.5e-6
 HEADS = [(64, 64), (64, 128), (128, 64), (128, 128), (40, 24)]
@@ -215,6 +215,140 @@ def test_weights_behind_gates_that_are_nearly_closed(form):
     r = ref[0][:, to:]
     off = ((y * r).sum(-1) / (r * r).sum(-1) - 1).mean((0, 2))
     assert float(off.square().mean().sqrt()) < 4e-5, off
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_which_form_takes_a_call(dtype):
+    """tcgen05 takes 16-bit heads of at most 128 keys and values, more than 64 steps and rows on 16 bytes; mma.sync the rest"""
+    _lib.set_option(1, 0)
+
+    def name(change, b=2, n=200, h=4, kd=64, vd=64, backward=True):
+        q, k, v, f, hin, dy, dh = _inputs(dtype, b, n, h, kd, vd)
+        q, k, v, f, dy = change(q, k, v, f, dy)
+        with torch.no_grad():
+            M.decayed_attention(q, k, v, f)
+        forward = _lib.last_kernel()
+        if backward:
+            run(q, k, v, f, hin, dy=dy, dh=dh)
+            assert _lib.last_kernel() == forward
+        return forward
+
+    def same(*x):
+        return x
+
+    def columns(extra):   # of one projection, `extra` values off
+        def change(q, k, v, f, dy):
+            z = torch.zeros(*q.shape[:2], extra + 8 + sum(t[0, 0].numel() for t in (q, k, v, f)), dtype=q.dtype, device="cuda")
+            out, at = [], extra
+            for t in (q, k, v, f):
+                w = t[0, 0].numel()
+                z[..., at:at + w] = t.flatten(2)
+                out.append(z[..., at:at + w].view(t.shape))
+                at += w
+            return (*out, dy)
+        return change
+
+    def time_major(*x):
+        return tuple(t.transpose(0, 1).contiguous().transpose(0, 1) for t in x)
+
+    def shared(q, k, v, f, dy):
+        return q, k[:, :, :1].expand_as(k), v[:, :, :1].expand_as(v), f, dy
+
+    def thrice(q, k, v, f, dy):   # the same sequence for all
+        return (*(t[:1].expand_as(t) for t in (q, k, v, f)), dy)
+    taken = "decayed_attention_tc" if dtype != "fp32" else "other"
+    for kd, vd in HEADS + [(8, 8), (72, 16), (16, 120)]:
+        assert name(same, kd=kd, vd=vd) == taken, (kd, vd)
+    assert name(same, n=65) == taken and name(time_major) == taken and name(shared) == taken and name(thrice) == taken
+    assert name(same, b=1, h=1) == taken
+    assert name(columns(0), h=8) == taken   # (8 heads: rows of 1544 + 8 values)
+    assert name(same, n=64) == "other" and name(same, kd=136) == "other" and name(same, vd=144) == "other" and name(same, kd=36) == "other"
+    assert name(columns(1), h=8) == "other" and name(columns(0), h=12) == "other"   # (rows of 2324 + 8 values)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("size", [(2, 130, 3, 64, 128), (1, 129, 1, 128, 128), (3, 257, 2, 48, 96), (1, 65, 2, 32, 40), (2, 300, 2, 64, 64)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_both_forms_at_the_same_sizes(form, dtype, size, reverse):
+    b, n, h, kd, vd = size
+    g = torch.Generator().manual_seed(6)
+    pad, reset = (torch.rand(b, n, generator=g) < 0.3).cuda(), (torch.rand(b, n, generator=g) < 0.05).cuda()
+    both(dtype, *size, reverse=reverse)
+    assert _lib.last_kernel() == ("decayed_attention_tc" if form == "tcgen05" else "other")
+    both(dtype, *size, pad, reset, reverse=reverse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads", [8, 12])
+@pytest.mark.parametrize("b,n", [(2, 200), (10, 300)])
+def test_one_projection(dtype, heads, b, n):
+    """the module's layout: z's gradient, written in place of its parts, on tcgen05 (8 heads) and mma.sync (12)"""
+    _lib.set_option(1, 0)
+    q, k, v, f, hin, dy, dh = _inputs(dtype, b, n, heads, 64, 64, shift=3.0)
+    pad = torch.arange(n, device="cuda")[None].expand(b, n) >= torch.arange(n - 10 * b, n, 10, device="cuda")[:, None]
+    z = torch.cat([t.flatten(2) for t in (q, k, v, f)], -1).requires_grad_()
+    y, h = M.functions.decayed_attention_packed(z, heads, 64, pad, None, hin, 0.125, True)
+    form = "decayed_attention_tc" if heads == 8 else "other"
+    assert _lib.last_kernel() == form
+    dz, = torch.autograd.grad([y, h], [z], [dy, dh])
+    assert _lib.last_kernel() == form
+    kw = dict(hin=hin, pad=pad, scale=0.125, dy=dy, dh=dh)
+    ref, _ = reference(q, k, v, f, **kw)
+    u = torch.finfo(DT[dtype]).eps / 2
+    want = torch.cat([t.flatten(2) for t in ref[2:6]], -1)
+    step = 2.0 ** -25 if dtype == "fp16" else 0.0
+    near(y, ref[0], u, step)
+    near(h, ref[1], STATE)
+    for part, (a, c) in enumerate(zip(dz.split([64 * heads] * 3 + [heads], -1), want.split([64 * heads] * 3 + [heads], -1))):
+        # (the gates' gradient: one rounding more, and that of products which may be larger than their sum)
+        near(a, c, u * (1.5 if part == 3 else 1.0), step)
+    assert float(dz.detach()[pad].abs().max()) == 0
+    parts = run(*(t for t in (q, k, v, f)), **kw)
+    assert torch.equal(dz, torch.cat([t.flatten(2) for t in parts[2:6]], -1)) or heads == 12   # (rows of 12 heads by themselves: tcgen05)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_the_module_on_tcgen05(dtype):
+    torch.manual_seed(0)
+    _lib.set_option(1, 0)
+    m = M.DecayedAttention(96, 8, zdim=256, hdim=512, bidirectional=True).cuda().to(DT[dtype])
+    u = torch.randn(3, 260, 96, device="cuda").to(DT[dtype])
+    pad = torch.arange(260, device="cuda")[None] >= torch.tensor([[260], [100], [201]], device="cuda")
+    with torch.no_grad():
+        y = m(u, pad)
+        z, r = m.in_proj(u), m.back_proj(u)
+        a = M.decayed_attention(*m._parts(z), pad, scale=m.scale)
+        assert _lib.last_kernel() == "decayed_attention_tc"
+        c = M.decayed_attention(*m._parts(r), pad, scale=m.scale, reverse=True)
+        assert torch.equal(y, (a + c).flatten(-2))
+    m(u, pad).float().square().sum().backward()
+    assert _lib.last_kernel() == "decayed_attention_tc"
+    assert all(torch.isfinite(p.grad).all() and float(p.grad.abs().max()) > 0 for p in m.parameters())
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_the_31_values():
+    """the last heads of a call whose offsets pass 32 bits, forward and backward, against a call of their own"""
+    b, n, h, kd, vd = 1, 34000, 512, 128, 128
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    _lib.set_option(1, 0)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v, dy = (torch.randn(b, n, h, kd, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(4))
+    f = torch.randn(b, n, h, device="cuda", dtype=torch.float32, generator=g) + 3.0
+    assert v.numel() > 2 ** 31
+    last = slice(h - 2, h)
+    part = run(*(t[:, :, last].contiguous() for t in (q, k, v, f)), None, None, None, 0.1, False, dy[:, :, last].contiguous(),
+               torch.zeros(b, 2, kd, vd, device="cuda"))
+    whole = run(q, k, v, f, None, None, None, 0.1, False, dy, torch.zeros(b, h, kd, vd, device="cuda"))
+    for i in range(6):
+        x, y = (whole[i][:, last] if i == 1 else whole[i][:, :, last]).detach().double(), part[i].detach().double()
+        # (few heads have segments, whose states are joined in another order: last bits, and a rounding that goes the other way)
+        assert float((x - y).norm()) < 2.0 ** -8 * float(y.norm()), i
 
 
 def test_the_longest_sequences_have_their_chunks_counted():
