@@ -35,6 +35,8 @@ struct Walk {
   int B, L, H, tiles, chunks, per, segs;
   float p_scale, o_scale, s_scale;
   int rev, excl;
+  long long wait_limit;   // SM cycles after which a wait of the tensor memory's form gives up
+  int withhold;           // a test: chunk of each block whose keys are never loaded, or -1
 };
 
 // The walk of dq leaves a chunk's state where its weight in the next one is above zero; that of dk, whose sum of the same gates may round

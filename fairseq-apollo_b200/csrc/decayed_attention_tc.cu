@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
 // barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it
 enum { kQFull, kQEmpty = kQFull + 3, kQRaw = kQEmpty + 3, kKFull = kQRaw + 3, kKEmpty = kKFull + 3, kKRaw = kKEmpty + 3, kVFull = kKRaw + 3,
        kVEmpty = kVFull + 3, kVRaw = kVEmpty + 3, kXFull = kVRaw + 3, kXEmpty = kXFull + 2, kXRaw = kXEmpty + 2, kGFull = kXRaw + 2, kGEmpty = kGFull + 2,
-       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead = kO1Done + 2, kSReady = kORead + 2, kDsDone, kUnit, kWReady = kUnit + 4, kBars = kWReady + 2 };
+       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead = kO1Done + 2, kSReady = kORead + 2, kDsDone, kUnit, kAllDone = kUnit + 4, kWReady = kAllDone + 2, kBars = kWReady + 2 };
 
 // kOut: outputs; else the state that a segment leaves by itself.  kDots: sums for the gates' gradient (1: walk of dq, 2: of dk).
 template <typename T, int KD, int VD, bool kOut, int kDots>
@@ -150,15 +150,24 @@ __device__ __forceinline__ bool tried(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// A wait that gives up (after seconds: never expected) raises `gone`; from then on no wait lasts, and everything runs out on whatever the
-// buffers hold.  (Short: the roles' loops together are to stay in the instruction cache.)
-__device__ __forceinline__ void wait_for(uint32_t bar, uint32_t parity, volatile int* gone) {
+// A wait that gives up (never expected) raises `gone` and returns false; from then on no wait lasts.  Warps that meet others by name run out on
+// whatever the buffers hold; loads and products are issued no more, and what is under way is waited for before the block ends.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* gone, long long limit) {
+  if (tried(bar, parity)) return true;
+  const long long from = clock64();
 #pragma unroll 1
-  for (int i = 0; !tried(bar, parity); ++i)
-    if (i > 1 << 24 || *gone) {   // (a try itself lasts a fraction of a microsecond)
+  while (!tried(bar, parity))
+    if (*gone || clock64() - from > limit) {
       g_device_error = *gone = 1;
-      break;
+      return false;
     }
+  return true;
+}
+// what the block itself has under way, however short the limit of the other waits is
+__device__ __forceinline__ void settle(uint32_t bar, uint32_t parity, long long limit) {
+  const long long from = clock64();
+#pragma unroll 1
+  while (!tried(bar, parity) && clock64() - from < 2 * limit + 4000000) {}
 }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // `THREADS` threads, whole warps, meet
@@ -269,8 +278,9 @@ __device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap* m, i
 }
 // 128 steps of an operand; rows behind the last one and columns it does not have become zeros.  An axis whose stride is 0 has one place.
 template <int D>
-__device__ __forceinline__ void load_tile(uint32_t to, const CUtensorMap* m, const Operand& o, int t0, int h, int b, uint32_t bar) {
+__device__ __forceinline__ void load_tile(uint32_t to, const CUtensorMap* m, const Operand& o, int t0, int h, int b, uint32_t bar, bool go = true) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(D * kC * 2) : "memory");
+  if (!go) return;   // (a test: what waits for it gives up)
 #pragma unroll
   for (int c = 0; c < D; c += 64) tma_load_4d(to + c / 64 * kBox, m, c, t0, o.sh ? h : 0, o.sb ? b : 0, bar);
 }
@@ -298,7 +308,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
   int first = seg * w.per, chunks = min(w.per, w.chunks - first);   // in the order of the walk
   const bool ends = first + chunks == w.chunks;
   auto bar = [&](int i) { return base + L::kOffBar + i * 8; };
-  auto wait = [&](int i, uint32_t parity) { wait_for(bar(i), parity, gone); };
+  auto wait = [&](int i, uint32_t parity) { return wait_for(bar(i), parity, gone, w.wait_limit); };
   auto done = [&](int i) {   // (a warp arrives as one: barriers take their threads one after another)
     __syncwarp();
     if (lane == 0) arrive(bar(i));
@@ -785,41 +795,73 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     if (umma_elect()) {
       const TcGates* const table = static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks;
       bool next = w.pad && chunks && table[tile_of(0)].padded;
+      // loads so far: of keys, queries, values, x, gates; by place (bit 3 of what + place): parity of the uses of kQRaw..., whether the last was one
+      int loaded[5] = {0, 0, 0, 0, 0};
+      uint32_t used = 0, last = 0;
+      auto note = [&](int what, int place, bool raw) {
+        const uint32_t bit = 1u << (3 * what + place);
+        ++loaded[what];
+        if (raw) used ^= bit, last |= bit;
+        else last &= ~bit;
+      };
 #pragma unroll 1
       for (int n = 0; n < chunks; ++n) {
         const int t0 = tile_of(n) * kC;
         const bool raw = next;   // (the others' loads are seen as they land)
         next = w.pad && n + 1 < chunks && table[tile_of(n + 1)].padded;
-        if (n >= L::kKs) wait(kKEmpty + Kr::place(n), Kr::parity(n) ^ 1);
-        load_tile<KD>(base + L::kOffK + Kr::place(n) * L::kTk, &maps.k, w.k, t0, h, b, bar((raw ? kKRaw : kKFull) + Kr::place(n)));
+        if (n >= L::kKs && !wait(kKEmpty + Kr::place(n), Kr::parity(n) ^ 1)) break;
+        load_tile<KD>(base + L::kOffK + Kr::place(n) * L::kTk, &maps.k, w.k, t0, h, b, bar((raw ? kKRaw : kKFull) + Kr::place(n)), n != w.withhold);
+        note(0, Kr::place(n), raw);
         auto values = [&]() {
-          if (n >= L::kVs) wait(kVEmpty + Vr::place(n), Vr::parity(n) ^ 1);
+          if (n >= L::kVs && !wait(kVEmpty + Vr::place(n), Vr::parity(n) ^ 1)) return false;
           load_tile<VD>(base + L::kOffV + Vr::place(n) * L::kTv, &maps.v, w.v, t0, h, b, bar((raw ? kVRaw : kVFull) + Vr::place(n)));
+          note(2, Vr::place(n), raw);
+          return true;
         };
-        if (L::kVs > 1) values();
+        if (L::kVs > 1 && !values()) break;
         if (kOut) {
-          if (n >= L::kQs) wait(kQEmpty + Qr::place(n), Qr::parity(n) ^ 1);
+          if (n >= L::kQs && !wait(kQEmpty + Qr::place(n), Qr::parity(n) ^ 1)) break;
           load_tile<KD>(base + L::kOffQ + Qr::place(n) * L::kTk, &maps.q, w.q, t0, h, b, bar((raw ? kQRaw : kQFull) + Qr::place(n)));
+          note(1, Qr::place(n), raw);
         }
-        if (n > 1) wait(kGEmpty + (n & 1), (n >> 1 & 1) ^ 1);
+        if (n > 1 && !wait(kGEmpty + (n & 1), (n >> 1 & 1) ^ 1)) break;
         uint64_t* const got = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1);
         mbar_expect_tx(got, sizeof(TcGates));
         bulk_load_1d(&gates(n), table + tile_of(n), sizeof(TcGates), got);
+        note(4, n & 1, false);
         if (L::kX) {
-          if (n >= L::kXs) wait(kXEmpty + Xr::place(n), Xr::parity(n) ^ 1);
+          if (n >= L::kXs && !wait(kXEmpty + Xr::place(n), Xr::parity(n) ^ 1)) break;
           load_tile<VD>(base + L::kOffX + Xr::place(n) * L::kTv, &maps.x, w.x, t0, h, b, bar((raw ? kXRaw : kXFull) + Xr::place(n)));
+          note(3, Xr::place(n), raw);
         }
-        if (L::kVs == 1) values();
+        if (L::kVs == 1 && !values()) break;
       }
+      // (the last load of each place lands before the block ends, also where no one has waited for it)
+      auto landed = [&](int what, int places, int full, int raw) {
+#pragma unroll 1
+        for (int m = max(loaded[what] - places, 0); m < loaded[what]; ++m) {
+          if (what == 0 && m == w.withhold) continue;
+          const int place = m % places, at = 3 * what + place;
+          if (last >> at & 1) settle(bar(raw + place), (used >> at & 1) ^ 1, w.wait_limit);
+          else settle(bar(full + place), m / places & 1, w.wait_limit);
+        }
+      };
+      landed(0, L::kKs, kKFull, kKRaw);
+      landed(1, L::kQs, kQFull, kQRaw);
+      landed(2, L::kVs, kVFull, kVRaw);
+      landed(3, L::kXs, kXFull, kXRaw);
+      landed(4, 2, kGFull, kGFull);
     }
     __syncwarp();
   } else if (warp == 17) {
     // ================================================================================ padded steps: whatever lies there becomes zeros
     if (w.pad) {
       uint32_t used = 0;   // parity of each place's uses by chunks with padding
-      for (int n = 0; n < chunks; ++n) {
+      auto together = [&](int i, uint32_t parity) { return __all_sync(~0u, wait(i, parity)); };
+      bool go = true;
+      for (int n = 0; go && n < chunks; ++n) {
         const TcGates& g = gates(n);
-        wait(kGFull + (n & 1), n >> 1 & 1);
+        if (!together(kGFull + (n & 1), n >> 1 & 1)) break;
         const uint32_t pad[4] = {g.pad[0], g.pad[1], g.pad[2], g.pad[3]};
         const bool any = g.padded;
         done(kGEmpty + (n & 1));
@@ -832,7 +874,8 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
           const int raw = (what == 0 ? kKRaw : what == 1 ? kQRaw : what == 2 ? kVRaw : kXRaw) + place;
           const int full = (what == 0 ? kKFull : what == 1 ? kQFull : what == 2 ? kVFull : kXFull) + place;
           const uint32_t at = base + (what == 0 ? L::kOffK : what == 1 ? L::kOffQ : what == 2 ? L::kOffV : L::kOffX) + place * (what < 2 ? L::kTk : L::kTv);
-          wait(raw, used >> (3 * what + place) & 1);
+          go = together(raw, used >> (3 * what + place) & 1);
+          if (!go) break;
           used ^= 1u << (3 * what + place);
           clear_rows(at, what < 2 ? KD / 8 : VD / 8, pad, lane);
           fence_proxy_async();
@@ -845,30 +888,35 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     if (kOut && umma_elect()) {
       constexpr uint32_t kPairs = idesc<T>(128, false, false, 128), kRows = idesc<T>(VD, false, true, 128);
       constexpr int kAhead = L::kTwo ? 1 : 0;
+      bool begun = false;
 #pragma unroll 1
       for (int n = -kAhead; n < chunks; ++n) {
         if (const int m = n + kAhead; m < chunks) {
-          wait(kQFull + Qr::place(m), Qr::parity(m));
-          wait(kKFull + Kr::place(m), Kr::parity(m));
+          if (!wait(kQFull + Qr::place(m), Qr::parity(m)) || !wait(kKFull + Kr::place(m), Kr::parity(m))) break;
           // (a barrier tells two phases apart: the warps of weights have seen these products of two chunks ago, not only those of pairs)
-          if (m > 1) wait(kWReady + (m & 1), (m >> 1 & 1) ^ 1);
+          if (m > 1 && !wait(kWReady + (m & 1), (m >> 1 & 1) ^ 1)) break;
           tm_after();
           const uint64_t q = tile_desc(base + L::kOffQ + Qr::place(m) * L::kTk), kt = tile_desc(base + L::kOffK + Kr::place(m) * L::kTk);
 #pragma unroll
           for (int k = 0; k < KD / 16; ++k) umma(tm + L::col_p(m), q + kAlong(k), kt + kAlong(k), kPairs, k > 0);
+          begun = true;
           umma_commit(bar(kPDone + (m & 1)));
           umma_commit(bar(kQEmpty + Qr::place(m)));
         }
         if (n < 0) continue;
         const uint64_t vt = tile_desc(base + L::kOffV + Vr::place(n) * L::kTv);
-        wait(kVFull + Vr::place(n), Vr::parity(n));
-        if (n) wait(kORead + ((n - 1) & 1), (n - 1) >> 1 & 1);
-        wait(kPReady + (n & 1), n >> 1 & 1);
+        if (!wait(kVFull + Vr::place(n), Vr::parity(n)) || (n && !wait(kORead + ((n - 1) & 1), (n - 1) >> 1 & 1)) ||
+            !wait(kPReady + (n & 1), n >> 1 & 1))
+          break;
         tm_after();
 #pragma unroll
         for (int k = 0; k < kC / 16; ++k) umma_tm(tm + L::kColO2, tm + L::col_p(n) + k / 4 * 64 + k % 4 * 8, vt + kOver(k), kRows, k > 0);
         umma_commit(bar(kODone));
         umma_commit(bar(kVEmpty + Vr::place(n)));
+      }
+      if (begun) {   // (nothing of this block's products is on its way when it ends)
+        umma_commit(bar(kAllDone));
+        settle(bar(kAllDone), 0, w.wait_limit);
       }
     }
     __syncwarp();
@@ -877,24 +925,21 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     if (umma_elect()) {
       constexpr uint32_t kRows = idesc<T>(VD, false, true, 128), kBoth = idesc<T>(VD, true, true, KD);
       const uint64_t s = over(base + L::kOffS, KD * 16), lo = over(base + L::kOffLo, kPlane), lo2 = over(base + L::kOffLo2, kPlane);
+      bool begun = false;
 #pragma unroll 1
       for (int n = 0; n < chunks; ++n) {
         if constexpr (kOut) {
-          wait(kQFull + Qr::place(n), Qr::parity(n));
-          wait(kSReady, n & 1);
-          if (L::kTwo ? n > 1 : n > 0) {   // (the place is free)
-            const int m = L::kTwo ? n - 2 : n - 1;
-            wait(kORead + (m & 1), m >> 1 & 1);
-          }
+          if (!wait(kQFull + Qr::place(n), Qr::parity(n)) || !wait(kSReady, n & 1)) break;
+          if (const int m = L::kTwo ? n - 2 : n - 1; m >= 0 && !wait(kORead + (m & 1), m >> 1 & 1)) break;   // (the place is free)
           tm_after();
           const uint64_t q = tile_desc(base + L::kOffQ + Qr::place(n) * L::kTk);
 #pragma unroll
           for (int k = 0; k < KD / 16; ++k) umma(tm + L::col_o1(n), q + kAlong(k), s + k * 16, kRows, k > 0);
+          begun = true;
           umma_commit(bar(kO1Done + (n & 1)));
           umma_commit(bar(kQEmpty + Qr::place(n)));
         }
-        wait(kVFull + Vr::place(n), Vr::parity(n));
-        wait(kWReady + (n & 1), n >> 1 & 1);
+        if (!wait(kVFull + Vr::place(n), Vr::parity(n)) || !wait(kWReady + (n & 1), n >> 1 & 1)) break;
         tm_after();
         const uint64_t kt = tile_desc(base + L::kOffK + Kr::place(n) * L::kTk), vt = tile_desc(base + L::kOffV + Vr::place(n) * L::kTv);
         if constexpr (L::kPieces == 3)
@@ -904,12 +949,15 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
         for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, lo + k * 16, vt + kOver(k), kBoth, k > 0 || L::kPieces == 3);
 #pragma unroll
         for (int k = 0; k < kC / 16; ++k) umma(tm + L::kColS, kt + kOver(k), vt + kOver(k), kBoth, true);
+        begun = true;
         umma_commit(bar(kDsDone));
         umma_commit(bar(kKEmpty + Kr::place(n)));
         umma_commit(bar(kVEmpty + Vr::place(n)));
       }
-      // (nothing of this block's products is on its way when it ends)
-      if (chunks) wait(kVEmpty + Vr::place(chunks - 1), Vr::parity(chunks - 1));
+      if (begun) {
+        umma_commit(bar(kAllDone + 1));
+        settle(bar(kAllDone + 1), 0, w.wait_limit);
+      }
     }
     __syncwarp();
   }
@@ -990,7 +1038,11 @@ bool tc_takes(int dtype, const Walk& w) {
 int tc_walk(int dtype, const Walk& w, int dots, void* stream) {
   Maps m;
   if (!maps_of(&m, dtype, w)) return MEGA_ERR_UNSUPPORTED;
-  with_width(dtype, w, [&](auto width) { width.run(w, m, dots, stream); });
+  Walk bounded = w;
+  const int limit = g_options[OPT_WAIT_LIMIT].load(), withhold = g_options[OPT_WITHHOLD_LOAD].load();
+  bounded.wait_limit = limit > 0 ? (long long)limit : 4000000000LL;
+  bounded.withhold = withhold > 0 ? withhold : -1;
+  with_width(dtype, w, [&](auto width) { width.run(bounded, m, dots, stream); });
   g_last_kernel.store("decayed_attention_tc", std::memory_order_relaxed);
   return MEGA_OK;
 }

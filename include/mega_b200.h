@@ -91,7 +91,8 @@ MEGA_API uint64_t mega_launch_count(void);
 #define MEGA_OPT_WITHHOLD_LOAD 4 /* test aid, value k > 0: the tensor-core kernel never issues the TMA load of its
                                     step k (the barrier keeps expecting its bytes), so that every waiter of that
                                     stage runs into the wait limit, the kernel returns early without its final
-                                    stores and raises the device error word; nothing faults or traps */
+                                    stores and raises the device error word; nothing faults or traps.  Decayed
+                                    attention on tcgen05: the keys of each block's chunk k */
 #define MEGA_OPT_SPLIT 5 /* TimestepNorm -> EMA calls: 1: only the kernels that walk a sequence as one chain, 2: the forms
                             parallel over time wherever they apply (3: the scan among them), 0: whichever is estimated
                             to be faster.  TimestepNorm by itself: 3: the scan, 4: the form without tensor cores that

@@ -15,6 +15,7 @@ there is room for no more: 2^-17 of a key besides).
 """
 import ctypes
 import threading
+import time
 
 import pytest
 import torch
@@ -349,6 +350,38 @@ def test_more_than_2_to_the_31_values():
         x, y = (whole[i][:, last] if i == 1 else whole[i][:, :, last]).detach().double(), part[i].detach().double()
         # (few heads have segments, whose states are joined in another order: last bits, and a rounding that goes the other way)
         assert float((x - y).norm()) < 2.0 ** -8 * float(y.norm()), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("kd,vd", HEADS[:4])
+@pytest.mark.parametrize("b,n,h", [(5, 700, 16), (1, 2100, 16)])
+@pytest.mark.parametrize("padded", [False, True])
+def test_a_wait_that_runs_out(dtype, kd, vd, b, n, h, padded):
+    """keys of a chunk that never arrive (a test aid; the limit of waits is then a millisecond): every walk of the call ends by itself
+    and raises the error word, and the next call is as if nothing had been"""
+    q, k, v, f, hin, dy, dh = _inputs(dtype, b, n, h, kd, vd, shift=4.0)
+    pad = (torch.arange(n, device="cuda")[None].expand(b, n) % 200 >= 150) if padded else None
+    _lib.set_option(1, 0)
+
+    def call():
+        return run(q, k, v, f, hin, pad, None, 0.1, False, dy, dh)
+    want = call()
+    assert _lib.last_kernel() == "decayed_attention_tc" and _lib.device_error(reset=True) == 0
+    _lib.set_option(3, 2_000_000)
+    _lib.set_option(4, 1)
+    try:
+        begun = time.time()
+        call()
+        torch.cuda.synchronize()
+        assert time.time() - begun < 5.0
+        assert _lib.device_error(reset=True) != 0
+    finally:
+        _lib.set_option(3, 0)
+        _lib.set_option(4, 0)
+    for x, y in zip(call(), want):
+        assert torch.equal(x, y)
+    assert _lib.device_error() == 0
 
 
 def test_the_longest_sequences_have_their_chunks_counted():
