@@ -1176,7 +1176,7 @@ std::tuple<Tensor, OptTensor> decayed_attention(const Tensor& q, const Tensor& k
   return {y, h};
 }
 
-// whether any value of t lies where `out` (contiguous) has one
+// whether t lies apart from `out` (contiguous): no place from its first value to its last is one of `out`'s
 bool apart(const Tensor& out, const Tensor& t) {
   if (!t.defined() || t.numel() == 0 || out.numel() == 0) return true;
   const char *to = static_cast<const char*>(out.data_ptr()), *from = static_cast<const char*>(t.data_ptr());
