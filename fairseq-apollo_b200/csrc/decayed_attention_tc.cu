@@ -795,61 +795,71 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
     if (umma_elect()) {
       const TcGates* const table = static_cast<const TcGates*>(w.gates) + (long long)bh * w.chunks;
       bool next = w.pad && chunks && table[tile_of(0)].padded;
-      // loads so far: of keys, queries, values, x, gates; by place (bit 3 of what + place): parity of the uses of kQRaw..., whether the last was one
-      int loaded[5] = {0, 0, 0, 0, 0};
-      uint32_t used = 0, last = 0;
-      auto note = [&](int what, int place, bool raw) {
-        const uint32_t bit = 1u << (3 * what + place);
-        ++loaded[what];
-        if (raw) used ^= bit, last |= bit;
-        else last &= ~bit;
-      };
+      // parity of the uses of kQRaw..., for rings of one, two and three places
+      uint32_t uses = 0;
+      auto used = [](int n) { return 1u | 2u << (n & 1) | 8u << n % 3; };
+      int n = 0, begun = 0;   // where it ended: loads of chunk n that were issued, bits of keys, queries, values, x, gates
 #pragma unroll 1
-      for (int n = 0; n < chunks; ++n) {
+      for (; n < chunks; ++n) {
         const int t0 = tile_of(n) * kC;
         const bool raw = next;   // (the others' loads are seen as they land)
         next = w.pad && n + 1 < chunks && table[tile_of(n + 1)].padded;
+        constexpr int kFirst = L::kVs > 1 ? 5 : 1;   // keys, and values where they come next
         if (n >= L::kKs && !wait(kKEmpty + Kr::place(n), Kr::parity(n) ^ 1)) break;
         load_tile<KD>(base + L::kOffK + Kr::place(n) * L::kTk, &maps.k, w.k, t0, h, b, bar((raw ? kKRaw : kKFull) + Kr::place(n)), n != w.withhold);
-        note(0, Kr::place(n), raw);
         auto values = [&]() {
           if (n >= L::kVs && !wait(kVEmpty + Vr::place(n), Vr::parity(n) ^ 1)) return false;
           load_tile<VD>(base + L::kOffV + Vr::place(n) * L::kTv, &maps.v, w.v, t0, h, b, bar((raw ? kVRaw : kVFull) + Vr::place(n)));
-          note(2, Vr::place(n), raw);
           return true;
         };
-        if (L::kVs > 1 && !values()) break;
-        if (kOut) {
-          if (n >= L::kQs && !wait(kQEmpty + Qr::place(n), Qr::parity(n) ^ 1)) break;
-          load_tile<KD>(base + L::kOffQ + Qr::place(n) * L::kTk, &maps.q, w.q, t0, h, b, bar((raw ? kQRaw : kQFull) + Qr::place(n)));
-          note(1, Qr::place(n), raw);
+        if (L::kVs > 1 && !values()) {
+          begun = 1;
+          break;
         }
-        if (n > 1 && !wait(kGEmpty + (n & 1), (n >> 1 & 1) ^ 1)) break;
+        if (kOut) {
+          if (n >= L::kQs && !wait(kQEmpty + Qr::place(n), Qr::parity(n) ^ 1)) {
+            begun = kFirst;
+            break;
+          }
+          load_tile<KD>(base + L::kOffQ + Qr::place(n) * L::kTk, &maps.q, w.q, t0, h, b, bar((raw ? kQRaw : kQFull) + Qr::place(n)));
+        }
+        if (n > 1 && !wait(kGEmpty + (n & 1), (n >> 1 & 1) ^ 1)) {
+          begun = kFirst | 2;
+          break;
+        }
         uint64_t* const got = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + kGFull + (n & 1);
         mbar_expect_tx(got, sizeof(TcGates));
         bulk_load_1d(&gates(n), table + tile_of(n), sizeof(TcGates), got);
-        note(4, n & 1, false);
         if (L::kX) {
-          if (n >= L::kXs && !wait(kXEmpty + Xr::place(n), Xr::parity(n) ^ 1)) break;
+          if (n >= L::kXs && !wait(kXEmpty + Xr::place(n), Xr::parity(n) ^ 1)) {
+            begun = kFirst | 2 | 16;
+            break;
+          }
           load_tile<VD>(base + L::kOffX + Xr::place(n) * L::kTv, &maps.x, w.x, t0, h, b, bar((raw ? kXRaw : kXFull) + Xr::place(n)));
-          note(3, Xr::place(n), raw);
         }
-        if (L::kVs == 1 && !values()) break;
+        if (L::kVs == 1 && !values()) {
+          begun = kFirst | 2 | 16 | 8;
+          break;
+        }
+        if (raw) uses ^= used(n);
       }
       // (the last load of each place lands before the block ends, also where no one has waited for it)
       auto landed = [&](int what, int places, int full, int raw) {
+        const int count = n + (begun >> what & 1);
+        auto is_raw = [&](int m) { return raw != full && w.pad && table[tile_of(m)].padded; };
+        const uint32_t parity = count > n && is_raw(n) ? uses ^ used(n) : uses;
 #pragma unroll 1
-        for (int m = max(loaded[what] - places, 0); m < loaded[what]; ++m) {
+        for (int m = max(count - places, 0); m < count; ++m) {
           if (what == 0 && m == w.withhold) continue;
-          const int place = m % places, at = 3 * what + place;
-          if (last >> at & 1) settle(bar(raw + place), (used >> at & 1) ^ 1, w.wait_limit);
+          const int place = m % places;
+          if (is_raw(m)) settle(bar(raw + place), (parity >> (places == 1 ? 0 : places == 2 ? 1 + place : 3 + place) & 1) ^ 1, w.wait_limit);
           else settle(bar(full + place), m / places & 1, w.wait_limit);
         }
       };
       landed(0, L::kKs, kKFull, kKRaw);
-      landed(1, L::kQs, kQFull, kQRaw);
+      if (kOut) landed(1, L::kQs, kQFull, kQRaw);
       landed(2, L::kVs, kVFull, kVRaw);
-      landed(3, L::kXs, kXFull, kXRaw);
+      if (L::kX) landed(3, L::kXs, kXFull, kXRaw);
       landed(4, 2, kGFull, kGFull);
     }
     __syncwarp();
