@@ -562,7 +562,8 @@ def decayed_attention_step(q, k, v, forget, h=None, scale=1.0, h_out=None):
 # -------------------------------------------- root-mean-square norm with a residual
 def rms_norm_fwd(x, weight, residual=None, num_groups=1, eps=1e-5):
     """r = x + residual, rounded to x's type, y = r / sqrt(mean(r^2) + eps) * (1 + weight) for x (B, ..., D): the mean over each group of
-    D / num_groups adjacent channels.  Returns y, or (y, r) with a residual (of x's shape and dtype)."""
+    D / num_groups adjacent channels (in fp32: the norm of a row is to stay below 2^64).  Returns y, or (y, r) with a residual (of x's
+    shape and dtype)."""
     y, r = _lib.host().rms_norm(x, weight, residual, int(num_groups), float(eps))
     return y if residual is None else (y, r)
 

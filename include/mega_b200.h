@@ -699,7 +699,8 @@ MEGA_API int mega_group_norm_bwd(const void* dy, const void* x, void* dx, int dt
  * mega_decayed_attention_fwd: y, h_out.
  * mega_decayed_attention_bwd: from q, k, v, f, h_in, dy and dh_out the gradients dq, dk, dv, df (0 at padded steps) and dh_in.
  * mega_decayed_attention_step: one step of every sequence (L = 1, the second stride of each operand is not used, no masks): y, h_out.
- * In 16-bit types the products' operands (pairs' weights, the state) are rounded to that type, sums and the state are fp32.
+ * In 16-bit types the products' operands (pairs' weights, the state; in fp16 each times a power of two that keeps them in range) are
+ * rounded to that type, sums and the state are fp32.
  */
 #define MEGA_ATT_REVERSE 1u
 #define MEGA_ATT_MOST 256
@@ -731,7 +732,8 @@ MEGA_API int mega_decayed_attention_step(const mega_decayed_attention_args* args
  * ---- Root-mean-square norm with a residual -----------------------------------------------------
  * Rows of D contiguous channels in num_groups groups of D / num_groups adjacent ones: r = x + residual, rounded to the activations'
  * type (residual == NULL: r = x), y = r / sqrt(mean(r^2) + eps) * (1 + weight), the mean over a group.  Operands are (B, L, D),
- * strides of the first two axes free; weight (D) fp32.
+ * strides of the first two axes free, outputs overlap neither one another nor an input; weight (D) fp32.  Squares are summed in fp32: the
+ * norm of a row is to stay below 2^64.
  * mega_rms_norm_fwd: y, and r where `sum` is not NULL (it is required with a residual).
  * mega_rms_norm_bwd: from dy, dr (r's own gradient, NULL: zero) and r the gradient dx of x, which is the residual's too, and dweight
  * (D) fp32, summed over rows in a fixed order.  `work`: device memory of mega_rms_norm_work() bytes, 16-byte aligned, used by this
