@@ -17,7 +17,7 @@
 // This file: chunks of 64 steps on mma.sync, for fp32 (three products of TF32 pieces for each), heads of more than 128 keys or values, operands
 // that TMA cannot address, and short calls; everything else goes to the form on tcgen05 (decayed_attention_tc.cu).  A block of four warps
 // has 64 (32) values of a head; the state stays in its registers in fp32, the next chunk is on its way by cp.async.  What bounds it: the
-// rate of mma.sync with few warps to a multiprocessor (8 x 4096 x 16 heads of 64 in bf16 328 us, the time to move q, k, v, y is 41;
+// rate of mma.sync with few warps to a multiprocessor (8 x 4096 x 16 heads of 64 in bf16 345 us, the time to move q, k, v, y is 41;
 // fp32, 4 x 2805 x 7 heads of 50 x 83, rows on 4- and 8-byte boundaries, 284 us for 13).
 //
 // Resets (and gates so closed that their decay is zero in fp32) are counted rather than summed: a pair with another count between

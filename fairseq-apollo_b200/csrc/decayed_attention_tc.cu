@@ -18,12 +18,14 @@
 // writes it without bank conflicts.  (Loads by cp.async, three warps of them, took 140 cycles each and held up every other access to
 // shared memory: they were what bounded it: 209 us, by TMA 135, 8 x 4096 x 16 heads of 64.)
 //
-// Measured (8 sequences x 4096 steps x 16 heads in bf16, forward, no padding): heads of 64 89 us, 3.0 TB/s of q, k, v and y; of 128
-// 149 us, 3.6 TB/s; the products of chunks on mma.sync (decayed_attention.cu) 328 and 585 us.  What bounds it: a chunk of 64 x 64 heads
-// takes 4000 cycles, its loads 1300, its products 1900; 6500 warp instructions at 1.2 a cycle and the exchanges between roles (250 cycles
-// a wait) are the rest.  Heads of 128 also saturate shared memory: products read 350 KB of operands a chunk at 128 bytes a cycle, and
-// the pieces of keys are 100 KB more (two pieces instead of three: 138 us for 152).  Steps on the way: gates by a kernel before (123 -> 101
-// us at 64), two places for pairs (101 -> 91), products from two warps (91 -> 88).
+// Measured (8 sequences x 4096 steps x 16 heads in bf16, forward, no padding): heads of 64 84 to 88 us, 3.1 TB/s of q, k, v and y; of 128
+// 140 us, 3.8 TB/s; the products of chunks on mma.sync (decayed_attention.cu) 345 and 559 us.  What bounds it: a chunk of 64 x 64 heads
+// takes 4600 cycles (from the difference to 8192 steps), in which its products keep the tensor cores busy for 1600; 8000 warp instructions at 1.75 a
+// cycle and the exchanges between roles (250 cycles a wait) are the rest.  Heads of 128 also saturate shared memory: products read
+// 350 KB of operands a chunk at 128 bytes a cycle, and the pieces of keys are 100 KB more (two pieces instead of three: 138 us for 152).
+// Steps on the way: gates by a kernel before (123 -> 101 us at 64), two places for pairs (101 -> 91), products from two warps (91 -> 88).
+// fp16 is scaled where it enters products (decayed_attention.cuh), for which the roles look their operands through once more and meet: heads of
+// 64 100 us (86 without), of 128 153 (131), training at 64 516 (425), at 64 x 128 660 (610).
 //
 // The state is accumulated by each chunk's own sum, which is then added in fp32: a long chain inside the tensor cores' accumulator
 // would be cut off, not rounded, thousands of times.
@@ -107,10 +109,11 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
   if (lane == 0) g.enter = r.enter, g.padded = !r.padded ? 0 : all && !r.total ? 2 : 1;
 }
 
-// barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it
+// barriers; kQRaw...: what a load completes where padded steps have to be cleared before the rest may see it; kUnit: fp16's scale of the state
 enum { kQFull, kQEmpty = kQFull + 3, kQRaw = kQEmpty + 3, kKFull = kQRaw + 3, kKEmpty = kKFull + 3, kKRaw = kKEmpty + 3, kVFull = kKRaw + 3,
        kVEmpty = kVFull + 3, kVRaw = kVEmpty + 3, kXFull = kVRaw + 3, kXEmpty = kXFull + 2, kXRaw = kXEmpty + 2, kGFull = kXRaw + 2, kGEmpty = kGFull + 2,
-       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead = kO1Done + 2, kSReady = kORead + 2, kDsDone, kUnit, kAllDone = kUnit + 4, kWReady = kAllDone + 2, kBars = kWReady + 2 };
+       kPDone = kGEmpty + 2, kPReady = kPDone + 2, kODone = kPReady + 2, kO1Done, kORead = kO1Done + 2, kSReady = kORead + 2, kDsDone,
+       kUnit, kAllDone = kUnit + 4, kWReady = kAllDone + 2, kBars = kWReady + 2 };
 
 // kOut: outputs; else the state that a segment leaves by itself.  kDots: sums for the gates' gradient (1: walk of dq, 2: of dk).
 template <typename T, int KD, int VD, bool kOut, int kDots>
