@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(Lay<T, KD, VD, kOut, kDots>::kThreads, 1) tc_k
               unpack2(mul2(pack2(v[4 * j], v[4 * j + 1]), mul2(ff, pack2(c[j].x, c[j].y))), v[4 * j], v[4 * j + 1]);
               unpack2(mul2(pack2(v[4 * j + 2], v[4 * j + 3]), mul2(ff, pack2(c[j].z, c[j].w))), v[4 * j + 2], v[4 * j + 3]);
             }
-          } else {   // resets among these steps, or a decay by more than 2^-100: a power of two for each pair
+          } else {   // resets among these steps, or a decay by more than 2^-100 (fp16: 2^-60): a power of two for each pair
 #pragma unroll
             for (int j = 0; j < kW; ++j) {
               const float p = v[j] * (p_scale * ex2(0x1p-18f * (float)min(ri - g.rel[j0 + j], 0)));

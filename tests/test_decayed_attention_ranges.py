@@ -353,6 +353,71 @@ def test_more_than_2_to_the_31_values():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("scale", [-0.5, 0.0, 30.0, 1e-6])
+@pytest.mark.parametrize("kd,vd", [(64, 64), (64, 128), (128, 128)])
+def test_scales_of_any_sign_and_size(form, dtype, scale, kd, vd):
+    q, k, v, f, hin, dy, dh = _inputs(dtype, 2, 200, 2, kd, vd, gate_dtype=torch.float32)
+    kw = dict(hin=hin, scale=scale, dy=dy, dh=dh)
+    ref, _ = reference(q, k, v, f, **kw)
+    got = run(q, k, v, f, **kw)
+    # (fp32: two products in a row leave out 2^-22 each; queries times keys and pairs times values are cut off at each group of 8 places, at
+    # 128 keys 16 + 8 times by 2^-25 on average; weights as above: 5e-7 + 7e-7 + 6e-7 = 1.8e-6)
+    u, step = torch.finfo(DT[dtype]).eps / 2 if dtype != "fp32" else 2.0 ** -19, 2.0 ** -25 if dtype == "fp16" else 0.0
+    for i in (0, 2, 3, 4):
+        near(got[i], ref[i], u, step)
+    near(got[5], ref[5], u, size=gate_sizes(q, k, v, f, **kw))
+    near(got[1], ref[1], STATE)
+    # (with a scale of 0 the state's gradient is dh times the whole sequence's decay 2^-G, a weight far below the 2^-8 that STATE reckons with:
+    # its logarithm, 2^-24 of itself off in its terms and once more as a float, is G 2^-23 ln 2 off)
+    whole = 0.0 if scale else float(torch.nn.functional.logsigmoid(f.double()).sum(1).abs().max()) * 2.0 ** -23
+    near(got[6], ref[6], STATE + whole + (2.0 ** -17 if dtype == "bf16" and form == "tcgen05" and kd > 64 and vd > 64 else 0.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kd,vd", [(64, 64), (128, 128)])
+def test_fp16_calls_at_once_and_captured(form, kd, vd):
+    q, k, v, f, hin, dy, dh = _inputs("fp16", 2, 900, 2, kd, vd)
+
+    def call():
+        return run(q, k, v, f, hin, None, None, 0.1, False, dy, dh)
+    want = call()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for r in got for x, y in zip(r, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for t in out:
+        t.detach().zero_()
+    graph.replay()
+    assert all(torch.equal(x, y) for x, y in zip(out, want))
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_a_prompt_on_tcgen05_and_single_steps_behind_it(dtype):
+    torch.manual_seed(2)
+    _lib.set_option(1, 0)
+    m = M.DecayedAttention(128, 8, zdim=512, hdim=512).cuda().to(DT[dtype]).eval()
+    u = torch.randn(3, 210, 128, device="cuda").to(DT[dtype])
+    with torch.no_grad():
+        q, k, v, f = m._parts(m.in_proj(u))
+        ref, _ = reference(q, k, v, f, scale=m.scale)
+        state = {}
+        parts = [m(u[:, :200], None, state)]
+        assert _lib.last_kernel() == "decayed_attention_tc"
+        parts += [m(u[:, t:t + 1], None, state) for t in range(200, 210)]
+    # (single steps' projections are other library products: a rounding of each operand more)
+    near(torch.cat(parts, 1).unflatten(-1, (8, 64)), ref[0], 2 * torch.finfo(DT[dtype]).eps / 2, 2.0 ** -25 if dtype == "fp16" else 0.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("kd,vd", HEADS[:4])
 @pytest.mark.parametrize("b,n,h", [(5, 700, 16), (1, 2100, 16)])
