@@ -1,7 +1,7 @@
 """Linear attention with a decay for each head where states, gradients or gates leave their usual range, and which form takes a call.
 
-Every test runs both forms of whole sequences (tcgen05, and mma.sync by way of the option that leaves the first one out), against the
-recurrence in 64 bits.  Tolerances are on norms: an elementwise bound adds up every share's largest error, under which a lost piece of
+A test that takes `form` runs both forms of whole sequences (tcgen05, and mma.sync by way of the option that leaves the first one out).
+The reference is the recurrence in 64 bits.  Tolerances are on norms: an elementwise bound adds up every share's largest error, under which a lost piece of
 an operand would not show.
 
 Outputs and gradients in 16-bit types have three roundings on their way (a pair's weight, the state that is read, the result), of which
