@@ -703,37 +703,55 @@ __global__ void __launch_bounds__(128) gate_grad_kernel(const GateGrad a) {
   const GateIn<N> in = gates_fetch<T, N>(w, b, h, tile, lane);
   float through = 0.f;
   for (int i = 0; i < a.parts; ++i) through += a.through[at * a.parts + i];
-  float ends[N], kept[N], behind = 0.f, before = 0.f;   // pairs and reads that end at a step; what a step leaves behind the chunk
+  // Pairs that end at a step less those that begin at it, reads of the state that entered, what a step leaves behind the chunk.  The first is
+  // summed up between steps that let nothing through (resets, and decays below fp32's resolution, 2^-24): pairs on one side of
+  // such a step cancel but for roundings, beside which the gradient of a closed gate is next to nothing.
+  float pairs[N], reads[N], kept[N], behind = 0.f, before = 0.f, within = 0.f;
+  bool cut[N], open = true;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    ends[i] = kept[i] = 0.f;
+    pairs[i] = reads[i] = kept[i] = 0.f;
+    cut[i] = (in.reset >> i & 1) || (!(in.pad >> i & 1) && log2_gate(in.f[i]) < -24.f);
     const long long t = (long long)tile * (32 * N) + gate_row<N>(w, lane, i);
     if (t >= w.L) continue;
     for (int k = 0; k < a.dq_tiles; ++k) {
       const float2 u = a.dq[(k * bhs + bh) * w.L + t];
-      ends[i] += u.x + u.y;
+      reads[i] += u.x, pairs[i] += u.y;
     }
     for (int k = 0; k < a.dk_tiles; ++k) {
       const float2 u = a.dk[(k * bhs + bh) * w.L + t];
-      kept[i] += u.x, ends[i] -= u.y;
+      kept[i] += u.x, pairs[i] -= u.y;
     }
-    behind += ends[i], before += kept[i];
+    behind += reads[i], before += kept[i];
+  }
+#pragma unroll
+  for (int i = N - 1; i >= 0; --i) {   // (of the pairs, what reaches the step before this lane's, and whether what is behind them does)
+    within += pairs[i];
+    if (cut[i]) within = 0.f, open = false;
   }
   float suffix = behind, prefix = before;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const float u = __shfl_down_sync(~0u, suffix, o), v = __shfl_up_sync(~0u, prefix, o);
-    if (lane + o < 32) suffix += u;
+    const float u = __shfl_down_sync(~0u, suffix, o), v = __shfl_up_sync(~0u, prefix, o), x = __shfl_down_sync(~0u, within, o);
+    const bool y = __shfl_down_sync(~0u, (int)open, o);
+    if (lane + o < 32) {
+      suffix += u;
+      if (open) within += x;
+      open = open && y;
+    }
     if (lane >= o) prefix += v;
   }
   suffix = __shfl_down_sync(~0u, suffix, 1), prefix = __shfl_up_sync(~0u, prefix, 1);   // (of the lanes behind, before)
-  if (lane == 31) suffix = 0.f;
+  within = __shfl_down_sync(~0u, within, 1);
+  if (lane == 31) suffix = within = 0.f;
   if (lane == 0) prefix = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float da = suffix + prefix + through;
+  for (int i = N - 1; i >= 0; --i) {
+    within += pairs[i];
+    if (cut[i]) within = 0.f;
+    float da = suffix + prefix + through + within;
 #pragma unroll
-    for (int j = 0; j < N; ++j) da += j >= i ? ends[j] : kept[j];
+    for (int j = 0; j < N; ++j) da += j >= i ? reads[j] : kept[j];
     const long long t = (long long)tile * (32 * N) + gate_row<N>(w, lane, i);
     if (t >= w.L) continue;
     // log sigmoid(f)' = sigmoid(-f)

@@ -220,6 +220,37 @@ def test_weights_behind_gates_that_are_nearly_closed(form):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("kd,vd", [(64, 64), (64, 128), (128, 128)])
+@pytest.mark.parametrize("pattern", ["half", "some", "documents"])
+def test_gradients_of_closed_gates_beside_open_ones(form, dtype, kd, vd, pattern):
+    """nothing passes a closed gate: its gradient is next to nothing however much the steps on either side of it have to do with one
+    another, and open gates, whose slope is 3e-4, have a small one"""
+    q, k, v, f, hin, dy, dh = _inputs(dtype, 2, 300, 2, kd, vd, gate_dtype=torch.float32, shift=8.0, spread=0.5)
+    reset = None
+    if pattern == "half":
+        f[:, 40:100] = -70.0
+        f[:, 200:290] = -25.0
+    elif pattern == "some":
+        f[:, ::23] = -40.0
+        f[:, 7::31] = -20.0
+    else:
+        reset = torch.zeros(2, 300, dtype=torch.bool, device="cuda")
+        reset[:, 5::40] = True
+        f[:, ::29] = -90.0
+    kw = dict(hin=hin, scale=kd ** -0.5, dy=dy, dh=dh)
+    ref, _ = reference(q, k, v, f, reset=reset, **kw)
+    got = run(q, k, v, f, reset=reset, **kw)
+    u = torch.finfo(DT[dtype]).eps / 2 if dtype != "fp32" else 2.0 ** -19
+    # (shares of pairs, of both states and of what passes a chunk, each rounded once: 4 u / sqrt(3) / 2, with room for pairs that one walk
+    # rounds up and the other down)
+    near(got[5], ref[5], 1.5 * u, size=gate_sizes(q, k, v, f if reset is None else f.masked_fill(reset[..., None], -float("inf")), **kw))
+    shut = (f < -19)
+    # (a decay of e^-20 times products of states of 10 by 10, 128 x 128 of them, is below 1e-4)
+    assert float(got[5][shut].abs().max()) < 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 def test_which_form_takes_a_call(dtype):
     """tcgen05 takes 16-bit heads of at most 128 keys and values, more than 64 steps and rows on 16 bytes; mma.sync the rest"""
     _lib.set_option(1, 0)
