@@ -12,7 +12,8 @@
 // W_ij = (dy_i . v_j) (q_i . k_j) of a pair with its weight, summed over j by the walk of dq and over i by that of dk, the first is
 // sum_{i >= t} of the one less the other (fp32 products both, unrounded: the pairs on one side of t cancel); the next two are sums of
 // q_i . dq_i and k_j . dk_j of the parts that come from states, the last is the product of both states, for which the walk of dq leaves
-// every chunk's state in the activations' type.  Nothing is carried from chunk to chunk, where roundings would pile up.
+// every chunk's state in the activations' type (fp16: with its scale).  Nothing is carried from chunk to chunk, where roundings would pile
+// up, and pairs' sums are not carried past steps that let nothing through.
 //
 // This file: chunks of 64 steps on mma.sync, for fp32 (three products of TF32 pieces for each), heads of more than 128 keys or values, operands
 // that TMA cannot address, and short calls; everything else goes to the form on tcgen05 (decayed_attention_tc.cu).  A block of four warps

@@ -7,7 +7,8 @@
 //   dS = (w K)^T V                  w K in pieces of 8 (bf16, three) or 11 (fp16, two) bits, the first in K's place
 //   O2 = (weighted pairs) V
 // and y = e O1 + O2 with a row's factor e.  The sums for the gates' gradient are those of x with e O1 and with O2: of the latter, taken from
-// the walks of dq and dk, the pairs on one side of a step cancel because both walks round the same weights the same way.
+// the walks of dq and dk, the pairs on one side of a step cancel because both walks round the same weights the same way (but for the one pair
+// in some thousand whose weight, two units apart, lies next to a rounding's border: such a pair is off by one rounding).
 // Roles: eight warps of pairs and outputs (a thread has half of a row of the chunk), eight of weights and state (a thread has half of a
 // step's keys, then half of a row of the state, whose fp32 values stay in its registers), one that loads, one for
 // padded steps, and two that issue products: those of pairs, and those with the state (one warp for both takes longer to wait and to issue
@@ -76,6 +77,9 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
   // (eight lanes hold 32 steps; the last of them in the order of the walk is the last one's)
   const long long end = __shfl_sync(~0u, r.sum[3], lane | 7);
   const int there = __shfl_sync(~0u, r.count[3], lane | 7);
+  // (cut off alike for the walk that goes the other way, whose sums leave out a step's own gate: differences between steps are the same there)
+  const int way = w.excl ? -1 : 1;
+  auto place = [&](long long sum) { return (w.excl ? r.all - sum : sum) >> 22; };
   unsigned mask = 0;   // of this lane's rows in their word
   int rel[4];
   float col[4];
@@ -83,7 +87,7 @@ __global__ void __launch_bounds__(128) tc_gates_kernel(const __grid_constant__ W
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int to = w.rev ? 3 - k : k;   // rows ascend
-    rel[to] = (int)((r.sum[k] - end) >> 22), count[to] = (uint8_t)r.count[k];
+    rel[to] = way * (int)(place(r.sum[k]) - place(end)), count[to] = (uint8_t)r.count[k];
     col[to] = r.count[k] == there && !(in.pad >> k & 1) ? exp2f(gate_sum(end - r.sum[k]) + r.bad) : 0.f;
     mask |= (in.pad >> k & 1) << to;
   }

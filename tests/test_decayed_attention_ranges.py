@@ -250,6 +250,19 @@ def test_gradients_of_closed_gates_beside_open_ones(form, dtype, kd, vd, pattern
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mean,shut", [(-2.0, False), (-2.0, True), (2.0, True)])
+def test_gates_that_go_from_next_to_closed_to_open(form, mean, shut):
+    """the gradient's walks weigh a pair alike, to the last bit where each pair has a power of two of its own"""
+    q, k, v, f, hin, dy, dh = _inputs("fp16", 2, 260, 4, 128, 128, gate_dtype=torch.float32, shift=mean, spread=6.0)
+    if shut:
+        f[:, :130] = -70.0
+    kw = dict(hin=hin, scale=128 ** -0.5, dy=dy, dh=dh)
+    ref, _ = reference(q, k, v, f, **kw)
+    got = run(q, k, v, f, **kw)
+    near(got[5], ref[5], 1.2 * 2.0 ** -11)   # (four shares, each rounded once: 2 u / sqrt(3))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 def test_which_form_takes_a_call(dtype):
     """tcgen05 takes 16-bit heads of at most 128 keys and values, more than 64 steps and rows on 16 bytes; mma.sync the rest"""
